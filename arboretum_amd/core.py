@@ -22,6 +22,7 @@ def _load_lib():
             "libarboretum.so is not built: run `python arboretum_amd/build.py` (needs hipcc)")
     lib = ctypes.cdll.LoadLibrary(path)
     c_char_p, c_void_p, c_int, c_float = ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    c_long = ctypes.c_longlong
     P = ctypes.POINTER
     sigs = {
         # reference boundary (python-wrapper/arboretum_wrapper.h:6-39)
@@ -73,6 +74,15 @@ def _load_lib():
         "AHistSumPlan": [ctypes.c_longlong, c_int, P(ctypes.c_uint), P(ctypes.c_uint)],
         "AHistSumNoAlloc": [c_void_p] * 10 + [ctypes.c_ulonglong, ctypes.c_longlong, c_int, c_int, c_int, c_int,
                                               c_int, c_void_p, c_void_p],
+        "AEmbedding": [c_void_p] * 3 + [c_long, c_int, c_long, c_int] + [c_long] * 4 + [c_int, c_int, c_float, c_void_p,
+                                                                                   c_void_p],
+        "AEmbeddingSortBytes": [c_long, c_int, c_long, P(ctypes.c_ulonglong)],
+        "AEmbeddingSort": [c_void_p] * 3 + [c_long, c_int] + [c_long] * 3 + [c_int, c_void_p, ctypes.c_ulonglong,
+                                                                             c_void_p, c_void_p],
+        "AEmbeddingGradBytes": [c_long, c_int, c_int, P(ctypes.c_ulonglong)],
+        "AEmbeddingGrad": [c_void_p] * 4 + [c_long, c_int, c_long, c_int, c_long, c_long, c_int, c_int, c_float, c_int,
+                                            c_void_p, ctypes.c_ulonglong, c_void_p],
+        "AAdamW": [c_int] + [c_void_p] * 5 + [c_int, c_int] + [ctypes.c_double] * 6 + [c_long] + [c_void_p] * 3,
     }
     for name, args in sigs.items():
         fn = getattr(lib, name)
@@ -131,6 +141,74 @@ def hist_sum_no_alloc(sum_g, sum_h, bin_count, grad, hess, node_size, bins, stri
     _check(_LIB.AHistSumNoAlloc(sum_g, sum_h, bin_count, parent_g, parent_h, parent_c, grad, hess, node_size,
                                 bins, int(stride), int(nrow), int(ncol), int(nodes), int(bool(use_trick)),
                                 int(shift_g), int(shift_h), stream, status))
+
+
+_TYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+
+
+def _type(name):
+    try:
+        return _TYPES[name]
+    except (KeyError, TypeError):
+        raise ArboretumError(ValueError("element type %r is not one of %s" % (name, ", ".join(_TYPES)))) from None
+
+
+def embedding(out, table, tokens, n, vocab, dim, bag=1, scale=1.0, dtype="float32", token_bits=32, out_stride=None,
+              table_stride=None, token_stride=None, bag_stride=1, status=None, stream=None):
+    """out[i] = scale * (sum over the bag of table[token]), rows of `dim` elements of `dtype` ("float32", "bfloat16",
+    "float16") on the GPU (AEmbedding).  Array arguments are DEVICE addresses; token j of bag i is at
+    i * token_stride + j * bag_stride (elements; token_stride is `bag` unless given), -1 stands for none.
+    `status`: an optional device word, set to 1 by a token outside the table.  Does not wait."""
+    _check(_LIB.AEmbedding(out, table, tokens, n, bag, vocab, dim, dim if out_stride is None else out_stride,
+                           dim if table_stride is None else table_stride, bag if token_stride is None else token_stride,
+                           bag_stride, _type(dtype), token_bits, scale, status, stream))
+
+
+def embedding_sort_bytes(n, vocab, bag=1):
+    """Bytes of device memory embedding_sort works in (AEmbeddingSortBytes; no GPU needed)."""
+    v = ctypes.c_ulonglong()
+    _check(_LIB.AEmbeddingSortBytes(n, bag, vocab, ctypes.byref(v)))
+    return v.value
+
+
+def embedding_sort(keys, rows, tokens, n, vocab, work, work_bytes, bag=1, token_bits=32, token_stride=None,
+                   bag_stride=1, status=None, stream=None):
+    """The (token, bag) pairs of n bags in order of tokens, for embedding_grad (AEmbeddingSort): keys and rows take
+    n * bag 32-bit words each.  Tokens as in embedding(); `work`: embedding_sort_bytes() of device memory.  Does not wait."""
+    _check(_LIB.AEmbeddingSort(keys, rows, tokens, n, bag, vocab, bag if token_stride is None else token_stride, bag_stride,
+                               token_bits, work, work_bytes, status, stream))
+
+
+def embedding_grad_bytes(n, dim, bag=1):
+    """Bytes of device memory embedding_grad works in (AEmbeddingGradBytes; no GPU needed)."""
+    v = ctypes.c_ulonglong()
+    _check(_LIB.AEmbeddingGradBytes(n, bag, dim, ctypes.byref(v)))
+    return v.value
+
+
+def embedding_grad(grad_table, grad_out, keys, rows, n, vocab, dim, work, work_bytes, bag=1, scale=1.0, dtype="float32",
+                   grad_dtype="float32", accumulate=False, table_stride=None, out_stride=None, stream=None):
+    """Gradient of embedding()'s table (AEmbeddingGrad): grad_table[v] = scale * (sum of grad_out[row] over the pairs of
+    embedding_sort with key v), added to what is there with `accumulate`.  dtype: of grad_out; grad_dtype: of grad_table, that or
+    "float32".  The same from run to run.  Does not wait."""
+    _check(_LIB.AEmbeddingGrad(grad_table, grad_out, keys, rows, n, bag, vocab, dim,
+                               dim if table_stride is None else table_stride, dim if out_stride is None else out_stride,
+                               _type(dtype), _type(grad_dtype), scale, int(bool(accumulate)), work, work_bytes, stream))
+
+
+def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
+          grad_scale=1.0, dtype="float32", grad_dtype=None, lr_device=None, step_device=None, stream=None):
+    """One AdamW step over a list of tensors on the GPU (AAdamW).  params, grads, exp_avgs, exp_avg_sqs: DEVICE addresses, a list or
+    an integer array of them each; sizes: elements of each tensor.  params have `dtype`, grads `grad_dtype` (dtype unless
+    given), the two states float32.  `step` counts from 1.  lr_device, step_device: optional device words (float32, int64)
+    read instead of lr and step.  Does not wait."""
+    lists = [np.ascontiguousarray(a, dtype=np.uint64) for a in (params, grads, exp_avgs, exp_avg_sqs)]
+    sizes = np.ascontiguousarray(sizes, dtype=np.int64)
+    if sizes.ndim != 1 or any(a.shape != sizes.shape for a in lists):
+        raise ArboretumError(ValueError("the lists of tensors differ in length"))
+    _check(_LIB.AAdamW(sizes.size, *(a.ctypes.data for a in lists), sizes.ctypes.data, _type(dtype),
+                       _type(dtype if grad_dtype is None else grad_dtype), lr, beta1, beta2, eps, weight_decay, grad_scale,
+                       step, lr_device, step_device, stream))
 
 
 def _fptr(a):

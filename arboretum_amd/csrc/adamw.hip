@@ -1,0 +1,184 @@
+// AdamW over many tensors at once.  For every element, in 32 bits,
+//   g = grad_scale * grad            m = beta1 m + (1 - beta1) g
+//   p = p - lr weight_decay p        v = beta2 v + (1 - beta2) g^2
+//   p = p - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+// (Loshchilov and Hutter, "Decoupled weight decay regularization").  The states m and v stay in 32 bits; p is rounded once,
+// to its own type.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "operators_device.h"
+
+namespace arb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kVec = 4;                            // elements of a load
+constexpr int kChunk = kThreads * kVec * 8;        // elements of a workgroup
+constexpr int kTensorsAtOnce = 88;                 // a launch's tensors travel in its arguments (4 KB of them)
+
+struct Tensor {
+  void *p;
+  const void *g;
+  float *m, *v;
+  long long size;
+};
+
+struct Scalars {
+  float decay, beta1, beta2, rest1, rest2, step_size, root, eps, grad_scale;
+};
+
+// What depends on the step and the learning rate: in 64 bits, rounded once.
+__host__ __device__ inline void SetStep(Scalars *s, double lr, double weight_decay, double beta1, double beta2, double t) {
+  s->decay = (float)(1.0 - lr * weight_decay);
+  s->step_size = (float)(lr / (1.0 - pow(beta1, t)));
+  s->root = (float)sqrt(1.0 - pow(beta2, t));
+}
+
+struct Launch {
+  Tensor tensor[kTensorsAtOnce];
+  unsigned first[kTensorsAtOnce + 1];  // workgroup that begins each tensor
+  int count;
+  Scalars s;
+  double lr, weight_decay, beta1, beta2;
+  long long step;
+  const float *lr_device;
+  const long long *step_device;
+};
+static_assert(sizeof(Launch) <= 4096, "kernel arguments");
+
+template <typename P, typename G>
+__device__ __forceinline__ void Update(const Scalars &s, P &p, G grad, float &m, float &v) {
+  const float g = static_cast<float>(grad) * s.grad_scale;
+  m = s.beta1 * m + s.rest1 * g;
+  v = s.beta2 * v + s.rest2 * (g * g);
+  const float x = static_cast<float>(p) * s.decay;
+  p = Round<P>(x - s.step_size * m / (sqrtf(v) / s.root + s.eps));
+}
+
+template <typename P, typename G>
+__global__ void __launch_bounds__(kThreads) k_adamw(const Launch a) {
+  __shared__ Scalars s_scalars;
+  Scalars s = a.s;
+  if (a.lr_device != nullptr || a.step_device != nullptr) {
+    if (threadIdx.x == 0) {
+      s_scalars = a.s;
+      const double lr = a.lr_device != nullptr ? (double)*a.lr_device : a.lr;
+      const long long t = a.step_device != nullptr ? *a.step_device : a.step;
+      SetStep(&s_scalars, lr, a.weight_decay, a.beta1, a.beta2, (double)max(t, 1ll));
+    }
+    __syncthreads();
+    s = s_scalars;
+  }
+  int low = 0, high = a.count;  // first[low] <= blockIdx.x < first[high]
+  while (high - low > 1) {
+    const int mid = (low + high) / 2;
+    if (a.first[mid] <= blockIdx.x) low = mid;
+    else high = mid;
+  }
+  const Tensor t = a.tensor[low];
+  const long long begin = (long long)(blockIdx.x - a.first[low]) * kChunk, end = min(t.size, begin + kChunk);
+  P *p = static_cast<P *>(t.p);
+  const G *g = static_cast<const G *>(t.g);
+  for (long long i = begin + threadIdx.x; i < end; i += kThreads) Update(s, p[i], g[i], t.m[i], t.v[i]);
+}
+
+// Two ranges of one list that meet would be updated twice, by two workgroups at once.
+template <typename Ptr>
+void CheckApart(const AdamWArgs &a, Ptr list, size_t bytes, const char *what) {
+  auto begin = [&](int i) { return reinterpret_cast<uintptr_t>(list[i]); };
+  auto meet = [&](int i, int j) { return begin(i) + (size_t)a.sizes[i] * bytes > begin(j); };
+  int last = -1;
+  bool rising = true;
+  for (int i = 0; i < a.count; ++i) {
+    if (a.sizes[i] == 0) continue;
+    if (last >= 0 && begin(i) < begin(last)) rising = false;
+    else if (last >= 0 && meet(last, i)) throw std::runtime_error(std::string(what) + " overlap");
+    last = i;
+  }
+  if (rising) return;
+  std::vector<int> order;
+  for (int i = 0; i < a.count; ++i)
+    if (a.sizes[i] != 0) order.push_back(i);
+  std::sort(order.begin(), order.end(), [&](int i, int j) { return begin(i) < begin(j); });
+  for (size_t k = 1; k < order.size(); ++k)
+    if (meet(order[k - 1], order[k])) throw std::runtime_error(std::string(what) + " overlap");
+}
+
+void Validate(const AdamWArgs &a) {
+  CheckType(a.type);
+  CheckType(a.grad_type);
+  if (a.count < 0) throw std::runtime_error("bad tensor count");
+  if (a.count > 0 && (!a.params || !a.grads || !a.exp_avg || !a.exp_avg_sq || !a.sizes)) throw std::runtime_error("null pointer argument");
+  for (int i = 0; i < a.count; ++i) {
+    if (a.sizes[i] < 0 || a.sizes[i] >= (1ll << 40)) throw std::runtime_error("bad tensor size");
+    if (a.sizes[i] == 0) continue;
+    if (!a.params[i] || !a.grads[i] || !a.exp_avg[i] || !a.exp_avg_sq[i]) throw std::runtime_error("null tensor");
+    CheckAligned(a.params[i], ElementBytes(a.type), "a parameter");
+    CheckAligned(a.grads[i], ElementBytes(a.grad_type), "a gradient");
+    CheckAligned(a.exp_avg[i], 4, "a state");
+    CheckAligned(a.exp_avg_sq[i], 4, "a state");
+    if (a.params[i] == a.exp_avg[i] || a.params[i] == a.exp_avg_sq[i] || a.exp_avg[i] == a.exp_avg_sq[i])
+      throw std::runtime_error("a tensor and its states overlap");
+  }
+  // (comparisons that a NaN fails)
+  if (!(a.lr >= 0) || !(a.eps >= 0) || !(a.weight_decay >= 0)) throw std::runtime_error("lr, eps and weight_decay must not be negative");
+  if (!(a.beta1 >= 0 && a.beta1 < 1) || !(a.beta2 >= 0 && a.beta2 < 1)) throw std::runtime_error("beta1 and beta2 must be in [0, 1)");
+  if (!std::isfinite(a.lr) || !std::isfinite(a.eps) || !std::isfinite(a.weight_decay) || !std::isfinite(a.grad_scale))
+    throw std::runtime_error("lr, eps, weight_decay and grad_scale must be finite");
+  if (!a.step_device && a.step < 1) throw std::runtime_error("step counts from 1");
+  CheckAligned(a.lr_device, 4, "lr_device");
+  CheckAligned(a.step_device, 8, "step_device");
+  CheckApart(a, a.params, ElementBytes(a.type), "params");
+  CheckApart(a, a.exp_avg, 4, "states");
+  CheckApart(a, a.exp_avg_sq, 4, "states");
+}
+
+}  // namespace
+
+void AdamW(const AdamWArgs &a) {
+  Validate(a);
+  Launch l;
+  l.s.beta1 = (float)a.beta1;
+  l.s.beta2 = (float)a.beta2;
+  l.s.rest1 = (float)(1.0 - a.beta1);
+  l.s.rest2 = (float)(1.0 - a.beta2);
+  l.s.eps = (float)a.eps;
+  l.s.grad_scale = (float)a.grad_scale;
+  SetStep(&l.s, a.lr, a.weight_decay, a.beta1, a.beta2, (double)std::max(a.step, 1ll));
+  l.lr = a.lr;
+  l.weight_decay = a.weight_decay;
+  l.beta1 = a.beta1;
+  l.beta2 = a.beta2;
+  l.step = a.step;
+  l.lr_device = a.lr_device;
+  l.step_device = a.step_device;
+  int at = 0;
+  while (at < a.count) {
+    unsigned long long blocks = 0;
+    l.count = 0;
+    const void *first = nullptr;
+    for (; at < a.count && l.count < kTensorsAtOnce; ++at) {
+      if (a.sizes[at] == 0) continue;
+      const unsigned long long more = (unsigned long long)(a.sizes[at] + kChunk - 1) / kChunk;
+      if (blocks + more > (1ull << 30)) break;
+      if (l.count == 0) first = a.params[at];
+      l.tensor[l.count] = Tensor{a.params[at], a.grads[at], a.exp_avg[at], a.exp_avg_sq[at], a.sizes[at]};
+      l.first[l.count++] = (unsigned)blocks;
+      blocks += more;
+    }
+    if (l.count == 0) break;
+    l.first[l.count] = (unsigned)blocks;
+    OnDeviceOf device(first);
+    WithType(a.type, [&](auto p) {
+      WithType(a.grad_type, [&](auto g) {
+        hipLaunchKernelGGL((k_adamw<decltype(p), decltype(g)>), dim3((unsigned)blocks), dim3(kThreads), 0,
+                           static_cast<hipStream_t>(a.stream), l);
+      });
+    });
+    HIP_OK(hipGetLastError());
+  }
+}
+
+}  // namespace arb

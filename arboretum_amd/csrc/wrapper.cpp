@@ -14,6 +14,7 @@
 #include "booster.h"
 #include "hist_sum.h"
 #include "memory_pool.h"
+#include "operators.h"
 #include "parallel.h"
 
 using namespace arb;
@@ -420,6 +421,58 @@ const char *AHistSumNoAlloc(long long *sum_g, long long *sum_h, unsigned *bin_co
     HistSumArgs a{bins, stride, ncol, nrow, grad, hess, node_size, nodes, use_trick, parent_g, parent_h, parent_c,
                   shift_g, shift_h, sum_g, sum_h, bin_count, stream};
     HistSumNoAlloc(a, status);
+  });
+}
+
+const char *AEmbedding(void *out, const void *table, const void *tokens, long long n, int bag, long long vocab, int dim,
+                       long long out_stride, long long table_stride, long long token_stride, long long bag_stride,
+                       int type, int token_bits, float scale, unsigned *status, void *stream) {
+  return Guard([&] {
+    Embedding(EmbeddingArgs{{tokens, token_bits, n, bag, token_stride, bag_stride, vocab, status}, table, table_stride, out,
+                            out_stride, dim, type, scale, stream});
+  });
+}
+
+const char *AEmbeddingSortBytes(long long n, int bag, long long vocab, unsigned long long *bytes) {
+  return Guard([&] {
+    if (!bytes) throw std::runtime_error("bad arguments");
+    *bytes = EmbeddingSortBytes(n, bag, vocab);
+  });
+}
+
+const char *AEmbeddingSort(unsigned *keys, unsigned *rows, const void *tokens, long long n, int bag, long long vocab,
+                           long long token_stride, long long bag_stride, int token_bits, void *work,
+                           unsigned long long work_bytes, unsigned *status, void *stream) {
+  return Guard([&] {
+    EmbeddingSort(EmbeddingSortArgs{{tokens, token_bits, n, bag, token_stride, bag_stride, vocab, status}, keys, rows, work,
+                                    work_bytes, stream});
+  });
+}
+
+const char *AEmbeddingGradBytes(long long n, int bag, int dim, unsigned long long *bytes) {
+  return Guard([&] {
+    if (!bytes) throw std::runtime_error("bad arguments");
+    *bytes = EmbeddingGradBytes(n, bag, dim);
+  });
+}
+
+const char *AEmbeddingGrad(void *grad_table, const void *grad_out, const unsigned *keys, const unsigned *rows,
+                           long long n, int bag, long long vocab, int dim, long long table_stride, long long out_stride,
+                           int type, int table_type, float scale, int accumulate, void *work,
+                           unsigned long long work_bytes, void *stream) {
+  return Guard([&] {
+    EmbeddingGrad(EmbeddingGradArgs{keys, rows, n, bag, vocab, grad_out, out_stride, grad_table, table_stride, dim, type, table_type,
+                                    scale, accumulate != 0, work, work_bytes, stream});
+  });
+}
+
+const char *AAdamW(int count, void *const *params, const void *const *grads, float *const *exp_avg,
+                   float *const *exp_avg_sq, const long long *sizes, int type, int grad_type, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, double grad_scale, long long step,
+                   const float *lr_device, const long long *step_device, void *stream) {
+  return Guard([&] {
+    AdamW(AdamWArgs{count, params, grads, exp_avg, exp_avg_sq, sizes, type, grad_type, lr, beta1, beta2, eps, weight_decay,
+                    grad_scale, step, lr_device, step_device, stream});
   });
 }
 
