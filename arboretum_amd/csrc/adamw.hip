@@ -16,6 +16,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kVec = 4;                            // elements of a load
 constexpr int kChunk = kThreads * kVec * 8;        // elements of a workgroup
+constexpr int kAhead = 2;
 constexpr int kTensorsAtOnce = 88;                 // a launch's tensors travel in its arguments (4 KB of them)
 
 struct Tensor {
@@ -81,7 +82,36 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const Launch a) {
   const long long begin = (long long)(blockIdx.x - a.first[low]) * kChunk, end = min(t.size, begin + kChunk);
   P *p = static_cast<P *>(t.p);
   const G *g = static_cast<const G *>(t.g);
-  for (long long i = begin + threadIdx.x; i < end; i += kThreads) Update(s, p[i], g[i], t.m[i], t.v[i]);
+  typedef Pack<P, kVec> Ps;
+  typedef Pack<G, kVec> Gs;
+  typedef Pack<float, kVec> Fs;
+  constexpr long long kStep = kThreads * kVec;
+  long long i = begin + threadIdx.x * kVec;
+  // kAhead vectors of each array in flight
+  for (; i + (kAhead - 1) * kStep + kVec <= end; i += kAhead * kStep) {
+    Ps ps[kAhead];
+    Gs gs[kAhead];
+    Fs ms[kAhead], vs[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const long long at = i + k * kStep;
+      gs[k] = *reinterpret_cast<const Gs *>(g + at);
+      ps[k] = *reinterpret_cast<const Ps *>(p + at);
+      ms[k] = *reinterpret_cast<const Fs *>(t.m + at);
+      vs[k] = *reinterpret_cast<const Fs *>(t.v + at);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const long long at = i + k * kStep;
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) Update(s, ps[k].v[c], gs[k].v[c], ms[k].v[c], vs[k].v[c]);
+      *reinterpret_cast<Ps *>(p + at) = ps[k];
+      *reinterpret_cast<Fs *>(t.m + at) = ms[k];
+      *reinterpret_cast<Fs *>(t.v + at) = vs[k];
+    }
+  }
+  for (; i < end; i += kStep)
+    for (long long at = i; at < min(end, i + kVec); ++at) Update(s, p[at], g[at], t.m[at], t.v[at]);
 }
 
 // Two ranges of one list that meet would be updated twice, by two workgroups at once.
