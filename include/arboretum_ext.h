@@ -217,7 +217,7 @@ const char *AHistSumNoAlloc(long long *sum_g, long long *sum_h, unsigned *bin_co
  * count elements and are not negative; rows may begin at any element.
  * Tokens: token j of bag i is tokens[i * token_stride + j * bag_stride], a signed integer of token_bits (32 or 64).  -1
  * stands for none.  Any other outside [0, vocab) is treated as none too, and sets *status (a device word, may be
- * NULL, never cleared here) to 1.  n * bag and vocab are below 2^31; both n and bag may be 0. */
+ * NULL, never cleared here) to 1.  n * bag and vocab are below 2^31, dim below 2^24; both n and bag may be 0. */
 
 /* out[i] = scale * (sum over j of table[token(i, j)]), rows of `dim` elements; 0 for a bag without tokens. */
 const char *AEmbedding(void *out, const void *table, const void *tokens, long long n, int bag, long long vocab, int dim,

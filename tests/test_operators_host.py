@@ -58,6 +58,7 @@ TOKENS = [
 @pytest.mark.parametrize("change, says", TOKENS + [
     (dict(dtype="float64"), "element type"),
     (dict(dim=0), "bad dimension"),
+    (dict(dim=1 << 24), "bad dimension"),
     (dict(out=None), "null pointer"),
     (dict(table=None), "null pointer"),
     (dict(out=A + 2), "not aligned"),
@@ -87,6 +88,7 @@ def test_embedding_sort_refuses(arb, change, says):
     (dict(n=1 << 24, bag=1 << 7), "below 2\\^31"),
     (dict(vocab=0), "bad vocabulary"),
     (dict(dim=0), "bad dimension"),
+    (dict(dim=1 << 24), "bad dimension"),
     (dict(dtype="int8"), "element type"),
     (dict(dtype="bfloat16", grad_dtype="float16"), "float32 or of the type"),
     (dict(dtype="float32", grad_dtype="bfloat16"), "float32 or of the type"),
