@@ -202,11 +202,14 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta
     an integer array of them each; sizes: elements of each tensor.  params have `dtype`, grads `grad_dtype` (dtype unless
     given), the two states float32.  `step` counts from 1.  lr_device, step_device: optional device words (float32, int64)
     read instead of lr and step.  Does not wait."""
-    lists = [np.ascontiguousarray(a, dtype=np.uint64) for a in (params, grads, exp_avgs, exp_avg_sqs)]
-    sizes = np.ascontiguousarray(sizes, dtype=np.int64)
-    if sizes.ndim != 1 or any(a.shape != sizes.shape for a in lists):
-        raise ArboretumError(ValueError("the lists of tensors differ in length"))
-    _check(_LIB.AAdamW(sizes.size, *(a.ctypes.data for a in lists), sizes.ctypes.data, _type(dtype),
+    try:  # the five lists one after the other
+        table = np.array((params, grads, exp_avgs, exp_avg_sqs, sizes), dtype=np.int64)
+    except (ValueError, TypeError, OverflowError):
+        table = None
+    if table is None or table.ndim != 2:
+        raise ArboretumError(ValueError("the lists of tensors differ in length or hold other than addresses and sizes"))
+    count, at = table.shape[1], table.ctypes.data
+    _check(_LIB.AAdamW(count, at, at + 8 * count, at + 16 * count, at + 24 * count, at + 32 * count, _type(dtype),
                        _type(dtype if grad_dtype is None else grad_dtype), lr, beta1, beta2, eps, weight_decay, grad_scale,
                        step, lr_device, step_device, stream))
 

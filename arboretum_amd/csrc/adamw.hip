@@ -15,7 +15,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVec = 4;                            // elements of a load
-constexpr int kChunk = kThreads * kVec * 8;        // elements of a workgroup
+constexpr int kLeastChunk = kThreads * kVec;       // elements of a workgroup, and at most
+constexpr int kMostChunk = kThreads * kVec * 8;
+constexpr unsigned long long kEnoughBlocks = 2048;
 constexpr int kAhead = 2;
 constexpr int kTensorsAtOnce = 88;                 // a launch's tensors travel in its arguments (4 KB of them)
 
@@ -40,7 +42,7 @@ __host__ __device__ inline void SetStep(Scalars *s, double lr, double weight_dec
 struct Launch {
   Tensor tensor[kTensorsAtOnce];
   unsigned first[kTensorsAtOnce + 1];  // workgroup that begins each tensor
-  int count;
+  int count, chunk;
   Scalars s;
   double lr, weight_decay, beta1, beta2;
   long long step;
@@ -79,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const Launch a) {
     else high = mid;
   }
   const Tensor t = a.tensor[low];
-  const long long begin = (long long)(blockIdx.x - a.first[low]) * kChunk, end = min(t.size, begin + kChunk);
+  const long long begin = (long long)(blockIdx.x - a.first[low]) * a.chunk, end = min(t.size, begin + a.chunk);
   P *p = static_cast<P *>(t.p);
   const G *g = static_cast<const G *>(t.g);
   typedef Pack<P, kVec> Ps;
@@ -184,6 +186,11 @@ void AdamW(const AdamWArgs &a) {
   l.step = a.step;
   l.lr_device = a.lr_device;
   l.step_device = a.step_device;
+  // few elements are spread over the chip, a vector a thread; many in chunks that keep a workgroup busy for a while
+  unsigned long long all = 0;
+  for (int i = 0; i < a.count; ++i) all += (unsigned long long)a.sizes[i];
+  l.chunk = kLeastChunk;
+  while (l.chunk < kMostChunk && all / l.chunk > kEnoughBlocks) l.chunk *= 2;
   int at = 0;
   while (at < a.count) {
     unsigned long long blocks = 0;
@@ -191,7 +198,7 @@ void AdamW(const AdamWArgs &a) {
     const void *first = nullptr;
     for (; at < a.count && l.count < kTensorsAtOnce; ++at) {
       if (a.sizes[at] == 0) continue;
-      const unsigned long long more = (unsigned long long)(a.sizes[at] + kChunk - 1) / kChunk;
+      const unsigned long long more = (unsigned long long)(a.sizes[at] + l.chunk - 1) / l.chunk;
       if (blocks + more > (1ull << 30)) break;
       if (l.count == 0) first = a.params[at];
       l.tensor[l.count] = Tensor{a.params[at], a.grads[at], a.exp_avg[at], a.exp_avg_sq[at], a.sizes[at]};

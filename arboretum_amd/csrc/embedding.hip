@@ -25,10 +25,9 @@ struct Bags {
   int bag;
   unsigned vocab;
   unsigned *status;
-  // The row of the table that token j of bag i names; `vocab` for none.
-  __device__ __forceinline__ unsigned At(long long i, long long j) const {
-    return Row(tokens[i * token_stride + j * bag_stride]);
-  }
+  __device__ __forceinline__ Token At(long long i, long long j) const { return tokens[i * token_stride + j * bag_stride]; }
+  // The row of the table that a token names; `vocab` for none.  (Called when all tokens of a step have been asked for: behind the
+  // store to *status no load is started early.)
   __device__ __forceinline__ unsigned Row(Token t) const {
     typedef std::make_unsigned_t<Token> Word;
     if ((Word)t < (Word)vocab) return (unsigned)t;
@@ -88,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> ba
   const unsigned lane = threadIdx.x & ((1u << lanes_log) - 1u);
   const int step = kVec << lanes_log;
   const int first = (int)blockIdx.y * (step * kPieces) + (int)lane * kVec;
-  const unsigned t = bags.At(i, 0);
+  const unsigned t = bags.Row(bags.At(i, 0));
   const T *from = r.table + (long long)t * r.table_stride;
   T *to = r.out + i * r.out_stride;
   Pack<T, kVec> x[kPieces];
@@ -127,12 +126,12 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
     const Token *at = bags.tokens + i * bags.token_stride + share * bags.bag_stride;
     const long long step = (long long)shares * bags.bag_stride;
     for (int j = share; j < bags.bag; j += kAhead * shares) {
+      Token token[kAhead];
       unsigned t[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        t[k] = bags.vocab;
-        if (j + k * shares < bags.bag) t[k] = bags.Row(at[k * step]);
-      }
+      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bags.bag ? at[k * step] : Token(-1);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) t[k] = bags.Row(token[k]);
       at += kAhead * step;
       Pack<T, kVec> x[kAhead];
 #pragma unroll
@@ -190,44 +189,186 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
 }
 
 // -------------------------------------------------------------------- sort
-//
-// Least significant digit first, up to 9 bits at a time: two passes up to a vocabulary of 262,143.  A tile of 4096 pairs is put in
-// order in the LDS, so that the pairs of a digit leave as one run.
 
-constexpr int kSortThreads = 512;
-constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kSortRounds = 8;                         // pairs per thread
-constexpr int kSortTile = kSortThreads * kSortRounds;  // 4096
-constexpr int kWavePairs = kSortTile / kSortWaves;
-constexpr int kDigitBits = 9;
-constexpr int kDigits = 1 << kDigitBits;
-
-// Where a pass takes its pairs from: the tokens themselves, or keys and rows.
+// The pairs of a call, numbered in the order the tokens lie in memory.
 template <typename Token>
-struct FromTokens {
+struct Pairs {
   Bags<Token> bags;
   unsigned m;
   bool by_column;  // pair p is token p / n of bag p % n, else token p % bag of bag p / bag
-  __device__ __forceinline__ void Get(unsigned p, unsigned *key, unsigned *row) const {
-    unsigned i, j;
-    if (by_column) {
-      j = p / (unsigned)bags.n;
-      i = p - j * (unsigned)bags.n;
-    } else {
-      i = p / (unsigned)bags.bag;
-      j = p - i * (unsigned)bags.bag;
-    }
-    *key = bags.At(i, j);
-    *row = i;
+  bool flat;       // ... and stands at tokens[p]
+  __device__ __forceinline__ unsigned Bag(unsigned p) const {
+    return by_column ? p % (unsigned)bags.n : p / (unsigned)bags.bag;
   }
+  __device__ __forceinline__ Token At(unsigned p) const {
+    if (flat) return bags.tokens[p];
+    const unsigned i = Bag(p);
+    return bags.At(i, by_column ? p / (unsigned)bags.n : p - i * (unsigned)bags.bag);
+  }
+};
+
+template <typename Token>
+Pairs<Token> PairsOf(const TokenBags &b, unsigned m) {
+  const bool by_column = b.token_stride < b.bag_stride;
+  const bool flat = by_column ? (b.token_stride == 1 || b.n == 1) && (b.bag_stride == b.n || b.bag == 1)
+                              : (b.bag_stride == 1 || b.bag == 1) && (b.token_stride == b.bag || b.n == 1);
+  return Pairs<Token>{BagsOf<Token>(b), m, by_column, flat};
+}
+
+// Lanes of the wave that hold the same digit of kBits bits as this one.
+template <int kBits>
+__device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid) {
+  unsigned long long peers = __ballot(valid);
+#pragma unroll
+  for (int b = 0; b < kBits; ++b) {
+    const unsigned long long m = __ballot((d >> b) & 1u);
+    peers &= ((d >> b) & 1u) ? m : ~m;
+  }
+  return peers;
+}
+
+// ---- few pairs: one launch
+//
+// Every workgroup has a range of the vocabulary.  It reads all tokens (they come out of the L2), counts those below its range, which is
+// where its pairs start in the result, keeps those within, and sorts them in the LDS.  Nothing passes between workgroups.
+
+constexpr int kRangeThreads = 1024;
+constexpr int kRangeWaves = kRangeThreads / 64;
+constexpr int kRangeBits = 6;  // of a digit
+constexpr unsigned kMostRangePairs = 32768;
+constexpr unsigned kMostRanges = 256;  // a workgroup per CU
+
+// Pairs are kept as (key - first key of the range) << place_bits | place.
+template <int kRounds, typename Token>
+__global__ void __launch_bounds__(kRangeThreads)
+k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits, unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
+  __shared__ unsigned s_pair[kRounds * kRangeThreads];
+  __shared__ unsigned s_count[kRangeWaves << kRangeBits];  // pairs of a digit, then their place; the waves of a digit beside each other
+  __shared__ unsigned s_sum[2][kRangeWaves];
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned v0 = blockIdx.x * span;
+  Token token[kRounds];
+  unsigned key[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const unsigned p = k * kRangeThreads + threadIdx.x;
+    token[k] = p < in.m ? in.At(p) : Token(-1);
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) key[k] = k * kRangeThreads + threadIdx.x < in.m ? in.bags.Row(token[k]) : ~0u;
+  unsigned within = 0, below = 0;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const bool real = key[k] <= in.bags.vocab;
+    within += (unsigned)__popcll(__ballot(real && key[k] >= v0 && key[k] - v0 < span));
+    below += (unsigned)__popcll(__ballot(key[k] < v0));
+  }
+  if (lane == 0) {
+    s_sum[0][wave] = within;
+    s_sum[1][wave] = below;
+  }
+  __syncthreads();
+  unsigned at = 0, held = 0, start = 0;
+#pragma unroll
+  for (unsigned w = 0; w < kRangeWaves; ++w) {
+    if (w < wave) at += s_sum[0][w];
+    held += s_sum[0][w];
+    start += s_sum[1][w];
+  }
+  if (held == 0) return;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const bool mine = key[k] <= in.bags.vocab && key[k] >= v0 && key[k] - v0 < span;
+    const unsigned long long all = __ballot(mine);
+    if (mine) s_pair[at + (unsigned)__popcll(all & ((1ull << lane) - 1ull))] = (key[k] - v0) << place_bits | (k * kRangeThreads + threadIdx.x);
+    at += (unsigned)__popcll(all);
+  }
+  const int passes = (key_bits + kRangeBits - 1) / kRangeBits;
+  // a wave's pairs are a run of them: `rounds` times 64
+  const unsigned rounds = (held + kRangeThreads - 1) / kRangeThreads, first = wave * rounds * 64u;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int bits = (key_bits + passes - 1) / passes, shift = place_bits + pass * bits;
+    unsigned pair[kRounds], place[kRounds];
+    s_count[threadIdx.x] = 0;
+    __syncthreads();  // (the pairs are in place, too)
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      if (k < (int)rounds) {
+        const unsigned i = first + k * 64u + lane;
+        const bool valid = i < held;
+        pair[k] = valid ? s_pair[i] : 0u;
+        const unsigned d = (pair[k] >> shift) & ((1u << bits) - 1u);
+        const unsigned long long peers = DigitPeers<kRangeBits>(d, valid);
+        const unsigned less = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
+        unsigned *count = &s_count[d * kRangeWaves + wave];
+        const unsigned before = *count;
+        place[k] = before + less;
+        __builtin_amdgcn_wave_barrier();  // every lane has read its counter
+        if (valid && less == 0) *count = before + (unsigned)__popcll(peers);
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    __syncthreads();
+    // exclusive sum over (digit, wave), a counter a thread
+    const unsigned mine = s_count[threadIdx.x];
+    unsigned sum = mine;
+    for (int off = 1; off < 64; off <<= 1) {
+      const unsigned o = __shfl_up(sum, off);
+      if (lane >= (unsigned)off) sum += o;
+    }
+    if (lane == 63) s_sum[0][wave] = sum;
+    __syncthreads();
+    for (unsigned w = 0; w < wave; ++w) sum += s_sum[0][w];
+    s_count[threadIdx.x] = sum - mine;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      if (k < (int)rounds && first + k * 64u + lane < held) {
+        const unsigned d = (pair[k] >> shift) & ((1u << bits) - 1u);
+        s_pair[s_count[d * kRangeWaves + wave] + place[k]] = pair[k];
+      }
+    }
+    __syncthreads();
+  }
+  if (passes == 0) __syncthreads();
+  for (unsigned i = threadIdx.x; i < held; i += kRangeThreads) {
+    const unsigned pair = s_pair[i], p = pair & ((1u << place_bits) - 1u);
+    keys[start + i] = v0 + (pair >> place_bits);
+    rows[start + i] = in.Bag(p);
+  }
+}
+
+// ---- many pairs: least significant digit first
+//
+// Up to 9 bits a pass (two passes up to a vocabulary of 262,143), three or four launches each.  A tile of 8192 pairs is put
+// in order in the LDS, so that the pairs of a digit leave as one run.
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kSortRounds = 8;                         // pairs per thread
+constexpr int kSortTile = kSortThreads * kSortRounds;  // 8192
+constexpr int kWavePairs = kSortTile / kSortWaves;
+constexpr int kDigitBits = 9;
+constexpr int kDigits = 1 << kDigitBits;
+constexpr unsigned kGroupTiles = 32;  // tiles whose counts are summed up by one workgroup
+
+// Where a pass takes its pairs from: the tokens themselves, or the keys and rows of the pass before.
+template <typename Token>
+struct FromTokens {
+  Pairs<Token> pairs;
+  unsigned m;
+  typedef Token Raw;
+  __device__ __forceinline__ Token At(unsigned p) const { return pairs.At(p); }
+  __device__ __forceinline__ unsigned Key(Token t) const { return pairs.bags.Row(t); }
+  __device__ __forceinline__ unsigned Row(unsigned p) const { return pairs.Bag(p); }
 };
 struct FromPairs {
   const unsigned *keys, *rows;
   unsigned m;
-  __device__ __forceinline__ void Get(unsigned p, unsigned *key, unsigned *row) const {
-    *key = keys[p];
-    *row = rows[p];
-  }
+  typedef unsigned Raw;
+  __device__ __forceinline__ unsigned At(unsigned p) const { return keys[p]; }
+  __device__ __forceinline__ unsigned Key(unsigned key) const { return key; }
+  __device__ __forceinline__ unsigned Row(unsigned p) const { return rows[p]; }
 };
 
 struct Digit {
@@ -236,122 +377,147 @@ struct Digit {
   __device__ __forceinline__ unsigned Of(unsigned key) const { return (key >> shift) & mask; }
 };
 
-// Digit counts of one tile: counts[digit * tiles + tile].
+// Digit counts of one tile: counts[tile * kDigits + digit].  A thread's pairs lie beside each other and equal neighbours are counted
+// as one, and a wave of one digit only as one: pairs that are nearly in order (leaves, tree by tree; the last pass) would
+// otherwise queue for one counter of the LDS.
 template <typename Source>
-__global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts, unsigned tiles) {
+__global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
   __shared__ unsigned s_count[kDigits];
-  s_count[threadIdx.x] = 0;
+  if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
   __syncthreads();
-  const unsigned base = blockIdx.x * kSortTile;
+  const unsigned base = blockIdx.x * kSortTile + threadIdx.x * kSortRounds;
+  typename Source::Raw raw[kSortRounds];
+  unsigned d[kSortRounds];
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
-    const unsigned p = base + k * kSortThreads + threadIdx.x;
-    if (p < in.m) {
-      unsigned key, row;
-      in.Get(p, &key, &row);
-      atomicAdd(&s_count[digit.Of(key)], 1u);
+  for (int k = 0; k < kSortRounds; ++k) raw[k] = in.At(min(base + k, in.m - 1));
+#pragma unroll
+  for (int k = 0; k < kSortRounds; ++k) d[k] = base + k < in.m ? digit.Of(in.Key(raw[k])) : kDigits;
+  bool same = true;
+#pragma unroll
+  for (int k = 1; k < kSortRounds; ++k) same = same && d[k] == d[0];
+  const unsigned one = __builtin_amdgcn_readfirstlane(d[0]);
+  if (__ballot(!(same && d[0] == one)) == 0ull) {
+    if ((threadIdx.x & 63u) == 0 && one < kDigits) atomicAdd(&s_count[one], 64u * kSortRounds);
+  } else {
+    unsigned run = 0;
+#pragma unroll
+    for (int k = 0; k < kSortRounds; ++k) {
+      ++run;
+      if (k + 1 == kSortRounds || d[k + 1 < kSortRounds ? k + 1 : k] != d[k]) {
+        if (d[k] < kDigits) atomicAdd(&s_count[d[k]], run);
+        run = 0;
+      }
     }
   }
   __syncthreads();
-  counts[(size_t)threadIdx.x * tiles + blockIdx.x] = s_count[threadIdx.x];
+  if (threadIdx.x <= digit.mask) counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = s_count[threadIdx.x];
 }
 
-// Exclusive scan of the tile counts of a digit, in place, and the digit's total.  A workgroup per digit.
-__global__ void __launch_bounds__(256) k_sort_scan(unsigned *__restrict__ counts, unsigned tiles, unsigned *__restrict__ totals) {
-  __shared__ unsigned s_wave[4];
-  unsigned *v = counts + (size_t)blockIdx.x * tiles;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned carry = 0;
-  for (unsigned base = 0; base < tiles; base += 256) {
-    const unsigned i = base + threadIdx.x;
-    const unsigned c = i < tiles ? v[i] : 0u;
-    unsigned incl = c;
-    for (int off = 1; off < 64; off <<= 1) {
-      const unsigned o = __shfl_up(incl, off);
-      if (lane >= off) incl += o;
-    }
-    if (lane == 63) s_wave[wave] = incl;
-    __syncthreads();
-    unsigned before = carry;
+// Exclusive sums over the tiles of a group, in place, and the group's totals.  A thread per digit.
+__global__ void __launch_bounds__(kDigits) k_sort_sum_tiles(unsigned *__restrict__ counts, unsigned tiles, unsigned *__restrict__ groups) {
+  unsigned *v = counts + (size_t)blockIdx.x * kGroupTiles * kDigits + threadIdx.x;
+  const unsigned held = min(kGroupTiles, tiles - blockIdx.x * kGroupTiles);
+  unsigned c[kGroupTiles];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += s_wave[w];
-      carry += s_wave[w];
-    }
-    if (i < tiles) v[i] = before + incl - c;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
-}
-
-// Lanes of the wave that hold the same digit as this one.
-__device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid) {
-  unsigned long long peers = __ballot(valid);
+  for (unsigned k = 0; k < kGroupTiles; ++k) c[k] = k < held ? v[k * kDigits] : 0u;
+  unsigned sum = 0;
 #pragma unroll
-  for (int b = 0; b < kDigitBits; ++b) {
-    const unsigned long long m = __ballot((d >> b) & 1u);
-    peers &= ((d >> b) & 1u) ? m : ~m;
+  for (unsigned k = 0; k < kGroupTiles; ++k) {
+    if (k < held) v[k * kDigits] = sum;
+    sum += c[k];
   }
-  return peers;
+  groups[(size_t)blockIdx.x * kDigits + threadIdx.x] = sum;
 }
 
-// Stable scatter of one tile.  counts (scanned): pairs of the same digit in the tiles before.
+// The same over groups, and the totals of all behind them.  64 digits a workgroup, its waves share the groups.
+__global__ void __launch_bounds__(1024) k_sort_sum_groups(unsigned *__restrict__ groups, unsigned count) {
+  __shared__ unsigned s_sum[16][64];
+  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, digit = blockIdx.x * 64 + lane;
+  const unsigned per = (count + 15) / 16, b = min(count, wave * per), e = min(count, b + per);
+  unsigned sum = 0;
+#pragma unroll 8
+  for (unsigned i = b; i < e; ++i) sum += groups[(size_t)i * kDigits + digit];
+  s_sum[wave][lane] = sum;
+  __syncthreads();
+  unsigned run = 0, total = 0;
+#pragma unroll
+  for (unsigned w = 0; w < 16; ++w) {
+    if (w < wave) run += s_sum[w][lane];
+    total += s_sum[w][lane];
+  }
+#pragma unroll 8
+  for (unsigned i = b; i < e; ++i) {
+    const unsigned c = groups[(size_t)i * kDigits + digit];
+    groups[(size_t)i * kDigits + digit] = run;
+    run += c;
+  }
+  if (wave == 0) groups[(size_t)count * kDigits + digit] = total;
+}
+
+// Stable scatter of one tile.  counts, groups: pairs of the same digit in the tiles of the group before, in the groups before;
+// totals: pairs of each digit.
 template <typename Source>
 __global__ void __launch_bounds__(kSortThreads)
-k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ counts, unsigned tiles, const unsigned *__restrict__ totals,
-               unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
-  __shared__ unsigned s_key[kSortTile], s_row[kSortTile];
-  __shared__ unsigned s_wave[kSortWaves][kDigits];  // pairs of each digit of a wave; then those of the waves before
-  __shared__ unsigned s_first[kDigits];             // place in the tile of the first pair of each digit
-  __shared__ unsigned s_out[kDigits];               // output position of that pair
-  __shared__ unsigned s_sum[2][kSortWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ counts, const unsigned *__restrict__ groups,
+               const unsigned *__restrict__ totals, unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
+  __shared__ unsigned s_pair[kSortTile];                  // the keys, then the rows
+  __shared__ unsigned short s_wave[kSortWaves][kDigits];  // pairs of each digit of a wave; then those of the waves before
+  __shared__ unsigned s_first[kDigits];                   // place in the tile of the first pair of each digit
+  __shared__ unsigned s_out[kDigits];                     // output position of that pair
+  __shared__ unsigned s_sum[2][kDigits / 64];
+  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const unsigned base = blockIdx.x * kSortTile, held = min((unsigned)kSortTile, in.m - base);
-  for (int w = 0; w < kSortWaves; ++w) s_wave[w][threadIdx.x] = 0;
-  unsigned key[kSortRounds], row[kSortRounds], rank[kSortRounds];
+  for (int i = threadIdx.x; i < kSortWaves * kDigits / 2; i += kSortThreads) reinterpret_cast<unsigned *>(s_wave)[i] = 0;
+  typename Source::Raw raw[kSortRounds];
+  unsigned key[kSortRounds], place[kSortRounds];
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
-    const unsigned i = wave * kWavePairs + k * 64 + lane;
-    key[k] = row[k] = 0;
-    if (i < held) in.Get(base + i, &key[k], &row[k]);
+  for (int k = 0; k < kSortRounds; ++k) raw[k] = in.At(base + min(wave * kWavePairs + k * 64 + lane, held - 1));
+#pragma unroll
+  for (int k = 0; k < kSortRounds; ++k) key[k] = in.Key(raw[k]);  // (past the end: the last one's, which goes nowhere)
+  unsigned total = 0, before = 0;
+  if (threadIdx.x <= digit.mask) {
+    total = totals[threadIdx.x];
+    before = counts[(size_t)blockIdx.x * kDigits + threadIdx.x];
+    if (groups != nullptr) before += groups[(size_t)(blockIdx.x / kGroupTiles) * kDigits + threadIdx.x];
   }
-  const unsigned total = totals[threadIdx.x], before = counts[(size_t)threadIdx.x * tiles + blockIdx.x];
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortRounds; ++k) {
     const bool valid = wave * kWavePairs + k * 64 + lane < held;
     const unsigned d = digit.Of(key[k]);
-    const unsigned long long peers = DigitPeers(d, valid);
-    const unsigned below = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
+    const unsigned long long peers = DigitPeers<kDigitBits>(d, valid);
+    const unsigned less = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
     const unsigned held_of = s_wave[wave][d];
-    rank[k] = held_of + below;
+    place[k] = held_of + less;
     __builtin_amdgcn_wave_barrier();  // every lane has read its counter
-    if (valid && below == 0) s_wave[wave][d] = held_of + (unsigned)__popcll(peers);
+    if (valid && less == 0) s_wave[wave][d] = (unsigned short)(held_of + (unsigned)__popcll(peers));
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  {
-    // thread = digit: pairs of smaller digits in the tile, and in all
-    unsigned mine = 0;
+  // thread = digit: pairs of smaller digits in the tile, and in all
+  unsigned mine = 0;
+  if (threadIdx.x < kDigits) {
     for (int w = 0; w < kSortWaves; ++w) {
       const unsigned c = s_wave[w][threadIdx.x];
-      s_wave[w][threadIdx.x] = mine;
+      s_wave[w][threadIdx.x] = (unsigned short)mine;
       mine += c;
     }
-    unsigned in_tile = mine, in_all = total;
-    for (int off = 1; off < 64; off <<= 1) {
-      const unsigned a = __shfl_up(in_tile, off), b = __shfl_up(in_all, off);
-      if (lane >= off) {
-        in_tile += a;
-        in_all += b;
-      }
+  }
+  unsigned in_tile = mine, in_all = total;
+  for (int off = 1; off < 64; off <<= 1) {
+    const unsigned a = __shfl_up(in_tile, off), b = __shfl_up(in_all, off);
+    if (lane >= (unsigned)off) {
+      in_tile += a;
+      in_all += b;
     }
-    if (lane == 63) {
-      s_sum[0][wave] = in_tile;
-      s_sum[1][wave] = in_all;
-    }
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) {
+  }
+  if (lane == 63 && wave < kDigits / 64) {
+    s_sum[0][wave] = in_tile;
+    s_sum[1][wave] = in_all;
+  }
+  __syncthreads();
+  if (threadIdx.x < kDigits) {
+    for (unsigned w = 0; w < wave; ++w) {
       in_tile += s_sum[0][w];
       in_all += s_sum[1][w];
     }
@@ -363,43 +529,76 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   for (int k = 0; k < kSortRounds; ++k) {
     if (wave * kWavePairs + k * 64 + lane < held) {
       const unsigned d = digit.Of(key[k]);
-      const unsigned at = s_first[d] + s_wave[wave][d] + rank[k];
-      s_key[at] = key[k];
-      s_row[at] = row[k];
+      place[k] += s_first[d] + s_wave[wave][d];
+      s_pair[place[k]] = key[k];
+    }
+  }
+  __syncthreads();
+  unsigned to[kSortRounds];
+#pragma unroll
+  for (int k = 0; k < kSortRounds; ++k) {
+    const unsigned i = k * kSortThreads + threadIdx.x;
+    if (i < held) {
+      const unsigned v = s_pair[i], d = digit.Of(v);
+      to[k] = s_out[d] + (i - s_first[d]);
+      keys[to[k]] = v;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortRounds; ++k) {
+    const unsigned i = wave * kWavePairs + k * 64 + lane;
+    if (i < held) s_pair[place[k]] = in.Row(base + i);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSortRounds; ++k) {
     const unsigned i = k * kSortThreads + threadIdx.x;
-    if (i < held) {
-      const unsigned d = digit.Of(s_key[i]);
-      const unsigned to = s_out[d] + (i - s_first[d]);
-      keys[to] = s_key[i];
-      rows[to] = s_row[i];
-    }
+    if (i < held) rows[to[k]] = s_pair[i];
   }
 }
 
-// Passes and bits of a digit for keys in [0, vocab].
+int BitsOf(unsigned long long v) {
+  int bits = 0;
+  while (v >> bits) ++bits;
+  return bits;
+}
+
+// Which way a call goes, for keys in [0, vocab].
 struct SortPlan {
-  int passes, bits;
-  unsigned m, tiles;
-  size_t counts_bytes, pairs_bytes, bytes;
+  unsigned m;
+  // one launch: workgroups, keys of each, bits of a key within its range and of a pair's place; 0 workgroups: many pairs
+  unsigned ranges, span;
+  int key_bits, place_bits;
+  int passes, bits;  // many pairs
+  unsigned tiles, groups;
+  size_t counts_bytes, groups_bytes, pairs_bytes, bytes;
 };
 constexpr size_t Align256(size_t v) { return (v + 255) / 256 * 256; }
 
 SortPlan PlanSort(long long n, int bag, long long vocab) {
-  SortPlan s;
-  int bits = 1;
-  while (vocab >> bits) ++bits;
+  SortPlan s = {};
+  s.bytes = 256;  // (so that nobody allocates nothing)
+  s.m = (unsigned)(n * bag);
+  if (s.m == 0) return s;
+  if (s.m <= kMostRangePairs) {
+    // 256 keys a workgroup: two passes of four bits
+    s.ranges = (unsigned)std::min<long long>(vocab / 256 + 1, kMostRanges);
+    s.span = (unsigned)(vocab / s.ranges + 1);
+    s.key_bits = BitsOf(s.span - 1);
+    s.place_bits = BitsOf(s.m - 1);
+    if (s.key_bits + s.place_bits <= 32) return s;
+    s.ranges = 0;
+  }
+  const int bits = BitsOf((unsigned long long)vocab);
   s.passes = (bits + kDigitBits - 1) / kDigitBits;
   s.bits = (bits + s.passes - 1) / s.passes;
-  s.m = (unsigned)(n * bag);
   s.tiles = (s.m + kSortTile - 1) / kSortTile;
+  s.groups = (s.tiles + kGroupTiles - 1) / kGroupTiles;
   s.counts_bytes = Align256((size_t)s.tiles * kDigits * sizeof(unsigned));
+  s.groups_bytes = (size_t)(s.groups + 1) * kDigits * sizeof(unsigned);
   s.pairs_bytes = s.passes > 1 ? Align256((size_t)s.m * sizeof(unsigned)) : 0;
-  s.bytes = s.counts_bytes + kDigits * sizeof(unsigned) + 2 * s.pairs_bytes;
+  s.bytes = s.counts_bytes + s.groups_bytes + 2 * s.pairs_bytes;
   return s;
 }
 
@@ -441,6 +640,13 @@ struct Gradient {
   unsigned fill_blocks, slots;  // workgroups that write the rows no token names, rows of each
   int lanes_log;
   unsigned pieces;
+
+  // Whether this workgroup writes zeros, and the how many-th of its kind it is.
+  __device__ __forceinline__ bool Fills(unsigned *block) const {
+    const bool fills = blockIdx.x < fill_blocks;
+    *block = fills ? blockIdx.x : blockIdx.x - fill_blocks;
+    return fills;
+  }
 
   template <int kVec>
   __device__ __forceinline__ void Write(unsigned v, int d, const float (&sum)[kVec]) const {
@@ -514,11 +720,11 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
 // Rows of more than kNarrow elements: 2^lanes_log lanes hold kVec columns each and walk a chunk pair by pair, kAhead rows in flight.
 template <typename T, typename O, int kVec>
 __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) {
-  if (blockIdx.x < g.fill_blocks) {
-    FillRows(g, blockIdx.x);
+  unsigned block;
+  if (g.Fills(&block)) {
+    FillRows(g, block);
     return;
   }
-  const unsigned block = blockIdx.x - g.fill_blocks;
   const unsigned piece = block % g.pieces;
   unsigned w = ((block / g.pieces) * kThreads + threadIdx.x) >> g.lanes_log;
   if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);  // (the wave's own: keys and rows are scalar loads then)
@@ -579,11 +785,12 @@ __device__ __forceinline__ float WaveSum(float v) {
 // the same the lanes add up what is theirs; when it changes they meet.
 template <typename T, typename O, int kDim>
 __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g) {
-  if (blockIdx.x < g.fill_blocks) {
-    FillRows(g, blockIdx.x);
+  unsigned block;
+  if (g.Fills(&block)) {
+    FillRows(g, block);
     return;
   }
-  const unsigned w = __builtin_amdgcn_readfirstlane(((blockIdx.x - g.fill_blocks) * kThreads + threadIdx.x) >> 6);
+  const unsigned w = __builtin_amdgcn_readfirstlane((block * kThreads + threadIdx.x) >> 6);
   if (w >= g.chunks) return;
   const unsigned lane = threadIdx.x & 63u;
   const unsigned begin = w * g.chunk, end = min(g.m, begin + g.chunk);
@@ -659,29 +866,46 @@ __device__ __forceinline__ bool GoesOn(const Gradient<T, O> &g, unsigned w, unsi
   *v = g.keys[end];
   if (*v >= g.vocab || g.keys[end - 1] != *v) return false;
   if (g.keys[begin] == *v && begin != 0 && g.keys[begin - 1] == *v) return false;
-  *last = (WaveLowerBound(g.keys + end, g.m - end, *v + 1u) + end - 1u) / g.chunk;
+  // the chunks after it that the run still begins: most often one or two, so 64 are asked at once
+  const unsigned x = w + 1u + (threadIdx.x & 63u);
+  const unsigned long long other = ~__ballot(x < g.chunks && g.keys[(size_t)x * g.chunk] == *v);
+  if (other != 0ull) *last = w + (unsigned)__builtin_ctzll(other);
+  else *last = (WaveLowerBound(g.keys + end, g.m - end, *v + 1u) + end - 1u) / g.chunk;
   return true;
 }
 
 // The parts of the runs that go on, wide rows: a lane per column, the waves of a workgroup share the parts.
 template <typename T, typename O>
 __global__ void __launch_bounds__(kThreads) k_grad_join_wide(const Gradient<T, O> g) {
-  __shared__ float s_sum[kThreads / 64][64];
+  constexpr unsigned kWaves = kThreads / 64;
+  constexpr int kVec = 4;
+  __shared__ float s_sum[kWaves][64][kVec];
   unsigned v, last;
   const unsigned w = blockIdx.x;
   if (!GoesOn(g, w, &v, &last)) return;
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  constexpr unsigned kWaves = kThreads / 64;
-  for (int d0 = (int)blockIdx.y * 64; d0 < g.dim; d0 += 64 * (int)gridDim.y) {
-    const int d = min(d0 + (int)lane, g.dim - 1);
-    float sum[1] = {wave == 0 ? g.parts[((size_t)w * 2 + 1) * g.dim + d] : 0.0f};
+  for (int d0 = (int)blockIdx.y * 64 * kVec; d0 < g.dim; d0 += 64 * kVec * (int)gridDim.y) {
+    const int d = d0 + (int)lane * kVec, held = g.dim - d;
+    float sum[kVec] = {};
+    auto add = [&](size_t row) {
+      Pack<float, kVec> x;
+      Load<float, kVec>(g.parts + row * g.dim + d, held, &x);
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) sum[c] += x.v[c];
+    };
+    if (held > 0) {
+      if (wave == 0) add((size_t)w * 2 + 1);
 #pragma unroll 8
-    for (unsigned x = w + 1u + wave; x <= last; x += kWaves) sum[0] += g.parts[(size_t)x * 2 * g.dim + d];
-    s_sum[wave][lane] = sum[0];
+      for (unsigned x = w + 1u + wave; x <= last; x += kWaves) add((size_t)x * 2);
+    }
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) s_sum[wave][lane][c] = sum[c];
     __syncthreads();
-    if (wave == 0 && d0 + (int)lane < g.dim) {
-      for (unsigned k = 1; k < kWaves; ++k) sum[0] += s_sum[k][lane];
-      g.template Write<1>(v, d, sum);
+    if (wave == 0 && held > 0) {
+      for (unsigned k = 1; k < kWaves; ++k)
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) sum[c] += s_sum[k][lane][c];
+      g.template Write<kVec>(v, d, sum);
     }
     __syncthreads();
   }
@@ -781,11 +1005,26 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
   if (a.work_bytes < plan.bytes) throw std::runtime_error("work memory too small");
   OnDeviceOf device(a.keys);
   hipStream_t st = static_cast<hipStream_t>(a.stream);
+  if (plan.ranges > 0) {
+    WithToken(a.bags.bits, [&](auto token) {
+      typedef decltype(token) Token;
+      const Pairs<Token> in = PairsOf<Token>(a.bags, plan.m);
+      auto launch = [&](auto rounds) {
+        hipLaunchKernelGGL((k_sort_ranges<decltype(rounds)::value, Token>), dim3(plan.ranges), dim3(kRangeThreads), 0, st, in, plan.span,
+                           plan.key_bits, plan.place_bits, a.keys, a.rows);
+      };
+      if (plan.m <= 1 * kRangeThreads) launch(std::integral_constant<int, 1>());
+      else if (plan.m <= 8 * kRangeThreads) launch(std::integral_constant<int, 8>());
+      else launch(std::integral_constant<int, 32>());
+    });
+    HIP_OK(hipGetLastError());
+    return;
+  }
   unsigned char *work = static_cast<unsigned char *>(a.work);
   unsigned *counts = reinterpret_cast<unsigned *>(work);
-  unsigned *totals = reinterpret_cast<unsigned *>(work + plan.counts_bytes);
+  unsigned *groups = reinterpret_cast<unsigned *>(work + plan.counts_bytes);
   unsigned *spare[2];
-  spare[0] = totals + kDigits;
+  spare[0] = groups + plan.groups_bytes / sizeof(unsigned);
   spare[1] = spare[0] + plan.pairs_bytes / sizeof(unsigned);
   unsigned *last[2] = {a.keys, a.rows};
   for (int pass = 0; pass < plan.passes; ++pass) {
@@ -794,19 +1033,19 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
     const Digit digit{pass * plan.bits, (1u << plan.bits) - 1u};
     auto launch = [&](const auto &in) {
       typedef std::decay_t<decltype(in)> Source;
-      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts, plan.tiles);
-      hipLaunchKernelGGL(k_sort_scan, dim3(kDigits), dim3(256), 0, st, counts, plan.tiles, totals);
-      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts, plan.tiles, totals, to[0],
-                         to[1]);
+      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts);
+      hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
+      const bool several = plan.groups > 1;  // (the totals of the only group are those of all)
+      if (several) hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
+      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts,
+                         several ? groups : (const unsigned *)nullptr, several ? groups + (size_t)plan.groups * kDigits : groups, to[0], to[1]);
     };
     if (pass > 0) {
       launch(FromPairs{from[0], from[1], plan.m});
     } else {
-      // pairs in the order the tokens lie in memory
-      const bool by_column = a.bags.token_stride < a.bags.bag_stride;
       WithToken(a.bags.bits, [&](auto token) {
         typedef decltype(token) Token;
-        launch(FromTokens<Token>{BagsOf<Token>(a.bags), plan.m, by_column});
+        launch(FromTokens<Token>{PairsOf<Token>(a.bags, plan.m), plan.m});
       });
     }
   }
@@ -868,7 +1107,7 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       if (blocks >= (1ull << 31)) throw std::runtime_error("too many tokens of this width");
       if (blocks > 0) hipLaunchKernelGGL((k_grad_wide<T, O, kVec>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g);
       if (g.chunks > 1)
-        hipLaunchKernelGGL((k_grad_join_wide<T, O>), dim3(g.chunks, std::min((a.dim + 63) / 64, 64)), dim3(kThreads), 0, st, g);
+        hipLaunchKernelGGL((k_grad_join_wide<T, O>), dim3(g.chunks, std::min((a.dim + 255) / 256, 16)), dim3(kThreads), 0, st, g);
     } else {
       const unsigned wave_blocks = (g.chunks + kThreads / 64 - 1) / (kThreads / 64), blocks = wave_blocks + g.fill_blocks;
       auto run = [&](auto width) {
