@@ -26,13 +26,20 @@ struct Bags {
   unsigned vocab;
   unsigned *status;
   __device__ __forceinline__ Token At(long long i, long long j) const { return tokens[i * token_stride + j * bag_stride]; }
-  // The row of the table that a token names; `vocab` for none.  (Called when all tokens of a step have been asked for: behind the
-  // store to *status no load is started early.)
+  // The row of the table that a token names; `vocab` for none (negative tokens are large ones without a sign).
   __device__ __forceinline__ unsigned Row(Token t) const {
     typedef std::make_unsigned_t<Token> Word;
-    if ((Word)t < (Word)vocab) return (unsigned)t;
-    if (t != -1 && status != nullptr) *status = 1u;
-    return vocab;
+    return (unsigned)min((Word)t, (Word)vocab);
+  }
+  __device__ __forceinline__ bool Wrong(Token t) const { return t != -1 && Row(t) == vocab; }
+  // (a branch that a call without a status word passes by)
+  template <int kTokens>
+  __device__ __forceinline__ void Report(const Token (&t)[kTokens]) const {
+    if (status == nullptr) return;
+    bool wrong = false;
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) wrong = wrong || Wrong(t[k]);
+    if (wrong) *status = 1u;
   }
 };
 
@@ -78,7 +85,8 @@ struct Rows {
 };
 
 // Bags of one token: rows are copied, scaled.  2^lanes_log lanes take a piece of kPieces vectors a lane of a row, so that all
-// its loads are in flight at once (blockIdx.y: which piece).
+// its loads are in flight at once (blockIdx.y: which piece).  Here and below the last vector of a row that is not whole
+// vectors wide is moved back to end with the row: two lanes then write the same values to the same place.
 constexpr int kPieces = 4;
 template <typename T, int kVec, typename Token>
 __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> bags, const Rows<T> r, int lanes_log) {
@@ -87,29 +95,25 @@ __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> ba
   const unsigned lane = threadIdx.x & ((1u << lanes_log) - 1u);
   const int step = kVec << lanes_log;
   const int first = (int)blockIdx.y * (step * kPieces) + (int)lane * kVec;
-  const unsigned t = bags.Row(bags.At(i, 0));
-  const T *from = r.table + (long long)t * r.table_stride;
+  const Token token[1] = {bags.At(i, 0)};
+  const unsigned t = bags.Row(token[0]);
+  if (blockIdx.y == 0 && lane == 0) bags.Report(token);
+  const T *from = r.table + (long long)min(t, bags.vocab - 1u) * r.table_stride;
   T *to = r.out + i * r.out_stride;
   Pack<T, kVec> x[kPieces];
 #pragma unroll
-  for (int k = 0; k < kPieces; ++k) {
-    const int d = first + k * step;
-    if (t < bags.vocab) Load<T, kVec>(from + d, r.dim - d, &x[k]);
-    else
-#pragma unroll
-      for (int c = 0; c < kVec; ++c) x[k].v[c] = T(0);
-  }
+  for (int k = 0; k < kPieces; ++k) x[k] = *reinterpret_cast<const Pack<T, kVec> *>(from + min(first + k * step, r.dim - kVec));
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
-    const int d = first + k * step;
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) x[k].v[c] = Round<T>(static_cast<float>(x[k].v[c]) * r.scale);
-    if (d < r.dim) Store<T, kVec>(to + d, r.dim - d, x[k]);
+    for (int c = 0; c < kVec; ++c) x[k].v[c] = t < bags.vocab ? Round<T>(static_cast<float>(x[k].v[c]) * r.scale) : T(0);
+    if (first + k * step < r.dim) *reinterpret_cast<Pack<T, kVec> *>(to + min(first + k * step, r.dim - kVec)) = x[k];
   }
 }
 
 // Bags of several tokens.  A row of the result is 2^lanes_log lanes wide (kVec elements a lane), and 2^shares_log shares of
-// them take every so many-th token each and meet in the end, by steps of halves.  kAhead tokens of a lane are in flight.
+// them take every so many-th token each and meet in the end, by steps of halves.  kAhead tokens of a lane are in flight; where
+// there is no token the last row of the table is read and not added.
 constexpr int kAhead = 8;
 template <typename T, int kVec, typename Token>
 __global__ void __launch_bounds__(kThreads)
@@ -118,42 +122,46 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
   const bool live = i < bags.n;
   const unsigned lane = threadIdx.x & ((1u << lanes_log) - 1u);
   const int share = (int)((threadIdx.x >> lanes_log) & ((1u << shares_log) - 1u)), shares = 1 << shares_log;
-  const int d = ((int)blockIdx.y << lanes_log) * kVec + (int)lane * kVec;
+  const int column = ((int)blockIdx.y << lanes_log) * kVec + (int)lane * kVec, d = min(column, r.dim - kVec);
   float sum[kVec];
 #pragma unroll
   for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
-  if (live && d < r.dim) {
+  if (live && column < r.dim) {
     const Token *at = bags.tokens + i * bags.token_stride + share * bags.bag_stride;
+    const T *table = r.table + d;
     const long long step = (long long)shares * bags.bag_stride;
-    for (int j = share; j < bags.bag; j += kAhead * shares) {
-      Token token[kAhead];
-      unsigned t[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bags.bag ? at[k * step] : Token(-1);
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) t[k] = bags.Row(token[k]);
-      at += kAhead * step;
+    auto add = [&](const Token (&token)[kAhead]) {
       Pack<T, kVec> x[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) x[k].v[c] = T(0);
-        if (t[k] < bags.vocab) Load<T, kVec>(r.table + (long long)t[k] * r.table_stride + d, r.dim - d, &x[k]);
-      }
+      for (int k = 0; k < kAhead; ++k)
+        x[k] = *reinterpret_cast<const Pack<T, kVec> *>(table + (long long)min(bags.Row(token[k]), bags.vocab - 1u) * r.table_stride);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) sum[c] += static_cast<float>(x[k].v[c]);
+        for (int c = 0; c < kVec; ++c) sum[c] += bags.Row(token[k]) < bags.vocab ? static_cast<float>(x[k].v[c]) : 0.0f;
+      if (blockIdx.y == 0 && lane == 0) bags.Report(token);
+    };
+    Token token[kAhead];
+    int j = share;
+    for (; j + (kAhead - 1) * shares < bags.bag; j += kAhead * shares, at += kAhead * step) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) token[k] = at[k * step];
+      add(token);
+    }
+    if (j < bags.bag) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bags.bag ? at[k * step] : Token(-1);
+      add(token);
     }
   }
   for (int s = shares_log - 1; s >= 0; --s)
 #pragma unroll
     for (int c = 0; c < kVec; ++c) sum[c] += __shfl_xor(sum[c], 1 << (lanes_log + s));
-  if (live && share == 0 && d < r.dim) {
+  if (live && share == 0 && column < r.dim) {
     Pack<T, kVec> y;
 #pragma unroll
     for (int c = 0; c < kVec; ++c) y.v[c] = Round<T>(sum[c] * r.scale);
-    Store<T, kVec>(r.out + i * r.out_stride + d, r.dim - d, y);
+    *reinterpret_cast<Pack<T, kVec> *>(r.out + i * r.out_stride + d) = y;
   }
 }
 
@@ -247,6 +255,8 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   __shared__ unsigned s_sum[2][kRangeWaves];
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned v0 = blockIdx.x * span;
+  if (v0 > in.bags.vocab) return;
+  const unsigned here = min(span, in.bags.vocab + 1u - v0);  // keys of the range (a key less v0 wraps to a large one below it)
   Token token[kRounds];
   unsigned key[kRounds];
 #pragma unroll
@@ -256,11 +266,11 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   }
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) key[k] = k * kRangeThreads + threadIdx.x < in.m ? in.bags.Row(token[k]) : ~0u;
+  if (blockIdx.x == 0) in.bags.Report(token);
   unsigned within = 0, below = 0;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const bool real = key[k] <= in.bags.vocab;
-    within += (unsigned)__popcll(__ballot(real && key[k] >= v0 && key[k] - v0 < span));
+    within += (unsigned)__popcll(__ballot(key[k] - v0 < here));
     below += (unsigned)__popcll(__ballot(key[k] < v0));
   }
   if (lane == 0) {
@@ -278,7 +288,7 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   if (held == 0) return;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const bool mine = key[k] <= in.bags.vocab && key[k] >= v0 && key[k] - v0 < span;
+    const bool mine = key[k] - v0 < here;
     const unsigned long long all = __ballot(mine);
     if (mine) s_pair[at + (unsigned)__popcll(all & ((1ull << lane) - 1ull))] = (key[k] - v0) << place_bits | (k * kRangeThreads + threadIdx.x);
     at += (unsigned)__popcll(all);
@@ -360,6 +370,10 @@ struct FromTokens {
   typedef Token Raw;
   __device__ __forceinline__ Token At(unsigned p) const { return pairs.At(p); }
   __device__ __forceinline__ unsigned Key(Token t) const { return pairs.bags.Row(t); }
+  template <int kTokens>
+  __device__ __forceinline__ void Report(const Token (&t)[kTokens]) const {
+    pairs.bags.Report(t);
+  }
   __device__ __forceinline__ unsigned Row(unsigned p) const { return pairs.Bag(p); }
 };
 struct FromPairs {
@@ -368,6 +382,8 @@ struct FromPairs {
   typedef unsigned Raw;
   __device__ __forceinline__ unsigned At(unsigned p) const { return keys[p]; }
   __device__ __forceinline__ unsigned Key(unsigned key) const { return key; }
+  template <int kKeys>
+  __device__ __forceinline__ void Report(const unsigned (&)[kKeys]) const {}
   __device__ __forceinline__ unsigned Row(unsigned p) const { return rows[p]; }
 };
 
@@ -390,6 +406,7 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, co
   unsigned d[kSortRounds];
 #pragma unroll
   for (int k = 0; k < kSortRounds; ++k) raw[k] = in.At(min(base + k, in.m - 1));
+  in.Report(raw);
 #pragma unroll
   for (int k = 0; k < kSortRounds; ++k) d[k] = base + k < in.m ? digit.Of(in.Key(raw[k])) : kDigits;
   bool same = true;
