@@ -665,9 +665,15 @@ struct Gradient {
     return fills;
   }
 
+  // kVec columns of row v from d on.  The first `skip` of them are another lane's, too: to be added only once.
   template <int kVec>
-  __device__ __forceinline__ void Write(unsigned v, int d, const float (&sum)[kVec]) const {
+  __device__ __forceinline__ void Write(unsigned v, int d, int skip, const float (&sum)[kVec]) const {
     O *at = grad_table + (long long)v * table_stride + d;
+    if (accumulate && skip > 0) {
+      for (int c = 0; c < kVec; ++c)
+        if (c >= skip) at[c] = Round<O>(static_cast<float>(at[c]) + sum[c] * scale);
+      return;
+    }
     Pack<O, kVec> y;
     if (accumulate) Load<O, kVec>(at, dim - d, &y);
 #pragma unroll
@@ -679,10 +685,10 @@ struct Gradient {
   }
   // The end of a run of key v in chunk w.
   template <int kVec>
-  __device__ __forceinline__ void Finish(unsigned v, unsigned w, int d, bool begins, bool ends, const float (&sum)[kVec]) const {
+  __device__ __forceinline__ void Finish(unsigned v, unsigned w, int d, int skip, bool begins, bool ends, const float (&sum)[kVec]) const {
     if (v >= vocab) return;
     if (begins && ends) {
-      Write<kVec>(v, d, sum);
+      Write<kVec>(v, d, skip, sum);
     } else {
       Pack<float, kVec> y;
 #pragma unroll
@@ -745,16 +751,16 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
   const unsigned piece = block % g.pieces;
   unsigned w = ((block / g.pieces) * kThreads + threadIdx.x) >> g.lanes_log;
   if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);  // (the wave's own: keys and rows are scalar loads then)
-  const int d = (int)(((piece << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
-  if (w >= g.chunks || d >= g.dim) return;
+  const int column = (int)(((piece << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
+  if (w >= g.chunks || column >= g.dim) return;
+  const int d = min(column, g.dim - kVec), skip = column - d;
   const unsigned begin = w * g.chunk, end = min(g.m, begin + g.chunk);
   unsigned cur = g.keys[begin];
   bool begins = begin == 0 || g.keys[begin - 1] != cur;
   float sum[kVec];
 #pragma unroll
   for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
-  const T *column = g.grad_out + d;
-  const int held = g.dim - d;
+  const T *from = g.grad_out + d;
   for (unsigned p = begin; p < end; p += kAhead) {
     Pack<unsigned, kAhead> key, row;
     if (p + kAhead <= end) {
@@ -767,30 +773,25 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
         row.v[k] = p + k < end ? g.rows[p + k] : g.n;
       }
     }
+    // every load is asked for: what a pair has no row for is the last one's, and not added
     Pack<T, kVec> x[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (row.v[k] < g.n && key.v[k] < g.vocab) {
-        Load<T, kVec>(column + (long long)row.v[k] * g.out_stride, held, &x[k]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) x[k].v[c] = T(0);
-      }
-    }
+    for (int k = 0; k < kAhead; ++k)
+      x[k] = *reinterpret_cast<const Pack<T, kVec> *>(from + (long long)min(row.v[k], g.n - 1u) * g.out_stride);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (key.v[k] != cur) {
-        g.template Finish<kVec>(cur, w, d, begins, true, sum);
+        g.template Finish<kVec>(cur, w, d, skip, begins, true, sum);
         cur = key.v[k];
         begins = true;
 #pragma unroll
         for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
       }
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) sum[c] += static_cast<float>(x[k].v[c]);
+      for (int c = 0; c < kVec; ++c) sum[c] += row.v[k] < g.n ? static_cast<float>(x[k].v[c]) : 0.0f;
     }
   }
-  g.template Finish<kVec>(cur, w, d, begins, end == g.m || g.keys[end] != cur, sum);
+  g.template Finish<kVec>(cur, w, d, skip, begins, end == g.m || g.keys[end] != cur, sum);
 }
 
 __device__ __forceinline__ float WaveSum(float v) {
@@ -818,40 +819,55 @@ __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g
   for (int c = 0; c < kDim; ++c) sum[c] = 0.0f;
   constexpr int kRounds = 4;
   for (unsigned p = begin; p < end; p += 64 * kRounds) {
-    unsigned key[kRounds];
-    Pack<T, kDim> x[kRounds];
+    unsigned key[kRounds], row[kRounds];
 #pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
+    for (int k = 0; k < kRounds; ++k) {  // past the end the last key stands, without a row
       const unsigned at = p + k * 64 + lane;
       key[k] = g.keys[min(at, end - 1)];
-      const unsigned row = g.rows[min(at, end - 1)];
-      if (at < end && row < g.n && key[k] < g.vocab) {
-        Load<T, kDim>(g.grad_out + (long long)row * g.out_stride, g.dim, &x[k]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < kDim; ++c) x[k].v[c] = T(0);
-      }
+      row[k] = g.rows[min(at, end - 1)];
+      if (at >= end) row[k] = g.n;
     }
+    float x[kRounds][kDim];
+    if (g.dim == kDim) {
+      Pack<T, kDim> held[kRounds];
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k)
+        held[k] = *reinterpret_cast<const Pack<T, kDim> *>(g.grad_out + (long long)min(row[k], g.n - 1u) * g.out_stride);
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+        for (int c = 0; c < kDim; ++c) x[k][c] = static_cast<float>(held[k].v[c]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+        for (int c = 0; c < kDim; ++c)
+          x[k][c] = static_cast<float>(g.grad_out[(long long)min(row[k], g.n - 1u) * g.out_stride + min(c, g.dim - 1)]);
+    }
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+      for (int c = 0; c < kDim; ++c) x[k][c] = row[k] < g.n ? x[k][c] : 0.0f;
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
       const bool same = key[k] == cur;
       if (__ballot(!same) == 0ull) {
 #pragma unroll
-        for (int c = 0; c < kDim; ++c) sum[c] += static_cast<float>(x[k].v[c]);
+        for (int c = 0; c < kDim; ++c) sum[c] += x[k][c];
         continue;
       }
       // the run that came in ends here
       float total[kDim];
 #pragma unroll
-      for (int c = 0; c < kDim; ++c) total[c] = WaveSum(sum[c] + (same ? static_cast<float>(x[k].v[c]) : 0.0f));
-      if (lane == 0) g.template Finish<kDim>(cur, w, 0, begins, true, total);
+      for (int c = 0; c < kDim; ++c) total[c] = WaveSum(sum[c] + (same ? x[k][c] : 0.0f));
+      if (lane == 0) g.template Finish<kDim>(cur, w, 0, 0, begins, true, total);
       // the last key goes on; those between are whole: sums over runs of equal keys, by steps of doubled length
       const unsigned last = __builtin_amdgcn_readlane(key[k], 63);
       const bool between = !same && key[k] != last;
       if (__ballot(between) != 0ull) {
         float run[kDim];
 #pragma unroll
-        for (int c = 0; c < kDim; ++c) run[c] = static_cast<float>(x[k].v[c]);
+        for (int c = 0; c < kDim; ++c) run[c] = x[k][c];
         for (int off = 1; off < 64; off <<= 1) {
           const bool joins = __shfl_up(key[k], off) == key[k] && lane >= (unsigned)off;
 #pragma unroll
@@ -861,10 +877,10 @@ __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g
           }
         }
         const unsigned after = __shfl_down(key[k], 1);
-        if (between && after != key[k]) g.template Finish<kDim>(key[k], w, 0, true, true, run);
+        if (between && after != key[k]) g.template Finish<kDim>(key[k], w, 0, 0, true, true, run);
       }
 #pragma unroll
-      for (int c = 0; c < kDim; ++c) sum[c] = key[k] == last ? static_cast<float>(x[k].v[c]) : 0.0f;
+      for (int c = 0; c < kDim; ++c) sum[c] = key[k] == last ? x[k][c] : 0.0f;
       cur = last;
       begins = true;
     }
@@ -872,7 +888,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g
   float total[kDim];
 #pragma unroll
   for (int c = 0; c < kDim; ++c) total[c] = WaveSum(sum[c]);
-  if (lane == 0) g.template Finish<kDim>(cur, w, 0, begins, end == g.m || g.keys[end] != cur, total);
+  if (lane == 0) g.template Finish<kDim>(cur, w, 0, 0, begins, end == g.m || g.keys[end] != cur, total);
 }
 
 // Chunk w: whether a run begins in it that goes on beyond its end, and the last chunk that run reaches.
@@ -922,7 +938,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_join_wide(const Gradient<T, O
       for (unsigned k = 1; k < kWaves; ++k)
 #pragma unroll
         for (int c = 0; c < kVec; ++c) sum[c] += s_sum[k][lane][c];
-      g.template Write<kVec>(v, d, sum);
+      g.template Write<kVec>(v, d, 0, sum);
     }
     __syncthreads();
   }
@@ -939,7 +955,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_join_narrow(const Gradient<T,
 #pragma unroll 4
     for (unsigned x = w + 1u + lane; x <= last; x += 64u) sum[0] += g.parts[(size_t)x * 2 * g.dim + d];
     sum[0] = WaveSum(sum[0]);
-    if (lane == 0) g.template Write<1>(v, d, sum);
+    if (lane == 0) g.template Write<1>(v, d, 0, sum);
   }
 }
 
