@@ -223,16 +223,17 @@ Pairs<Token> PairsOf(const TokenBags &b, unsigned m) {
   return Pairs<Token>{BagsOf<Token>(b), m, by_column, flat};
 }
 
-// Lanes of the wave that hold the same digit of kBits bits as this one.
-template <int kBits>
-__device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid) {
-  unsigned long long peers = __ballot(valid);
-#pragma unroll
-  for (int b = 0; b < kBits; ++b) {
-    const unsigned long long m = __ballot((d >> b) & 1u);
-    peers &= ((d >> b) & 1u) ? m : ~m;
+// Lanes of the wave that hold the same digit as this one.
+__device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid, int bits) {
+  const unsigned long long all = __ballot(valid);
+  unsigned low = (unsigned)all, high = (unsigned)(all >> 32);
+  for (int b = 0; b < bits; ++b) {
+    const int set = (int)(d << (31 - b)) >> 31;  // -1 or 0
+    const unsigned long long m = __ballot(set != 0);
+    low &= ~((unsigned)m ^ (unsigned)set);
+    high &= ~((unsigned)(m >> 32) ^ (unsigned)set);
   }
-  return peers;
+  return (unsigned long long)high << 32 | low;
 }
 
 // ---- few pairs: one launch
@@ -242,7 +243,7 @@ __device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid)
 
 constexpr int kRangeThreads = 1024;
 constexpr int kRangeWaves = kRangeThreads / 64;
-constexpr int kRangeBits = 6;  // of a digit
+constexpr int kRangeBits = 8;  // of a digit, at most
 constexpr unsigned kMostRangePairs = 32768;
 constexpr unsigned kMostRanges = 256;  // a workgroup per CU
 
@@ -251,7 +252,8 @@ template <int kRounds, typename Token>
 __global__ void __launch_bounds__(kRangeThreads)
 k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits, unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
   __shared__ unsigned s_pair[kRounds * kRangeThreads];
-  __shared__ unsigned s_count[kRangeWaves << kRangeBits];  // pairs of a digit, then their place; the waves of a digit beside each other
+  constexpr int kCounters = kRangeWaves << kRangeBits, kOwn = kCounters / kRangeThreads;
+  __shared__ __align__(16) unsigned s_count[kCounters];  // pairs of a digit, then their place; the waves of a digit beside each other
   __shared__ unsigned s_sum[2][kRangeWaves];
   const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned v0 = blockIdx.x * span;
@@ -299,7 +301,8 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   for (int pass = 0; pass < passes; ++pass) {
     const int bits = (key_bits + passes - 1) / passes, shift = place_bits + pass * bits;
     unsigned pair[kRounds], place[kRounds];
-    s_count[threadIdx.x] = 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) s_count[k * kRangeThreads + threadIdx.x] = 0;
     __syncthreads();  // (the pairs are in place, too)
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
@@ -308,7 +311,7 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
         const bool valid = i < held;
         pair[k] = valid ? s_pair[i] : 0u;
         const unsigned d = (pair[k] >> shift) & ((1u << bits) - 1u);
-        const unsigned long long peers = DigitPeers<kRangeBits>(d, valid);
+        const unsigned long long peers = DigitPeers(d, valid, bits);
         const unsigned less = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
         unsigned *count = &s_count[d * kRangeWaves + wave];
         const unsigned before = *count;
@@ -319,8 +322,13 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
       }
     }
     __syncthreads();
-    // exclusive sum over (digit, wave), a counter a thread
-    const unsigned mine = s_count[threadIdx.x];
+    // exclusive sum over (digit, wave), kOwn counters a thread
+    unsigned own[kOwn], mine = 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      own[k] = s_count[threadIdx.x * kOwn + k];
+      mine += own[k];
+    }
     unsigned sum = mine;
     for (int off = 1; off < 64; off <<= 1) {
       const unsigned o = __shfl_up(sum, off);
@@ -329,7 +337,12 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
     if (lane == 63) s_sum[0][wave] = sum;
     __syncthreads();
     for (unsigned w = 0; w < wave; ++w) sum += s_sum[0][w];
-    s_count[threadIdx.x] = sum - mine;
+    sum -= mine;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      s_count[threadIdx.x * kOwn + k] = sum;
+      sum += own[k];
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
@@ -388,7 +401,7 @@ struct FromPairs {
 };
 
 struct Digit {
-  int shift;
+  int shift, bits;
   unsigned mask;
   __device__ __forceinline__ unsigned Of(unsigned key) const { return (key >> shift) & mask; }
 };
@@ -396,31 +409,34 @@ struct Digit {
 // Digit counts of one tile: counts[tile * kDigits + digit].  A thread's pairs lie beside each other and equal neighbours are counted
 // as one, and a wave of one digit only as one: pairs that are nearly in order (leaves, tree by tree; the last pass) would
 // otherwise queue for one counter of the LDS.
+constexpr int kCountThreads = 512;
+constexpr int kCountRounds = kSortTile / kCountThreads;
+static_assert(kCountThreads == kDigits, "a thread per counter");
 template <typename Source>
-__global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
+__global__ void __launch_bounds__(kCountThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
   __shared__ unsigned s_count[kDigits];
-  if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
+  s_count[threadIdx.x] = 0;
   __syncthreads();
-  const unsigned base = blockIdx.x * kSortTile + threadIdx.x * kSortRounds;
-  typename Source::Raw raw[kSortRounds];
-  unsigned d[kSortRounds];
+  const unsigned base = blockIdx.x * kSortTile + threadIdx.x * kCountRounds;
+  typename Source::Raw raw[kCountRounds];
+  unsigned d[kCountRounds];
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) raw[k] = in.At(min(base + k, in.m - 1));
+  for (int k = 0; k < kCountRounds; ++k) raw[k] = in.At(min(base + k, in.m - 1));
   in.Report(raw);
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) d[k] = base + k < in.m ? digit.Of(in.Key(raw[k])) : kDigits;
+  for (int k = 0; k < kCountRounds; ++k) d[k] = base + k < in.m ? digit.Of(in.Key(raw[k])) : kDigits;
   bool same = true;
 #pragma unroll
-  for (int k = 1; k < kSortRounds; ++k) same = same && d[k] == d[0];
+  for (int k = 1; k < kCountRounds; ++k) same = same && d[k] == d[0];
   const unsigned one = __builtin_amdgcn_readfirstlane(d[0]);
   if (__ballot(!(same && d[0] == one)) == 0ull) {
-    if ((threadIdx.x & 63u) == 0 && one < kDigits) atomicAdd(&s_count[one], 64u * kSortRounds);
+    if ((threadIdx.x & 63u) == 0 && one < kDigits) atomicAdd(&s_count[one], 64u * kCountRounds);
   } else {
     unsigned run = 0;
 #pragma unroll
-    for (int k = 0; k < kSortRounds; ++k) {
+    for (int k = 0; k < kCountRounds; ++k) {
       ++run;
-      if (k + 1 == kSortRounds || d[k + 1 < kSortRounds ? k + 1 : k] != d[k]) {
+      if (k + 1 == kCountRounds || d[k + 1 < kCountRounds ? k + 1 : k] != d[k]) {
         if (d[k] < kDigits) atomicAdd(&s_count[d[k]], run);
         run = 0;
       }
@@ -502,7 +518,9 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   for (int k = 0; k < kSortRounds; ++k) {
     const bool valid = wave * kWavePairs + k * 64 + lane < held;
     const unsigned d = digit.Of(key[k]);
-    const unsigned long long peers = DigitPeers<kDigitBits>(d, valid);
+    // (the last pass finds most waves in order: one digit)
+    const bool other = valid && d != __builtin_amdgcn_readfirstlane(d);
+    const unsigned long long peers = __ballot(other) == 0ull ? __ballot(valid) : DigitPeers(d, valid, digit.bits);
     const unsigned less = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
     const unsigned held_of = s_wave[wave][d];
     place[k] = held_of + less;
@@ -599,7 +617,7 @@ SortPlan PlanSort(long long n, int bag, long long vocab) {
   s.m = (unsigned)(n * bag);
   if (s.m == 0) return s;
   if (s.m <= kMostRangePairs) {
-    // 256 keys a workgroup: two passes of four bits
+    // 256 keys a workgroup are one pass
     s.ranges = (unsigned)std::min<long long>(vocab / 256 + 1, kMostRanges);
     s.span = (unsigned)(vocab / s.ranges + 1);
     s.key_bits = BitsOf(s.span - 1);
@@ -658,10 +676,12 @@ struct Gradient {
   int lanes_log;
   unsigned pieces;
 
-  // Whether this workgroup writes zeros, and the how many-th of its kind it is.
+  // Whether this workgroup writes zeros, and the how many-th of its kind it is.  The others start first: they wait for rows
+  // that they gather, these only write (32,768 x 4096: 256 us, 272 the other way round, 445 in turns).
   __device__ __forceinline__ bool Fills(unsigned *block) const {
-    const bool fills = blockIdx.x < fill_blocks;
-    *block = fills ? blockIdx.x : blockIdx.x - fill_blocks;
+    const unsigned walk = gridDim.x - fill_blocks;
+    const bool fills = blockIdx.x >= walk;
+    *block = fills ? blockIdx.x - walk : blockIdx.x;
     return fills;
   }
 
@@ -726,17 +746,23 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
     if (low < end && g.keys[low] == v0 + threadIdx.x) atomicOr(&s_named[threadIdx.x / 32], 1u << (threadIdx.x % 32));
   }
   __syncthreads();
+  // a row in pieces of 16 aligned bytes, whole ones past the caches (345 -> 272 us where 0.8 GB are zeros), elements at its ends
   constexpr int kVec = 16 / sizeof(O);
-  const int lanes = min(64, (g.dim + kVec - 1) / kVec);  // lanes of a row
+  const int pieces = g.dim / kVec + 2, lanes = min(64, pieces);
   const int groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
   if (group >= groups) return;
-  Pack<O, kVec> zero;
-#pragma unroll
-  for (int c = 0; c < kVec; ++c) zero.v[c] = O(0);
   for (unsigned k = group; k < slots; k += groups) {
     if (s_named[k / 32] >> (k % 32) & 1u) continue;
     O *row = g.grad_table + (long long)(v0 + k) * g.table_stride;
-    for (int d = lane * kVec; d < g.dim; d += lanes * kVec) Store<O, kVec>(row + d, g.dim - d, zero);
+    const int before = (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(O));  // elements of the first piece in front of the row
+    for (int d = lane * kVec - before; d < g.dim; d += lanes * kVec) {
+      if (d >= 0 && d + kVec <= g.dim) {
+        typedef float Piece __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(Piece{0.0f, 0.0f, 0.0f, 0.0f}, reinterpret_cast<Piece *>(row + d));
+      } else {
+        for (int c = max(d, 0); c < min(d + kVec, g.dim); ++c) row[c] = O(0);
+      }
+    }
   }
 }
 
@@ -761,23 +787,30 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
 #pragma unroll
   for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
   const T *from = g.grad_out + d;
-  for (unsigned p = begin; p < end; p += kAhead) {
-    Pack<unsigned, kAhead> key, row;
+  Pack<unsigned, kAhead> key, row, next_key, next_row;
+  auto pairs = [&](unsigned p) {
     if (p + kAhead <= end) {
-      key = *reinterpret_cast<const Pack<unsigned, kAhead> *>(g.keys + p);
-      row = *reinterpret_cast<const Pack<unsigned, kAhead> *>(g.rows + p);
+      next_key = *reinterpret_cast<const Pack<unsigned, kAhead> *>(g.keys + p);
+      next_row = *reinterpret_cast<const Pack<unsigned, kAhead> *>(g.rows + p);
     } else {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {  // past the end the last key stands, without a row
-        key.v[k] = g.keys[min(p + k, end - 1)];
-        row.v[k] = p + k < end ? g.rows[p + k] : g.n;
+        const unsigned at = min(p + k, end - 1);
+        next_key.v[k] = g.keys[at];
+        next_row.v[k] = p + k < end ? g.rows[at] : g.n;
       }
     }
+  };
+  pairs(begin);
+  for (unsigned p = begin; p < end; p += kAhead) {
+    key = next_key;
+    row = next_row;
     // every load is asked for: what a pair has no row for is the last one's, and not added
     Pack<T, kVec> x[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       x[k] = *reinterpret_cast<const Pack<T, kVec> *>(from + (long long)min(row.v[k], g.n - 1u) * g.out_stride);
+    if (p + kAhead < end) pairs(p + kAhead);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (key.v[k] != cur) {
@@ -959,12 +992,14 @@ __global__ void __launch_bounds__(kThreads) k_grad_join_narrow(const Gradient<T,
   }
 }
 
-// Pairs of a chunk.  Wide: 32, so that 32,768 pairs by 4096 columns are work for every CU, and more where the pairs
-// alone fill the chip, since each chunk leaves two rows of parts.  Narrow: from 64 (a round of a wave) on, by the same rule.
+// Pairs of a chunk: few, so that there are waves for every CU, and more where there are enough (4096), since each chunk leaves
+// two rows of parts to be joined.  (5,003 x 771: 28 us with 16 pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
 unsigned ChunkOf(unsigned m, int dim) {
-  const unsigned least = dim > kNarrow ? 32 : 64, most = dim > kNarrow ? 256 : 1024;
-  unsigned c = least;
-  while (c < most && m / c > 16384) c *= 2;
+  const bool wide = dim > kNarrow;
+  const unsigned most = wide ? 256 : 1024;
+  const unsigned long long per_64 = wide ? (dim + 7) / 8 : 64;  // waves of 64 chunks
+  unsigned c = wide ? 16 : 64;
+  while (c < most && m / c * per_64 / 64 > (wide ? 4096 : 16384)) c *= 2;
   return c;
 }
 
@@ -1063,10 +1098,10 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
   for (int pass = 0; pass < plan.passes; ++pass) {
     // the last pass writes to the caller's arrays, the passes before it in turn
     unsigned **to = (plan.passes - 1 - pass) % 2 == 0 ? last : spare, **from = to == last ? spare : last;
-    const Digit digit{pass * plan.bits, (1u << plan.bits) - 1u};
+    const Digit digit{pass * plan.bits, plan.bits, (1u << plan.bits) - 1u};
     auto launch = [&](const auto &in) {
       typedef std::decay_t<decltype(in)> Source;
-      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts);
+      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kCountThreads), 0, st, in, digit, counts);
       hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
       const bool several = plan.groups > 1;  // (the totals of the only group are those of all)
       if (several) hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
