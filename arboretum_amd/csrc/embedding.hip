@@ -387,6 +387,16 @@ struct FromTokens {
   __device__ __forceinline__ void Report(const Token (&t)[kTokens]) const {
     pairs.bags.Report(t);
   }
+  // kSome pairs from p on; past the end the last one's
+  template <int kSome>
+  __device__ __forceinline__ void Several(unsigned p, Token *to) const {
+    if (pairs.flat && p + kSome <= m) {
+      *reinterpret_cast<Pack<Token, kSome> *>(to) = *reinterpret_cast<const Pack<Token, kSome> *>(pairs.bags.tokens + p);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) to[k] = pairs.At(min(p + k, m - 1));
+  }
   __device__ __forceinline__ unsigned Row(unsigned p) const { return pairs.Bag(p); }
 };
 struct FromPairs {
@@ -397,6 +407,15 @@ struct FromPairs {
   __device__ __forceinline__ unsigned Key(unsigned key) const { return key; }
   template <int kKeys>
   __device__ __forceinline__ void Report(const unsigned (&)[kKeys]) const {}
+  template <int kSome>
+  __device__ __forceinline__ void Several(unsigned p, unsigned *to) const {
+    if (p + kSome <= m) {
+      *reinterpret_cast<Pack<unsigned, kSome> *>(to) = *reinterpret_cast<const Pack<unsigned, kSome> *>(keys + p);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) to[k] = keys[min(p + k, m - 1)];
+  }
   __device__ __forceinline__ unsigned Row(unsigned p) const { return rows[p]; }
 };
 
@@ -409,41 +428,42 @@ struct Digit {
 // Digit counts of one tile: counts[tile * kDigits + digit].  A thread's pairs lie beside each other and equal neighbours are counted
 // as one, and a wave of one digit only as one: pairs that are nearly in order (leaves, tree by tree; the last pass) would
 // otherwise queue for one counter of the LDS.
-constexpr int kCountThreads = 512;
-constexpr int kCountRounds = kSortTile / kCountThreads;
-static_assert(kCountThreads == kDigits, "a thread per counter");
 template <typename Source>
-__global__ void __launch_bounds__(kCountThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
+__global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
+  constexpr int kBeside = 4, kRounds = kSortRounds / kBeside;
   __shared__ unsigned s_count[kDigits];
-  s_count[threadIdx.x] = 0;
+  const unsigned tile = blockIdx.x;
+  if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
   __syncthreads();
-  const unsigned base = blockIdx.x * kSortTile + threadIdx.x * kCountRounds;
-  typename Source::Raw raw[kCountRounds];
-  unsigned d[kCountRounds];
+  const unsigned base = tile * kSortTile + threadIdx.x * kBeside;
+  typename Source::Raw raw[kSortRounds];
 #pragma unroll
-  for (int k = 0; k < kCountRounds; ++k) raw[k] = in.At(min(base + k, in.m - 1));
+  for (int r = 0; r < kRounds; ++r) in.template Several<kBeside>(base + r * kSortThreads * kBeside, raw + r * kBeside);
   in.Report(raw);
 #pragma unroll
-  for (int k = 0; k < kCountRounds; ++k) d[k] = base + k < in.m ? digit.Of(in.Key(raw[k])) : kDigits;
-  bool same = true;
+  for (int r = 0; r < kRounds; ++r) {
+    const unsigned p = base + r * kSortThreads * kBeside;
+    unsigned d[kBeside + 1];
 #pragma unroll
-  for (int k = 1; k < kCountRounds; ++k) same = same && d[k] == d[0];
-  const unsigned one = __builtin_amdgcn_readfirstlane(d[0]);
-  if (__ballot(!(same && d[0] == one)) == 0ull) {
-    if ((threadIdx.x & 63u) == 0 && one < kDigits) atomicAdd(&s_count[one], 64u * kCountRounds);
-  } else {
+    for (int k = 0; k < kBeside; ++k) d[k] = p + k < in.m ? digit.Of(in.Key(raw[r * kBeside + k])) : kDigits;
+    d[kBeside] = kDigits + 1;
+    const unsigned one = __builtin_amdgcn_readfirstlane(d[0]);
+    if (__ballot(d[0] != one || d[1] != one || d[2] != one || d[3] != one) == 0ull) {
+      if ((threadIdx.x & 63u) == 0 && one < kDigits) atomicAdd(&s_count[one], 64u * kBeside);
+      continue;
+    }
     unsigned run = 0;
 #pragma unroll
-    for (int k = 0; k < kCountRounds; ++k) {
+    for (int k = 0; k < kBeside; ++k) {
       ++run;
-      if (k + 1 == kCountRounds || d[k + 1 < kCountRounds ? k + 1 : k] != d[k]) {
+      if (d[k + 1] != d[k]) {
         if (d[k] < kDigits) atomicAdd(&s_count[d[k]], run);
         run = 0;
       }
     }
   }
   __syncthreads();
-  if (threadIdx.x <= digit.mask) counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = s_count[threadIdx.x];
+  if (threadIdx.x <= digit.mask) counts[(size_t)tile * kDigits + threadIdx.x] = s_count[threadIdx.x];
 }
 
 // Exclusive sums over the tiles of a group, in place, and the group's totals.  A thread per digit.
@@ -499,7 +519,8 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   __shared__ unsigned s_out[kDigits];                     // output position of that pair
   __shared__ unsigned s_sum[2][kDigits / 64];
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const unsigned base = blockIdx.x * kSortTile, held = min((unsigned)kSortTile, in.m - base);
+  const unsigned tile = blockIdx.x;
+  const unsigned base = tile * kSortTile, held = min((unsigned)kSortTile, in.m - base);
   for (int i = threadIdx.x; i < kSortWaves * kDigits / 2; i += kSortThreads) reinterpret_cast<unsigned *>(s_wave)[i] = 0;
   typename Source::Raw raw[kSortRounds];
   unsigned key[kSortRounds], place[kSortRounds];
@@ -510,8 +531,8 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   unsigned total = 0, before = 0;
   if (threadIdx.x <= digit.mask) {
     total = totals[threadIdx.x];
-    before = counts[(size_t)blockIdx.x * kDigits + threadIdx.x];
-    if (groups != nullptr) before += groups[(size_t)(blockIdx.x / kGroupTiles) * kDigits + threadIdx.x];
+    before = counts[(size_t)tile * kDigits + threadIdx.x];
+    if (groups != nullptr) before += groups[(size_t)(tile / kGroupTiles) * kDigits + threadIdx.x];
   }
   __syncthreads();
 #pragma unroll
@@ -856,8 +877,8 @@ __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {  // past the end the last key stands, without a row
       const unsigned at = p + k * 64 + lane;
-      key[k] = g.keys[min(at, end - 1)];
-      row[k] = g.rows[min(at, end - 1)];
+      key[k] = __builtin_nontemporal_load(g.keys + min(at, end - 1));
+      row[k] = __builtin_nontemporal_load(g.rows + min(at, end - 1));
       if (at >= end) row[k] = g.n;
     }
     float x[kRounds][kDim];
@@ -1101,7 +1122,7 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
     const Digit digit{pass * plan.bits, plan.bits, (1u << plan.bits) - 1u};
     auto launch = [&](const auto &in) {
       typedef std::decay_t<decltype(in)> Source;
-      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kCountThreads), 0, st, in, digit, counts);
+      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts);
       hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
       const bool several = plan.groups > 1;  // (the totals of the only group are those of all)
       if (several) hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
