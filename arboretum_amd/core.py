@@ -82,6 +82,8 @@ def _load_lib():
         "AEmbeddingGradBytes": [c_long, c_int, c_int, P(ctypes.c_ulonglong)],
         "AEmbeddingGrad": [c_void_p] * 4 + [c_long, c_int, c_long, c_int, c_long, c_long, c_int, c_int, c_float, c_int,
                                             c_void_p, ctypes.c_ulonglong, c_void_p],
+        "AGardenLeafTokens": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p, c_int],
+        "AGardenRefineLeaves": [c_void_p, c_void_p, c_int] + [ctypes.c_double] * 5,
         "AAdamW": [c_int] + [c_void_p] * 5 + [c_int, c_int] + [ctypes.c_double] * 6 + [c_long] + [c_void_p] * 3,
     }
     for name, args in sigs.items():
@@ -395,6 +397,25 @@ class Garden(object):
         """Tree walks of predict() on the GPU (default) or on the host; the results are bit-identical."""
         self._ensure()
         _check(_LIB.AGardenPredictOnDevice(self.handle, int(on)))
+
+    def leaf_tokens(self, data, tokens, stride=None, n_rounds=-1):
+        """The leaf of every row of `data` in each tree, as tokens for embedding() (AGardenLeafTokens): 32-bit words
+        [trees][stride] at the DEVICE address `tokens` (stride: data.rows unless given), the trees of a class together,
+        leaves numbered through them.  Returns the leaves of each class: the rows of its table.  Waits."""
+        self._ensure()
+        leaves = np.zeros(int(self.config.get('tree', {}).get('labels_count', 1)), dtype=np.int64)
+        _check(_LIB.AGardenLeafTokens(self.handle, data.handle, tokens, int(data.rows if stride is None else stride),
+                                      int(n_rounds), leaves.ctypes.data, leaves.size))
+        return leaves.tolist()
+
+    def refine_leaves(self, data=None, steps=100, lr=0.01, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
+        """Trains the leaf weights of all trees together, the splits as they are, by AdamW on the objective's mean over
+        `data` (the training matrix unless given; AGardenRefineLeaves).  The booster grows no tree afterwards."""
+        self._ensure()
+        data = self.data if data is None else data
+        if data is None:
+            raise ArboretumError(ValueError("no data matrix to refine on"))
+        _check(_LIB.AGardenRefineLeaves(self.handle, data.handle, int(steps), lr, beta1, beta2, eps, weight_decay))
 
     def set_inspect(self, on=True):
         self._ensure()

@@ -1,5 +1,6 @@
 #include "booster.h"
 
+#include "memory_pool.h"
 #include "parallel.h"
 
 #include <algorithm>
@@ -180,14 +181,19 @@ void Garden::FromInternal(const float *in, size_t count, float *out) const {
   }
 }
 
-void Garden::GrowTree(DataMatrix *data, const float *grad) {
-  if (cfg.method != kHist && cfg.method != kExact) throw std::runtime_error("unknown method");
-  if (grad != nullptr) throw std::runtime_error("user-supplied gradients are not supported");
+void Garden::CheckTarget(const DataMatrix *data) const {
   if (cfg.objective >= kSoftMaxOneVsAll) {
     if (data->labels.size() != data->rows) throw std::runtime_error("labels are not set");
   } else if (data->y.size() != data->rows) {
     throw std::runtime_error("y is not set");
   }
+}
+
+void Garden::GrowTree(DataMatrix *data, const float *grad) {
+  if (cfg.method != kHist && cfg.method != kExact) throw std::runtime_error("unknown method");
+  if (grad != nullptr) throw std::runtime_error("user-supplied gradients are not supported");
+  if (refined_) throw std::runtime_error("the leaves of this booster have been refined: it grows no more trees");
+  CheckTarget(data);
   // colsample checks of InitGrowingTree, garden.cu:126-140
   const size_t columns = data->columns_dense + data->columns_category;
   if ((int)(cfg.tree.colsample_bytree * columns) == 0)
@@ -244,6 +250,68 @@ void Garden::Predict(const DataMatrix *data, float *out, int n_rounds) const {
     }
   });
   FromInternal(tmp.data(), tmp.size(), out);
+}
+
+size_t Garden::CheckLeafWalk(const DataMatrix *data, int n_trees) const {
+  if (DeviceCount() <= 0) throw std::runtime_error("no HIP device available");
+  SyncTrees();
+  const size_t use = n_trees < 0 ? trees_.size() : std::min((size_t)n_trees, trees_.size());
+  if (use == 0) throw std::runtime_error("the booster has no trees");
+  if (data->rows == 0 || data->columns_dense == 0) throw std::runtime_error("empty data matrix");
+  if (data->rows >= ((size_t)1 << 31)) throw std::runtime_error("too many rows");
+  if (!DeviceWalkFits(*data, trees_, 0, use)) throw std::runtime_error("the trees or the rows are too large for the walk on the device");
+  return use;
+}
+
+void Garden::LeafTokens(const DataMatrix *data, int *tokens, size_t token_ld, int n_trees, long long *leaves_of) const {
+  if (!tokens || token_ld < data->rows) throw std::runtime_error("bad token array or stride");
+  const size_t use = CheckLeafWalk(data, n_trees), K = cfg.tree.labels_count;
+  if (leaves_of) {
+    std::fill(leaves_of, leaves_of + K, 0);
+    for (size_t t = 0; t < use; ++t)
+      if (trees_[t].label < K) leaves_of[trees_[t].label] += (long long)trees_[t].weights.size();
+  }
+  std::lock_guard<std::mutex> lock(predictor_mutex_);
+  if (!predictor_) predictor_.reset(CreateDevicePredictor());
+  LeavesOnDevice(predictor_.get(), *data, trees_, use, K, tokens, token_ld);
+}
+
+void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
+  if (options.steps < 0) throw std::runtime_error("bad number of steps");
+  if (cfg.objective < kSoftMaxOneVsAll && cfg.tree.labels_count > 1) throw std::runtime_error("several classes need a soft-max objective");
+  CheckTarget(data);
+  if (cfg.objective < kSoftMaxOneVsAll && !data->y_facts.finite) throw std::runtime_error("y must be finite");
+  const size_t use = CheckLeafWalk(data, -1), K = cfg.tree.labels_count, n = data->rows;
+  std::vector<size_t> trees_of(K, 0);
+  std::vector<std::vector<float>> tables(K);
+  for (size_t k = 0; k < K; ++k)
+    for (const RegTree &t : trees_) {
+      if (t.label != k) continue;
+      ++trees_of[k];
+      tables[k].insert(tables[k].end(), t.weights.begin(), t.weights.end());
+    }
+  for (size_t k = 0; k < K; ++k)
+    if (trees_of[k] * n >= ((size_t)1 << 31)) throw std::runtime_error("too many rows and trees: their product must be below 2^31");
+  const size_t token_ld = (n + 63) / 64 * 64;
+  struct Tokens {
+    int *p;
+    ~Tokens() { DevicePoolGive(p); }  // (nothing is pending: both calls below wait)
+  } tokens{static_cast<int *>(DevicePoolTake(use * token_ld * sizeof(int)))};
+  LeafTokens(data, tokens.p, token_ld, -1, nullptr);
+  RefineOnDevice(cfg, data, tokens.p, token_ld, trees_of, &tables, IntoInternal(cfg.tree.initial_y), options);
+  refined_ = true;
+  for (size_t k = 0; k < K; ++k) {
+    const float *from = tables[k].data();
+    for (RegTree &t : trees_) {
+      if (t.label != k) continue;
+      std::copy(from, from + t.weights.size(), t.weights.begin());
+      from += t.weights.size();
+    }
+  }
+  // (the predictors keep models laid out)
+  std::lock_guard<std::mutex> lock(predictor_mutex_);
+  predictor_.reset();
+  round_predictor_.reset();
 }
 
 // Floats of pinned memory AppendLastTree takes for its sums (128 MB).

@@ -191,9 +191,24 @@ void FreeDevicePredictor(DevicePredictor *p);
 const float *PredictOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees,
                              size_t begin, size_t end, size_t labels, float init, size_t row_begin = 0,
                              size_t row_end = SIZE_MAX);
+// The leaf every row of `data` reaches in each of trees[0, end): tokens[tree * token_ld + row], device memory, the trees in order
+// of labels (stable), leaves numbered through the trees of a label.  Waits for the result.
+void LeavesOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees, size_t end, size_t labels,
+                    int *tokens, size_t token_ld);
 // False for what only the host walks: 2 GB of trees and more, and rows on the host of which not even one fits a
 // staging block (a million features).
 bool DeviceWalkFits(const DataMatrix &data, const std::vector<RegTree> &trees, size_t begin, size_t end);
+
+// How Garden::RefineLeaves trains (AdamW).
+struct RefineOptions {
+  int steps;
+  double lr, beta1, beta2, eps, weight_decay;
+};
+
+// refine.hip: trains tables[label] (the leaf weights of that label's trees, one after the other), each over its rows of
+// `tokens` (LeavesOnDevice), against the objective of `cfg` and the target of `data`, starting from `init`.
+void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *tokens, size_t token_ld,
+                    const std::vector<size_t> &trees_of, std::vector<std::vector<float>> *tables, float init, const RefineOptions &options);
 
 class Garden {
  public:
@@ -206,6 +221,11 @@ class Garden {
   void Predict(const DataMatrix *data, float *out, int n_rounds) const;  // :643-657
   void UpdateByLastTree(DataMatrix *data);                   // :627-635
   void GetY(DataMatrix *data, float *out) const;             // :637-641; out: rows * labels_count floats
+  // Leaves of the rows of `data` in the first n_trees trees (all: negative), into device memory as LeavesOnDevice lays them;
+  // leaves_of[label]: leaves of that label's trees.  No counterpart in the reference, nor for the next.
+  void LeafTokens(const DataMatrix *data, int *tokens, size_t token_ld, int n_trees, long long *leaves_of) const;
+  // Trains the leaf weights of all trees together, the splits as they are.  The booster grows no tree afterwards.
+  void RefineLeaves(DataMatrix *data, const RefineOptions &options);
   const char *GetModel();                                    // :659-665
   void Restore(const char *json_model);                      // :667-677
 
@@ -241,6 +261,10 @@ class Garden {
   bool inspect_ = false;
   int timing_ = 0;
   bool predict_on_device_ = true;
+  bool refined_ = false;
+  // What LeafTokens and RefineLeaves ask of a matrix; the number of trees of the first n_trees (negative: all).
+  size_t CheckLeafWalk(const DataMatrix *data, int n_trees) const;
+  void CheckTarget(const DataMatrix *data) const;
   bool WalksOnDevice(const DataMatrix *data) const;
   mutable std::mutex predictor_mutex_;  // the predictors' results are read under it
   mutable std::unique_ptr<DevicePredictor, void (*)(DevicePredictor *)> round_predictor_{nullptr, FreeDevicePredictor};

@@ -41,7 +41,8 @@ constexpr size_t kMostModelBytes = (size_t)1 << 31;  // (trees are addressed by 
 // A tree as 8-byte words: its 2^(depth-1) - 1 nodes (feature, threshold bits) in heap order, then its
 // 2^(depth-1) leaf weights, two to a word.
 struct TreeRef {
-  unsigned off, depth, label, unused;
+  unsigned off, depth, label;
+  unsigned first;  // leaves of the trees of its label before it
 };
 
 size_t TreeWords(const RegTree &t) { return t.fid.size() + t.weights.size() / 2; }
@@ -108,7 +109,8 @@ typedef unsigned Node __attribute__((ext_vector_type(2)));
 // the trees start, LDS addresses or bytes from `words`.  The children of the node at byte p of its tree are at
 // 2 p + 8 and 2 p + 16, so there at 2 at - w + 8 (16): four vector instructions a level
 // beside the two reads (counting in nodes takes nine, and the walk is as much bound by them as by the LDS).
-template <bool IN_LDS, int N, typename F>
+// LEAVES: the numbers of the leaves (as bits) instead of their weights.
+template <bool IN_LDS, bool LEAVES, int N, typename F>
 __device__ __forceinline__ void WalkTrees(const unsigned char *words, const unsigned (&w)[N], unsigned depth,
                                           const F &fetch, float *leaf) {
   unsigned at[N], left[N], right[N];
@@ -133,6 +135,10 @@ __device__ __forceinline__ void WalkTrees(const unsigned char *words, const unsi
   const unsigned nodes = (1u << (depth - 1)) - 1u;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
+    if (LEAVES) {
+      leaf[k] = __uint_as_float(((at[k] - w[k]) >> 3) - nodes);
+      continue;
+    }
     const unsigned l = w[k] + 4u * nodes + ((at[k] - w[k]) >> 1);
     leaf[k] = IN_LDS ? LdsAt<float>(l) : *reinterpret_cast<const float *>(words + l);
   }
@@ -151,7 +157,8 @@ __device__ __forceinline__ void WalkTrees(const unsigned char *words, const unsi
 // 1,000,003 rows x 28 features, 200 trees of depth 8: 575 us (2370 with the values read from memory and
 // a tree at a time), of which the LDS is busy 210 and the vector units 270; 64 rows by 100 trees of
 // depth 6: 13 us (86).
-template <int SRC, bool TILE, bool TREES_IN_LDS>
+// LEAVES: no sums, but the leaf of every row and tree, as 32-bit words a.out[tree][row] numbered through the trees of a label.
+template <int SRC, bool TILE, bool TREES_IN_LDS, bool LEAVES>
 __global__ void __launch_bounds__(kWalkThreads) k_predict(const Walk a) {
   typedef typename Values<SRC>::T T;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(kWalkThreads) k_predict(const Walk a) {
       for (unsigned i = kAhead * kWalkThreads + threadIdx.x; b + i < e; i += kWalkThreads) s_words[i] = a.words[b + i];
       __syncthreads();
       if (t1 < a.n_trees) fetch_ahead(t1);
-    } else if (S > 1) {
+    } else if (S > 1 && !LEAVES) {
       __syncthreads();  // the leaf weights of the chunk before have been added
     }
     const unsigned char *words = reinterpret_cast<const unsigned char *>(a.words);
@@ -255,20 +262,24 @@ __global__ void __launch_bounds__(kWalkThreads) k_predict(const Walk a) {
         unsigned w[kChains];
 #pragma unroll
         for (unsigned k = 0; k < kChains; ++k) w[k] = tree(t + k * S);
-        WalkTrees<TREES_IN_LDS>(words, w, d, value, leaf);
+        WalkTrees<TREES_IN_LDS, LEAVES>(words, w, d, value, leaf);
       } else {
         const unsigned w[1] = {tree(t)};
-        WalkTrees<TREES_IN_LDS>(words, w, d, value, leaf);
+        WalkTrees<TREES_IN_LDS, LEAVES>(words, w, d, value, leaf);
       }
 #pragma unroll
       for (unsigned k = 0; k < kChains; ++k) {
         if (k > 0 && !four) break;
+        if (LEAVES) {
+          if (live) reinterpret_cast<unsigned *>(a.out)[(size_t)(t + k * S) * a.out_ld + row] = a.refs[t + k * S].first + __float_as_uint(leaf[k]);
+          continue;
+        }
         if (S == 1) add(t + k, leaf[k]);
         else s_leaf[(t + k * S - t0) * R + r] = leaf[k];
       }
       t += four ? kChains * S : S;
     }
-    if (S > 1) {
+    if (S > 1 && !LEAVES) {
       __syncthreads();
       if (slice == 0) {
         unsigned t = t0;
@@ -283,19 +294,19 @@ __global__ void __launch_bounds__(kWalkThreads) k_predict(const Walk a) {
       }
     }
   }
-  if (slice == 0 && live)
+  if (!LEAVES && slice == 0 && live)
     for (; cur < a.labels; ++cur, acc = a.init) a.out[(size_t)cur * a.out_ld + row] = acc;
 }
 
-template <int SRC, bool TILE, bool TREES_IN_LDS>
+template <int SRC, bool TILE, bool TREES_IN_LDS, bool LEAVES>
 void Launch(const Walk &a, size_t lds, hipStream_t stream) {
   static std::once_flag configured;
   std::call_once(configured, [] {
-    HIP_OK(hipFuncSetAttribute((const void *)k_predict<SRC, TILE, TREES_IN_LDS>,
+    HIP_OK(hipFuncSetAttribute((const void *)k_predict<SRC, TILE, TREES_IN_LDS, LEAVES>,
                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)kWalkLds));
   });
   const unsigned R = 1u << a.rows_log;
-  hipLaunchKernelGGL((k_predict<SRC, TILE, TREES_IN_LDS>), dim3((a.n + R - 1) / R), dim3(kWalkThreads), lds, stream, a);
+  hipLaunchKernelGGL((k_predict<SRC, TILE, TREES_IN_LDS, LEAVES>), dim3((a.n + R - 1) / R), dim3(kWalkThreads), lds, stream, a);
   HIP_OK(hipGetLastError());
 }
 
@@ -332,13 +343,15 @@ struct DevicePredictor {
         if (trees[t].label == k) order.push_back((unsigned)t);
     if (order.size() != e - b) throw std::runtime_error("tree label out of range");
     std::vector<TreeRef> refs;
-    size_t words = 0;
+    size_t words = 0, leaves = 0;
     largest = tree_words = 0;
     depth = trees[b].depth;
     bool same = true;
     for (unsigned t : order) {
       const size_t w = TreeWords(trees[t]);
-      refs.push_back(TreeRef{(unsigned)words, trees[t].depth, trees[t].label, 0u});
+      if (refs.empty() || refs.back().label != trees[t].label) leaves = 0;
+      refs.push_back(TreeRef{(unsigned)words, trees[t].depth, trees[t].label, (unsigned)leaves});
+      leaves += trees[t].weights.size();
       words += w;
       if (words * sizeof(uint2) >= kMostModelBytes) throw std::runtime_error("model too large for device prediction");
       largest = std::max(largest, (unsigned)w);
@@ -394,8 +407,8 @@ struct DevicePredictor {
     labels_of = labels;
   }
 
-  // rows [0, n) at `base` into out[label * out_ld + row]
-  void Rows(int src, const void *base, size_t ld, size_t n, size_t F, size_t labels, float init, float *out,
+  // rows [0, n) at `base` into out[label * out_ld + row]; their leaves into out[tree * out_ld + row]
+  void Rows(int src, const void *base, size_t ld, size_t n, size_t F, size_t labels, float init, bool leaves_only, float *out,
             size_t out_ld) {
     Walk a;
     a.base = base;
@@ -434,21 +447,26 @@ struct DevicePredictor {
     a.per_chunk = (unsigned)per;
     a.leaf_at = a.words_at + (unsigned)(trees_in_lds ? per * tree_bytes : 0);
     const size_t lds = a.leaf_at + per * leaf_bytes;
-#define ARB_WALK(S)                                                    \
-  do {                                                                 \
-    if (tile && trees_in_lds) Launch<S, true, true>(a, lds, stream);   \
-    else if (tile) Launch<S, true, false>(a, lds, stream);             \
-    else if (trees_in_lds) Launch<S, false, true>(a, lds, stream);     \
-    else Launch<S, false, false>(a, lds, stream);                      \
+#define ARB_WALK(S, L)                                                    \
+  do {                                                                    \
+    if (tile && trees_in_lds) Launch<S, true, true, L>(a, lds, stream);   \
+    else if (tile) Launch<S, true, false, L>(a, lds, stream);             \
+    else if (trees_in_lds) Launch<S, false, true, L>(a, lds, stream);     \
+    else Launch<S, false, false, L>(a, lds, stream);                      \
   } while (0)
-    if (src == kFloatRows) ARB_WALK(kFloatRows);
-    else if (src == kByteRows) ARB_WALK(kByteRows);
-    else ARB_WALK(kQuadCols);
+    if (leaves_only) {
+      if (src == kFloatRows) ARB_WALK(kFloatRows, true);
+      else if (src == kByteRows) ARB_WALK(kByteRows, true);
+      else ARB_WALK(kQuadCols, true);
+    } else if (src == kFloatRows) ARB_WALK(kFloatRows, false);
+    else if (src == kByteRows) ARB_WALK(kByteRows, false);
+    else ARB_WALK(kQuadCols, false);
 #undef ARB_WALK
   }
 
+  // The sums; with `tokens` (device memory, [trees][token_ld]) the leaves instead, and no sums.
   const float *Run(const DataMatrix &data, const std::vector<RegTree> &trees, size_t first, size_t use, size_t labels,
-                   float init, size_t row_begin, size_t row_end) {
+                   float init, size_t row_begin, size_t row_end, int *tokens = nullptr, size_t token_ld = 0) {
     const size_t n = std::min(row_end, data.rows) - row_begin, F = data.columns_dense;
     if (n == 0 || F == 0) throw std::runtime_error("empty data matrix");
     // only the block-wise walk of a streamed matrix indexes rows with 64 bits
@@ -459,13 +477,15 @@ struct DevicePredictor {
     LayOut(trees, first, use, F, labels);
     // Kernels write the sums where the host reads them: stores of 256 bytes a wave, at the rate of a copy
     // and beside the walk.
-    if (labels * n > result_floats) {
+    if (!tokens && labels * n > result_floats) {
       PinnedPoolGive(result);
       result = nullptr;
       result_floats = 0;
       result = static_cast<float *>(PinnedPoolTake(labels * n * sizeof(float)));
       result_floats = labels * n;
     }
+    float *const out = tokens ? reinterpret_cast<float *>(tokens) : result;
+    const size_t out_ld = tokens ? token_ld : n;
     // rows on the host: piece by piece through pinned memory into one device block (the stream keeps
     // a piece's copy behind the walk of the one before)
     auto through_block = [&](int src, const void *rows, size_t row_bytes) {
@@ -489,12 +509,12 @@ struct DevicePredictor {
                     [&](size_t k) {
                       if (k % group != group - 1 && k != pieces - 1) return;
                       const size_t r0 = k / group * group * piece;
-                      Rows(src, block.p, 0, std::min(group * piece, n - r0), F, labels, init, result + r0, n);
+                      Rows(src, block.p, 0, std::min(group * piece, n - r0), F, labels, init, tokens != nullptr, out + r0, out_ld);
                     }, stream);
       HIP_OK(hipStreamSynchronize(stream));
     };
     if (!data.is_prebinned) {
-      if (const float *rows = data.values->OnDevice()) Rows(kFloatRows, rows + row_begin * F, 0, n, F, labels, init, result, n);
+      if (const float *rows = data.values->OnDevice()) Rows(kFloatRows, rows + row_begin * F, 0, n, F, labels, init, tokens != nullptr, out, out_ld);
       else through_block(kFloatRows, data.values->OnHost() + row_begin * F, F * sizeof(float));
     } else if (!blocks) {
       through_block(kByteRows, data.prebinned.data() + row_begin * F, F);
@@ -507,7 +527,7 @@ struct DevicePredictor {
         for (size_t b = 0; b * br < n; ++b) {
           const size_t r0 = b * br;
           HIP_OK(hipMemcpyAsync(block, data.stream_blocks[row_begin / br + b], Q * br * sizeof(uint32_t), hipMemcpyHostToDevice, stream));
-          Rows(kQuadCols, block, br, std::min(br, n - r0), F, labels, init, result + r0, n);
+          Rows(kQuadCols, block, br, std::min(br, n - r0), F, labels, init, tokens != nullptr, out + r0, out_ld);
         }
         HIP_OK(hipStreamSynchronize(stream));
       } catch (...) {
@@ -527,6 +547,11 @@ void FreeDevicePredictor(DevicePredictor *p) { delete p; }
 const float *PredictOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees,
                              size_t begin, size_t end, size_t labels, float init, size_t row_begin, size_t row_end) {
   return p->Run(data, trees, begin, end, labels, init, row_begin, row_end);
+}
+
+void LeavesOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees, size_t end, size_t labels,
+                    int *tokens, size_t token_ld) {
+  p->Run(data, trees, 0, end, labels, 0.0f, 0, SIZE_MAX, tokens, token_ld);
 }
 
 bool DeviceWalkFits(const DataMatrix &data, const std::vector<RegTree> &trees, size_t begin, size_t end) {

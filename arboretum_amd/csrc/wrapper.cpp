@@ -424,6 +424,23 @@ const char *AHistSumNoAlloc(long long *sum_g, long long *sum_h, unsigned *bin_co
   });
 }
 
+const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens, long long stride, int n_rounds,
+                              long long *leaves, int classes) {
+  return Guard([&] {
+    const Garden &g = AsGarden(garden)->garden;
+    if (stride < 0) throw std::runtime_error("bad token array or stride");
+    if (leaves && classes != (int)g.cfg.tree.labels_count) throw std::runtime_error("the booster has " + std::to_string(g.cfg.tree.labels_count) + " classes");
+    g.LeafTokens(AsData(data), tokens, (size_t)stride, n_rounds, leaves);
+  });
+}
+
+const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
+                                double eps, double weight_decay) {
+  return Guard([&] {
+    AsGarden(garden)->garden.RefineLeaves(AsData(data), RefineOptions{steps, lr, beta1, beta2, eps, weight_decay});
+  });
+}
+
 const char *AEmbedding(void *out, const void *table, const void *tokens, long long n, int bag, long long vocab, int dim,
                        long long out_stride, long long table_stride, long long token_stride, long long bag_stride,
                        int type, int token_bits, float scale, unsigned *status, void *stream) {

@@ -210,8 +210,8 @@ const char *AHistSumNoAlloc(long long *sum_g, long long *sum_h, unsigned *bin_co
  * embedding of dimension 1 summed over the bag; the same operators serve embeddings of any dimension over
  * leaves, categories or the tokens of a text.  No counterpart in the reference.
  *
- * EVERY POINTER IS A DEVICE POINTER, but for the arrays of AAdamW and the `bytes` results.  All but the two calls that
- * return bytes enqueue on `stream` (a hipStream_t, NULL = default stream) of the device that their output is on, and return WITHOUT waiting.  They
+ * EVERY POINTER IS A DEVICE POINTER, but for the arrays of AAdamW and what is said to be the host's.  AEmbedding, AEmbeddingSort,
+ * AEmbeddingGrad and AAdamW enqueue on `stream` (a hipStream_t, NULL = default stream) of the device that their output is on, and return WITHOUT waiting.  They
  * allocate nothing, wait for nothing and may be captured into a graph.  Inputs and outputs must not overlap.
  * Element types: 0 float32, 1 bfloat16, 2 float16; sums are formed in float32 and rounded once, to nearest.  Strides
  * count elements and are not negative; rows may begin at any element.
@@ -243,6 +243,21 @@ const char *AEmbeddingGrad(void *grad_table, const void *grad_out, const unsigne
                            long long n, int bag, long long vocab, int dim, long long table_stride, long long out_stride,
                            int type, int table_type, float scale, int accumulate, void *work,
                            unsigned long long work_bytes, void *stream);
+
+/* The leaf every row of `data` reaches in each of the first n_rounds trees (-1: all): tokens[t * stride + row], DEVICE memory for
+ * 32-bit words of which nothing pending may make use, stride >= rows.  The trees of a class stand together (by class, then in the order they grew), and the
+ * leaves are numbered through the trees of a class: a class' columns are bags of tokens over a table of leaves[class] rows (a host array of
+ * `classes` counts, the booster's labels_count; may be NULL), token_stride 1 and bag_stride `stride`.  Waits for the result. */
+const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens, long long stride, int n_rounds,
+                              long long *leaves, int classes);
+
+/* Trains the leaf weights of all trees of the booster together, the splits as they are, against its objective on `data` (any matrix
+ * with a target): `steps` AdamW steps on the mean over all rows of half the
+ * squared error, or of the cross-entropy.  Works in 20 bytes of device memory per row and tree
+ * and waits for the result; rows times trees of a class are below 2^31.  The booster grows no tree afterwards (AGrowTree returns an
+ * error); predictions that matrices carry (AAppendLastTree) and the training predictions stay as they were. */
+const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
+                                double eps, double weight_decay);
 
 /* One AdamW step over `count` tensors at once, in float32 whatever the types of params (type) and grads (grad_type):
  *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;

@@ -183,6 +183,33 @@ def test_without_a_gpu_the_operators_say_so(arb):
             call(arb)
 
 
+def test_leaf_tokens_and_refinement_refuse_before_any_walk(arb):
+    data = arb.DMatrix(np.zeros((5, 3), np.float32), y=np.zeros(5))
+    booster = arb.Garden({"objective": 0, "method": 1, "tree": {"max_depth": 3}}, data)
+    says = "no trees" if arb.device_count() > 0 else "no HIP device"
+    with pytest.raises(arb.ArboretumError, match=says):
+        booster.leaf_tokens(data, A)
+    with pytest.raises(arb.ArboretumError, match=says):
+        booster.refine_leaves(data)
+    with pytest.raises(arb.ArboretumError, match="token array or stride"):
+        booster.leaf_tokens(data, A, stride=4)
+    with pytest.raises(arb.ArboretumError, match="token array or stride"):
+        booster.leaf_tokens(data, A, stride=-1)
+    with pytest.raises(arb.ArboretumError, match="token array or stride"):
+        booster.leaf_tokens(data, None)
+    with pytest.raises(arb.ArboretumError, match="bad number of steps"):
+        booster.refine_leaves(data, steps=-1)
+    with pytest.raises(arb.ArboretumError, match="y is not set"):
+        booster.refine_leaves(arb.DMatrix(np.zeros((5, 3), np.float32)))
+    with pytest.raises(arb.ArboretumError, match="finite"):
+        booster.refine_leaves(arb.DMatrix(np.zeros((5, 3), np.float32), y=np.full(5, np.inf)))
+    with pytest.raises(arb.ArboretumError, match="no data matrix"):
+        arb.Garden({"objective": 0}).refine_leaves()
+    several = arb.Garden({"objective": 0, "tree": {"labels_count": 2}}, data)
+    with pytest.raises(arb.ArboretumError, match="soft-max"):
+        several.refine_leaves()
+
+
 def test_every_operator_is_documented(arb):
     header = open(re.sub(r"arboretum_amd/__init__\.py$", "include/arboretum_ext.h", arb.__file__)).read()
     for name, symbol in [("embedding", "AEmbedding"), ("embedding_sort", "AEmbeddingSort"),
