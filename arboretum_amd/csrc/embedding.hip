@@ -127,9 +127,8 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
 #pragma unroll
   for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
   if (live && column < r.dim) {
-    const Token *at = bags.tokens + i * bags.token_stride + share * bags.bag_stride;
+    const Token *at = bags.tokens + i * bags.token_stride;
     const T *table = r.table + d;
-    const long long step = (long long)shares * bags.bag_stride;
     auto add = [&](const Token (&token)[kAhead]) {
       Pack<T, kVec> x[kAhead];
 #pragma unroll
@@ -143,14 +142,14 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
     };
     Token token[kAhead];
     int j = share;
-    for (; j + (kAhead - 1) * shares < bags.bag; j += kAhead * shares, at += kAhead * step) {
+    for (; j + (kAhead - 1) * shares < bags.bag; j += kAhead * shares) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) token[k] = at[k * step];
+      for (int k = 0; k < kAhead; ++k) token[k] = at[(j + k * shares) * bags.bag_stride];
       add(token);
     }
     if (j < bags.bag) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bags.bag ? at[k * step] : Token(-1);
+      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bags.bag ? at[(j + k * shares) * bags.bag_stride] : Token(-1);
       add(token);
     }
   }
@@ -165,6 +164,61 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
   }
 }
 
+// Rows of one element over so many bags that their tokens, column by column (the leaves of trees), come from memory and not
+// from the last-level cache of 256 MB.  A thread takes four neighbouring bags, whose tokens are one load, and the tokens of the next
+// columns are in flight while these are looked up.  Reading the tokens alone takes 135 us for a million bags of 200; the rest
+// is the lookups, of which the L1 answers little more than a lane a cycle.  (1,000,003 x 200: 223 us, 276 with a bag a thread;
+// 700,000 x 100, which the cache holds: 71 and 64; with the pieces of the table that a column names copied to the LDS first 290
+// and more: finding the pieces takes longer than the LDS saves.)
+constexpr int kColumns = 4;
+constexpr int kBagsOfThread = 4;
+constexpr long long kManyTokens = 1ll << 27;
+constexpr int kColumnBags = kThreads * kBagsOfThread;
+
+template <typename T, typename Token>
+__global__ void __launch_bounds__(kThreads) k_embedding_columns(const Bags<Token> bags, const Rows<T> r) {
+  const long long first = (long long)blockIdx.x * kColumnBags + threadIdx.x * kBagsOfThread;
+  const int held = (int)max(0ll, min((long long)kBagsOfThread, bags.n - first));
+  Token next[kColumns][kBagsOfThread];
+  auto fetch = [&](int j) {
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      const Token *at = bags.tokens + min(j + c, bags.bag - 1) * bags.bag_stride + first;
+      if (held == kBagsOfThread) {
+        *reinterpret_cast<Pack<Token, kBagsOfThread> *>(next[c]) = *reinterpret_cast<const Pack<Token, kBagsOfThread> *>(at);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kBagsOfThread; ++k) next[c][k] = k < held ? at[k] : Token(-1);
+      }
+#pragma unroll
+      for (int k = 0; k < kBagsOfThread; ++k)
+        if (j + c >= bags.bag) next[c][k] = Token(-1);
+    }
+  };
+  float sum[kBagsOfThread] = {};
+  fetch(0);
+  for (int j = 0; j < bags.bag; j += kColumns) {
+    unsigned t[kColumns][kBagsOfThread];
+    float x[kColumns][kBagsOfThread];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      bags.Report(next[c]);
+#pragma unroll
+      for (int k = 0; k < kBagsOfThread; ++k) t[c][k] = bags.Row(next[c][k]);
+    }
+    if (j + kColumns < bags.bag) fetch(j + kColumns);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+      for (int k = 0; k < kBagsOfThread; ++k) x[c][k] = static_cast<float>(r.table[(long long)min(t[c][k], bags.vocab - 1u) * r.table_stride]);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+      for (int k = 0; k < kBagsOfThread; ++k) sum[k] += t[c][k] < bags.vocab ? x[c][k] : 0.0f;
+  }
+  for (int k = 0; k < held; ++k) r.out[(first + k) * r.out_stride] = Round<T>(sum[k] * r.scale);
+}
+
 int LogAtLeast(long long v) {
   int log = 0;
   while ((1ll << log) < v) ++log;
@@ -175,6 +229,14 @@ template <typename T, int kVec, typename Token>
 void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
   const Bags<Token> bags = BagsOf<Token>(a.bags);
   const Rows<T> r{static_cast<const T *>(a.table), a.table_stride, static_cast<T *>(a.out), a.out_stride, a.dim, a.scale};
+  if constexpr (kVec == 1) {
+    if (a.dim == 1 && a.bags.bag > 1 && a.bags.token_stride == 1 && a.bags.bag_stride > 1 && a.bags.n * a.bags.bag >= kManyTokens &&
+        a.bags.n >= kColumnBags * 256) {
+      hipLaunchKernelGGL((k_embedding_columns<T, Token>), dim3((unsigned)((a.bags.n + kColumnBags - 1) / kColumnBags)), dim3(kThreads), 0, st,
+                         bags, r);
+      return;
+    }
+  }
   const long long vectors = (a.dim + kVec - 1) / kVec;
   const int lanes_log = std::min(LogAtLeast(vectors), 6);
   long long per_row = (vectors + (1ll << lanes_log) - 1) >> lanes_log;  // pieces of a row
@@ -184,7 +246,7 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
   } else {
     // Where the tokens of a bag lie beside each other the lanes of a wave read along them; otherwise they read along the
     // bags, unless these do not fill the chip (4 waves a CU).
-    const int most = std::min(6 - lanes_log, LogAtLeast((a.bags.bag + 15) / 16));
+    const int most = std::min(6 - lanes_log, LogAtLeast((a.bags.bag + 31) / 32));
     if (a.bags.bag_stride <= a.bags.token_stride) shares_log = most;
     else
       while (shares_log < most && ((a.bags.n * per_row) << (lanes_log + shares_log)) < 65536) ++shares_log;
@@ -871,7 +933,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g
   float sum[kDim];
 #pragma unroll
   for (int c = 0; c < kDim; ++c) sum[c] = 0.0f;
-  constexpr int kRounds = 4;
+  constexpr int kRounds = kDim == 1 ? 8 : 4;
   for (unsigned p = begin; p < end; p += 64 * kRounds) {
     unsigned key[kRounds], row[kRounds];
 #pragma unroll
@@ -949,67 +1011,81 @@ __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g
 template <typename T, typename O>
 __device__ __forceinline__ bool GoesOn(const Gradient<T, O> &g, unsigned w, unsigned *v, unsigned *last) {
   const unsigned begin = w * g.chunk, end = begin + g.chunk;
-  if (end >= g.m) return false;
-  *v = g.keys[end];
-  if (*v >= g.vocab || g.keys[end - 1] != *v) return false;
-  if (g.keys[begin] == *v && begin != 0 && g.keys[begin - 1] == *v) return false;
+  if (w >= g.chunks || end >= g.m) return false;
+  const unsigned next = g.keys[end], same = g.keys[end - 1], first = g.keys[begin], before = g.keys[max(begin, 1u) - 1u];
+  *v = next;
+  if (next >= g.vocab || same != next || (begin != 0 && first == next && before == next)) return false;
   // the chunks after it that the run still begins: most often one or two, so 64 are asked at once
   const unsigned x = w + 1u + (threadIdx.x & 63u);
-  const unsigned long long other = ~__ballot(x < g.chunks && g.keys[(size_t)x * g.chunk] == *v);
+  const unsigned long long other = ~__ballot(x < g.chunks && g.keys[(size_t)min(x, g.chunks - 1u) * g.chunk] == next);
   if (other != 0ull) *last = w + (unsigned)__builtin_ctzll(other);
-  else *last = (WaveLowerBound(g.keys + end, g.m - end, *v + 1u) + end - 1u) / g.chunk;
+  else *last = (WaveLowerBound(g.keys + end, g.m - end, next + 1u) + end - 1u) / g.chunk;
   return true;
 }
 
-// The parts of the runs that go on, wide rows: a lane per column, the waves of a workgroup share the parts.
+// The parts of the runs that go on, added up: every wave asks for a chunk of its own and sums the run that begins there, 2^lanes_log
+// lanes side by side over the columns (four each) and the others over the parts.  A run of many parts is left to all waves of the workgroup.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinVec = 4;
+constexpr unsigned kManyParts = 8;  // of a lane
 template <typename T, typename O>
-__global__ void __launch_bounds__(kThreads) k_grad_join_wide(const Gradient<T, O> g) {
-  constexpr unsigned kWaves = kThreads / 64;
-  constexpr int kVec = 4;
-  __shared__ float s_sum[kWaves][64][kVec];
-  unsigned v, last;
-  const unsigned w = blockIdx.x;
-  if (!GoesOn(g, w, &v, &last)) return;
-  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  for (int d0 = (int)blockIdx.y * 64 * kVec; d0 < g.dim; d0 += 64 * kVec * (int)gridDim.y) {
-    const int d = d0 + (int)lane * kVec, held = g.dim - d;
-    float sum[kVec] = {};
-    auto add = [&](size_t row) {
-      Pack<float, kVec> x;
-      Load<float, kVec>(g.parts + row * g.dim + d, held, &x);
+__global__ void __launch_bounds__(kJoinThreads) k_grad_join(const Gradient<T, O> g, int lanes_log) {
+  constexpr unsigned kWaves = kJoinThreads / 64;
+  __shared__ float s_sum[kWaves][64][kJoinVec];
+  __shared__ unsigned s_key[kWaves], s_last[kWaves];
+  const unsigned lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned share = lane >> lanes_log, shares = 64u >> lanes_log;  // of the parts, within the wave
+  const int column = (int)(lane & ((1u << lanes_log) - 1u)) * kJoinVec, step = kJoinVec << lanes_log;
+  float sum[kJoinVec];
+  // parts of the run from chunk w on, beginning with the `from`-th and taking every `by`-th: the first is what the run left in w itself
+  auto add = [&](unsigned w, unsigned last, int d, unsigned from, unsigned by) {
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) sum[c] += x.v[c];
-    };
-    if (held > 0) {
-      if (wave == 0) add((size_t)w * 2 + 1);
+    for (int c = 0; c < kJoinVec; ++c) sum[c] = 0.0f;
+    if (d >= g.dim) return;
 #pragma unroll 8
-      for (unsigned x = w + 1u + wave; x <= last; x += kWaves) add((size_t)x * 2);
-    }
+    for (unsigned x = w + from; x <= last; x += by) {
+      Pack<float, kJoinVec> y;
+      Load<float, kJoinVec>(g.parts + ((size_t)x * 2 + (x == w ? 1 : 0)) * g.dim + d, g.dim - d, &y);
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) s_sum[wave][lane][c] = sum[c];
-    __syncthreads();
-    if (wave == 0 && held > 0) {
-      for (unsigned k = 1; k < kWaves; ++k)
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) sum[c] += s_sum[k][lane][c];
-      g.template Write<kVec>(v, d, 0, sum);
+      for (int c = 0; c < kJoinVec; ++c) sum[c] += y.v[c];
     }
-    __syncthreads();
+  };
+  auto meet = [&] {
+    for (int off = 32; off >= 1 << lanes_log; off >>= 1)
+#pragma unroll
+      for (int c = 0; c < kJoinVec; ++c) sum[c] += __shfl_xor(sum[c], off);
+  };
+  const unsigned w0 = blockIdx.x * kWaves;
+  unsigned v = 0, last = 0;
+  const bool goes = GoesOn(g, w0 + wave, &v, &last), many = goes && last - (w0 + wave) > kManyParts * shares;
+  if (goes && !many) {
+    for (int d0 = (int)blockIdx.y * step; d0 < g.dim; d0 += (int)gridDim.y * step) {
+      add(w0 + wave, last, d0 + column, share, shares);
+      meet();
+      if (share == 0 && d0 + column < g.dim) g.template Write<kJoinVec>(v, d0 + column, 0, sum);
+    }
   }
-}
-
-// The same for narrow rows: a wave per run, its lanes share the parts.
-template <typename T, typename O>
-__global__ void __launch_bounds__(kThreads) k_grad_join_narrow(const Gradient<T, O> g) {
-  const unsigned w = __builtin_amdgcn_readfirstlane((blockIdx.x * kThreads + threadIdx.x) >> 6), lane = threadIdx.x & 63u;
-  unsigned v, last;
-  if (w >= g.chunks || !GoesOn(g, w, &v, &last)) return;
-  for (int d = 0; d < g.dim; ++d) {
-    float sum[1] = {lane == 0 ? g.parts[((size_t)w * 2 + 1) * g.dim + d] : 0.0f};
-#pragma unroll 4
-    for (unsigned x = w + 1u + lane; x <= last; x += 64u) sum[0] += g.parts[(size_t)x * 2 * g.dim + d];
-    sum[0] = WaveSum(sum[0]);
-    if (lane == 0) g.template Write<1>(v, d, 0, sum);
+  if (lane == 0) {
+    s_key[wave] = v;
+    s_last[wave] = many ? last : 0u;  // (a run that goes on ends behind chunk 0)
+  }
+  __syncthreads();
+  for (unsigned k = 0; k < kWaves; ++k) {
+    if (s_last[k] == 0u) continue;
+    for (int d0 = (int)blockIdx.y * step; d0 < g.dim; d0 += (int)gridDim.y * step) {
+      add(w0 + k, s_last[k], d0 + column, wave * shares + share, kWaves * shares);
+      meet();
+#pragma unroll
+      for (int c = 0; c < kJoinVec; ++c) s_sum[wave][lane][c] = sum[c];
+      __syncthreads();
+      if (wave == 0 && share == 0 && d0 + column < g.dim) {
+        for (unsigned x = 1; x < kWaves; ++x)
+#pragma unroll
+          for (int c = 0; c < kJoinVec; ++c) sum[c] += s_sum[x][lane][c];
+        g.template Write<kJoinVec>(s_key[k], d0 + column, 0, sum);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -1182,7 +1258,7 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
     g.chunk = ChunkOf(m, a.dim);
     g.chunks = (m + g.chunk - 1) / g.chunk;
     g.parts = static_cast<float *>(a.work);
-    g.slots = (unsigned)std::min<size_t>(std::max<size_t>(65536 / (a.dim * sizeof(O)), 1), kMostSlots);
+    g.slots = (unsigned)std::min<size_t>(std::max<size_t>(16384 / (a.dim * sizeof(O)), 1), kMostSlots);
     g.fill_blocks = a.accumulate ? 0 : (unsigned)((a.vocab + g.slots - 1) / g.slots);
     g.lanes_log = 6;
     g.pieces = 1;
@@ -1195,8 +1271,6 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
           ((((unsigned long long)g.chunks << g.lanes_log) + kThreads - 1) / kThreads) * g.pieces + g.fill_blocks;
       if (blocks >= (1ull << 31)) throw std::runtime_error("too many tokens of this width");
       if (blocks > 0) hipLaunchKernelGGL((k_grad_wide<T, O, kVec>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g);
-      if (g.chunks > 1)
-        hipLaunchKernelGGL((k_grad_join_wide<T, O>), dim3(g.chunks, std::min((a.dim + 255) / 256, 16)), dim3(kThreads), 0, st, g);
     } else {
       const unsigned wave_blocks = (g.chunks + kThreads / 64 - 1) / (kThreads / 64), blocks = wave_blocks + g.fill_blocks;
       auto run = [&](auto width) {
@@ -1208,7 +1282,12 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
         else if (a.dim <= 4) run(std::integral_constant<int, 4>());
         else run(std::integral_constant<int, 8>());
       }
-      if (g.chunks > 1) hipLaunchKernelGGL((k_grad_join_narrow<T, O>), dim3(wave_blocks), dim3(kThreads), 0, st, g);
+    }
+    if (g.chunks > 1) {
+      constexpr unsigned kWaves = kJoinThreads / 64;
+      const int lanes_log = std::min(LogAtLeast((a.dim + kJoinVec - 1) / kJoinVec), 6), pieces = (a.dim + 64 * kJoinVec - 1) / (64 * kJoinVec);
+      hipLaunchKernelGGL((k_grad_join<T, O>), dim3((g.chunks + kWaves - 1) / kWaves, std::min(pieces, 16)), dim3(kJoinThreads), 0, st, g,
+                         lanes_log);
     }
   };
   WithType(a.type, [&](auto t) {

@@ -533,3 +533,81 @@ def test_two_streams_at_once(arb):
     for model, w in zip(models, want):
         for a, b in zip(model.results(), w):
             assert torch.equal(a, b)
+
+
+MANY = 1 << 27  # tokens, column by column, from which on rows of one element are looked up four bags a thread
+
+
+@pytest.mark.parametrize("kind,bits,dtype", [("leaves", 32, "float32"), ("leaves", 64, "float16"), ("wide", 32, "bfloat16"),
+                                             ("padded", 32, "float32"), ("padded", 64, "float32")])
+def test_scalar_embeddings_of_many_columns(arb, kind, bits, dtype):
+    bag, T = 13, TYPES[dtype]
+    n = MANY // bag + 1027
+    vocab = 13 * 1500
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    piece = {"leaves": 256, "wide": 1500, "padded": 1024}[kind]
+    stride = n + 3
+    held = torch.full((bag, stride), 1 << 30, dtype=torch.int32 if bits == 32 else torch.int64, device="cuda")
+    for j in range(bag):
+        held[j, :n] = torch.randint(0, piece, (n,), generator=gen, device="cuda") + j * 1500
+        if kind == "padded":
+            held[j, :n][torch.rand(n, generator=gen, device="cuda") < 0.3] = -1
+    if kind == "padded":
+        held[4, :n] = -1
+        held[:, 5000:8000] = -1
+    table = torch.randn(vocab, 1, generator=gen, device="cuda").to(T)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full((n + 1, 2), 9.0, device="cuda", dtype=T)
+    arb.embedding(out.data_ptr(), table.data_ptr(), held.data_ptr(), n, vocab, 1, bag=bag, scale=0.75, dtype=dtype, token_bits=bits,
+                  token_stride=1, bag_stride=stride, out_stride=2, status=status.data_ptr())
+    want, mag = (torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2))
+    for j in range(bag):
+        t = held[j, :n].long()
+        x = torch.where(t >= 0, table.double()[t.clamp(min=0), 0], 0.0) * 0.75
+        want += x
+        mag += x.abs()
+    within(out[:n, 0], want.cpu(), (bag + 3) * U * mag.cpu(), T)
+    assert (out[:, 1] == 9).all() and (out[n] == 9).all() and status.item() == 0
+
+
+def test_scalar_embeddings_report_a_wrong_token_in_any_column(arb):
+    bag, vocab = 9, 2304
+    n = MANY // bag + 1
+    held = torch.arange(bag, dtype=torch.int32, device="cuda")[:, None].repeat(1, n) * 256
+    table = torch.ones(vocab, 1, device="cuda")
+    for column, row, token in [(0, 0, vocab), (8, n - 1, -2), (3, 77_777, 2 ** 31 - 1)]:
+        right = held[column, row].item()
+        held[column, row] = token
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.empty(n, device="cuda")
+        arb.embedding(out.data_ptr(), table.data_ptr(), held.data_ptr(), n, vocab, 1, bag=bag, token_stride=1, bag_stride=n,
+                      status=status.data_ptr())
+        held[column, row] = right
+        want = torch.full((n,), 9.0, device="cuda")
+        want[row] = 8.0
+        assert torch.equal(out, want) and status.item() == 1
+
+
+def test_gradients_of_many_pairs_the_tokens_out_of_order(arb):
+    # more pairs than one launch sorts: several tiles and groups of tiles, one, two and three digits
+    for n, bag, vocab, dim in [(300_000, 3, 400, 1), (33_000, 1, 100_000, 9), (150_000, 2, 300_000, 2), (300_000, 1, 70, 3)]:
+        gen = torch.Generator(device="cuda").manual_seed(vocab)
+        tokens = (torch.rand(n, bag, generator=gen, device="cuda") ** 2 * vocab).long()
+        tokens[torch.rand(n, bag, generator=gen, device="cuda") < 0.1] = -1
+        for strides, held in (((bag, 1), tokens.to(torch.int32)), ((1, n), tokens.t().to(torch.int32).contiguous()),
+                              ((bag + 1, 1), torch.cat([tokens, tokens[:, :1]], 1).to(torch.int32))):
+            s = Sorted(arb, held, n, bag, vocab, strides)
+            key = torch.where(tokens >= 0, tokens, vocab).reshape(-1)
+            assert torch.equal(s.keys.long(), key.sort().values)
+            pair = key * n + torch.arange(n, device="cuda").repeat_interleave(bag)
+            assert torch.equal((s.keys.long() * n + s.rows.long()).sort().values, pair.sort().values)
+            g = torch.randn(n, dim, generator=gen, device="cuda")
+            got = s.grad(g, torch.full((vocab, dim), float("nan"), device="cuda"))
+            rows = torch.arange(n, device="cuda").repeat_interleave(bag)
+            want = torch.zeros(vocab + 1, dim, dtype=torch.float64, device="cuda").index_add_(0, key, g.double()[rows])
+            mag = torch.zeros(vocab + 1, dim, dtype=torch.float64, device="cuda").index_add_(0, key, g.double().abs()[rows])
+            # sums are formed in parts (a lane's share of a chunk, chunks of a run): no part and no joining of parts takes more
+            # than 20,000 additions one after the other
+            terms = torch.bincount(key, minlength=vocab + 1)[:-1, None].clamp(max=20_000).cpu()
+            within(got, want[:-1].cpu(), (terms + 3) * U * mag[:-1].cpu(), torch.float32)
+            assert torch.equal(got, s.grad(g, torch.empty(vocab, dim, device="cuda")))
