@@ -260,6 +260,21 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
 
 // -------------------------------------------------------------------- sort
 
+// Division of numbers below 2^31 by a number that stays the same (Granlund and Montgomery, "Division by invariant integers
+// using multiplication"): with 2^(l-1) < d <= 2^l, factor = floor(2^(31+l) / d) + 1 makes p factor / 2^(31+l) exceed p / d by less than 1 / d.
+struct Divider {
+  unsigned by, factor;
+  int shift;
+  explicit Divider(unsigned d) : by(d), factor(0), shift(0) {
+    if (d < 2) return;  // (factor 0)
+    int l = 1;
+    while ((1ull << l) < d) ++l;
+    factor = (unsigned)((1ull << (31 + l)) / d + 1);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ unsigned Quotient(unsigned p) const { return factor == 0 ? p : __umulhi(p, factor) >> shift; }
+};
+
 // The pairs of a call, numbered in the order the tokens lie in memory.
 template <typename Token>
 struct Pairs {
@@ -267,13 +282,24 @@ struct Pairs {
   unsigned m;
   bool by_column;  // pair p is token p / n of bag p % n, else token p % bag of bag p / bag
   bool flat;       // ... and stands at tokens[p]
+  Divider line;    // n or bag
   __device__ __forceinline__ unsigned Bag(unsigned p) const {
-    return by_column ? p % (unsigned)bags.n : p / (unsigned)bags.bag;
+    const unsigned q = line.Quotient(p);
+    return by_column ? p - q * line.by : q;
   }
-  __device__ __forceinline__ Token At(unsigned p) const {
-    if (flat) return bags.tokens[p];
-    const unsigned i = Bag(p);
-    return bags.At(i, by_column ? p / (unsigned)bags.n : p - i * (unsigned)bags.bag);
+  // Tokens of the pairs first, first + step, ... ; past the last pair that one's.
+  template <int kTokens>
+  __device__ __forceinline__ void Get(unsigned first, unsigned step, Token (&to)[kTokens]) const {
+    if (flat) {
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) to[k] = bags.tokens[min(first + k * step, m - 1)];
+    } else {
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) {
+        const unsigned p = min(first + k * step, m - 1), q = line.Quotient(p), rest = p - q * line.by;
+        to[k] = bags.At(by_column ? rest : q, by_column ? q : rest);
+      }
+    }
   }
 };
 
@@ -282,7 +308,7 @@ Pairs<Token> PairsOf(const TokenBags &b, unsigned m) {
   const bool by_column = b.token_stride < b.bag_stride;
   const bool flat = by_column ? (b.token_stride == 1 || b.n == 1) && (b.bag_stride == b.n || b.bag == 1)
                               : (b.bag_stride == 1 || b.bag == 1) && (b.token_stride == b.bag || b.n == 1);
-  return Pairs<Token>{BagsOf<Token>(b), m, by_column, flat};
+  return Pairs<Token>{BagsOf<Token>(b), m, by_column, flat, Divider(by_column ? (unsigned)b.n : (unsigned)b.bag)};
 }
 
 // Lanes of the wave that hold the same digit as this one.
@@ -323,11 +349,7 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   const unsigned here = min(span, in.bags.vocab + 1u - v0);  // keys of the range (a key less v0 wraps to a large one below it)
   Token token[kRounds];
   unsigned key[kRounds];
-#pragma unroll
-  for (int k = 0; k < kRounds; ++k) {
-    const unsigned p = k * kRangeThreads + threadIdx.x;
-    token[k] = p < in.m ? in.At(p) : Token(-1);
-  }
+  in.Get(threadIdx.x, kRangeThreads, token);
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) key[k] = k * kRangeThreads + threadIdx.x < in.m ? in.bags.Row(token[k]) : ~0u;
   if (blockIdx.x == 0) in.bags.Report(token);
@@ -443,41 +465,40 @@ struct FromTokens {
   Pairs<Token> pairs;
   unsigned m;
   typedef Token Raw;
-  __device__ __forceinline__ Token At(unsigned p) const { return pairs.At(p); }
-  __device__ __forceinline__ unsigned Key(Token t) const { return pairs.bags.Row(t); }
-  template <int kTokens>
-  __device__ __forceinline__ void Report(const Token (&t)[kTokens]) const {
+  template <int kSome>
+  __device__ __forceinline__ void Get(unsigned first, unsigned step, Token (&to)[kSome]) const {
+    pairs.Get(first, step, to);
+  }
+  // kSome pairs side by side
+  template <int kSome>
+  __device__ __forceinline__ void Beside(unsigned p, Token (&to)[kSome]) const {
+    if (pairs.flat && p + kSome <= m) *reinterpret_cast<Pack<Token, kSome> *>(to) = *reinterpret_cast<const Pack<Token, kSome> *>(pairs.bags.tokens + p);
+    else pairs.Get(p, 1, to);
+  }
+  template <int kSome>
+  __device__ __forceinline__ void Report(const Token (&t)[kSome]) const {
     pairs.bags.Report(t);
   }
-  // kSome pairs from p on; past the end the last one's
-  template <int kSome>
-  __device__ __forceinline__ void Several(unsigned p, Token *to) const {
-    if (pairs.flat && p + kSome <= m) {
-      *reinterpret_cast<Pack<Token, kSome> *>(to) = *reinterpret_cast<const Pack<Token, kSome> *>(pairs.bags.tokens + p);
-      return;
-    }
-#pragma unroll
-    for (int k = 0; k < kSome; ++k) to[k] = pairs.At(min(p + k, m - 1));
-  }
+  __device__ __forceinline__ unsigned Key(Token t) const { return pairs.bags.Row(t); }
   __device__ __forceinline__ unsigned Row(unsigned p) const { return pairs.Bag(p); }
 };
 struct FromPairs {
   const unsigned *keys, *rows;
   unsigned m;
   typedef unsigned Raw;
-  __device__ __forceinline__ unsigned At(unsigned p) const { return keys[p]; }
-  __device__ __forceinline__ unsigned Key(unsigned key) const { return key; }
-  template <int kKeys>
-  __device__ __forceinline__ void Report(const unsigned (&)[kKeys]) const {}
   template <int kSome>
-  __device__ __forceinline__ void Several(unsigned p, unsigned *to) const {
-    if (p + kSome <= m) {
-      *reinterpret_cast<Pack<unsigned, kSome> *>(to) = *reinterpret_cast<const Pack<unsigned, kSome> *>(keys + p);
-      return;
-    }
+  __device__ __forceinline__ void Get(unsigned first, unsigned step, unsigned (&to)[kSome]) const {
 #pragma unroll
-    for (int k = 0; k < kSome; ++k) to[k] = keys[min(p + k, m - 1)];
+    for (int k = 0; k < kSome; ++k) to[k] = keys[min(first + k * step, m - 1)];
   }
+  template <int kSome>
+  __device__ __forceinline__ void Beside(unsigned p, unsigned (&to)[kSome]) const {
+    if (p + kSome <= m) *reinterpret_cast<Pack<unsigned, kSome> *>(to) = *reinterpret_cast<const Pack<unsigned, kSome> *>(keys + p);
+    else Get(p, 1, to);
+  }
+  template <int kSome>
+  __device__ __forceinline__ void Report(const unsigned (&)[kSome]) const {}
+  __device__ __forceinline__ unsigned Key(unsigned key) const { return key; }
   __device__ __forceinline__ unsigned Row(unsigned p) const { return rows[p]; }
 };
 
@@ -498,16 +519,17 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, co
   if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
   __syncthreads();
   const unsigned base = tile * kSortTile + threadIdx.x * kBeside;
-  typename Source::Raw raw[kSortRounds];
+  typename Source::Raw raw[kRounds][kBeside];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) in.template Several<kBeside>(base + r * kSortThreads * kBeside, raw + r * kBeside);
-  in.Report(raw);
+  for (int r = 0; r < kRounds; ++r) in.Beside(base + r * kSortThreads * kBeside, raw[r]);
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) in.Report(raw[r]);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const unsigned p = base + r * kSortThreads * kBeside;
     unsigned d[kBeside + 1];
 #pragma unroll
-    for (int k = 0; k < kBeside; ++k) d[k] = p + k < in.m ? digit.Of(in.Key(raw[r * kBeside + k])) : kDigits;
+    for (int k = 0; k < kBeside; ++k) d[k] = p + k < in.m ? digit.Of(in.Key(raw[r][k])) : kDigits;
     d[kBeside] = kDigits + 1;
     const unsigned one = __builtin_amdgcn_readfirstlane(d[0]);
     if (__ballot(d[0] != one || d[1] != one || d[2] != one || d[3] != one) == 0ull) {
@@ -572,7 +594,7 @@ __global__ void __launch_bounds__(1024) k_sort_sum_groups(unsigned *__restrict__
 // Stable scatter of one tile.  counts, groups: pairs of the same digit in the tiles of the group before, in the groups before;
 // totals: pairs of each digit.
 template <typename Source>
-__global__ void __launch_bounds__(kSortThreads)
+__global__ void __launch_bounds__(kSortThreads, 8)  // (8 waves a SIMD: two workgroups on a CU)
 k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ counts, const unsigned *__restrict__ groups,
                const unsigned *__restrict__ totals, unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
   __shared__ unsigned s_pair[kSortTile];                  // the keys, then the rows
@@ -586,8 +608,7 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   for (int i = threadIdx.x; i < kSortWaves * kDigits / 2; i += kSortThreads) reinterpret_cast<unsigned *>(s_wave)[i] = 0;
   typename Source::Raw raw[kSortRounds];
   unsigned key[kSortRounds], place[kSortRounds];
-#pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) raw[k] = in.At(base + min(wave * kWavePairs + k * 64 + lane, held - 1));
+  in.Get(base + wave * kWavePairs + lane, 64, raw);
 #pragma unroll
   for (int k = 0; k < kSortRounds; ++k) key[k] = in.Key(raw[k]);  // (past the end: the last one's, which goes nowhere)
   unsigned total = 0, before = 0;
