@@ -144,7 +144,7 @@ void Validate(const AdamWArgs &a) {
   if (a.count < 0) throw std::runtime_error("bad tensor count");
   if (a.count > 0 && (!a.params || !a.grads || !a.exp_avg || !a.exp_avg_sq || !a.sizes)) throw std::runtime_error("null pointer argument");
   for (int i = 0; i < a.count; ++i) {
-    if (a.sizes[i] < 0 || a.sizes[i] >= (1ll << 40)) throw std::runtime_error("bad tensor size");
+    if (a.sizes[i] < 0 || a.sizes[i] >= (1ll << 36)) throw std::runtime_error("bad tensor size");
     if (a.sizes[i] == 0) continue;
     if (!a.params[i] || !a.grads[i] || !a.exp_avg[i] || !a.exp_avg_sq[i]) throw std::runtime_error("null tensor");
     CheckAligned(a.params[i], ElementBytes(a.type), "a parameter");
@@ -199,7 +199,7 @@ void AdamW(const AdamWArgs &a) {
     for (; at < a.count && l.count < kTensorsAtOnce; ++at) {
       if (a.sizes[at] == 0) continue;
       const unsigned long long more = (unsigned long long)(a.sizes[at] + l.chunk - 1) / l.chunk;
-      if (blocks + more > (1ull << 30)) break;
+      if (l.count > 0 && blocks + more > (1ull << 23)) break;  // (a launch counts its threads with 32 bits)
       if (l.count == 0) first = a.params[at];
       l.tensor[l.count] = Tensor{a.params[at], a.grads[at], a.exp_avg[at], a.exp_avg_sq[at], a.sizes[at]};
       l.first[l.count++] = (unsigned)blocks;

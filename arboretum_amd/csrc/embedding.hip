@@ -121,7 +121,7 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
   const long long i = (long long)(((unsigned long long)blockIdx.x * kThreads + threadIdx.x) >> (lanes_log + shares_log));
   const bool live = i < bags.n;
   const unsigned lane = threadIdx.x & ((1u << lanes_log) - 1u);
-  const int share = (int)((threadIdx.x >> lanes_log) & ((1u << shares_log) - 1u)), shares = 1 << shares_log;
+  const unsigned share = (threadIdx.x >> lanes_log) & ((1u << shares_log) - 1u), shares = 1u << shares_log;
   const int column = ((int)blockIdx.y << lanes_log) * kVec + (int)lane * kVec, d = min(column, r.dim - kVec);
   float sum[kVec];
 #pragma unroll
@@ -140,16 +140,17 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
         for (int c = 0; c < kVec; ++c) sum[c] += bags.Row(token[k]) < bags.vocab ? static_cast<float>(x[k].v[c]) : 0.0f;
       if (blockIdx.y == 0 && lane == 0) bags.Report(token);
     };
+    const unsigned bag = (unsigned)bags.bag;
     Token token[kAhead];
-    int j = share;
-    for (; j + (kAhead - 1) * shares < bags.bag; j += kAhead * shares) {
+    unsigned j = share;
+    for (; j + (kAhead - 1) * shares < bag; j += kAhead * shares) {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) token[k] = at[(j + k * shares) * bags.bag_stride];
       add(token);
     }
-    if (j < bags.bag) {
+    if (j < bag) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bags.bag ? at[(j + k * shares) * bags.bag_stride] : Token(-1);
+      for (int k = 0; k < kAhead; ++k) token[k] = j + k * shares < bag ? at[(j + k * shares) * bags.bag_stride] : Token(-1);
       add(token);
     }
   }
@@ -252,10 +253,18 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
       while (shares_log < most && ((a.bags.n * per_row) << (lanes_log + shares_log)) < 65536) ++shares_log;
     group_log += shares_log;
   }
-  const long long blocks = ((a.bags.n << group_log) + kThreads - 1) / kThreads;
-  const dim3 grid((unsigned)blocks, (unsigned)per_row);
-  if (a.bags.bag == 1) hipLaunchKernelGGL((k_embedding_one<T, kVec, Token>), grid, dim3(kThreads), 0, st, bags, r, lanes_log);
-  else hipLaunchKernelGGL((k_embedding_bag<T, kVec, Token>), grid, dim3(kThreads), 0, st, bags, r, lanes_log, shares_log);
+  // (a launch counts its threads with 32 bits)
+  const long long most = (1ll << 31) >> group_log;
+  for (long long i = 0; i < a.bags.n; i += most) {
+    Bags<Token> some = bags;
+    some.n = std::min(most, a.bags.n - i);
+    if (some.tokens) some.tokens += i * some.token_stride;
+    Rows<T> to = r;
+    to.out += i * r.out_stride;
+    const dim3 grid((unsigned)(((some.n << group_log) + kThreads - 1) / kThreads), (unsigned)per_row);
+    if (a.bags.bag == 1) hipLaunchKernelGGL((k_embedding_one<T, kVec, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log);
+    else hipLaunchKernelGGL((k_embedding_bag<T, kVec, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log, shares_log);
+  }
 }
 
 // -------------------------------------------------------------------- sort
@@ -1111,19 +1120,19 @@ __global__ void __launch_bounds__(kJoinThreads) k_grad_join(const Gradient<T, O>
 }
 
 // Pairs of a chunk: few, so that there are waves for every CU, and more where there are enough (4096), since each chunk leaves
-// two rows of parts to be joined.  (5,003 x 771: 28 us with 16 pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
+// two rows of parts to be joined; never more than four million waves.  (5,003 x 771: 28 us with 16 pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
 unsigned ChunkOf(unsigned m, int dim) {
   const bool wide = dim > kNarrow;
   const unsigned most = wide ? 256 : 1024;
   const unsigned long long per_64 = wide ? (dim + 7) / 8 : 64;  // waves of 64 chunks
   unsigned c = wide ? 16 : 64;
-  while (c < most && m / c * per_64 / 64 > (wide ? 4096 : 16384)) c *= 2;
+  while ((c < most && m / c * per_64 / 64 > (wide ? 4096 : 16384)) || m / c * per_64 / 64 > (1 << 22)) c *= 2;
   return c;
 }
 
 // ------------------------------------------------------------------ checks
 
-constexpr int kMostDim = (1 << 24) - 1;  // (a grid's second dimension counts 65,535 pieces of a row of 256 elements at least)
+constexpr int kMostDim = 65535 * 256;  // (a grid's second dimension counts 65,535 pieces of a row of 256 elements at least)
 
 void CheckShape(long long n, int bag, long long vocab) {
   if (n < 0 || bag < 0) throw std::runtime_error("bad row count or bag size");
@@ -1280,6 +1289,8 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
     g.chunks = (m + g.chunk - 1) / g.chunk;
     g.parts = static_cast<float *>(a.work);
     g.slots = (unsigned)std::min<size_t>(std::max<size_t>(16384 / (a.dim * sizeof(O)), 1), kMostSlots);
+    while (g.slots < kMostSlots && a.vocab / g.slots > (1 << 22)) g.slots *= 2;  // (a launch counts its threads with 32 bits)
+    g.slots = std::min(g.slots, kMostSlots);
     g.fill_blocks = a.accumulate ? 0 : (unsigned)((a.vocab + g.slots - 1) / g.slots);
     g.lanes_log = 6;
     g.pieces = 1;
@@ -1290,7 +1301,6 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       g.pieces = (vectors + (1u << g.lanes_log) - 1) >> g.lanes_log;
       const unsigned long long blocks =
           ((((unsigned long long)g.chunks << g.lanes_log) + kThreads - 1) / kThreads) * g.pieces + g.fill_blocks;
-      if (blocks >= (1ull << 31)) throw std::runtime_error("too many tokens of this width");
       if (blocks > 0) hipLaunchKernelGGL((k_grad_wide<T, O, kVec>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g);
     } else {
       const unsigned wave_blocks = (g.chunks + kThreads / 64 - 1) / (kThreads / 64), blocks = wave_blocks + g.fill_blocks;

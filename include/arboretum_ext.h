@@ -217,7 +217,8 @@ const char *AHistSumNoAlloc(long long *sum_g, long long *sum_h, unsigned *bin_co
  * count elements and are not negative; rows may begin at any element.
  * Tokens: token j of bag i is tokens[i * token_stride + j * bag_stride], a signed integer of token_bits (32 or 64).  -1
  * stands for none.  Any other outside [0, vocab) is treated as none too, and sets *status (a device word, may be
- * NULL, never cleared here) to 1.  n * bag and vocab are below 2^31, dim below 2^24; both n and bag may be 0. */
+ * NULL, never cleared here) to 1.  n * bag and vocab are below 2^31, dim is at most 65,535 * 256; both n and bag may be 0.
+ * The first call of a kind in a process loads its kernels: a program that captures graphs makes one beforehand. */
 
 /* out[i] = scale * (sum over j of table[token(i, j)]), rows of `dim` elements; 0 for a bag without tokens. */
 const char *AEmbedding(void *out, const void *table, const void *tokens, long long n, int bag, long long vocab, int dim,
@@ -255,7 +256,8 @@ const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens,
  * with a target): `steps` AdamW steps on the mean over all rows of half the
  * squared error, or of the cross-entropy.  Works in 20 bytes of device memory per row and tree
  * and waits for the result; rows times trees of a class are below 2^31.  The booster grows no tree afterwards (AGrowTree returns an
- * error); predictions that matrices carry (AAppendLastTree) and the training predictions stay as they were. */
+ * error); predictions that matrices carry (AAppendLastTree) and the training predictions stay as they were.  No other thread may use
+ * the booster meanwhile. */
 const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
                                 double eps, double weight_decay);
 
@@ -263,7 +265,7 @@ const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps,
  *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * params, grads, exp_avg (m), exp_avg_sq (v), sizes: HOST arrays of `count` device pointers and element counts, read before
- * the call returns; tensors of one list must not overlap.  A size may be 0, its pointers are then not looked at.
+ * the call returns; tensors of one list must not overlap.  Sizes are below 2^36; one may be 0, its pointers are then not looked at.
  * All tensors are on one device.  step counts from 1.
  * lr_device, step_device: device words read instead of lr and step (for a captured graph that is replayed with
  * others); may be NULL.  (A step below 1 there counts as 1.) */

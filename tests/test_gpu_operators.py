@@ -611,3 +611,27 @@ def test_gradients_of_many_pairs_the_tokens_out_of_order(arb):
             terms = torch.bincount(key, minlength=vocab + 1)[:-1, None].clamp(max=20_000).cpu()
             within(got, want[:-1].cpu(), (terms + 3) * U * mag[:-1].cpu(), torch.float32)
             assert torch.equal(got, s.grad(g, torch.empty(vocab, dim, device="cuda")))
+
+
+def test_more_rows_than_one_launch_takes(arb):
+    n, vocab, dim = (1 << 30) + 7, 1000, 16  # two lanes a row
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    held = torch.randint(0, vocab, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    table = torch.randn(vocab, dim, generator=gen, device="cuda").half()
+    out = torch.empty(n, dim, dtype=torch.float16, device="cuda")
+    arb.embedding(out.data_ptr(), table.data_ptr(), held.data_ptr(), n, vocab, dim, dtype="float16")
+    for i in range(0, n, 1 << 23):  # (torch's own gather takes a workgroup per index, which a launch counts with 32 bits)
+        assert torch.equal(out[i:i + (1 << 23)], table[held[i:i + (1 << 23)].long()])
+
+
+def test_one_bag_of_very_many_tokens(arb):
+    # a single row of the result: all lanes of one group walk the bag
+    bag, vocab = 5_000_003, 8
+    held = (torch.arange(bag, device="cuda") % vocab).to(torch.int32)
+    table = torch.tensor([1.0, -1.0, 2.0, -2.0, 0.5, -0.5, 0.25, -0.25], device="cuda")[:, None].contiguous()
+    out = torch.empty(1, device="cuda")
+    arb.embedding(out.data_ptr(), table.data_ptr(), held.data_ptr(), 1, vocab, 1, bag=bag)
+    assert out.item() == 2.0  # (whole quarters: every sum is exact) 5,000,003 = 8 * 625,000 + 3
+    s = Sorted(arb, held, 1, bag, vocab, (bag, 1))
+    got = s.grad(torch.ones(1, 1, device="cuda"), torch.empty(vocab, 1, device="cuda"))
+    assert got[:, 0].tolist() == [625_001.0] * 3 + [625_000.0] * 5

@@ -119,6 +119,7 @@ def test_embedding_grad_refuses(arb, change, says):
     (dict(beta2=-0.1), "in \\[0, 1\\)"),
     (dict(beta2=float("nan")), "in \\[0, 1\\)"),
     (dict(sizes=[-1]), "bad tensor size"),
+    (dict(sizes=[1 << 36]), "bad tensor size"),
     (dict(sizes=[100, 3]), "differ in length"),
     (dict(grads=[A, A]), "differ in length"),
     (dict(params=[0]), "null tensor"),
@@ -149,6 +150,14 @@ def test_adamw_refuses_tensors_that_meet(arb, which, at):
         lists[which][-1] = 20 * A + 796
     with pytest.raises(arb.ArboretumError, match="overlap"):
         adamw(arb, sizes=[100] * k, **lists)
+
+
+def test_the_widest_row(arb):
+    for call in (lookup, grad):
+        with pytest.raises(arb.ArboretumError, match="bad dimension"):
+            call(arb, dim=65_535 * 256 + 1)
+        with pytest.raises(arb.ArboretumError, match="overlap"):  # of the right width, but too close to each other
+            call(arb, dim=65_535 * 256, out_stride=-1 if call is grad else 5)
 
 
 def test_nothing_to_do_is_no_error(arb):
