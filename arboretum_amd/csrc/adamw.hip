@@ -15,10 +15,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVec = 4;                            // elements of a load
-constexpr int kLeastChunk = kThreads * kVec;       // elements of a workgroup, and at most
-constexpr int kMostChunk = kThreads * kVec * 8;
-constexpr unsigned long long kEnoughBlocks = 2048;
-constexpr int kAhead = 2;
+// Elements of a workgroup: a vector a thread, more only where a launch would count more workgroups than it can.  What bounds the
+// step is memory (28 bytes an element in 32 bits, 22 with params and grads in 16): workgroups that come and go keep more of it in flight than
+// ones that walk (150 M elements in 300 tensors: 797 us, 5.3 TB/s; eight vectors a thread 860, thirty-two 947; 16 tensors of 182 M in 16
+// bits: 742, 770, 802).
+constexpr int kChunk = kThreads * kVec;
+constexpr unsigned long long kMostBlocks = 1ull << 22;  // (a launch counts its threads with 32 bits)
 constexpr int kTensorsAtOnce = 88;                 // a launch's tensors travel in its arguments (4 KB of them)
 
 struct Tensor {
@@ -32,19 +34,21 @@ struct Scalars {
   float decay, beta1, beta2, rest1, rest2, step_size, root, eps, grad_scale;
 };
 
-// What depends on the step and the learning rate: in 64 bits, rounded once.
-__host__ __device__ inline void SetStep(Scalars *s, double lr, double weight_decay, double beta1, double beta2, double t) {
+// What depends on the step and the learning rate: in 64 bits, rounded once.  Powers by the logarithms (base 2) of the betas: where the step
+// is read on the device, every workgroup computes them.
+__host__ __device__ inline void SetStep(Scalars *s, double lr, double weight_decay, double log_beta1, double log_beta2, double t) {
   s->decay = (float)(1.0 - lr * weight_decay);
-  s->step_size = (float)(lr / (1.0 - pow(beta1, t)));
-  s->root = (float)sqrt(1.0 - pow(beta2, t));
+  s->step_size = (float)(lr / (1.0 - exp2(t * log_beta1)));
+  s->root = (float)sqrt(1.0 - exp2(t * log_beta2));
 }
 
 struct Launch {
   Tensor tensor[kTensorsAtOnce];
   unsigned first[kTensorsAtOnce + 1];  // workgroup that begins each tensor
-  int count, chunk;
+  int count;
+  long long chunk;
   Scalars s;
-  double lr, weight_decay, beta1, beta2;
+  double lr, weight_decay, log_beta1, log_beta2;
   long long step;
   const float *lr_device;
   const long long *step_device;
@@ -69,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const Launch a) {
       s_scalars = a.s;
       const double lr = a.lr_device != nullptr ? (double)*a.lr_device : a.lr;
       const long long t = a.step_device != nullptr ? *a.step_device : a.step;
-      SetStep(&s_scalars, lr, a.weight_decay, a.beta1, a.beta2, (double)max(t, 1ll));
+      SetStep(&s_scalars, lr, a.weight_decay, a.log_beta1, a.log_beta2, (double)max(t, 1ll));
     }
     __syncthreads();
     s = s_scalars;
@@ -87,33 +91,20 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const Launch a) {
   typedef Pack<P, kVec> Ps;
   typedef Pack<G, kVec> Gs;
   typedef Pack<float, kVec> Fs;
-  constexpr long long kStep = kThreads * kVec;
-  long long i = begin + threadIdx.x * kVec;
-  // kAhead vectors of each array in flight
-  for (; i + (kAhead - 1) * kStep + kVec <= end; i += kAhead * kStep) {
-    Ps ps[kAhead];
-    Gs gs[kAhead];
-    Fs ms[kAhead], vs[kAhead];
+  for (long long i = begin + threadIdx.x * kVec; i < end; i += kThreads * kVec) {
+    if (i + kVec <= end) {
+      const Gs gs = *reinterpret_cast<const Gs *>(g + i);
+      Ps ps = *reinterpret_cast<const Ps *>(p + i);
+      Fs ms = *reinterpret_cast<const Fs *>(t.m + i), vs = *reinterpret_cast<const Fs *>(t.v + i);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const long long at = i + k * kStep;
-      gs[k] = *reinterpret_cast<const Gs *>(g + at);
-      ps[k] = *reinterpret_cast<const Ps *>(p + at);
-      ms[k] = *reinterpret_cast<const Fs *>(t.m + at);
-      vs[k] = *reinterpret_cast<const Fs *>(t.v + at);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const long long at = i + k * kStep;
-#pragma unroll
-      for (int c = 0; c < kVec; ++c) Update(s, ps[k].v[c], gs[k].v[c], ms[k].v[c], vs[k].v[c]);
-      *reinterpret_cast<Ps *>(p + at) = ps[k];
-      *reinterpret_cast<Fs *>(t.m + at) = ms[k];
-      *reinterpret_cast<Fs *>(t.v + at) = vs[k];
+      for (int c = 0; c < kVec; ++c) Update(s, ps.v[c], gs.v[c], ms.v[c], vs.v[c]);
+      *reinterpret_cast<Ps *>(p + i) = ps;
+      *reinterpret_cast<Fs *>(t.m + i) = ms;
+      *reinterpret_cast<Fs *>(t.v + i) = vs;
+    } else {
+      for (long long at = i; at < end; ++at) Update(s, p[at], g[at], t.m[at], t.v[at]);
     }
   }
-  for (; i < end; i += kStep)
-    for (long long at = i; at < min(end, i + kVec); ++at) Update(s, p[at], g[at], t.m[at], t.v[at]);
 }
 
 // Two ranges of one list that meet would be updated twice, by two workgroups at once.
@@ -178,19 +169,18 @@ void AdamW(const AdamWArgs &a) {
   l.s.rest2 = (float)(1.0 - a.beta2);
   l.s.eps = (float)a.eps;
   l.s.grad_scale = (float)a.grad_scale;
-  SetStep(&l.s, a.lr, a.weight_decay, a.beta1, a.beta2, (double)std::max(a.step, 1ll));
   l.lr = a.lr;
   l.weight_decay = a.weight_decay;
-  l.beta1 = a.beta1;
-  l.beta2 = a.beta2;
+  l.log_beta1 = std::log2(a.beta1);  // (of 0: minus infinity, and its powers are 0)
+  l.log_beta2 = std::log2(a.beta2);
+  SetStep(&l.s, a.lr, a.weight_decay, l.log_beta1, l.log_beta2, (double)std::max(a.step, 1ll));
   l.step = a.step;
   l.lr_device = a.lr_device;
   l.step_device = a.step_device;
-  // few elements are spread over the chip, a vector a thread; many in chunks that keep a workgroup busy for a while
   unsigned long long all = 0;
   for (int i = 0; i < a.count; ++i) all += (unsigned long long)a.sizes[i];
-  l.chunk = kLeastChunk;
-  while (l.chunk < kMostChunk && all / l.chunk > kEnoughBlocks) l.chunk *= 2;
+  l.chunk = kChunk;
+  while (all / l.chunk > kMostBlocks) l.chunk *= 2;
   int at = 0;
   while (at < a.count) {
     unsigned long long blocks = 0;
@@ -199,7 +189,7 @@ void AdamW(const AdamWArgs &a) {
     for (; at < a.count && l.count < kTensorsAtOnce; ++at) {
       if (a.sizes[at] == 0) continue;
       const unsigned long long more = (unsigned long long)(a.sizes[at] + l.chunk - 1) / l.chunk;
-      if (l.count > 0 && blocks + more > (1ull << 23)) break;  // (a launch counts its threads with 32 bits)
+      
       if (l.count == 0) first = a.params[at];
       l.tensor[l.count] = Tensor{a.params[at], a.grads[at], a.exp_avg[at], a.exp_avg_sq[at], a.sizes[at]};
       l.first[l.count++] = (unsigned)blocks;

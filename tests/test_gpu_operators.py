@@ -635,3 +635,19 @@ def test_one_bag_of_very_many_tokens(arb):
     s = Sorted(arb, held, 1, bag, vocab, (bag, 1))
     got = s.grad(torch.ones(1, 1, device="cuda"), torch.empty(vocab, 1, device="cuda"))
     assert got[:, 0].tolist() == [625_001.0] * 3 + [625_000.0] * 5
+
+
+@pytest.mark.parametrize("beta1,beta2", [(0.0, 0.0), (0.0, 0.999), (0.9, 0.0), (0.95, 0.9999)])
+def test_adamw_with_other_betas(arb, beta1, beta2):
+    gen = torch.Generator().manual_seed(2)
+    *host, at = make_tensors(gen, [3000], torch.float32, torch.float32)
+    for step in (1, 2, 1000):
+        for on_device in (False, True):
+            dev = [t.cuda() for t in host]
+            step_d = torch.tensor([step], device="cuda")
+            more = dict(step=1, step_device=step_d.data_ptr()) if on_device else dict(step=step)
+            run_adamw(arb, dev, at, [3000], beta1=beta1, beta2=beta2, **more)
+            want, bound = adamw_64(*host, step, 0.01, beta1, beta2, 1e-6, 0.1, 0.5)
+            within(dev[0], want[0], bound[0], torch.float32)
+            for k in (1, 2):
+                assert ((dev[k + 1].cpu().double() - want[k]).abs() <= bound[k] + 2.0 ** -149).all()
