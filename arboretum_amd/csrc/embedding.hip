@@ -73,6 +73,26 @@ __device__ __forceinline__ void Store(T *__restrict__ at, int held, const Pack<T
   }
 }
 
+// Results larger than the L2 caches of all XCDs (32 MB) go past them: nobody would find them there, and the table's rows stay (a
+// lookup of 65,536 x 4096 bf16 152 -> 130 us).
+constexpr size_t kStreamedBytes = (size_t)32 << 20;
+template <typename T, int kVec>
+__device__ __forceinline__ void StorePast(T *__restrict__ at, const Pack<T, kVec> &from) {
+  constexpr int kBytes = sizeof(T) * kVec;
+  if constexpr (kBytes % 16 == 0) {
+    typedef float Part __attribute__((ext_vector_type(4), aligned(2)));  // (of the smallest element)
+    struct Parts {
+      Pack<float, 4> v[kBytes / 16];
+    };
+    const Parts parts = __builtin_bit_cast(Parts, from);
+#pragma unroll
+    for (int k = 0; k < kBytes / 16; ++k)
+      __builtin_nontemporal_store(Part{parts.v[k].v[0], parts.v[k].v[1], parts.v[k].v[2], parts.v[k].v[3]}, reinterpret_cast<Part *>(at) + k);
+  } else {
+    *reinterpret_cast<Pack<T, kVec> *>(at) = from;
+  }
+}
+
 // Rows of the two matrices of a lookup.
 template <typename T>
 struct Rows {
@@ -88,7 +108,7 @@ struct Rows {
 // its loads are in flight at once (blockIdx.y: which piece).  Here and below the last vector of a row that is not whole
 // vectors wide is moved back to end with the row: two lanes then write the same values to the same place.
 constexpr int kPieces = 4;
-template <typename T, int kVec, typename Token>
+template <typename T, int kVec, bool kPast, typename Token>
 __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> bags, const Rows<T> r, int lanes_log) {
   const long long i = (long long)(((unsigned long long)blockIdx.x * kThreads + threadIdx.x) >> lanes_log);
   if (i >= bags.n) return;
@@ -107,7 +127,10 @@ __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> ba
   for (int k = 0; k < kPieces; ++k) {
 #pragma unroll
     for (int c = 0; c < kVec; ++c) x[k].v[c] = t < bags.vocab ? Round<T>(static_cast<float>(x[k].v[c]) * r.scale) : T(0);
-    if (first + k * step < r.dim) *reinterpret_cast<Pack<T, kVec> *>(to + min(first + k * step, r.dim - kVec)) = x[k];
+    if (first + k * step >= r.dim) continue;
+    T *at = to + min(first + k * step, r.dim - kVec);
+    if (kPast) StorePast<T, kVec>(at, x[k]);
+    else *reinterpret_cast<Pack<T, kVec> *>(at) = x[k];
   }
 }
 
@@ -230,6 +253,7 @@ template <typename T, int kVec, typename Token>
 void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
   const Bags<Token> bags = BagsOf<Token>(a.bags);
   const Rows<T> r{static_cast<const T *>(a.table), a.table_stride, static_cast<T *>(a.out), a.out_stride, a.dim, a.scale};
+  const bool past = (size_t)a.bags.n * a.dim * sizeof(T) > kStreamedBytes;
   if constexpr (kVec == 1) {
     if (a.dim == 1 && a.bags.bag > 1 && a.bags.token_stride == 1 && a.bags.bag_stride > 1 && a.bags.n * a.bags.bag >= kManyTokens &&
         a.bags.n >= kColumnBags * 256) {
@@ -262,7 +286,8 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
     Rows<T> to = r;
     to.out += i * r.out_stride;
     const dim3 grid((unsigned)(((some.n << group_log) + kThreads - 1) / kThreads), (unsigned)per_row);
-    if (a.bags.bag == 1) hipLaunchKernelGGL((k_embedding_one<T, kVec, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log);
+    if (a.bags.bag == 1 && past) hipLaunchKernelGGL((k_embedding_one<T, kVec, true, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log);
+    else if (a.bags.bag == 1) hipLaunchKernelGGL((k_embedding_one<T, kVec, false, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log);
     else hipLaunchKernelGGL((k_embedding_bag<T, kVec, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log, shares_log);
   }
 }
@@ -859,7 +884,7 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
     if (low < end && g.keys[low] == v0 + threadIdx.x) atomicOr(&s_named[threadIdx.x / 32], 1u << (threadIdx.x % 32));
   }
   __syncthreads();
-  // a row in pieces of 16 aligned bytes, whole ones past the caches (345 -> 272 us where 0.8 GB are zeros), elements at its ends
+  // a row in pieces of 16 aligned bytes (past the caches: 345 -> 272 us where 0.8 GB are zeros; the sums are better left in them, 267 and 274), elements at its ends
   constexpr int kVec = 16 / sizeof(O);
   const int pieces = g.dim / kVec + 2, lanes = min(64, pieces);
   const int groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
