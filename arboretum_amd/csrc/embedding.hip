@@ -491,6 +491,7 @@ constexpr int kSortTile = kSortThreads * kSortRounds;  // 8192
 constexpr int kWavePairs = kSortTile / kSortWaves;
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
+constexpr unsigned kXcds = 8;
 constexpr unsigned kGroupTiles = 32;  // tiles whose counts are summed up by one workgroup
 
 // Where a pass takes its pairs from: the tokens themselves, or the keys and rows of the pass before.
@@ -637,7 +638,10 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   __shared__ unsigned s_out[kDigits];                     // output position of that pair
   __shared__ unsigned s_sum[2][kDigits / 64];
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const unsigned tile = blockIdx.x;
+  // Workgroups are dealt to the eight XCDs in turn.  Tiles that follow each other, whose runs of a digit meet inside a line of memory, go to
+  // the same one (50 M pairs: 214 -> 199 us).
+  const unsigned tile = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  if (tile * (unsigned long long)kSortTile >= in.m) return;
   const unsigned base = tile * kSortTile, held = min((unsigned)kSortTile, in.m - base);
   for (int i = threadIdx.x; i < kSortWaves * kDigits / 2; i += kSortThreads) reinterpret_cast<unsigned *>(s_wave)[i] = 0;
   typename Source::Raw raw[kSortRounds];
@@ -1257,7 +1261,7 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
       hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
       const bool several = plan.groups > 1;  // (the totals of the only group are those of all)
       if (several) hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
-      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts,
+      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3((plan.tiles + kXcds - 1) / kXcds * kXcds), dim3(kSortThreads), 0, st, in, digit, counts,
                          several ? groups : (const unsigned *)nullptr, several ? groups + (size_t)plan.groups * kDigits : groups, to[0], to[1]);
     };
     if (pass > 0) {
