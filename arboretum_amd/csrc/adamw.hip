@@ -15,10 +15,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVec = 4;                            // elements of a load
-// Elements of a workgroup: a vector a thread, more only where a launch would count more workgroups than it can.  What bounds the
-// step is memory (28 bytes an element in 32 bits, 22 with params and grads in 16): workgroups that come and go keep more of it in flight than
-// ones that walk (150 M elements in 300 tensors: 797 us, 5.3 TB/s; eight vectors a thread 860, thirty-two 947; 16 tensors of 182 M in 16
-// bits: 742, 770, 802).
+// Elements of a workgroup: a vector a thread, more only where a launch would count more workgroups than it can.  What
+// bounds the step is memory (28 bytes an element in 32 bits, 22 with params and grads in 16): workgroups that come
+// and go keep more of it in flight than ones that walk (150 M elements in 300 tensors: 797 us, 5.3 TB/s; eight
+// vectors a thread 860, thirty-two 947; 16 tensors of 182 M in 16 bits: 742, 770, 802).
 constexpr int kChunk = kThreads * kVec;
 constexpr unsigned long long kMostBlocks = 1ull << 22;  // (a launch counts its threads with 32 bits)
 constexpr int kTensorsAtOnce = 88;                 // a launch's tensors travel in its arguments (4 KB of them)
@@ -34,8 +34,8 @@ struct Scalars {
   float decay, beta1, beta2, rest1, rest2, step_size, root, eps, grad_scale;
 };
 
-// What depends on the step and the learning rate: in 64 bits, rounded once.  Powers by the logarithms (base 2) of the betas: where the step
-// is read on the device, every workgroup computes them.
+// What depends on the step and the learning rate: in 64 bits, rounded once.  Powers by the logarithms (base 2) of the
+// betas: where the step is read on the device, every workgroup computes them.
 __host__ __device__ inline void SetStep(Scalars *s, double lr, double weight_decay, double log_beta1, double log_beta2, double t) {
   s->decay = (float)(1.0 - lr * weight_decay);
   s->step_size = (float)(lr / (1.0 - exp2(t * log_beta1)));

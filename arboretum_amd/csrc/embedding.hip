@@ -6,8 +6,6 @@
 // The gradient gathers: the (token, bag) pairs are put in order of tokens first (a stable radix sort), so that every sum is
 // formed in an order that depends on the tokens alone, and no atomic decides it.
 #include <algorithm>
-#include <cstring>
-#include <limits>
 #include <type_traits>
 
 #include "operators_device.h"
@@ -73,8 +71,8 @@ __device__ __forceinline__ void Store(T *__restrict__ at, int held, const Pack<T
   }
 }
 
-// Results larger than the L2 caches of all XCDs (32 MB) go past them: nobody would find them there, and the table's rows stay (a
-// lookup of 65,536 x 4096 bf16 152 -> 130 us).
+// Results larger than the L2 caches of all XCDs (32 MB) go past them: nobody would find them there, and the table's
+// rows stay (a lookup of 65,536 x 4096 bf16 152 -> 130 us).
 constexpr size_t kStreamedBytes = (size_t)32 << 20;
 template <typename T, int kVec>
 __device__ __forceinline__ void StorePast(T *__restrict__ at, const Pack<T, kVec> &from) {
@@ -87,7 +85,8 @@ __device__ __forceinline__ void StorePast(T *__restrict__ at, const Pack<T, kVec
     const Parts parts = __builtin_bit_cast(Parts, from);
 #pragma unroll
     for (int k = 0; k < kBytes / 16; ++k)
-      __builtin_nontemporal_store(Part{parts.v[k].v[0], parts.v[k].v[1], parts.v[k].v[2], parts.v[k].v[3]}, reinterpret_cast<Part *>(at) + k);
+      __builtin_nontemporal_store(Part{parts.v[k].v[0], parts.v[k].v[1], parts.v[k].v[2], parts.v[k].v[3]},
+                                  reinterpret_cast<Part *>(at) + k);
   } else {
     *reinterpret_cast<Pack<T, kVec> *>(at) = from;
   }
@@ -104,9 +103,10 @@ struct Rows {
   float scale;
 };
 
-// Bags of one token: rows are copied, scaled.  2^lanes_log lanes take a piece of kPieces vectors a lane of a row, so that all
-// its loads are in flight at once (blockIdx.y: which piece).  Here and below the last vector of a row that is not whole
-// vectors wide is moved back to end with the row: two lanes then write the same values to the same place.
+// Bags of one token: rows are copied, scaled.  2^lanes_log lanes take a piece of kPieces vectors a lane of a row, so
+// that all its loads are in flight at once (blockIdx.y: which piece).  Here and below the last vector of a row that
+// is not whole vectors wide is moved back to end with the row: two lanes then write the same values to the same
+// place.
 constexpr int kPieces = 4;
 template <typename T, int kVec, bool kPast, typename Token>
 __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> bags, const Rows<T> r, int lanes_log) {
@@ -134,9 +134,9 @@ __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> ba
   }
 }
 
-// Bags of several tokens.  A row of the result is 2^lanes_log lanes wide (kVec elements a lane), and 2^shares_log shares of
-// them take every so many-th token each and meet in the end, by steps of halves.  kAhead tokens of a lane are in flight; where
-// there is no token the last row of the table is read and not added.
+// Bags of several tokens.  A row of the result is 2^lanes_log lanes wide (kVec elements a lane), and 2^shares_log
+// shares of them take every so many-th token each and meet in the end, by steps of halves.  kAhead tokens of a lane
+// are in flight; where there is no token the last row of the table is read and not added.
 constexpr int kAhead = 8;
 template <typename T, int kVec, typename Token>
 __global__ void __launch_bounds__(kThreads)
@@ -188,12 +188,13 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
   }
 }
 
-// Rows of one element over so many bags that their tokens, column by column (the leaves of trees), come from memory and not
-// from the last-level cache of 256 MB.  A thread takes four neighbouring bags, whose tokens are one load, and the tokens of the next
-// columns are in flight while these are looked up.  Reading the tokens alone takes 135 us for a million bags of 200; the rest
-// is the lookups, of which the L1 answers little more than a lane a cycle.  (1,000,003 x 200: 223 us, 276 with a bag a thread;
-// 700,000 x 100, which the cache holds: 71 and 64; with the pieces of the table that a column names copied to the LDS first 290
-// and more: finding the pieces takes longer than the LDS saves.)
+// Rows of one element over so many bags that their tokens, column by column (the leaves of trees), come from memory
+// and not from the last-level cache of 256 MB.  A thread takes four neighbouring bags, whose tokens are one load, and
+// the tokens of the next columns are in flight while these are looked up.  Reading the tokens alone takes 135 us for
+// a million bags of 200; the rest is the lookups, of which the L1 answers little more than a lane a cycle.
+// (1,000,003 x 200: 223 us, 276 with a bag a thread; 700,000 x 100, which the cache holds: 71 and 64; with the pieces
+// of the table that a column names copied to the LDS first 290 and more: finding the pieces takes longer than the LDS
+// saves.)
 constexpr int kColumns = 4;
 constexpr int kBagsOfThread = 4;
 constexpr long long kManyTokens = 1ll << 27;
@@ -234,7 +235,8 @@ __global__ void __launch_bounds__(kThreads) k_embedding_columns(const Bags<Token
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-      for (int k = 0; k < kBagsOfThread; ++k) x[c][k] = static_cast<float>(r.table[(long long)min(t[c][k], bags.vocab - 1u) * r.table_stride]);
+      for (int k = 0; k < kBagsOfThread; ++k)
+        x[c][k] = static_cast<float>(r.table[(long long)min(t[c][k], bags.vocab - 1u) * r.table_stride]);
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
@@ -257,8 +259,8 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
   if constexpr (kVec == 1) {
     if (a.dim == 1 && a.bags.bag > 1 && a.bags.token_stride == 1 && a.bags.bag_stride > 1 && a.bags.n * a.bags.bag >= kManyTokens &&
         a.bags.n >= kColumnBags * 256) {
-      hipLaunchKernelGGL((k_embedding_columns<T, Token>), dim3((unsigned)((a.bags.n + kColumnBags - 1) / kColumnBags)), dim3(kThreads), 0, st,
-                         bags, r);
+      const unsigned blocks = (unsigned)((a.bags.n + kColumnBags - 1) / kColumnBags);
+      hipLaunchKernelGGL((k_embedding_columns<T, Token>), dim3(blocks), dim3(kThreads), 0, st, bags, r);
       return;
     }
   }
@@ -286,16 +288,18 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
     Rows<T> to = r;
     to.out += i * r.out_stride;
     const dim3 grid((unsigned)(((some.n << group_log) + kThreads - 1) / kThreads), (unsigned)per_row);
-    if (a.bags.bag == 1 && past) hipLaunchKernelGGL((k_embedding_one<T, kVec, true, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log);
-    else if (a.bags.bag == 1) hipLaunchKernelGGL((k_embedding_one<T, kVec, false, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log);
-    else hipLaunchKernelGGL((k_embedding_bag<T, kVec, Token>), grid, dim3(kThreads), 0, st, some, to, lanes_log, shares_log);
+    const dim3 block(kThreads);
+    if (a.bags.bag != 1) hipLaunchKernelGGL((k_embedding_bag<T, kVec, Token>), grid, block, 0, st, some, to, lanes_log, shares_log);
+    else if (past) hipLaunchKernelGGL((k_embedding_one<T, kVec, true, Token>), grid, block, 0, st, some, to, lanes_log);
+    else hipLaunchKernelGGL((k_embedding_one<T, kVec, false, Token>), grid, block, 0, st, some, to, lanes_log);
   }
 }
 
 // -------------------------------------------------------------------- sort
 
-// Division of numbers below 2^31 by a number that stays the same (Granlund and Montgomery, "Division by invariant integers
-// using multiplication"): with 2^(l-1) < d <= 2^l, factor = floor(2^(31+l) / d) + 1 makes p factor / 2^(31+l) exceed p / d by less than 1 / d.
+// Division of numbers below 2^31 by a number that stays the same (Granlund and Montgomery, "Division by invariant
+// integers using multiplication"): with 2^(l-1) < d <= 2^l, factor = floor(2^(31+l) / d) + 1 makes p factor /
+// 2^(31+l) exceed p / d by less than 1 / d.
 struct Divider {
   unsigned by, factor;
   int shift;
@@ -360,8 +364,9 @@ __device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid,
 
 // ---- few pairs: one launch
 //
-// Every workgroup has a range of the vocabulary.  It reads all tokens (they come out of the L2), counts those below its range, which is
-// where its pairs start in the result, keeps those within, and sorts them in the LDS.  Nothing passes between workgroups.
+// Every workgroup has a range of the vocabulary.  It reads all tokens (they come out of the L2), counts those below
+// its range, which is where its pairs start in the result, keeps those within, and sorts them in the LDS.  Nothing
+// passes between workgroups.
 
 constexpr int kRangeThreads = 1024;
 constexpr int kRangeWaves = kRangeThreads / 64;
@@ -372,7 +377,8 @@ constexpr unsigned kMostRanges = 256;  // a workgroup per CU
 // Pairs are kept as (key - first key of the range) << place_bits | place.
 template <int kRounds, typename Token>
 __global__ void __launch_bounds__(kRangeThreads)
-k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits, unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
+k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits, unsigned *__restrict__ keys,
+              unsigned *__restrict__ rows) {
   __shared__ unsigned s_pair[kRounds * kRangeThreads];
   constexpr int kCounters = kRangeWaves << kRangeBits, kOwn = kCounters / kRangeThreads;
   __shared__ __align__(16) unsigned s_count[kCounters];  // pairs of a digit, then their place; the waves of a digit beside each other
@@ -410,7 +416,8 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   for (int k = 0; k < kRounds; ++k) {
     const bool mine = key[k] - v0 < here;
     const unsigned long long all = __ballot(mine);
-    if (mine) s_pair[at + (unsigned)__popcll(all & ((1ull << lane) - 1ull))] = (key[k] - v0) << place_bits | (k * kRangeThreads + threadIdx.x);
+    const unsigned to = at + (unsigned)__popcll(all & ((1ull << lane) - 1ull));
+    if (mine) s_pair[to] = (key[k] - v0) << place_bits | (k * kRangeThreads + threadIdx.x);
     at += (unsigned)__popcll(all);
   }
   const int passes = (key_bits + kRangeBits - 1) / kRangeBits;
@@ -507,7 +514,8 @@ struct FromTokens {
   // kSome pairs side by side
   template <int kSome>
   __device__ __forceinline__ void Beside(unsigned p, Token (&to)[kSome]) const {
-    if (pairs.flat && p + kSome <= m) *reinterpret_cast<Pack<Token, kSome> *>(to) = *reinterpret_cast<const Pack<Token, kSome> *>(pairs.bags.tokens + p);
+    typedef Pack<Token, kSome> Some;
+    if (pairs.flat && p + kSome <= m) *reinterpret_cast<Some *>(to) = *reinterpret_cast<const Some *>(pairs.bags.tokens + p);
     else pairs.Get(p, 1, to);
   }
   template <int kSome>
@@ -543,9 +551,9 @@ struct Digit {
   __device__ __forceinline__ unsigned Of(unsigned key) const { return (key >> shift) & mask; }
 };
 
-// Digit counts of one tile: counts[tile * kDigits + digit].  A thread's pairs lie beside each other and equal neighbours are counted
-// as one, and a wave of one digit only as one: pairs that are nearly in order (leaves, tree by tree; the last pass) would
-// otherwise queue for one counter of the LDS.
+// Digit counts of one tile: counts[tile * kDigits + digit].  A thread's pairs lie beside each other and equal
+// neighbours are counted as one, and a wave of one digit only as one: pairs that are nearly in order (leaves, tree by
+// tree; the last pass) would otherwise queue for one counter of the LDS.
 template <typename Source>
 __global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
   constexpr int kBeside = 4, kRounds = kSortRounds / kBeside;
@@ -626,8 +634,8 @@ __global__ void __launch_bounds__(1024) k_sort_sum_groups(unsigned *__restrict__
   if (wave == 0) groups[(size_t)count * kDigits + digit] = total;
 }
 
-// Stable scatter of one tile.  counts, groups: pairs of the same digit in the tiles of the group before, in the groups before;
-// totals: pairs of each digit.
+// Stable scatter of one tile.  counts, groups: pairs of the same digit in the tiles of the group before, in the
+// groups before; totals: pairs of each digit.
 template <typename Source>
 __global__ void __launch_bounds__(kSortThreads, 8)  // (8 waves a SIMD: two workgroups on a CU)
 k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ counts, const unsigned *__restrict__ groups,
@@ -638,8 +646,8 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   __shared__ unsigned s_out[kDigits];                     // output position of that pair
   __shared__ unsigned s_sum[2][kDigits / 64];
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  // Workgroups are dealt to the eight XCDs in turn.  Tiles that follow each other, whose runs of a digit meet inside a line of memory, go to
-  // the same one (50 M pairs: 214 -> 199 us).
+  // Workgroups are dealt to the eight XCDs in turn.  Tiles that follow each other, whose runs of a digit meet inside
+  // a line of memory, go to the same one (50 M pairs: 214 -> 199 us).
   const unsigned tile = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
   if (tile * (unsigned long long)kSortTile >= in.m) return;
   const unsigned base = tile * kSortTile, held = min((unsigned)kSortTile, in.m - base);
@@ -781,12 +789,13 @@ SortPlan PlanSort(long long n, int bag, long long vocab) {
 
 // ---------------------------------------------------------------- gradient
 //
-// The sorted pairs are cut into chunks of equal length, whatever the tokens are: a token that half of all bags name is
-// the work of many waves.  A run of equal keys inside one chunk is summed and written there; of a run that goes on beyond its
-// chunk each chunk leaves its part of the sum in the work memory, and a second launch (k_grad_join) adds the parts in order.
+// The sorted pairs are cut into chunks of equal length, whatever the tokens are: a token that half of all bags name
+// is the work of many waves.  A run of equal keys inside one chunk is summed and written there; of a run that goes on
+// beyond its chunk each chunk leaves its part of the sum in the work memory, and a second launch (k_grad_join) adds
+// the parts in order.
 
-// First pair whose key is at least v: the whole wave asks, 64 probes a step (five steps for 2^30 pairs, where halving takes thirty loads
-// one after the other).
+// First pair whose key is at least v: the whole wave asks, 64 probes a step (five steps for 2^30 pairs, where halving
+// takes thirty loads one after the other).
 __device__ __forceinline__ unsigned WaveLowerBound(const unsigned *__restrict__ keys, unsigned m, unsigned v) {
   unsigned low = 0, high = m;  // the answer is in [low, high]
   while (low < high) {
@@ -888,7 +897,8 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
     if (low < end && g.keys[low] == v0 + threadIdx.x) atomicOr(&s_named[threadIdx.x / 32], 1u << (threadIdx.x % 32));
   }
   __syncthreads();
-  // a row in pieces of 16 aligned bytes (past the caches: 345 -> 272 us where 0.8 GB are zeros; the sums are better left in them, 267 and 274), elements at its ends
+  // a row in pieces of 16 aligned bytes (past the caches: 345 -> 272 us where 0.8 GB are zeros; the sums are better
+  // left in them, 267 and 274), elements at its ends
   constexpr int kVec = 16 / sizeof(O);
   const int pieces = g.dim / kVec + 2, lanes = min(64, pieces);
   const int groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
@@ -908,7 +918,8 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
   }
 }
 
-// Rows of more than kNarrow elements: 2^lanes_log lanes hold kVec columns each and walk a chunk pair by pair, kAhead rows in flight.
+// Rows of more than kNarrow elements: 2^lanes_log lanes hold kVec columns each and walk a chunk pair by pair, kAhead
+// rows in flight.
 template <typename T, typename O, int kVec>
 __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) {
   unsigned block;
@@ -974,8 +985,8 @@ __device__ __forceinline__ float WaveSum(float v) {
   return v;
 }
 
-// Rows of up to kDim <= kNarrow elements: a lane takes a pair with its whole row, a wave 64 pairs of a chunk at a time.  While the key stays
-// the same the lanes add up what is theirs; when it changes they meet.
+// Rows of up to kDim <= kNarrow elements: a lane takes a pair with its whole row, a wave 64 pairs of a chunk at a
+// time.  While the key stays the same the lanes add up what is theirs; when it changes they meet.
 template <typename T, typename O, int kDim>
 __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g) {
   unsigned block;
@@ -1082,8 +1093,9 @@ __device__ __forceinline__ bool GoesOn(const Gradient<T, O> &g, unsigned w, unsi
   return true;
 }
 
-// The parts of the runs that go on, added up: every wave asks for a chunk of its own and sums the run that begins there, 2^lanes_log
-// lanes side by side over the columns (four each) and the others over the parts.  A run of many parts is left to all waves of the workgroup.
+// The parts of the runs that go on, added up: every wave asks for a chunk of its own and sums the run that begins
+// there, 2^lanes_log lanes side by side over the columns (four each) and the others over the parts.  A run of many
+// parts is left to all waves of the workgroup.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinVec = 4;
 constexpr unsigned kManyParts = 8;  // of a lane
@@ -1096,7 +1108,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_grad_join(const Gradient<T, O>
   const unsigned share = lane >> lanes_log, shares = 64u >> lanes_log;  // of the parts, within the wave
   const int column = (int)(lane & ((1u << lanes_log) - 1u)) * kJoinVec, step = kJoinVec << lanes_log;
   float sum[kJoinVec];
-  // parts of the run from chunk w on, beginning with the `from`-th and taking every `by`-th: the first is what the run left in w itself
+  // parts of the run from chunk w on, beginning with the `from`-th and taking every `by`-th: the first is what the
+  // run left in w itself
   auto add = [&](unsigned w, unsigned last, int d, unsigned from, unsigned by) {
 #pragma unroll
     for (int c = 0; c < kJoinVec; ++c) sum[c] = 0.0f;
@@ -1148,8 +1161,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_grad_join(const Gradient<T, O>
   }
 }
 
-// Pairs of a chunk: few, so that there are waves for every CU, and more where there are enough (4096), since each chunk leaves
-// two rows of parts to be joined; never more than four million waves.  (5,003 x 771: 28 us with 16 pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
+// Pairs of a chunk: few, so that there are waves for every CU, and more where there are enough (4096), since each
+// chunk leaves two rows of parts to be joined; never more than four million waves.  (5,003 x 771: 28 us with 16
+// pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
 unsigned ChunkOf(unsigned m, int dim) {
   const bool wide = dim > kNarrow;
   const unsigned most = wide ? 256 : 1024;
@@ -1261,8 +1275,9 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
       hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
       const bool several = plan.groups > 1;  // (the totals of the only group are those of all)
       if (several) hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
-      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3((plan.tiles + kXcds - 1) / kXcds * kXcds), dim3(kSortThreads), 0, st, in, digit, counts,
-                         several ? groups : (const unsigned *)nullptr, several ? groups + (size_t)plan.groups * kDigits : groups, to[0], to[1]);
+      const unsigned *before = several ? groups : nullptr, *totals = several ? groups + (size_t)plan.groups * kDigits : groups;
+      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3((plan.tiles + kXcds - 1) / kXcds * kXcds), dim3(kSortThreads), 0, st, in, digit,
+                         counts, before, totals, to[0], to[1]);
     };
     if (pass > 0) {
       launch(FromPairs{from[0], from[1], plan.m});
@@ -1286,7 +1301,8 @@ size_t EmbeddingGradBytes(long long n, int bag, int dim) {
 void EmbeddingGrad(const EmbeddingGradArgs &a) {
   CheckType(a.type);
   CheckType(a.table_type);
-  if (a.table_type != kFloat32 && a.table_type != a.type) throw std::runtime_error("the table's gradient is float32 or of the type of grad_out");
+  if (a.table_type != kFloat32 && a.table_type != a.type)
+    throw std::runtime_error("the table's gradient is float32 or of the type of grad_out");
   CheckShape(a.n, a.bag, a.vocab);
   CheckRows(a.grad_out, a.n, a.out_stride, a.dim, a.type, false, "grad_out");
   CheckRows(a.grad_table, a.vocab, a.table_stride, a.dim, a.table_type, true, "grad_table");
@@ -1345,7 +1361,8 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
     }
     if (g.chunks > 1) {
       constexpr unsigned kWaves = kJoinThreads / 64;
-      const int lanes_log = std::min(LogAtLeast((a.dim + kJoinVec - 1) / kJoinVec), 6), pieces = (a.dim + 64 * kJoinVec - 1) / (64 * kJoinVec);
+      const int lanes_log = std::min(LogAtLeast((a.dim + kJoinVec - 1) / kJoinVec), 6);
+      const int pieces = (a.dim + 64 * kJoinVec - 1) / (64 * kJoinVec);
       hipLaunchKernelGGL((k_grad_join<T, O>), dim3((g.chunks + kWaves - 1) / kWaves, std::min(pieces, 16)), dim3(kJoinThreads), 0, st, g,
                          lanes_log);
     }

@@ -1,8 +1,7 @@
-// Leaf weights trained together, the splits as they are: a row of the matrix is a bag of tokens, one leaf per tree, the sum of
-// their weights is what the booster answers, and the weights are a table of embeddings of dimension 1.  Every step is
-// the lookup, the gradient of the objective, the gradient of the table and AdamW, all on the device; the tokens are
-// sorted once.
-#include <cstring>
+// Leaf weights trained together, the splits as they are: a row of the matrix is a bag of tokens, one leaf per tree,
+// the sum of their weights is what the booster answers, and the weights are a table of embeddings of dimension 1.
+// Every step is the lookup, the gradient of the objective, the gradient of the table and AdamW, all on the device;
+// the tokens are sorted once.
 #include <memory>
 #include <vector>
 

@@ -206,73 +206,77 @@ const char *AHistSumNoAlloc(long long *sum_g, long long *sum_h, unsigned *bin_co
 
 /* ---- Embeddings over tokens, and the optimizer's step over their tables.
  *
- * A row of a data matrix is a bag of tokens, one leaf per tree (AGardenLeafTokens), and what a booster answers is an
- * embedding of dimension 1 summed over the bag; the same operators serve embeddings of any dimension over
+ * A row of a data matrix is a bag of tokens, one leaf per tree (AGardenLeafTokens), and what a booster answers is
+ * an embedding of dimension 1 summed over the bag; the same operators serve embeddings of any dimension over
  * leaves, categories or the tokens of a text.  No counterpart in the reference.
  *
- * EVERY POINTER IS A DEVICE POINTER, but for the arrays of AAdamW and what is said to be the host's.  AEmbedding, AEmbeddingSort,
- * AEmbeddingGrad and AAdamW enqueue on `stream` (a hipStream_t, NULL = default stream) of the device that their output is on, and return WITHOUT waiting.  They
- * allocate nothing, wait for nothing and may be captured into a graph.  Inputs and outputs must not overlap.
- * Element types: 0 float32, 1 bfloat16, 2 float16; sums are formed in float32 and rounded once, to nearest.  Strides
- * count elements and are not negative; rows may begin at any element.
- * Tokens: token j of bag i is tokens[i * token_stride + j * bag_stride], a signed integer of token_bits (32 or 64).  -1
- * stands for none.  Any other outside [0, vocab) is treated as none too, and sets *status (a device word, may be
- * NULL, never cleared here) to 1.  n * bag and vocab are below 2^31, dim is at most 65,535 * 256; both n and bag may be 0.
- * The first call of a kind in a process loads its kernels: a program that captures graphs makes one beforehand. */
+ * EVERY POINTER IS A DEVICE POINTER, but for the arrays of AAdamW and what is said to be the host's.  AEmbedding,
+ * AEmbeddingSort, AEmbeddingGrad and AAdamW enqueue on `stream` (a hipStream_t, NULL = default stream) of the
+ * device that their output is on, and return WITHOUT waiting.  They allocate nothing, wait for nothing and may be
+ * captured into a graph.  Inputs and outputs must not overlap.
+ * Element types: 0 float32, 1 bfloat16, 2 float16; sums are formed in float32 and rounded once, to nearest.
+ * Strides count elements and are not negative; rows may begin at any element.
+ * Tokens: token j of bag i is tokens[i * token_stride + j * bag_stride], a signed integer of token_bits (32 or
+ * 64).  -1 stands for none.  Any other outside [0, vocab) is treated as none too, and sets *status (a device word,
+ * may be NULL, never cleared here) to 1.  n * bag and vocab are below 2^31, dim is at most 65,535 * 256; both n
+ * and bag may be 0. The first call of a kind in a process loads its kernels: a program that captures graphs makes
+ * one beforehand. */
 
 /* out[i] = scale * (sum over j of table[token(i, j)]), rows of `dim` elements; 0 for a bag without tokens. */
 const char *AEmbedding(void *out, const void *table, const void *tokens, long long n, int bag, long long vocab, int dim,
                        long long out_stride, long long table_stride, long long token_stride, long long bag_stride,
                        int type, int token_bits, float scale, unsigned *status, void *stream);
 
-/* The pairs (token, bag) in order of tokens, for AEmbeddingGrad: keys[p] is the token and rows[p] the bag of pair p, n * bag of
- * them.  Pairs of one token stand in an order that depends on the arguments alone; what stands for none comes last,
- * with the key `vocab`.  A caller whose tokens stay the same sorts them once.
+/* The pairs (token, bag) in order of tokens, for AEmbeddingGrad: keys[p] is the token and rows[p] the bag of pair
+ * p, n * bag of them.  Pairs of one token stand in an order that depends on the arguments alone; what stands for
+ * none comes last, with the key `vocab`.  A caller whose tokens stay the same sorts them once.
  * work: 16-byte aligned, AEmbeddingSortBytes of it, undefined before and after. */
 const char *AEmbeddingSortBytes(long long n, int bag, long long vocab, unsigned long long *bytes);
 const char *AEmbeddingSort(unsigned *keys, unsigned *rows, const void *tokens, long long n, int bag, long long vocab,
                            long long token_stride, long long bag_stride, int token_bits, void *work,
                            unsigned long long work_bytes, unsigned *status, void *stream);
 
-/* Gradient of AEmbedding's table: grad_table[v] = scale * (sum of grad_out[rows[p]] over the pairs p of key v), 0 for a row that
- * no token names.  accumulate != 0 adds it to what is there (rows that no token names are not touched).
- * The result is the same from run to run.  table_type: 0, or `type`, the type of grad_out.
- * keys, rows: of AEmbeddingSort with the same n, bag and vocab.  work: as there, AEmbeddingGradBytes of it (may be the
- * same memory). */
+/* Gradient of AEmbedding's table: grad_table[v] = scale * (sum of grad_out[rows[p]] over the pairs p of key v), 0
+ * for a row that no token names.  accumulate != 0 adds it to what is there (rows that no token names are not
+ * touched). The result is the same from run to run.  table_type: 0, or `type`, the type of grad_out.
+ * keys, rows: of AEmbeddingSort with the same n, bag and vocab.  work: as there, AEmbeddingGradBytes of it (may be
+ * the same memory). */
 const char *AEmbeddingGradBytes(long long n, int bag, int dim, unsigned long long *bytes);
 const char *AEmbeddingGrad(void *grad_table, const void *grad_out, const unsigned *keys, const unsigned *rows,
                            long long n, int bag, long long vocab, int dim, long long table_stride, long long out_stride,
                            int type, int table_type, float scale, int accumulate, void *work,
                            unsigned long long work_bytes, void *stream);
 
-/* The leaf every row of `data` reaches in each of the first n_rounds trees (-1: all): tokens[t * stride + row], DEVICE memory for
- * 32-bit words of which nothing pending may make use, stride >= rows.  The trees of a class stand together (by class, then in the order they grew), and the
- * leaves are numbered through the trees of a class: a class' columns are bags of tokens over a table of leaves[class] rows (a host array of
- * `classes` counts, the booster's labels_count; may be NULL), token_stride 1 and bag_stride `stride`.  Waits for the result. */
-const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens, long long stride, int n_rounds,
-                              long long *leaves, int classes);
-
-/* Trains the leaf weights of all trees of the booster together, the splits as they are, against its objective on `data` (any matrix
- * with a target): `steps` AdamW steps on the mean over all rows of half the
- * squared error, or of the cross-entropy.  Works in 20 bytes of device memory per row and tree
- * and waits for the result; rows times trees of a class are below 2^31.  The booster grows no tree afterwards (AGrowTree returns an
- * error); predictions that matrices carry (AAppendLastTree) and the training predictions stay as they were.  No other thread may use
- * the booster meanwhile. */
-const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
-                                double eps, double weight_decay);
-
-/* One AdamW step over `count` tensors at once, in float32 whatever the types of params (type) and grads (grad_type):
+/* One AdamW step over `count` tensors at once, in float32 whatever the types of params (type) and grads
+ * (grad_type):
  *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * params, grads, exp_avg (m), exp_avg_sq (v), sizes: HOST arrays of `count` device pointers and element counts, read before
- * the call returns; tensors of one list must not overlap.  Sizes are below 2^36; one may be 0, its pointers are then not looked at.
- * All tensors are on one device.  step counts from 1.
+ * params, grads, exp_avg (m), exp_avg_sq (v), sizes: HOST arrays of `count` device pointers and element counts,
+ * read before the call returns; tensors of one list must not overlap.  Sizes are below 2^36; one may be 0, its
+ * pointers are then not looked at. All tensors are on one device.  step counts from 1.
  * lr_device, step_device: device words read instead of lr and step (for a captured graph that is replayed with
  * others); may be NULL.  (A step below 1 there counts as 1.) */
 const char *AAdamW(int count, void *const *params, const void *const *grads, float *const *exp_avg,
                    float *const *exp_avg_sq, const long long *sizes, int type, int grad_type, double lr, double beta1,
                    double beta2, double eps, double weight_decay, double grad_scale, long long step,
                    const float *lr_device, const long long *step_device, void *stream);
+
+/* The leaf every row of `data` reaches in each of the first n_rounds trees (-1: all): tokens[t * stride + row],
+ * DEVICE memory for 32-bit words of which nothing pending may make use, stride >= rows.  The trees of a class
+ * stand together (by class, then in the order they grew), and the leaves are numbered through the trees of a
+ * class: a class' columns are bags of tokens over a table of leaves[class] rows (a host array of `classes` counts,
+ * the booster's labels_count; may be NULL), token_stride 1 and bag_stride `stride`.  Waits for the result. */
+const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens, long long stride, int n_rounds,
+                              long long *leaves, int classes);
+
+/* Trains the leaf weights of all trees of the booster together, the splits as they are, against its objective on
+ * `data` (any matrix with a target): `steps` AdamW steps on the mean over all rows of half the squared error, or
+ * of the cross-entropy.  Works in 20 bytes of device memory per row and tree and waits for the result; rows times
+ * trees of a class are below 2^31.  The booster grows no tree afterwards (AGrowTree returns an error); predictions
+ * that matrices carry (AAppendLastTree) and the training predictions stay as they were.  No other thread may use
+ * the booster meanwhile. */
+const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
+                                double eps, double weight_decay);
 
 #ifdef __cplusplus
 }
