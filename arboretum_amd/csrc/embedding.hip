@@ -870,7 +870,7 @@ struct Gradient {
 };
 
 // Zeros for the rows [block * slots, ...) that no token names.  Which these are is found from the few pairs of those rows.
-template <typename T, typename O>
+template <int kBlock, typename T, typename O>
 __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block) {
   __shared__ unsigned s_range[2], s_named[kMostSlots / 32];
   const unsigned wave = threadIdx.x >> 6;
@@ -882,8 +882,8 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
   }
   __syncthreads();
   const unsigned begin = s_range[0], end = s_range[1];
-  if (end - begin <= 8 * kThreads) {
-    for (unsigned p = begin + threadIdx.x; p < end; p += kThreads) {
+  if (end - begin <= 8 * kBlock) {
+    for (unsigned p = begin + threadIdx.x; p < end; p += kBlock) {
       const unsigned k = g.keys[p] - v0;
       if (k < slots) atomicOr(&s_named[k / 32], 1u << (k % 32));
     }
@@ -901,7 +901,7 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
   // left in them, 267 and 274), elements at its ends
   constexpr int kVec = 16 / sizeof(O);
   const int pieces = g.dim / kVec + 2, lanes = min(64, pieces);
-  const int groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  const int groups = kBlock / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
   if (group >= groups) return;
   for (unsigned k = group; k < slots; k += groups) {
     if (s_named[k / 32] >> (k % 32) & 1u) continue;
@@ -918,21 +918,10 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
   }
 }
 
-// Rows of more than kNarrow elements: 2^lanes_log lanes hold kVec columns each and walk a chunk pair by pair, kAhead
-// rows in flight.
-template <typename T, typename O, int kVec>
-__global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) {
-  unsigned block;
-  if (g.Fills(&block)) {
-    FillRows(g, block);
-    return;
-  }
-  const unsigned piece = block % g.pieces;
-  unsigned w = ((block / g.pieces) * kThreads + threadIdx.x) >> g.lanes_log;
-  if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);  // (the wave's own: keys and rows are scalar loads then)
-  const int column = (int)(((piece << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
-  if (w >= g.chunks || column >= g.dim) return;
-  const int d = min(column, g.dim - kVec), skip = column - d;
+// The runs of chunk w, columns [d, d + kVec): done(key, begins, ends, sum) for each, whether it begins and ends in
+// the chunk. kAhead rows are in flight, and the pairs of the next step.
+template <int kVec, typename T, typename O, typename Done>
+__device__ __forceinline__ void WalkChunk(const Gradient<T, O> &g, unsigned w, int d, const Done &done) {
   const unsigned begin = w * g.chunk, end = min(g.m, begin + g.chunk);
   unsigned cur = g.keys[begin];
   bool begins = begin == 0 || g.keys[begin - 1] != cur;
@@ -967,7 +956,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (key.v[k] != cur) {
-        g.template Finish<kVec>(cur, w, d, skip, begins, true, sum);
+        done(cur, begins, true, sum);
         cur = key.v[k];
         begins = true;
 #pragma unroll
@@ -977,7 +966,71 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
       for (int c = 0; c < kVec; ++c) sum[c] += row.v[k] < g.n ? static_cast<float>(x[k].v[c]) : 0.0f;
     }
   }
-  g.template Finish<kVec>(cur, w, d, skip, begins, end == g.m || g.keys[end] != cur, sum);
+  done(cur, begins, end == g.m || g.keys[end] != cur, sum);
+}
+
+// Rows of more than kNarrow elements: 2^lanes_log lanes hold kVec columns each and walk a chunk pair by pair.
+template <typename T, typename O, int kVec>
+__global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) {
+  unsigned block;
+  if (g.Fills(&block)) {
+    FillRows<kThreads>(g, block);
+    return;
+  }
+  const unsigned piece = block % g.pieces;
+  unsigned w = ((block / g.pieces) * kThreads + threadIdx.x) >> g.lanes_log;
+  if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);  // (the wave's own: keys and rows are scalar loads then)
+  const int column = (int)(((piece << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
+  if (w >= g.chunks || column >= g.dim) return;
+  const int d = min(column, g.dim - kVec);
+  WalkChunk<kVec>(g, w, d, [&](unsigned v, bool begins, bool ends, const float (&sum)[kVec]) {
+    g.template Finish<kVec>(v, w, d, column - d, begins, ends, sum);
+  });
+}
+
+// The same for so few pairs that one workgroup holds all chunks of a piece: the parts of runs that go on meet in the
+// LDS, and there is no second launch (64 pairs x 64: 5.8 us; with it 6.2 and 2.2, and 3.5 more of the host).
+constexpr int kFewThreads = 1024;
+constexpr unsigned kFewPairs = 512;
+template <typename T, typename O, int kVec>
+__global__ void __launch_bounds__(kFewThreads) k_grad_few(const Gradient<T, O> g) {
+  unsigned block;
+  if (g.Fills(&block)) {
+    FillRows<kFewThreads>(g, block);
+    return;
+  }
+  __shared__ float s_part[kVec][kFewThreads];  // of the run that comes in
+  unsigned w = threadIdx.x >> g.lanes_log;
+  if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);
+  const int column = (int)(((block << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
+  const int d = min(column, g.dim - kVec);
+  const bool live = w < g.chunks && column < g.dim;
+  unsigned goes_on = g.vocab;  // key of the run that goes on
+  float rest[kVec];
+#pragma unroll
+  for (int c = 0; c < kVec; ++c) rest[c] = 0.0f;
+  if (live) {
+    WalkChunk<kVec>(g, w, d, [&](unsigned v, bool begins, bool ends, const float (&sum)[kVec]) {
+      if (v >= g.vocab) return;
+      if (begins && ends) {
+        g.template Write<kVec>(v, d, column - d, sum);
+      } else if (begins) {
+        goes_on = v;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) rest[c] = sum[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) s_part[c][threadIdx.x] = sum[c];
+      }
+    });
+  }
+  __syncthreads();
+  if (goes_on >= g.vocab) return;
+  for (unsigned x = w + 1; x < g.chunks && g.keys[x * g.chunk] == goes_on; ++x) {
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) rest[c] += s_part[c][threadIdx.x + ((x - w) << g.lanes_log)];
+  }
+  g.template Write<kVec>(goes_on, d, column - d, rest);
 }
 
 __device__ __forceinline__ float WaveSum(float v) {
@@ -991,7 +1044,7 @@ template <typename T, typename O, int kDim>
 __global__ void __launch_bounds__(kThreads) k_grad_narrow(const Gradient<T, O> g) {
   unsigned block;
   if (g.Fills(&block)) {
-    FillRows(g, block);
+    FillRows<kThreads>(g, block);
     return;
   }
   const unsigned w = __builtin_amdgcn_readfirstlane((block * kThreads + threadIdx.x) >> 6);
@@ -1168,7 +1221,7 @@ unsigned ChunkOf(unsigned m, int dim) {
   const bool wide = dim > kNarrow;
   const unsigned most = wide ? 256 : 1024;
   const unsigned long long per_64 = wide ? (dim + 7) / 8 : 64;  // waves of 64 chunks
-  unsigned c = wide ? 16 : 64;
+  unsigned c = wide ? 16 : m <= most ? most : 64;  // (few narrow pairs: one wave, and nothing to join)
   while ((c < most && m / c * per_64 / 64 > (wide ? 4096 : 16384)) || m / c * per_64 / 64 > (1 << 22)) c *= 2;
   return c;
 }
@@ -1344,6 +1397,13 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       const unsigned vectors = (unsigned)(a.dim + kVec - 1) / kVec;
       g.lanes_log = std::min(LogAtLeast(vectors), 6);
       g.pieces = (vectors + (1u << g.lanes_log) - 1) >> g.lanes_log;
+      const unsigned walkers = kFewThreads >> g.lanes_log;
+      if (m > 0 && m <= std::min(kFewPairs, 32 * walkers)) {
+        g.chunk = (m + walkers - 1) / walkers;
+        g.chunks = (m + g.chunk - 1) / g.chunk;
+        hipLaunchKernelGGL((k_grad_few<T, O, kVec>), dim3(g.pieces + g.fill_blocks), dim3(kFewThreads), 0, st, g);
+        return;
+      }
       const unsigned long long blocks =
           ((((unsigned long long)g.chunks << g.lanes_log) + kThreads - 1) / kThreads) * g.pieces + g.fill_blocks;
       if (blocks > 0) hipLaunchKernelGGL((k_grad_wide<T, O, kVec>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g);

@@ -651,3 +651,24 @@ def test_adamw_with_other_betas(arb, beta1, beta2):
             within(dev[0], want[0], bound[0], torch.float32)
             for k in (1, 2):
                 assert ((dev[k + 1].cpu().double() - want[k]).abs() <= bound[k] + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [9, 64, 260, 1100])
+@pytest.mark.parametrize("m", [2, 31, 63, 64, 65, 256, 511, 512, 513])
+def test_gradient_of_few_pairs(arb, m, dim, dtype):
+    # runs of every length within and across the chunks that one workgroup holds
+    gen = torch.Generator().manual_seed(m + dim)
+    T = TYPES[dtype]
+    for lengths in ([m], [1] * m, [m // 2, m - m // 2], [1, m - 1], [m - 1, 1], [3] * (m // 3) + [m % 3]):
+        tokens = torch.repeat_interleave(torch.arange(len(lengths)) * 2, torch.tensor(lengths))[torch.randperm(m, generator=gen)]
+        vocab = 2 * len(lengths) + 1
+        held = tokens.to(torch.int32).cuda()
+        grad_out = torch.randn(m, dim, generator=gen).to(T)
+        s = Sorted(arb, held, m, 1, vocab, (1, 1))
+        got = s.grad(grad_out.cuda(), torch.full((vocab, dim), float("nan"), dtype=T, device="cuda"))
+        want, mag, terms = grad_64(grad_out, tokens[:, None], vocab, 1.0)
+        within(got, want, (terms + 3) * U * mag, T)
+        old = torch.randn(vocab, dim, generator=gen).to(T)
+        got = s.grad(grad_out.cuda(), old.cuda(), accumulate=True)
+        within(got, want + old.double(), (terms + 3) * U * mag + 2 * U * (want.abs() + old.double().abs()), T)
