@@ -920,57 +920,80 @@ __device__ __forceinline__ void FillRows(const Gradient<T, O> &g, unsigned block
 
 // The runs of chunk w, columns [d, d + kVec): done(key, begins, ends, sum) for each, whether it begins and ends in
 // the chunk. kAhead rows are in flight, and the pairs of the next step.
-template <int kVec, typename T, typename O, typename Done>
+// kWave: the chunk is the whole wave's, and its keys and rows, which nobody writes meanwhile, are scalar loads.
+template <bool kWave>
+struct PairsAt {
+  typedef const unsigned *Pointer;
+};
+template <>
+struct PairsAt<true> {
+  typedef const __attribute__((address_space(4))) unsigned *Pointer;
+};
+template <int kVec, bool kWave, typename T, typename O, typename Done>
 __device__ __forceinline__ void WalkChunk(const Gradient<T, O> &g, unsigned w, int d, const Done &done) {
+  typedef typename PairsAt<kWave>::Pointer Pointer;
+  const Pointer keys = (Pointer)g.keys, rows = (Pointer)g.rows;
   const unsigned begin = w * g.chunk, end = min(g.m, begin + g.chunk);
-  unsigned cur = g.keys[begin];
-  bool begins = begin == 0 || g.keys[begin - 1] != cur;
+  unsigned cur = keys[begin];
+  bool begins = begin == 0 || keys[begin - 1] != cur;
   float sum[kVec];
 #pragma unroll
   for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
   const T *from = g.grad_out + d;
-  Pack<unsigned, kAhead> key, row, next_key, next_row;
+  unsigned key[kAhead], row[kAhead], next_key[kAhead], next_row[kAhead];
   auto pairs = [&](unsigned p) {
     if (p + kAhead <= end) {
-      next_key = *reinterpret_cast<const Pack<unsigned, kAhead> *>(g.keys + p);
-      next_row = *reinterpret_cast<const Pack<unsigned, kAhead> *>(g.rows + p);
+      typedef Pack<unsigned, kAhead> Some;
+      if constexpr (kWave) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          next_key[k] = keys[p + k];
+          next_row[k] = rows[p + k];
+        }
+      } else {
+        *reinterpret_cast<Some *>(next_key) = *reinterpret_cast<const Some *>(keys + p);
+        *reinterpret_cast<Some *>(next_row) = *reinterpret_cast<const Some *>(rows + p);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {  // past the end the last key stands, without a row
         const unsigned at = min(p + k, end - 1);
-        next_key.v[k] = g.keys[at];
-        next_row.v[k] = p + k < end ? g.rows[at] : g.n;
+        next_key[k] = keys[at];
+        next_row[k] = p + k < end ? rows[at] : g.n;
       }
     }
   };
   pairs(begin);
   for (unsigned p = begin; p < end; p += kAhead) {
-    key = next_key;
-    row = next_row;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      key[k] = next_key[k];
+      row[k] = next_row[k];
+    }
     // every load is asked for: what a pair has no row for is the last one's, and not added
     Pack<T, kVec> x[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      x[k] = *reinterpret_cast<const Pack<T, kVec> *>(from + (long long)min(row.v[k], g.n - 1u) * g.out_stride);
+      x[k] = *reinterpret_cast<const Pack<T, kVec> *>(from + (long long)min(row[k], g.n - 1u) * g.out_stride);
     if (p + kAhead < end) pairs(p + kAhead);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (key.v[k] != cur) {
+      if (key[k] != cur) {
         done(cur, begins, true, sum);
-        cur = key.v[k];
+        cur = key[k];
         begins = true;
 #pragma unroll
         for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
       }
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) sum[c] += row.v[k] < g.n ? static_cast<float>(x[k].v[c]) : 0.0f;
+      for (int c = 0; c < kVec; ++c) sum[c] += row[k] < g.n ? static_cast<float>(x[k].v[c]) : 0.0f;
     }
   }
-  done(cur, begins, end == g.m || g.keys[end] != cur, sum);
+  done(cur, begins, end == g.m || keys[end] != cur, sum);
 }
 
 // Rows of more than kNarrow elements: 2^lanes_log lanes hold kVec columns each and walk a chunk pair by pair.
-template <typename T, typename O, int kVec>
+template <typename T, typename O, int kVec, bool kWave>
 __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) {
   unsigned block;
   if (g.Fills(&block)) {
@@ -978,12 +1001,13 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
     return;
   }
   const unsigned piece = block % g.pieces;
-  unsigned w = ((block / g.pieces) * kThreads + threadIdx.x) >> g.lanes_log;
-  if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);  // (the wave's own: keys and rows are scalar loads then)
-  const int column = (int)(((piece << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
+  const int lanes_log = kWave ? 6 : g.lanes_log;
+  unsigned w = ((block / g.pieces) * kThreads + threadIdx.x) >> lanes_log;
+  if constexpr (kWave) w = __builtin_amdgcn_readfirstlane(w);
+  const int column = (int)(((piece << lanes_log) + (threadIdx.x & ((1u << lanes_log) - 1u))) * kVec);
   if (w >= g.chunks || column >= g.dim) return;
   const int d = min(column, g.dim - kVec);
-  WalkChunk<kVec>(g, w, d, [&](unsigned v, bool begins, bool ends, const float (&sum)[kVec]) {
+  WalkChunk<kVec, kWave>(g, w, d, [&](unsigned v, bool begins, bool ends, const float (&sum)[kVec]) {
     g.template Finish<kVec>(v, w, d, column - d, begins, ends, sum);
   });
 }
@@ -1000,8 +1024,7 @@ __global__ void __launch_bounds__(kFewThreads) k_grad_few(const Gradient<T, O> g
     return;
   }
   __shared__ float s_part[kVec][kFewThreads];  // of the run that comes in
-  unsigned w = threadIdx.x >> g.lanes_log;
-  if (g.lanes_log == 6) w = __builtin_amdgcn_readfirstlane(w);
+  const unsigned w = threadIdx.x >> g.lanes_log;
   const int column = (int)(((block << g.lanes_log) + (threadIdx.x & ((1u << g.lanes_log) - 1u))) * kVec);
   const int d = min(column, g.dim - kVec);
   const bool live = w < g.chunks && column < g.dim;
@@ -1010,7 +1033,7 @@ __global__ void __launch_bounds__(kFewThreads) k_grad_few(const Gradient<T, O> g
 #pragma unroll
   for (int c = 0; c < kVec; ++c) rest[c] = 0.0f;
   if (live) {
-    WalkChunk<kVec>(g, w, d, [&](unsigned v, bool begins, bool ends, const float (&sum)[kVec]) {
+    WalkChunk<kVec, false>(g, w, d, [&](unsigned v, bool begins, bool ends, const float (&sum)[kVec]) {
       if (v >= g.vocab) return;
       if (begins && ends) {
         g.template Write<kVec>(v, d, column - d, sum);
@@ -1149,10 +1172,9 @@ __device__ __forceinline__ bool GoesOn(const Gradient<T, O> &g, unsigned w, unsi
 // The parts of the runs that go on, added up: every wave asks for a chunk of its own and sums the run that begins
 // there, 2^lanes_log lanes side by side over the columns (four each) and the others over the parts.  A run of many
 // parts is left to all waves of the workgroup.
-constexpr int kJoinThreads = 256;
 constexpr int kJoinVec = 4;
 constexpr unsigned kManyParts = 8;  // of a lane
-template <typename T, typename O>
+template <int kJoinThreads, typename T, typename O>
 __global__ void __launch_bounds__(kJoinThreads) k_grad_join(const Gradient<T, O> g, int lanes_log) {
   constexpr unsigned kWaves = kJoinThreads / 64;
   __shared__ float s_sum[kWaves][64][kJoinVec];
@@ -1406,7 +1428,9 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       }
       const unsigned long long blocks =
           ((((unsigned long long)g.chunks << g.lanes_log) + kThreads - 1) / kThreads) * g.pieces + g.fill_blocks;
-      if (blocks > 0) hipLaunchKernelGGL((k_grad_wide<T, O, kVec>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g);
+      const dim3 grid((unsigned)blocks), block(kThreads);
+      if (blocks > 0 && g.lanes_log == 6) hipLaunchKernelGGL((k_grad_wide<T, O, kVec, true>), grid, block, 0, st, g);
+      else if (blocks > 0) hipLaunchKernelGGL((k_grad_wide<T, O, kVec, false>), grid, block, 0, st, g);
     } else {
       const unsigned wave_blocks = (g.chunks + kThreads / 64 - 1) / (kThreads / 64), blocks = wave_blocks + g.fill_blocks;
       auto run = [&](auto width) {
@@ -1420,11 +1444,18 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       }
     }
     if (g.chunks > 1) {
-      constexpr unsigned kWaves = kJoinThreads / 64;
       const int lanes_log = std::min(LogAtLeast((a.dim + kJoinVec - 1) / kJoinVec), 6);
       const int pieces = (a.dim + 64 * kJoinVec - 1) / (64 * kJoinVec);
-      hipLaunchKernelGGL((k_grad_join<T, O>), dim3((g.chunks + kWaves - 1) / kWaves, std::min(pieces, 16)), dim3(kJoinThreads), 0, st, g,
-                         lanes_log);
+      auto join = [&](auto threads) {
+        constexpr unsigned kJoin = decltype(threads)::value, kWaves = kJoin / 64;
+        hipLaunchKernelGGL((k_grad_join<kJoin, T, O>), dim3((g.chunks + kWaves - 1) / kWaves, std::min(pieces, 16)), dim3(kJoin), 0, st, g,
+                           lanes_log);
+      };
+      // few chunks: the longest run is what takes time, and eight waves share it (100,000 pairs x 256, one token in
+      // sixteen the same: 22 us, 37 by four); many: the workgroups that find nothing to do (50 M narrow pairs: 27 us
+      // by four, 32 by eight)
+      if (g.chunks < 32768) join(std::integral_constant<int, 512>());
+      else join(std::integral_constant<int, 256>());
     }
   };
   WithType(a.type, [&](auto t) {
