@@ -767,8 +767,9 @@ SortPlan PlanSort(long long n, int bag, long long vocab) {
   s.m = (unsigned)(n * bag);
   if (s.m == 0) return s;
   if (s.m <= kMostRangePairs) {
-    // 256 keys a workgroup are one pass
-    s.ranges = (unsigned)std::min<long long>(vocab / 256 + 1, kMostRanges);
+    // 256 keys a workgroup are one pass; where there are fewer keys than that for so many pairs, 256 pairs a workgroup
+    const long long wanted = std::max<long long>(vocab / 256 + 1, s.m / 256);
+    s.ranges = (unsigned)std::min({wanted, vocab + 1, (long long)kMostRanges});
     s.span = (unsigned)(vocab / s.ranges + 1);
     s.key_bits = BitsOf(s.span - 1);
     s.place_bits = BitsOf(s.m - 1);
@@ -1408,10 +1409,14 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
     g.chunk = ChunkOf(m, a.dim);
     g.chunks = (m + g.chunk - 1) / g.chunk;
     g.parts = static_cast<float *>(a.work);
-    g.slots = (unsigned)std::min<size_t>(std::max<size_t>(16384 / (a.dim * sizeof(O)), 1), kMostSlots);
-    while (g.slots < kMostSlots && a.vocab / g.slots > (1 << 22)) g.slots *= 2;  // (a launch counts its threads with 32 bits)
-    g.slots = std::min(g.slots, kMostSlots);
-    g.fill_blocks = a.accumulate ? 0 : (unsigned)((a.vocab + g.slots - 1) / g.slots);
+    // rows of zeros a workgroup: 16 KB of them for every four waves (more where a launch would count its threads beyond 32 bits)
+    auto fill = [&](int threads) {
+      g.slots = (unsigned)std::min<size_t>(std::max<size_t>(64 * threads / (a.dim * sizeof(O)), 1), kMostSlots);
+      while (g.slots < kMostSlots && a.vocab / g.slots > (1 << 22) / (threads / kThreads)) g.slots *= 2;
+      g.slots = std::min(g.slots, kMostSlots);
+      g.fill_blocks = a.accumulate ? 0 : (unsigned)((a.vocab + g.slots - 1) / g.slots);
+    };
+    fill(kThreads);
     g.lanes_log = 6;
     g.pieces = 1;
     if (a.dim > kNarrow) {
@@ -1421,6 +1426,7 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       g.pieces = (vectors + (1u << g.lanes_log) - 1) >> g.lanes_log;
       const unsigned walkers = kFewThreads >> g.lanes_log;
       if (m > 0 && m <= std::min(kFewPairs, 32 * walkers)) {
+        fill(kFewThreads);
         g.chunk = (m + walkers - 1) / walkers;
         g.chunks = (m + g.chunk - 1) / g.chunk;
         hipLaunchKernelGGL((k_grad_few<T, O, kVec>), dim3(g.pieces + g.fill_blocks), dim3(kFewThreads), 0, st, g);
