@@ -488,14 +488,12 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
 
 // ---- many pairs: least significant digit first
 //
-// Up to 9 bits a pass (two passes up to a vocabulary of 262,143), three or four launches each.  A tile of 8192 pairs is put
-// in order in the LDS, so that the pairs of a digit leave as one run.
+// Up to 9 bits a pass (two passes up to a vocabulary of 262,143), four launches each, and two where 32 tiles hold all
+// pairs.  A tile of up to 8192 pairs is put in order in the LDS, so that the pairs of a digit leave as one run.
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kSortRounds = 8;                         // pairs per thread
-constexpr int kSortTile = kSortThreads * kSortRounds;  // 8192
-constexpr int kWavePairs = kSortTile / kSortWaves;
+constexpr int kSortRounds = 8, kFewestRounds = 2;  // pairs per thread
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr unsigned kXcds = 8;
@@ -551,17 +549,17 @@ struct Digit {
   __device__ __forceinline__ unsigned Of(unsigned key) const { return (key >> shift) & mask; }
 };
 
-// Digit counts of one tile: counts[tile * kDigits + digit].  A thread's pairs lie beside each other and equal
-// neighbours are counted as one, and a wave of one digit only as one: pairs that are nearly in order (leaves, tree by
-// tree; the last pass) would otherwise queue for one counter of the LDS.
-template <typename Source>
+// Digit counts of one tile (kPairs pairs a thread): counts[tile * kDigits + digit].  A thread's pairs lie beside each
+// other and equal neighbours are counted as one, and a wave of one digit only as one: pairs that are nearly in order
+// (leaves, tree by tree; the last pass) would otherwise queue for one counter of the LDS.
+template <int kPairs, typename Source>
 __global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, const Digit digit, unsigned *__restrict__ counts) {
-  constexpr int kBeside = 4, kRounds = kSortRounds / kBeside;
+  constexpr int kBeside = kPairs < 4 ? kPairs : 4, kRounds = kPairs / kBeside;
   __shared__ unsigned s_count[kDigits];
   const unsigned tile = blockIdx.x;
   if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
   __syncthreads();
-  const unsigned base = tile * kSortTile + threadIdx.x * kBeside;
+  const unsigned base = tile * (kSortThreads * kPairs) + threadIdx.x * kBeside;
   typename Source::Raw raw[kRounds][kBeside];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) in.Beside(base + r * kSortThreads * kBeside, raw[r]);
@@ -575,7 +573,10 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_count(const Source in, co
     for (int k = 0; k < kBeside; ++k) d[k] = p + k < in.m ? digit.Of(in.Key(raw[r][k])) : kDigits;
     d[kBeside] = kDigits + 1;
     const unsigned one = __builtin_amdgcn_readfirstlane(d[0]);
-    if (__ballot(d[0] != one || d[1] != one || d[2] != one || d[3] != one) == 0ull) {
+    bool other = false;
+#pragma unroll
+    for (int k = 0; k < kBeside; ++k) other |= d[k] != one;
+    if (__ballot(other) == 0ull) {
       if ((threadIdx.x & 63u) == 0 && one < kDigits) atomicAdd(&s_count[one], 64u * kBeside);
       continue;
     }
@@ -634,12 +635,14 @@ __global__ void __launch_bounds__(1024) k_sort_sum_groups(unsigned *__restrict__
   if (wave == 0) groups[(size_t)count * kDigits + digit] = total;
 }
 
-// Stable scatter of one tile.  counts, groups: pairs of the same digit in the tiles of the group before, in the
-// groups before; totals: pairs of each digit.
-template <typename Source>
-__global__ void __launch_bounds__(kSortThreads, 8)  // (8 waves a SIMD: two workgroups on a CU)
-k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ counts, const unsigned *__restrict__ groups,
+// Stable scatter of one tile of kPairs pairs a thread.  counts, groups: pairs of the same digit in the tiles of the
+// group before, in the groups before; totals: pairs of each digit.  kFew: a single group, counts are those of each
+// tile, and every workgroup sums them up for itself.
+template <int kPairs, bool kFew, typename Source>
+__global__ void __launch_bounds__(kSortThreads, kFew ? 4 : 8)  // (8 waves a SIMD: two workgroups on a CU)
+k_sort_scatter(const Source in, const Digit digit, unsigned tiles, const unsigned *__restrict__ counts, const unsigned *__restrict__ groups,
                const unsigned *__restrict__ totals, unsigned *__restrict__ keys, unsigned *__restrict__ rows) {
+  constexpr unsigned kSortTile = kSortThreads * kPairs, kWavePairs = kPairs * 64;
   __shared__ unsigned s_pair[kSortTile];                  // the keys, then the rows
   __shared__ unsigned short s_wave[kSortWaves][kDigits];  // pairs of each digit of a wave; then those of the waves before
   __shared__ unsigned s_first[kDigits];                   // place in the tile of the first pair of each digit
@@ -648,24 +651,34 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   // Workgroups are dealt to the eight XCDs in turn.  Tiles that follow each other, whose runs of a digit meet inside
   // a line of memory, go to the same one (50 M pairs: 214 -> 199 us).
-  const unsigned tile = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
-  if (tile * (unsigned long long)kSortTile >= in.m) return;
-  const unsigned base = tile * kSortTile, held = min((unsigned)kSortTile, in.m - base);
+  const unsigned tile = kFew ? blockIdx.x : blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  if (tile >= tiles) return;
+  const unsigned base = tile * kSortTile, held = min(kSortTile, in.m - base);
   for (int i = threadIdx.x; i < kSortWaves * kDigits / 2; i += kSortThreads) reinterpret_cast<unsigned *>(s_wave)[i] = 0;
-  typename Source::Raw raw[kSortRounds];
-  unsigned key[kSortRounds], place[kSortRounds];
+  typename Source::Raw raw[kPairs];
+  unsigned key[kPairs], place[kPairs];
   in.Get(base + wave * kWavePairs + lane, 64, raw);
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) key[k] = in.Key(raw[k]);  // (past the end: the last one's, which goes nowhere)
+  for (int k = 0; k < kPairs; ++k) key[k] = in.Key(raw[k]);  // (past the end: the last one's, which goes nowhere)
   unsigned total = 0, before = 0;
   if (threadIdx.x <= digit.mask) {
-    total = totals[threadIdx.x];
-    before = counts[(size_t)tile * kDigits + threadIdx.x];
-    if (groups != nullptr) before += groups[(size_t)(tile / kGroupTiles) * kDigits + threadIdx.x];
+    if (kFew) {
+      unsigned c[kGroupTiles];
+#pragma unroll
+      for (unsigned k = 0; k < kGroupTiles; ++k) c[k] = counts[min(k, tiles - 1) * kDigits + threadIdx.x];
+#pragma unroll
+      for (unsigned k = 0; k < kGroupTiles; ++k) {
+        total += k < tiles ? c[k] : 0u;
+        before += k < tile ? c[k] : 0u;
+      }
+    } else {
+      total = totals[threadIdx.x];
+      before = counts[(size_t)tile * kDigits + threadIdx.x] + groups[(size_t)(tile / kGroupTiles) * kDigits + threadIdx.x];
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
+  for (int k = 0; k < kPairs; ++k) {
     const bool valid = wave * kWavePairs + k * 64 + lane < held;
     const unsigned d = digit.Of(key[k]);
     // (the last pass finds most waves in order: one digit)
@@ -711,7 +724,7 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
+  for (int k = 0; k < kPairs; ++k) {
     if (wave * kWavePairs + k * 64 + lane < held) {
       const unsigned d = digit.Of(key[k]);
       place[k] += s_first[d] + s_wave[wave][d];
@@ -719,9 +732,9 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
     }
   }
   __syncthreads();
-  unsigned to[kSortRounds];
+  unsigned to[kPairs];
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
+  for (int k = 0; k < kPairs; ++k) {
     const unsigned i = k * kSortThreads + threadIdx.x;
     if (i < held) {
       const unsigned v = s_pair[i], d = digit.Of(v);
@@ -731,13 +744,13 @@ k_sort_scatter(const Source in, const Digit digit, const unsigned *__restrict__ 
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
+  for (int k = 0; k < kPairs; ++k) {
     const unsigned i = wave * kWavePairs + k * 64 + lane;
     if (i < held) s_pair[place[k]] = in.Row(base + i);
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kSortRounds; ++k) {
+  for (int k = 0; k < kPairs; ++k) {
     const unsigned i = k * kSortThreads + threadIdx.x;
     if (i < held) rows[to[k]] = s_pair[i];
   }
@@ -756,6 +769,7 @@ struct SortPlan {
   unsigned ranges, span;
   int key_bits, place_bits;
   int passes, bits;  // many pairs
+  int pairs;         // of a thread
   unsigned tiles, groups;
   size_t counts_bytes, groups_bytes, pairs_bytes, bytes;
 };
@@ -779,7 +793,12 @@ SortPlan PlanSort(long long n, int bag, long long vocab) {
   const int bits = BitsOf((unsigned long long)vocab);
   s.passes = (bits + kDigitBits - 1) / kDigitBits;
   s.bits = (bits + s.passes - 1) / s.passes;
-  s.tiles = (s.m + kSortTile - 1) / kSortTile;
+  // small tiles, as long as they stay one group: a tile's work is one thing after the other (38,252 pairs, two passes:
+  // 37 us with tiles of 8192 and the sums in a launch of their own, 20 with tiles of 2048 that take the sums themselves)
+  s.pairs = kSortRounds;
+  while (s.pairs > kFewestRounds && s.m <= s.pairs / 2 * kSortThreads * kGroupTiles) s.pairs /= 2;
+  const unsigned tile = s.pairs * kSortThreads;
+  s.tiles = (s.m + tile - 1) / tile;
   s.groups = (s.tiles + kGroupTiles - 1) / kGroupTiles;
   s.counts_bytes = Align256((size_t)s.tiles * kDigits * sizeof(unsigned));
   s.groups_bytes = (size_t)(s.groups + 1) * kDigits * sizeof(unsigned);
@@ -1328,7 +1347,9 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
                            plan.key_bits, plan.place_bits, a.keys, a.rows);
       };
       if (plan.m <= 1 * kRangeThreads) launch(std::integral_constant<int, 1>());
+      else if (plan.m <= 4 * kRangeThreads) launch(std::integral_constant<int, 4>());
       else if (plan.m <= 8 * kRangeThreads) launch(std::integral_constant<int, 8>());
+      else if (plan.m <= 16 * kRangeThreads) launch(std::integral_constant<int, 16>());
       else launch(std::integral_constant<int, 32>());
     });
     HIP_OK(hipGetLastError());
@@ -1347,13 +1368,26 @@ void EmbeddingSort(const EmbeddingSortArgs &a) {
     const Digit digit{pass * plan.bits, plan.bits, (1u << plan.bits) - 1u};
     auto launch = [&](const auto &in) {
       typedef std::decay_t<decltype(in)> Source;
-      hipLaunchKernelGGL((k_sort_count<Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts);
-      hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
-      const bool several = plan.groups > 1;  // (the totals of the only group are those of all)
-      if (several) hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
-      const unsigned *before = several ? groups : nullptr, *totals = several ? groups + (size_t)plan.groups * kDigits : groups;
-      hipLaunchKernelGGL((k_sort_scatter<Source>), dim3((plan.tiles + kXcds - 1) / kXcds * kXcds), dim3(kSortThreads), 0, st, in, digit,
-                         counts, before, totals, to[0], to[1]);
+      auto few = [&](auto pairs) {
+        constexpr int kPairs = decltype(pairs)::value;
+        hipLaunchKernelGGL((k_sort_count<kPairs, Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts);
+        hipLaunchKernelGGL((k_sort_scatter<kPairs, true, Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, plan.tiles,
+                           counts, nullptr, nullptr, to[0], to[1]);
+      };
+      if (plan.groups > 1) {
+        hipLaunchKernelGGL((k_sort_count<kSortRounds, Source>), dim3(plan.tiles), dim3(kSortThreads), 0, st, in, digit, counts);
+        hipLaunchKernelGGL(k_sort_sum_tiles, dim3(plan.groups), dim3(kDigits), 0, st, counts, plan.tiles, groups);
+        hipLaunchKernelGGL(k_sort_sum_groups, dim3(kDigits / 64), dim3(1024), 0, st, groups, plan.groups);
+        hipLaunchKernelGGL((k_sort_scatter<kSortRounds, false, Source>), dim3((plan.tiles + kXcds - 1) / kXcds * kXcds),
+                           dim3(kSortThreads), 0, st, in, digit, plan.tiles, counts, groups, groups + (size_t)plan.groups * kDigits, to[0],
+                           to[1]);
+      } else if (plan.pairs == 2) {
+        few(std::integral_constant<int, 2>());
+      } else if (plan.pairs == 4) {
+        few(std::integral_constant<int, 4>());
+      } else {
+        few(std::integral_constant<int, 8>());
+      }
     };
     if (pass > 0) {
       launch(FromPairs{from[0], from[1], plan.m});
@@ -1409,7 +1443,8 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
     g.chunk = ChunkOf(m, a.dim);
     g.chunks = (m + g.chunk - 1) / g.chunk;
     g.parts = static_cast<float *>(a.work);
-    // rows of zeros a workgroup: 16 KB of them for every four waves (more where a launch would count its threads beyond 32 bits)
+    // rows of zeros a workgroup: 16 KB of them for every four waves (more where a launch would count its threads
+    // beyond 32 bits)
     auto fill = [&](int threads) {
       g.slots = (unsigned)std::min<size_t>(std::max<size_t>(64 * threads / (a.dim * sizeof(O)), 1), kMostSlots);
       while (g.slots < kMostSlots && a.vocab / g.slots > (1 << 22) / (threads / kThreads)) g.slots *= 2;

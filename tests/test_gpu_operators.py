@@ -672,3 +672,24 @@ def test_gradient_of_few_pairs(arb, m, dim, dtype):
         old = torch.randn(vocab, dim, generator=gen).to(T)
         got = s.grad(grad_out.cuda(), old.cuda(), accumulate=True)
         within(got, want + old.double(), (terms + 3) * U * mag + 2 * U * (want.abs() + old.double().abs()), T)
+
+
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("m", [4095, 4096, 4097, 16_384, 16_385, 32_769, 65_535, 65_536, 65_537, 131_072, 131_073, 262_144, 262_145])
+def test_order_of_pairs_where_the_tiles_change(arb, m, bits):
+    # both sides of every number of pairs from which on the sort takes other tiles or other launches
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    for vocab in (300, 40_000, 300_000):
+        tokens = torch.randint(0, vocab, (m,), generator=gen, device="cuda")
+        tokens[torch.rand(m, generator=gen, device="cuda") < 0.2] = vocab // 2
+        tokens[torch.rand(m, generator=gen, device="cuda") < 0.1] = -1
+        s = Sorted(arb, tokens.to(torch.int32 if bits == 32 else torch.int64), m, 1, vocab, (1, 1), bits=bits)
+        key = torch.where(tokens >= 0, tokens, vocab)
+        assert torch.equal(s.keys.long(), key.sort().values)
+        # every pair once, and pairs of a token in the same order from call to call
+        pair = key * m + torch.arange(m, device="cuda")
+        assert torch.equal((s.keys.long() * m + s.rows.long()).sort().values, pair.sort().values)
+        first = s.pairs.clone()
+        s.pairs.fill_(-7)
+        s.call()
+        assert torch.equal(s.pairs, first)
