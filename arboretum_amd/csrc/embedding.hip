@@ -349,17 +349,24 @@ Pairs<Token> PairsOf(const TokenBags &b, unsigned m) {
   return Pairs<Token>{BagsOf<Token>(b), m, by_column, flat, Divider(by_column ? (unsigned)b.n : (unsigned)b.bag)};
 }
 
-// Lanes of the wave that hold the same digit as this one.
-__device__ __forceinline__ unsigned long long DigitPeers(unsigned d, bool valid, int bits) {
-  const unsigned long long all = __ballot(valid);
-  unsigned low = (unsigned)all, high = (unsigned)(all >> 32);
+// Lanes of the wave that hold the same digit as this one, for kSome digits a lane: low and high come in as the lanes that
+// hold a digit at all.
+template <int kSome>
+__device__ __forceinline__ void DigitPeers(const unsigned (&d)[kSome], int bits, unsigned (&low)[kSome], unsigned (&high)[kSome]) {
   for (int b = 0; b < bits; ++b) {
-    const int set = (int)(d << (31 - b)) >> 31;  // -1 or 0
-    const unsigned long long m = __ballot(set != 0);
-    low &= ~((unsigned)m ^ (unsigned)set);
-    high &= ~((unsigned)(m >> 32) ^ (unsigned)set);
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) {
+      const int set = __builtin_amdgcn_sbfe((int)d[k], b, 1);  // -1 or 0
+      const unsigned long long m = __ballot(set != 0);
+      low[k] &= ~((unsigned)m ^ (unsigned)set);
+      high[k] &= ~((unsigned)(m >> 32) ^ (unsigned)set);
+    }
   }
-  return (unsigned long long)high << 32 | low;
+}
+
+// Lanes below this one in a mask.
+__device__ __forceinline__ unsigned LanesBelow(unsigned low, unsigned high) {
+  return __builtin_amdgcn_mbcnt_hi(high, __builtin_amdgcn_mbcnt_lo(low, 0u));
 }
 
 // ---- few pairs: one launch
@@ -416,7 +423,7 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
   for (int k = 0; k < kRounds; ++k) {
     const bool mine = key[k] - v0 < here;
     const unsigned long long all = __ballot(mine);
-    const unsigned to = at + (unsigned)__popcll(all & ((1ull << lane) - 1ull));
+    const unsigned to = at + LanesBelow((unsigned)all, (unsigned)(all >> 32));
     if (mine) s_pair[to] = (key[k] - v0) << place_bits | (k * kRangeThreads + threadIdx.x);
     at += (unsigned)__popcll(all);
   }
@@ -435,14 +442,16 @@ k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits
         const unsigned i = first + k * 64u + lane;
         const bool valid = i < held;
         pair[k] = valid ? s_pair[i] : 0u;
-        const unsigned d = (pair[k] >> shift) & ((1u << bits) - 1u);
-        const unsigned long long peers = DigitPeers(d, valid, bits);
-        const unsigned less = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
-        unsigned *count = &s_count[d * kRangeWaves + wave];
+        const unsigned d[1] = {(pair[k] >> shift) & ((1u << bits) - 1u)};
+        const unsigned long long all = __ballot(valid);
+        unsigned low[1] = {(unsigned)all}, high[1] = {(unsigned)(all >> 32)};
+        DigitPeers(d, bits, low, high);
+        const unsigned less = LanesBelow(low[0], high[0]);
+        unsigned *count = &s_count[d[0] * kRangeWaves + wave];
         const unsigned before = *count;
         place[k] = before + less;
         __builtin_amdgcn_wave_barrier();  // every lane has read its counter
-        if (valid && less == 0) *count = before + (unsigned)__popcll(peers);
+        if (valid && less == 0) *count = before + __popc(low[0]) + __popc(high[0]);
         __builtin_amdgcn_wave_barrier();
       }
     }
@@ -677,19 +686,29 @@ k_sort_scatter(const Source in, const Digit digit, unsigned tiles, const unsigne
     }
   }
   __syncthreads();
+  {
+    unsigned d[kPairs], low[kPairs], high[kPairs];
+    bool other = false;
 #pragma unroll
-  for (int k = 0; k < kPairs; ++k) {
-    const bool valid = wave * kWavePairs + k * 64 + lane < held;
-    const unsigned d = digit.Of(key[k]);
-    // (the last pass finds most waves in order: one digit)
-    const bool other = valid && d != __builtin_amdgcn_readfirstlane(d);
-    const unsigned long long peers = __ballot(other) == 0ull ? __ballot(valid) : DigitPeers(d, valid, digit.bits);
-    const unsigned less = (unsigned)__popcll(peers & ((1ull << lane) - 1ull));
-    const unsigned held_of = s_wave[wave][d];
-    place[k] = held_of + less;
-    __builtin_amdgcn_wave_barrier();  // every lane has read its counter
-    if (valid && less == 0) s_wave[wave][d] = (unsigned short)(held_of + (unsigned)__popcll(peers));
-    __builtin_amdgcn_wave_barrier();
+    for (int k = 0; k < kPairs; ++k) {
+      const bool valid = wave * kWavePairs + k * 64 + lane < held;
+      const unsigned long long all = __ballot(valid);
+      low[k] = (unsigned)all;
+      high[k] = (unsigned)(all >> 32);
+      d[k] = digit.Of(key[k]);
+      other |= valid && d[k] != __builtin_amdgcn_readfirstlane(d[k]);
+    }
+    if (__ballot(other) != 0ull) DigitPeers(d, digit.bits, low, high);  // (the last pass finds most waves in order: one digit)
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+      const bool valid = wave * kWavePairs + k * 64 + lane < held;
+      const unsigned less = LanesBelow(low[k], high[k]);
+      const unsigned held_of = s_wave[wave][d[k]];
+      place[k] = held_of + less;
+      __builtin_amdgcn_wave_barrier();  // every lane has read its counter
+      if (valid && less == 0) s_wave[wave][d[k]] = (unsigned short)(held_of + __popc(low[k]) + __popc(high[k]));
+      __builtin_amdgcn_wave_barrier();
+    }
   }
   __syncthreads();
   // thread = digit: pairs of smaller digits in the tile, and in all
