@@ -555,7 +555,7 @@ struct FromPairs {
 struct Digit {
   int shift, bits;
   unsigned mask;
-  __device__ __forceinline__ unsigned Of(unsigned key) const { return (key >> shift) & mask; }
+  __device__ __forceinline__ unsigned Of(unsigned key) const { return __builtin_amdgcn_ubfe(key, shift, bits); }
 };
 
 // Digit counts of one tile (kPairs pairs a thread): counts[tile * kDigits + digit].  A thread's pairs lie beside each
@@ -696,7 +696,7 @@ k_sort_scatter(const Source in, const Digit digit, unsigned tiles, const unsigne
       low[k] = (unsigned)all;
       high[k] = (unsigned)(all >> 32);
       d[k] = digit.Of(key[k]);
-      other |= valid && d[k] != __builtin_amdgcn_readfirstlane(d[k]);
+      other |= d[k] != (unsigned)__builtin_amdgcn_readfirstlane(d[k]);
     }
     if (__ballot(other) != 0ull) DigitPeers(d, digit.bits, low, high);  // (the last pass finds most waves in order: one digit)
 #pragma unroll
@@ -742,37 +742,41 @@ k_sort_scatter(const Source in, const Digit digit, unsigned tiles, const unsigne
     s_out[threadIdx.x] = in_all - total + before;
   }
   __syncthreads();
+  // From here on what stands past the end goes along, behind the pairs, up to the stores: no access of the LDS
+  // stands behind a branch.
 #pragma unroll
   for (int k = 0; k < kPairs; ++k) {
-    if (wave * kWavePairs + k * 64 + lane < held) {
-      const unsigned d = digit.Of(key[k]);
-      place[k] += s_first[d] + s_wave[wave][d];
-      s_pair[place[k]] = key[k];
-    }
+    const unsigned i = wave * kWavePairs + k * 64 + lane, d = digit.Of(key[k]);
+    const unsigned to = place[k] + s_first[d] + s_wave[wave][d];
+    place[k] = i < held ? to : i;
   }
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k) s_pair[place[k]] = key[k];
   __syncthreads();
   unsigned to[kPairs];
 #pragma unroll
-  for (int k = 0; k < kPairs; ++k) {
-    const unsigned i = k * kSortThreads + threadIdx.x;
-    if (i < held) {
-      const unsigned v = s_pair[i], d = digit.Of(v);
-      to[k] = s_out[d] + (i - s_first[d]);
-      keys[to[k]] = v;
-    }
-  }
-  __syncthreads();
+  for (int k = 0; k < kPairs; ++k) key[k] = s_pair[k * kSortThreads + threadIdx.x];
 #pragma unroll
   for (int k = 0; k < kPairs; ++k) {
-    const unsigned i = wave * kWavePairs + k * 64 + lane;
-    if (i < held) s_pair[place[k]] = in.Row(base + i);
+    const unsigned d = digit.Of(key[k]);
+    to[k] = s_out[d] - s_first[d] + k * kSortThreads + threadIdx.x;
   }
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k)
+    if (k * kSortThreads + threadIdx.x < held) keys[to[k]] = key[k];
+  __syncthreads();
+  unsigned again = base + wave * kWavePairs + lane;
+  asm volatile("" : "+v"(again));  // worked out anew: kept from the first loads on, the eight places would spill
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k) key[k] = in.Row(min(again + k * 64, in.m - 1));
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k) s_pair[place[k]] = key[k];
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kPairs; ++k) {
-    const unsigned i = k * kSortThreads + threadIdx.x;
-    if (i < held) rows[to[k]] = s_pair[i];
-  }
+  for (int k = 0; k < kPairs; ++k) key[k] = s_pair[k * kSortThreads + threadIdx.x];
+#pragma unroll
+  for (int k = 0; k < kPairs; ++k)
+    if (k * kSortThreads + threadIdx.x < held) rows[to[k]] = key[k];
 }
 
 int BitsOf(unsigned long long v) {
