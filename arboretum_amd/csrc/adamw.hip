@@ -189,7 +189,6 @@ void AdamW(const AdamWArgs &a) {
     for (; at < a.count && l.count < kTensorsAtOnce; ++at) {
       if (a.sizes[at] == 0) continue;
       const unsigned long long more = (unsigned long long)(a.sizes[at] + l.chunk - 1) / l.chunk;
-      
       if (l.count == 0) first = a.params[at];
       l.tensor[l.count] = Tensor{a.params[at], a.grads[at], a.exp_avg[at], a.exp_avg_sq[at], a.sizes[at]};
       l.first[l.count++] = (unsigned)blocks;

@@ -1059,6 +1059,7 @@ __global__ void __launch_bounds__(kThreads) k_grad_wide(const Gradient<T, O> g) 
 // LDS, and there is no second launch (64 pairs x 64: 5.8 us; with it 6.2 and 2.2, and 3.5 more of the host).
 constexpr int kFewThreads = 1024;
 constexpr unsigned kFewPairs = 512;
+constexpr long long kMostFewRows = 1ll << 29;
 template <typename T, typename O, int kVec>
 __global__ void __launch_bounds__(kFewThreads) k_grad_few(const Gradient<T, O> g) {
   unsigned block;
@@ -1483,7 +1484,9 @@ void EmbeddingGrad(const EmbeddingGradArgs &a) {
       g.lanes_log = std::min(LogAtLeast(vectors), 6);
       g.pieces = (vectors + (1u << g.lanes_log) - 1) >> g.lanes_log;
       const unsigned walkers = kFewThreads >> g.lanes_log;
-      if (m > 0 && m <= std::min(kFewPairs, 32 * walkers)) {
+      // (256 rows a workgroup and 1024 threads: a launch counts threads with 32 bits)
+      const bool counts = a.accumulate || a.vocab <= kMostFewRows;
+      if (m > 0 && m <= std::min(kFewPairs, 32 * walkers) && counts) {
         fill(kFewThreads);
         g.chunk = (m + walkers - 1) / walkers;
         g.chunks = (m + g.chunk - 1) / g.chunk;

@@ -679,7 +679,7 @@ def test_gradient_of_few_pairs(arb, m, dim, dtype):
 def test_order_of_pairs_where_the_tiles_change(arb, m, bits):
     # both sides of every number of pairs from which on the sort takes other tiles or other launches
     gen = torch.Generator(device="cuda").manual_seed(m)
-    for vocab in (300, 40_000, 300_000):
+    for vocab in (300, 40_000, 300_000, 2 ** 31 - 1):
         tokens = torch.randint(0, vocab, (m,), generator=gen, device="cuda")
         tokens[torch.rand(m, generator=gen, device="cuda") < 0.2] = vocab // 2
         tokens[torch.rand(m, generator=gen, device="cuda") < 0.1] = -1
@@ -693,3 +693,20 @@ def test_order_of_pairs_where_the_tiles_change(arb, m, bits):
         s.pairs.fill_(-7)
         s.call()
         assert torch.equal(s.pairs, first)
+
+
+def test_few_pairs_of_a_table_of_a_billion_rows(arb):
+    # more rows of zeros than one launch of large workgroups counts
+    vocab, dim = (1 << 30) + 7, 9
+    named = torch.tensor([vocab - 1, 0, 1 << 29, 0])
+    grad_out = torch.arange(1, 1 + 4 * dim).reshape(4, dim).half().cuda()
+    s = Sorted(arb, named.to(torch.int32).cuda(), 4, 1, vocab, (1, 1))
+    got = s.grad(grad_out, torch.full((vocab, dim), float("nan"), dtype=torch.float16, device="cuda"))
+    assert torch.equal(got[vocab - 1], grad_out[0]) and torch.equal(got[1 << 29], grad_out[2])
+    assert torch.equal(got[0], grad_out[1] + grad_out[3])  # (whole numbers: exact)
+    for row in (vocab - 1, 0, 1 << 29):
+        got[row] = 0
+    for i in range(0, vocab, 1 << 26):  # (a NaN counts)
+        assert torch.count_nonzero(got[i:i + (1 << 26)]).item() == 0
+    again = s.grad(grad_out, got, accumulate=True)
+    assert torch.equal(again[vocab - 1], grad_out[0]) and torch.equal(again[0], grad_out[1] + grad_out[3])
