@@ -3,7 +3,7 @@
 //   lookup    out[i]        = scale * sum_j table[token(i, j)]
 //   gradient  grad_table[v] = scale * sum of grad_out[i] over all (i, j) with token(i, j) = v
 //
-// The gradient gathers: the (token, bag) pairs are put in order of tokens first (a stable radix sort), so that every sum is
+// The gradient gathers: the (token, bag) pairs are put in order of tokens first (a radix sort), so that every sum is
 // formed in an order that depends on the tokens alone, and no atomic decides it.
 #include <algorithm>
 #include <type_traits>
