@@ -6,6 +6,7 @@
 // to its own type.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <vector>
 
 #include "operators_device.h"
@@ -150,6 +151,9 @@ void Validate(const AdamWArgs &a) {
   if (!(a.beta1 >= 0 && a.beta1 < 1) || !(a.beta2 >= 0 && a.beta2 < 1)) throw std::runtime_error("beta1 and beta2 must be in [0, 1)");
   if (!std::isfinite(a.lr) || !std::isfinite(a.eps) || !std::isfinite(a.weight_decay) || !std::isfinite(a.grad_scale))
     throw std::runtime_error("lr, eps, weight_decay and grad_scale must be finite");
+  // Elements whose gradient has always been 0 (rows of a table that no token names) have m = v = 0: they stay where they
+  // are as long as the denominator is not 0 and no constant of the kernel is infinite.
+  if ((float)a.eps < std::numeric_limits<float>::min()) throw std::runtime_error("eps must be at least 2^-126");
   if (!a.step_device && a.step < 1) throw std::runtime_error("step counts from 1");
   CheckAligned(a.lr_device, 4, "lr_device");
   CheckAligned(a.step_device, 8, "step_device");
@@ -174,6 +178,9 @@ void AdamW(const AdamWArgs &a) {
   l.log_beta1 = std::log2(a.beta1);  // (of 0: minus infinity, and its powers are 0)
   l.log_beta2 = std::log2(a.beta2);
   SetStep(&l.s, a.lr, a.weight_decay, l.log_beta1, l.log_beta2, (double)std::max(a.step, 1ll));
+  const bool words = a.lr_device || a.step_device;  // (what the kernel then works out is not known here)
+  if (!std::isfinite(l.s.eps) || !std::isfinite(l.s.grad_scale) || (!words && (!std::isfinite(l.s.step_size) || !std::isfinite(l.s.decay))))
+    throw std::runtime_error("a constant of the step is beyond float32");
   l.step = a.step;
   l.lr_device = a.lr_device;
   l.step_device = a.step_device;
