@@ -281,13 +281,21 @@ void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
   if (cfg.objective < kSoftMaxOneVsAll && cfg.tree.labels_count > 1) throw std::runtime_error("several classes need a soft-max objective");
   CheckTarget(data);
   if (cfg.objective < kSoftMaxOneVsAll && !data->y_facts.finite) throw std::runtime_error("y must be finite");
-  const size_t use = CheckLeafWalk(data, -1), K = cfg.tree.labels_count, n = data->rows;
+  const size_t K = cfg.tree.labels_count, n = data->rows;
+  if (cfg.objective >= kSoftMaxOneVsAll && K < 2) throw std::runtime_error("soft-max needs labels_count >= 2");
+  SyncTrees();
+  // Loaded trees all have the label 0, as in the reference: what class they were of is not known.  (Every round grows
+  // a tree of each class, so a booster of several classes has as many of each if and only if it grew them all.)
   std::vector<size_t> trees_of(K, 0);
+  for (const RegTree &t : trees_)
+    if (t.label < K) ++trees_of[t.label];
+  for (size_t count : trees_of)
+    if (count != trees_of[0]) throw std::runtime_error("refinement needs as many trees of each class: the trees of a loaded model have none");
+  const size_t use = CheckLeafWalk(data, -1);
   std::vector<std::vector<float>> tables(K);
   for (size_t k = 0; k < K; ++k)
     for (const RegTree &t : trees_) {
       if (t.label != k) continue;
-      ++trees_of[k];
       tables[k].insert(tables[k].end(), t.weights.begin(), t.weights.end());
     }
   for (size_t k = 0; k < K; ++k)

@@ -267,16 +267,18 @@ const char *AAdamW(int count, void *const *params, const void *const *grads, flo
  * DEVICE memory for 32-bit words of which nothing pending may make use, stride >= rows.  The trees of a class
  * stand together (by class, then in the order they grew), and the leaves are numbered through the trees of a
  * class: a class' columns are bags of tokens over a table of leaves[class] rows (a host array of `classes` counts,
- * the booster's labels_count; may be NULL), token_stride 1 and bag_stride `stride`.  Waits for the result. */
+ * the booster's labels_count; may be NULL), token_stride 1 and bag_stride `stride`.  Loaded trees all count as the
+ * first class', as they do for APredict.  Waits for the result. */
 const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens, long long stride, int n_rounds,
                               long long *leaves, int classes);
 
 /* Trains the leaf weights of all trees of the booster together, the splits as they are, against its objective on
  * `data` (any matrix with a target): `steps` AdamW steps on the mean over all rows of half the squared error, or
  * of the cross-entropy.  Works in 20 bytes of device memory per row and tree and waits for the result; rows times
- * trees of a class are below 2^31.  The booster grows no tree afterwards (AGrowTree returns an error); predictions
- * that matrices carry (AAppendLastTree) and the training predictions stay as they were.  No other thread may use
- * the booster meanwhile. */
+ * trees of a class are below 2^31.  A booster of several classes must have grown its trees: a model's text does
+ * not say which class a tree is of, and loaded ones are refused.  The booster grows no tree afterwards (AGrowTree
+ * returns an error); predictions that matrices carry (AAppendLastTree) and the training predictions stay as they
+ * were.  No other thread may use the booster meanwhile. */
 const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
                                 double eps, double weight_decay);
 
