@@ -307,6 +307,9 @@ void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
   } tokens{static_cast<int *>(DevicePoolTake(use * token_ld * sizeof(int)))};
   LeafTokens(data, tokens.p, token_ld, -1, nullptr);
   RefineOnDevice(cfg, data, tokens.p, token_ld, trees_of, &tables, IntoInternal(cfg.tree.initial_y), options);
+  for (const std::vector<float> &table : tables)
+    for (float w : table)
+      if (!std::isfinite(w)) throw std::runtime_error("the refined weights are not finite: the booster keeps its own");
   refined_ = true;
   for (size_t k = 0; k < K; ++k) {
     const float *from = tables[k].data();
