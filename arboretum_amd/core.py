@@ -410,7 +410,8 @@ class Garden(object):
 
     def refine_leaves(self, data=None, steps=100, lr=0.01, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
         """Trains the leaf weights of all trees together, the splits as they are, by AdamW on the objective's mean over
-        `data` (the training matrix unless given; AGardenRefineLeaves).  The booster grows no tree afterwards."""
+        `data` (the training matrix unless given; AGardenRefineLeaves).  max_leaf_weight is kept to, lambda and alpha
+        have no part in it.  The booster grows no tree afterwards."""
         self._ensure()
         data = self.data if data is None else data
         if data is None:

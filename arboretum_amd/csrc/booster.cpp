@@ -283,6 +283,7 @@ void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
   if (cfg.objective < kSoftMaxOneVsAll && !data->y_facts.finite) throw std::runtime_error("y must be finite");
   const size_t K = cfg.tree.labels_count, n = data->rows;
   if (cfg.objective >= kSoftMaxOneVsAll && K < 2) throw std::runtime_error("soft-max needs labels_count >= 2");
+  if (!(cfg.tree.max_leaf_weight >= 0.0f)) throw std::runtime_error("max_leaf_weight must not be negative");
   SyncTrees();
   // Loaded trees all have the label 0, as in the reference: what class they were of is not known.  (Every round grows
   // a tree of each class, so a booster of several classes has as many of each if and only if it grew them all.)

@@ -2,6 +2,8 @@
 // the sum of their weights is what the booster answers, and the weights are a table of embeddings of dimension 1.
 // Every step is the lookup, the gradient of the objective, the gradient of the table and AdamW, all on the device;
 // the tokens are sorted once.
+#include <algorithm>
+#include <cmath>
 #include <memory>
 #include <vector>
 
@@ -38,6 +40,12 @@ __global__ void k_direction_softmax(const uint8_t *__restrict__ labels, float *_
       y_hat[i + (size_t)k * n] = (labels[i] == k ? 1.0f : 0.0f) - p;
     }
   }
+}
+
+// A step of the weights ends where a grown leaf may end: within max_leaf_weight * eta.
+__global__ void k_limit(float *__restrict__ weight, float most, size_t n) {
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
+    weight[i] = weight[i] > most ? most : weight[i] < -most ? -most : weight[i];  // (a NaN stays one)
 }
 
 // Device memory and the stream of one call, given back when nothing is pending.
@@ -106,16 +114,18 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
     vs.push_back(t.v);
     sizes.push_back((long long)table.size());
   }
-  const unsigned grid = (unsigned)std::min<size_t>((n + 255) / 256, 4096);
+  const auto grid_of = [](size_t count) { return dim3((unsigned)std::min<size_t>((count + 255) / 256, 4096)); };
+  const dim3 grid = grid_of(n);
+  const float most = std::fabs(cfg.tree.max_leaf_weight * cfg.tree.eta);
   for (int step = 1; step <= options.steps; ++step) {
     for (size_t k = 0; k < K; ++k)  // (a class without trees has a sum of 0: bags of no tokens)
       Embedding(EmbeddingArgs{of[k].bags, of[k].weight ? of[k].weight : y_hat, 1, y_hat + k * n, 1, 1, kFloat32, 1.0f, work.stream});
     if (cfg.objective == kLinearRegression)
-      hipLaunchKernelGGL(k_direction_squared, dim3(grid), dim3(256), 0, work.stream, y.get(), y_hat, init, n);
+      hipLaunchKernelGGL(k_direction_squared, grid, dim3(256), 0, work.stream, y.get(), y_hat, init, n);
     else if (cfg.objective == kLogisticRegression)
-      hipLaunchKernelGGL(k_direction_logistic, dim3(grid), dim3(256), 0, work.stream, y.get(), y_hat, init, n);
+      hipLaunchKernelGGL(k_direction_logistic, grid, dim3(256), 0, work.stream, y.get(), y_hat, init, n);
     else
-      hipLaunchKernelGGL(k_direction_softmax, dim3(grid), dim3(256), 0, work.stream, labels.get(), y_hat, n, (int)K);
+      hipLaunchKernelGGL(k_direction_softmax, grid, dim3(256), 0, work.stream, labels.get(), y_hat, n, (int)K);
     HIP_OK(hipGetLastError());
     for (size_t k = 0; k < K; ++k) {
       if (!of[k].weight) continue;
@@ -125,6 +135,10 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
     AdamW(AdamWArgs{(int)weights.size(), weights.data(), grads.data(), ms.data(), vs.data(), sizes.data(), kFloat32, kFloat32,
                     options.lr, options.beta1, options.beta2, options.eps, options.weight_decay, 1.0, step, nullptr, nullptr,
                     work.stream});
+    if (cfg.tree.max_leaf_weight == 0.0f) continue;
+    for (size_t k = 0; k < K; ++k)
+      if (of[k].weight) hipLaunchKernelGGL(k_limit, grid_of((*tables)[k].size()), dim3(256), 0, work.stream, of[k].weight, most, (*tables)[k].size());
+    HIP_OK(hipGetLastError());
   }
   for (size_t k = 0; k < K; ++k) {
     std::vector<float> &table = (*tables)[k];

@@ -274,12 +274,14 @@ const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens,
 
 /* Trains the leaf weights of all trees of the booster together, the splits as they are, against its objective on
  * `data` (any matrix with a target): `steps` AdamW steps on the mean over all rows of half the squared error, or
- * of the cross-entropy.  Works in 20 bytes of device memory per row and tree and waits for the result; rows times
- * trees of a class are below 2^31.  A booster of several classes must have grown its trees: a model's text does
- * not say which class a tree is of, and loaded ones are refused.  If a weight comes out infinite or NaN (a
- * learning rate that is too large) that is an error, and the booster stays as it was.  The booster grows no tree
- * afterwards (AGrowTree returns an error); predictions that matrices carry (AAppendLastTree) and the training
- * predictions stay as they were.  No other thread may use the booster meanwhile. */
+ * of the cross-entropy.  lambda and alpha, which a grown leaf's weight answers to, have no part in it (weight_decay
+ * has); with a max_leaf_weight every step ends within max_leaf_weight * eta, as a grown leaf does.  Works in 20
+ * bytes of device memory per row and tree and waits for the result; rows times trees of a class are below 2^31.
+ * A booster of several classes must have grown its trees: a model's text does not say which class a tree is of, and
+ * loaded ones are refused.  If a weight comes out infinite or NaN (a learning rate that is too large) that is an
+ * error, and the booster stays as it was.  The booster grows no tree afterwards (AGrowTree returns an error);
+ * predictions that matrices carry (AAppendLastTree) and the training predictions stay as they were.  No other
+ * thread may use the booster meanwhile. */
 const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2,
                                 double eps, double weight_decay);
 

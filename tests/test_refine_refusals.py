@@ -39,3 +39,10 @@ def test_soft_max_of_one_class(arb, objective):
     booster = arb.load(model_text(2, objective=objective, labels_count=1))
     with pytest.raises(arb.ArboretumError, match="labels_count >= 2"):
         booster.refine_leaves(rows(arb, [0, 1, 0, 1]))
+
+
+def test_a_largest_leaf_weight_below_0(arb):
+    booster = arb.load(model_text(2, objective=0, labels_count=1, max_leaf_weight=-0.5))
+    data = arb.DMatrix(np.zeros((4, 1), np.float32), y=np.zeros(4, np.float32))
+    with pytest.raises(arb.ArboretumError, match="max_leaf_weight must not be negative"):
+        booster.refine_leaves(data)
