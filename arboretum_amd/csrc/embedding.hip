@@ -200,14 +200,19 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
 // Rows of one element over so many bags that their tokens, column by column (the leaves of trees), come from memory
 // and not from the last-level cache of 256 MB.  A thread takes four neighbouring bags, whose tokens are one load, and
 // the tokens of the next columns are in flight while these are looked up.  Reading the tokens alone takes 135 us for
-// a million bags of 200; the rest is the lookups, of which the L1 answers little more than a lane a cycle.
-// (1,000,003 x 200: 223 us, 276 with a bag a thread; 700,000 x 100, which the cache holds: 71 and 64; with the pieces
-// of the table that a column names copied to the LDS first 290 and more: finding the pieces takes longer than the LDS
-// saves.)
+// a million bags of 200; the rest is the lookups.  (With the pieces of the table that a column names copied to the
+// LDS first 290 and more: finding the pieces takes longer than the LDS saves.)
+// Taken from 512 MB of tokens on, where there are two workgroups for a CU.  Us with a bag a thread / here, 256 leaves
+// a column: tokens of 32 bits, 256 MB: 3,355,446 x 20 71 / 67, 671,091 x 100 75 / 76, 335,547 x 200 80 / 108; 512 MB:
+// 158 / 146, 177 / 162, 671,091 x 200 187 / 166, 335,547 x 400 206 / 233; 1 GB: 316 / 282, 350 / 289, 355 / 317.  Of
+// 64 bits, 256 MB: 53 / 49, 56 / 63, 54 / 84; 512 MB: 126 / 113, 133 / 117, 335,547 x 200 140 / 145; 1 GB: 252 / 223,
+// 251 / 225, 260 / 230.  A table that the L1 holds, or one whose rows are named all over, makes less of it: 512 MB of
+// 32 bits over 100 x 64 leaves 138 / 149, bags of three out of 200,000 514 / 542.
 constexpr int kColumns = 4;  // (SumOfFour)
 constexpr int kBagsOfThread = 4;
-constexpr long long kManyTokens = 1ll << 27;
 constexpr int kColumnBags = kThreads * kBagsOfThread;
+constexpr long long kManyTokenBytes = 1ll << 29;
+constexpr long long kManyBags = 2 * 256 * kColumnBags;
 
 template <typename T, typename Token>
 __global__ void __launch_bounds__(kThreads) k_embedding_columns(const Bags<Token> bags, const Rows<T> r) {
@@ -269,8 +274,8 @@ void LaunchLookup(const EmbeddingArgs &a, hipStream_t st) {
   const Rows<T> r{static_cast<const T *>(a.table), a.table_stride, static_cast<T *>(a.out), a.out_stride, a.dim, a.scale};
   const bool past = (size_t)a.bags.n * a.dim * sizeof(T) > kStreamedBytes;
   if constexpr (kVec == 1) {
-    if (a.dim == 1 && a.bags.bag > 1 && a.bags.token_stride == 1 && a.bags.bag_stride > 1 && a.bags.n * a.bags.bag >= kManyTokens &&
-        a.bags.n >= kColumnBags * 256) {
+    if (a.dim == 1 && a.bags.bag > 1 && a.bags.token_stride == 1 && a.bags.bag_stride > 1 && a.bags.n >= kManyBags &&
+        a.bags.n * a.bags.bag * (long long)sizeof(Token) >= kManyTokenBytes) {
       const unsigned blocks = (unsigned)((a.bags.n + kColumnBags - 1) / kColumnBags);
       hipLaunchKernelGGL((k_embedding_columns<T, Token>), dim3(blocks), dim3(kThreads), 0, st, bags, r);
       return;

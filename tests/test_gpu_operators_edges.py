@@ -1,4 +1,4 @@
-"""Sums of long bags."""
+"""Sums of long bags, and where bags are looked up another way."""
 import pytest
 import torch
 
@@ -35,3 +35,25 @@ def test_small_numbers_behind_a_large_one_are_not_lost(arb, n, bag, dim, columns
                       token_stride=1 if columns else bag, bag_stride=n if columns else 1)
         want = torch.full((n, dim), 1 + (bag - 1) * small, dtype=torch.float64)
         within(out, want, (bag / 4 + 12) * U * want, T)
+
+
+# both sides of 512 MB of tokens, and of 2^19 bags, from which on columns of scalars are read four bags a thread
+@pytest.mark.parametrize("n,bag,bits", [((1 << 19) - 1, 129, 64), (1 << 19, 128, 64), ((1 << 19) + 1, 127, 64), (1 << 19, 127, 64),
+                                        ((1 << 19) - 1, 257, 32), ((1 << 19) + 3, 256, 32), (1 << 19, 255, 32), ((1 << 26) + 5, 2, 32)])
+def test_columns_of_scalars_on_both_sides_of_the_rule(arb, n, bag, bits):
+    vocab, scale = 999, 1.5
+    gen = torch.Generator(device="cuda").manual_seed(bag + bits)
+    table = torch.randn(vocab, 1, generator=gen, device="cuda")
+    tokens = torch.randint(-1, vocab, (bag, n), generator=gen, device="cuda", dtype=torch.int32 if bits == 32 else torch.int64)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full((n + 1,), 7.0, device="cuda")
+    arb.embedding(out.data_ptr(), table.data_ptr(), tokens.data_ptr(), n, vocab, 1, bag=bag, scale=scale, token_bits=bits, token_stride=1,
+                  bag_stride=n, status=status.data_ptr())
+    held = torch.cat([table.double() * scale, torch.zeros(1, 1, dtype=torch.float64, device="cuda")])[:, 0]
+    want, mag = (torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2))
+    for one in tokens:
+        x = held[one.long()]  # (-1: the zero at the end)
+        want += x
+        mag += x.abs()
+    within(out[:n], want.cpu(), (bag / 4 + 12) * U * mag.cpu(), torch.float32)
+    assert out[n].item() == 7.0 and status.item() == 0
