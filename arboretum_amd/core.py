@@ -155,19 +155,32 @@ def _type(name):
         raise ArboretumError(ValueError("element type %r is not one of %s" % (name, ", ".join(_TYPES)))) from None
 
 
+def _refuse_wide(words, long_words):
+    """Refuses integers beyond 32 and 64 bits, of which the foreign call would only see the lower ones."""
+    for values, bits in ((words, 32), (long_words, 64)):
+        for v in values:
+            if not -(1 << (bits - 1)) <= v < 1 << (bits - 1):
+                raise ArboretumError(OverflowError("%d does not fit into %d bits" % (v, bits)))
+
+
 def embedding(out, table, tokens, n, vocab, dim, bag=1, scale=1.0, dtype="float32", token_bits=32, out_stride=None,
               table_stride=None, token_stride=None, bag_stride=1, status=None, stream=None):
     """out[i] = scale * (sum over the bag of table[token]), rows of `dim` elements of `dtype` ("float32", "bfloat16",
     "float16") on the GPU (AEmbedding).  Array arguments are DEVICE addresses; token j of bag i is at
     i * token_stride + j * bag_stride (elements; token_stride is `bag` unless given), -1 stands for none.
     `status`: an optional device word, set to 1 by a token outside the table.  Does not wait."""
-    _check(_LIB.AEmbedding(out, table, tokens, n, bag, vocab, dim, dim if out_stride is None else out_stride,
-                           dim if table_stride is None else table_stride, bag if token_stride is None else token_stride,
-                           bag_stride, _type(dtype), token_bits, scale, status, stream))
+    out_stride = dim if out_stride is None else out_stride
+    table_stride = dim if table_stride is None else table_stride
+    token_stride = bag if token_stride is None else token_stride
+    if (bag | dim | token_bits) >> 31 or (n | vocab | out_stride | table_stride | token_stride | bag_stride) >> 63:
+        _refuse_wide((bag, dim, token_bits), (n, vocab, out_stride, table_stride, token_stride, bag_stride))
+    _check(_LIB.AEmbedding(out, table, tokens, n, bag, vocab, dim, out_stride, table_stride, token_stride, bag_stride, _type(dtype),
+                           token_bits, scale, status, stream))
 
 
 def embedding_sort_bytes(n, vocab, bag=1):
     """Bytes of device memory embedding_sort works in (AEmbeddingSortBytes; no GPU needed)."""
+    _refuse_wide((bag,), (n, vocab))
     v = ctypes.c_ulonglong()
     _check(_LIB.AEmbeddingSortBytes(n, bag, vocab, ctypes.byref(v)))
     return v.value
@@ -177,12 +190,16 @@ def embedding_sort(keys, rows, tokens, n, vocab, work, work_bytes, bag=1, token_
                    bag_stride=1, status=None, stream=None):
     """The (token, bag) pairs of n bags in order of tokens, for embedding_grad (AEmbeddingSort): keys and rows take
     n * bag 32-bit words each.  Tokens as in embedding(); `work`: embedding_sort_bytes() of device memory.  Does not wait."""
-    _check(_LIB.AEmbeddingSort(keys, rows, tokens, n, bag, vocab, bag if token_stride is None else token_stride, bag_stride,
-                               token_bits, work, work_bytes, status, stream))
+    token_stride = bag if token_stride is None else token_stride
+    if (bag | token_bits) >> 31 or (n | vocab | token_stride | bag_stride) >> 63:
+        _refuse_wide((bag, token_bits), (n, vocab, token_stride, bag_stride))
+    _check(_LIB.AEmbeddingSort(keys, rows, tokens, n, bag, vocab, token_stride, bag_stride, token_bits, work,
+                               max(work_bytes, 0), status, stream))
 
 
 def embedding_grad_bytes(n, dim, bag=1):
     """Bytes of device memory embedding_grad works in (AEmbeddingGradBytes; no GPU needed)."""
+    _refuse_wide((bag, dim), (n,))
     v = ctypes.c_ulonglong()
     _check(_LIB.AEmbeddingGradBytes(n, bag, dim, ctypes.byref(v)))
     return v.value
@@ -193,9 +210,12 @@ def embedding_grad(grad_table, grad_out, keys, rows, n, vocab, dim, work, work_b
     """Gradient of embedding()'s table (AEmbeddingGrad): grad_table[v] = scale * (sum of grad_out[row] over the pairs of
     embedding_sort with key v), added to what is there with `accumulate`.  dtype: of grad_out; grad_dtype: of grad_table, that or
     "float32".  The same from run to run.  Does not wait."""
-    _check(_LIB.AEmbeddingGrad(grad_table, grad_out, keys, rows, n, bag, vocab, dim,
-                               dim if table_stride is None else table_stride, dim if out_stride is None else out_stride,
-                               _type(dtype), _type(grad_dtype), scale, int(bool(accumulate)), work, work_bytes, stream))
+    table_stride = dim if table_stride is None else table_stride
+    out_stride = dim if out_stride is None else out_stride
+    if (bag | dim) >> 31 or (n | vocab | table_stride | out_stride) >> 63:
+        _refuse_wide((bag, dim), (n, vocab, table_stride, out_stride))
+    _check(_LIB.AEmbeddingGrad(grad_table, grad_out, keys, rows, n, bag, vocab, dim, table_stride, out_stride, _type(dtype), _type(grad_dtype),
+                               scale, int(bool(accumulate)), work, max(work_bytes, 0), stream))
 
 
 def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
@@ -210,6 +230,8 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta
         table = None
     if table is None or table.ndim != 2:
         raise ArboretumError(ValueError("the lists of tensors differ in length or hold other than addresses and sizes"))
+    if step >> 63:
+        _refuse_wide((), (step,))
     count, at = table.shape[1], table.ctypes.data
     _check(_LIB.AAdamW(count, at, at + 8 * count, at + 16 * count, at + 24 * count, at + 32 * count, _type(dtype),
                        _type(dtype if grad_dtype is None else grad_dtype), lr, beta1, beta2, eps, weight_decay, grad_scale,
@@ -403,9 +425,10 @@ class Garden(object):
         [trees][stride] at the DEVICE address `tokens` (stride: data.rows unless given), the trees of a class together,
         leaves numbered through them.  Returns the leaves of each class: the rows of its table.  Waits."""
         self._ensure()
+        stride, n_rounds = int(data.rows if stride is None else stride), int(n_rounds)
+        _refuse_wide((n_rounds,), (stride,))
         leaves = np.zeros(int(self.config.get('tree', {}).get('labels_count', 1)), dtype=np.int64)
-        _check(_LIB.AGardenLeafTokens(self.handle, data.handle, tokens, int(data.rows if stride is None else stride),
-                                      int(n_rounds), leaves.ctypes.data, leaves.size))
+        _check(_LIB.AGardenLeafTokens(self.handle, data.handle, tokens, stride, n_rounds, leaves.ctypes.data, leaves.size))
         return leaves.tolist()
 
     def refine_leaves(self, data=None, steps=100, lr=0.01, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
@@ -416,6 +439,7 @@ class Garden(object):
         data = self.data if data is None else data
         if data is None:
             raise ArboretumError(ValueError("no data matrix to refine on"))
+        _refuse_wide((int(steps),), ())
         _check(_LIB.AGardenRefineLeaves(self.handle, data.handle, int(steps), lr, beta1, beta2, eps, weight_decay))
 
     def set_inspect(self, on=True):

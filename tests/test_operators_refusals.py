@@ -1,8 +1,9 @@
 """More calls that the tensor operators refuse, each of which would be answered wrongly: host code only, so nothing here
 reaches a GPU (addresses are never followed: every call is refused before a kernel is launched)."""
+import numpy as np
 import pytest
 
-from test_operators_host import A, adamw
+from test_operators_host import A, adamw, grad, lookup, sort
 
 
 @pytest.fixture(scope="module")
@@ -31,3 +32,43 @@ def test_adamw_refuses_constants_beyond_float32_whatever_the_device_words_replac
         adamw(arb, grad_scale=1e39, lr_device=A, step_device=A)
     with pytest.raises(arb.ArboretumError, match="eps must be at least"):
         adamw(arb, eps=0.0, lr_device=A, step_device=A)
+
+
+# Sizes that a call's 32- or 64-bit words do not hold: what is left of them after dropping the upper bits would pass every check.
+@pytest.mark.parametrize("call", ["embedding_sort_bytes", "embedding_grad_bytes"])
+def test_work_memory_of_sizes_that_do_not_fit(arb, call):
+    other = dict(vocab=10) if call == "embedding_sort_bytes" else dict(dim=8)
+    for change in (dict(bag=2 ** 32 + 1), dict(bag=-2 ** 32 + 1), dict(n=2 ** 64 + 4), dict(n=-2 ** 64 + 4), {k: v + 2 ** 32 * (1 + 2 ** 32 * (k == "vocab")) for k, v in other.items()}):
+        with pytest.raises(arb.ArboretumError, match="bits"):
+            getattr(arb, call)(**{**dict(n=4), **other, **change})
+
+
+@pytest.mark.parametrize("name,by", [("bag", 2 ** 32), ("dim", 2 ** 32), ("token_bits", 2 ** 32), ("dim", -2 ** 32), ("n", 2 ** 64), ("vocab", 2 ** 64),
+                                     ("vocab", -2 ** 64), ("out_stride", 2 ** 64), ("table_stride", 2 ** 64), ("token_stride", 2 ** 64),
+                                     ("bag_stride", 2 ** 64), ("bag_stride", -2 ** 65)])
+def test_sizes_that_do_not_fit(arb, name, by):
+    for call, takes in ((lookup, "bag dim token_bits n vocab out_stride table_stride token_stride bag_stride"),
+                        (sort, "bag token_bits n vocab token_stride bag_stride"), (grad, "bag dim n vocab out_stride table_stride")):
+        if name in takes.split():
+            value = dict(bag=1, dim=8, token_bits=32, n=4, vocab=10, out_stride=8, table_stride=8, token_stride=1, bag_stride=1)[name]
+            with pytest.raises(arb.ArboretumError, match="bits"):
+                call(arb, **{name: value + by})
+
+
+def test_steps_and_strides_that_do_not_fit(arb):
+    with pytest.raises(arb.ArboretumError, match="64 bits"):
+        adamw(arb, step=2 ** 64 + 1)
+    data = arb.DMatrix(np.zeros((5, 3), np.float32), y=np.zeros(5))
+    booster = arb.Garden({"objective": 0, "method": 1, "tree": {"max_depth": 3}}, data)
+    with pytest.raises(arb.ArboretumError, match="32 bits"):
+        booster.refine_leaves(steps=2 ** 32)
+    with pytest.raises(arb.ArboretumError, match="64 bits"):
+        booster.leaf_tokens(data, A, stride=2 ** 64 + 5)
+    with pytest.raises(arb.ArboretumError, match="32 bits"):
+        booster.leaf_tokens(data, A, n_rounds=2 ** 32 + 1)
+
+
+def test_work_memory_of_less_than_nothing(arb):
+    for call in (sort, grad):
+        with pytest.raises(arb.ArboretumError, match="too small"):
+            call(arb, work_bytes=-1)
