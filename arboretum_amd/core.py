@@ -5,6 +5,7 @@ boundary (core.py:21-48).  Everything here is marshalling; the work happens in
 the shared library (host C++ and HIP kernels)."""
 import ctypes
 import json
+import operator
 import os
 
 import numpy as np
@@ -218,14 +219,25 @@ def embedding_grad(grad_table, grad_out, keys, rows, n, vocab, dim, work, work_b
                                scale, int(bool(accumulate)), work, max(work_bytes, 0), stream))
 
 
+def _whole(values):
+    """Whether a list or array holds integers only (numpy would cut off what others have behind the point)."""
+    if isinstance(values, np.ndarray):
+        return values.dtype.kind in "iu" or values.size == 0
+    if not set(map(type, values)) <= {int}:
+        for v in values:
+            operator.index(v)
+    return True
+
+
 def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
           grad_scale=1.0, dtype="float32", grad_dtype=None, lr_device=None, step_device=None, stream=None):
     """One AdamW step over a list of tensors on the GPU (AAdamW).  params, grads, exp_avgs, exp_avg_sqs: DEVICE addresses, a list or
     an integer array of them each; sizes: elements of each tensor.  params have `dtype`, grads `grad_dtype` (dtype unless
     given), the two states float32.  `step` counts from 1.  lr_device, step_device: optional device words (float32, int64)
     read instead of lr and step.  Does not wait."""
+    lists = (params, grads, exp_avgs, exp_avg_sqs, sizes)
     try:  # the five lists one after the other
-        table = np.array((params, grads, exp_avgs, exp_avg_sqs, sizes), dtype=np.int64)
+        table = np.array(lists, dtype=np.int64) if all(map(_whole, lists)) else None
     except (ValueError, TypeError, OverflowError):
         table = None
     if table is None or table.ndim != 2:

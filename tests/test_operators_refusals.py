@@ -72,3 +72,22 @@ def test_work_memory_of_less_than_nothing(arb):
     for call in (sort, grad):
         with pytest.raises(arb.ArboretumError, match="too small"):
             call(arb, work_bytes=-1)
+
+
+@pytest.mark.parametrize("which", ["params", "grads", "exp_avgs", "exp_avg_sqs", "sizes"])
+@pytest.mark.parametrize("value", [3.7, "100", 64.0, np.float32(8), None, [4]])
+def test_adamw_refuses_lists_of_other_than_whole_numbers(arb, which, value):
+    for values in ([value], np.array([value])):
+        with pytest.raises(arb.ArboretumError, match="hold other than addresses and sizes"):
+            adamw(arb, **{which: values})
+
+
+def test_adamw_takes_lists_and_integer_arrays_alike(arb):
+    # (refused for its step: after the lists)
+    for kind in (list, tuple, lambda v: np.array(v, np.int64), lambda v: np.array(v, np.uint64), lambda v: [np.int64(x) for x in v],
+                 lambda v: np.array(v, np.int64)[::-1][::-1]):
+        lists = {name: kind([(k + 1) * A, (k + 9) * A]) for k, name in enumerate(["params", "grads", "exp_avgs", "exp_avg_sqs"])}
+        with pytest.raises(arb.ArboretumError, match="step counts from 1"):
+            adamw(arb, sizes=kind([100, 7]), step=0, **lists)
+    with pytest.raises(arb.ArboretumError, match="step counts from 1"):
+        adamw(arb, **{name: np.array([]) for name in ["params", "grads", "exp_avgs", "exp_avg_sqs", "sizes"]}, step=0)
