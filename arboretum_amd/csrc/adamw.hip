@@ -108,26 +108,42 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const Launch a) {
   }
 }
 
-// Two ranges of one list that meet would be updated twice, by two workgroups at once.
-template <typename Ptr>
-void CheckApart(const AdamWArgs &a, Ptr list, size_t bytes, const char *what) {
-  auto begin = [&](int i) { return reinterpret_cast<uintptr_t>(list[i]); };
-  auto meet = [&](int i, int j) { return begin(i) + (size_t)a.sizes[i] * bytes > begin(j); };
-  int last = -1;
-  bool rising = true;
-  for (int i = 0; i < a.count; ++i) {
-    if (a.sizes[i] == 0) continue;
-    if (last >= 0 && begin(i) < begin(last)) rising = false;
-    else if (last >= 0 && meet(last, i)) throw std::runtime_error(std::string(what) + " overlap");
-    last = i;
+// Elements that are written (of params and both states) and belong to another tensor too, or to a gradient, would be read
+// and written by two workgroups at once.  All ranges are looked at in order of where they begin: one that meets any
+// before it meets the one that ends last.
+struct Range {
+  uintptr_t begin, end;
+  bool written;
+};
+void CheckApart(const AdamWArgs &a) {
+  std::vector<Range> all;
+  all.reserve((size_t)a.count * 4);
+  const auto before = [](const Range &x, const Range &y) { return x.begin < y.begin; };
+  size_t joined = 0;  // ranges of the lists before, in order
+  const auto add = [&](auto list, size_t bytes, bool written) {
+    bool rising = true;
+    for (int i = 0; i < a.count; ++i) {
+      if (a.sizes[i] == 0) continue;
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(list[i]);
+      rising = rising && (all.size() == joined || all.back().begin <= begin);
+      all.push_back(Range{begin, begin + (size_t)a.sizes[i] * bytes, written});
+    }
+    if (!rising) std::sort(all.begin() + joined, all.end(), before);
+    if (joined > 0 && joined < all.size()) {
+      if (before(all.back(), all[0])) std::rotate(all.begin(), all.begin() + joined, all.end());
+      else if (before(all[joined], all[joined - 1])) std::inplace_merge(all.begin(), all.begin() + joined, all.end(), before);
+    }
+    joined = all.size();
+  };
+  add(a.params, ElementBytes(a.type), true);
+  add(a.grads, ElementBytes(a.grad_type), false);
+  add(a.exp_avg, 4, true);
+  add(a.exp_avg_sq, 4, true);
+  uintptr_t written = 0, read = 0;  // where those before end
+  for (const Range &r : all) {
+    if (r.begin < written || (r.written && r.begin < read)) throw std::runtime_error("params, states and grads overlap");
+    (r.written ? written : read) = std::max(r.written ? written : read, r.end);
   }
-  if (rising) return;
-  std::vector<int> order;
-  for (int i = 0; i < a.count; ++i)
-    if (a.sizes[i] != 0) order.push_back(i);
-  std::sort(order.begin(), order.end(), [&](int i, int j) { return begin(i) < begin(j); });
-  for (size_t k = 1; k < order.size(); ++k)
-    if (meet(order[k - 1], order[k])) throw std::runtime_error(std::string(what) + " overlap");
 }
 
 void Validate(const AdamWArgs &a) {
@@ -143,8 +159,6 @@ void Validate(const AdamWArgs &a) {
     CheckAligned(a.grads[i], ElementBytes(a.grad_type), "a gradient");
     CheckAligned(a.exp_avg[i], 4, "a state");
     CheckAligned(a.exp_avg_sq[i], 4, "a state");
-    if (a.params[i] == a.exp_avg[i] || a.params[i] == a.exp_avg_sq[i] || a.exp_avg[i] == a.exp_avg_sq[i])
-      throw std::runtime_error("a tensor and its states overlap");
   }
   // (comparisons that a NaN fails)
   if (!(a.lr >= 0) || !(a.eps >= 0) || !(a.weight_decay >= 0)) throw std::runtime_error("lr, eps and weight_decay must not be negative");
@@ -157,9 +171,7 @@ void Validate(const AdamWArgs &a) {
   if (!a.step_device && a.step < 1) throw std::runtime_error("step counts from 1");
   CheckAligned(a.lr_device, 4, "lr_device");
   CheckAligned(a.step_device, 8, "step_device");
-  CheckApart(a, a.params, ElementBytes(a.type), "params");
-  CheckApart(a, a.exp_avg, 4, "states");
-  CheckApart(a, a.exp_avg_sq, 4, "states");
+  CheckApart(a);
 }
 
 }  // namespace

@@ -252,10 +252,11 @@ const char *AEmbeddingGrad(void *grad_table, const void *grad_out, const unsigne
  *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * params, grads, exp_avg (m), exp_avg_sq (v), sizes: HOST arrays of `count` device pointers and element counts,
- * read before the call returns; tensors of one list must not overlap.  Sizes are below 2^36; one may be 0, its
- * pointers are then not looked at. All tensors are on one device.  step counts from 1.  eps is at least 2^-126 (an
- * element whose gradients have all been 0 stays where it is), and lr, its quotient by 1 - beta1^step, lr weight_decay, eps
- * and grad_scale lie within float32.
+ * read before the call returns.  What is written (params and both states) must be apart from all other tensors of
+ * the call (checked); gradients may be one another's.  Sizes are below 2^36; one may be 0, its pointers are then not
+ * looked at.  All tensors are on one device.  step counts from 1.  eps is at least 2^-126 (an element whose
+ * gradients have all been 0 stays where it is), and lr, its quotient by 1 - beta1^step, lr weight_decay, eps and
+ * grad_scale lie within float32.
  * lr_device, step_device: device words read instead of lr and step (for a captured graph that is replayed with
  * others); may be NULL.  (A step below 1 there counts as 1.) */
 const char *AAdamW(int count, void *const *params, const void *const *grads, float *const *exp_avg,

@@ -91,3 +91,74 @@ def test_adamw_takes_lists_and_integer_arrays_alike(arb):
             adamw(arb, sizes=kind([100, 7]), step=0, **lists)
     with pytest.raises(arb.ArboretumError, match="step counts from 1"):
         adamw(arb, **{name: np.array([]) for name in ["params", "grads", "exp_avgs", "exp_avg_sqs", "sizes"]}, step=0)
+
+
+NAMES = ["params", "grads", "exp_avgs", "exp_avg_sqs"]
+
+
+def places():
+    """Lists of three tensors that keep apart, 64 KB between two of them."""
+    return {name: [(k + 2) * A + 65536 * i for i in range(3)] for k, name in enumerate(NAMES)}
+
+
+# what is written must be apart from all else: the elements of two lists that meet would be read and written by two workgroups at once
+@pytest.mark.parametrize("first,second", [(a, b) for a in NAMES for b in NAMES if a != b])
+@pytest.mark.parametrize("i,j", [(0, 2), (2, 0), (1, 1)])
+@pytest.mark.parametrize("by", [0, 4, 396, -396])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_adamw_refuses_tensors_of_two_lists_that_meet(arb, first, second, i, j, by, order):
+    lists = places()
+    lists[second][j] = lists[first][i] + by
+    perm = {"rising": [0, 1, 2], "falling": [2, 1, 0], "mixed": [1, 0, 2]}[order]
+    with pytest.raises(arb.ArboretumError, match="overlap"):
+        adamw(arb, sizes=[100] * 3, **{name: [v[k] for k in perm] for name, v in lists.items()})
+
+
+@pytest.mark.parametrize("order", [[0, 1, 2, 3], [3, 1, 0, 2], [3, 2, 1, 0]])
+def test_adamw_takes_tensors_that_only_touch(arb, order):
+    # parameter, gradient and states of one tensor after the other, back to back, in 16 and 32 bits; a tensor of no elements anywhere
+    sizes, at, lists = [100, 7, 0, 31], 16 * A, {name: [] for name in NAMES}
+    for size in sizes:
+        for name, item in zip(NAMES, (2, 2, 4, 4)):
+            at += -at % item
+            lists[name].append(at)
+            at += size * item
+    lists["params"][2] = lists["exp_avgs"][0] + 4
+    if arb.device_count() == 0:
+        with pytest.raises(arb.ArboretumError, match="no HIP device"):
+            adamw(arb, sizes=[sizes[k] for k in order], dtype="bfloat16", **{name: [v[k] for k in order] for name, v in lists.items()})
+
+
+def test_adamw_takes_one_gradient_for_several_tensors(arb):
+    # (gradients are only read)
+    if arb.device_count() == 0:
+        lists = places()
+        lists["grads"] = [lists["grads"][0]] * 3
+        with pytest.raises(arb.ArboretumError, match="no HIP device"):
+            adamw(arb, sizes=[100] * 3, **lists)
+
+
+def test_adamw_finds_one_meeting_among_many(arb):
+    rng = np.random.default_rng(3)
+    for trial in range(40):
+        count = int(rng.integers(1, 400))
+        sizes = rng.integers(0, 50, count)
+        lists = {name: [] for name in NAMES}
+        at = A
+        slots = [(name, k) for name in NAMES for k in range(count)]
+        if trial % 2:
+            rng.shuffle(slots)
+        for name, k in slots:
+            lists[name] += [0] * (k + 1 - len(lists[name]))
+            lists[name][k] = at
+            at += 4 * int(sizes[k]) + 4 * int(rng.integers(0, 3))
+        if arb.device_count() == 0 and sizes.any():
+            with pytest.raises(arb.ArboretumError, match="no HIP device"):
+                adamw(arb, sizes=sizes, **lists)
+        if (sizes > 0).sum() < 2:
+            continue
+        one, other = rng.choice(np.flatnonzero(sizes > 0), 2, replace=False)
+        a, b = rng.choice(NAMES, 2, replace=False)
+        lists[a][one] = lists[b][other] + 4 * int(rng.integers(0, sizes[other]))
+        with pytest.raises(arb.ArboretumError, match="overlap"):
+            adamw(arb, sizes=sizes, **lists)
