@@ -124,3 +124,57 @@ def test_a_limit_of_0_holds_every_leaf(arb):
                        "tree": {"max_depth": 3, "eta": 0.0, "max_leaf_weight": 0.2}}, arb.DMatrix(X, y=y), 2)
     model.refine_leaves(steps=3)
     assert not weights(model).any()
+
+
+def sums_64(leaf, w, classes):
+    """Sums of leaf weights, and of their magnitudes: [classes][rows].  Tree t is of class t % classes."""
+    sums, size = np.zeros((classes, leaf.shape[1])), np.zeros((classes, leaf.shape[1]))
+    for t in range(len(leaf)):
+        sums[t % classes] += w[t][leaf[t]]
+        size[t % classes] += np.abs(w[t][leaf[t]])
+    return sums, size
+
+
+@pytest.mark.parametrize("objective,classes", [(0, 1), (1, 1), (4, 3), (3, 2)])
+def test_several_steps_of_every_objective(arb, objective, classes):
+    """Against 64 bits, the error carried from step to step.  With e the error of the weights so far (per leaf), a sum of a row's
+    weights is off by the e of its leaves and by (trees + 3) u of their magnitudes, and a direction by no more than that (the slopes of the links are at
+    most 1; of the soft-max, by the largest over the classes, twice) and 8 u of values around 1.  A gradient sums these over its rows and
+    is off by (rows + 4) u of the magnitudes besides.  The moments take such an error on with their factors and 5 and 8 roundings; the step
+    size m / (sqrt(v) / root + eps) is off by size (dm / den + |m| dr / den^2) and 13 roundings, dr = dv / (sqrt(v) root) or
+    sqrt(dv) / root, the lesser.  With eps = 0.05, large against most gradients, this stays small."""
+    from test_gpu_refine import U, directions_64, walk
+    model, data, X, y, labels = make(arb, objective, classes=classes, rounds=4, rows=2000)
+    n, trees, steps, lr, eps, decay, b1, b2 = len(X), model.num_trees(), 5, 0.02, 0.05, 0.1, 0.8, 0.9
+    init = {0: 0.5, 1: 0.0}.get(objective, 0.0)
+    leaf = walk(model, X)
+    w = np.array([model.tree(t)["weights"] for t in range(trees)], np.float64)
+    e, m, v, dm, dv = (np.zeros_like(w) for _ in range(5))
+    before = w.copy()
+    for step in range(1, steps + 1):
+        sums, size = sums_64(leaf, w, classes)
+        off, _ = sums_64(leaf, e, classes)
+        d = directions_64(objective, sums, init, y, labels)
+        dd = 2 * (off + (trees // classes + 3) * U * (size + off)).max(0) + 8 * U * (1 + np.abs(sums).max(0) + np.abs(d).max(0))
+        for t in range(trees):
+            g, dg, mag = (np.zeros(w.shape[1]) for _ in range(3))
+            np.add.at(g, leaf[t], -d[t % classes] / n)
+            np.add.at(dg, leaf[t], dd / n)
+            np.add.at(mag, leaf[t], np.abs(d[t % classes]) / n)
+            dg += (np.bincount(leaf[t], minlength=len(g)) + 4) * U * (mag + dg)
+            dm[t] = b1 * dm[t] + (1 - b1) * dg + 5 * U * (b1 * np.abs(m[t]) + (1 - b1) * np.abs(g))
+            dv[t] = b2 * dv[t] + (1 - b2) * (2 * np.abs(g) + dg) * dg + 8 * U * (b2 * v[t] + (1 - b2) * g * g)
+            m[t], v[t] = b1 * m[t] + (1 - b1) * g, b2 * v[t] + (1 - b2) * g * g
+            root, factor = np.sqrt(1 - b2 ** step), lr / (1 - b1 ** step)
+            den = np.sqrt(v[t]) / root + eps
+            dr = np.minimum(np.sqrt(dv[t]), dv[t] / np.maximum(np.sqrt(v[t]), 1e-300)) / root
+            moved = factor * m[t] / den
+            at = np.abs(w[t])
+            # (the denominator of the other side is no less than eps)
+            e[t] = e[t] * (1 - lr * decay) + 1.01 * factor * (dm[t] / den + np.abs(m[t]) * dr / (den * eps)) + 14 * U * np.abs(moved) + 3 * U * at
+            w[t] = w[t] * (1 - lr * decay) - moved
+    model.refine_leaves(steps=steps, lr=lr, eps=eps, weight_decay=decay, beta1=b1, beta2=b2)
+    got = weights(model).reshape(w.shape).astype(np.float64)
+    assert (np.abs(got - w) <= e).all()
+    # the bound tells a wrong step from a right one: it is far below what a weight moves
+    assert np.median(e) < 1e-3 * np.abs(w - before).max()
