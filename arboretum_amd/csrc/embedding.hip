@@ -398,7 +398,9 @@ constexpr int kRangeBits = 8;  // of a digit, at most
 constexpr unsigned kMostRangePairs = 32768;
 constexpr unsigned kMostRanges = 256;  // a workgroup per CU
 
-// Pairs are kept as (key - first key of the range) << place_bits | place.
+// Pairs are kept as (key - first key of the range) << place_bits | place.  All rounds are unrolled, each behind its
+// own test: with 32 of them 193 scalar registers are spilled into vector registers, and with tokens of 64 bits, which
+// are all in flight at once, 6 vector registers to scratch memory (32,768 pairs: 19.3 us, 21.2 with 64 bits).
 template <int kRounds, typename Token>
 __global__ void __launch_bounds__(kRangeThreads)
 k_sort_ranges(const Pairs<Token> in, unsigned span, int key_bits, int place_bits, unsigned *__restrict__ keys,
@@ -1298,8 +1300,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_grad_join(const Gradient<T, O>
 }
 
 // Pairs of a chunk: few, so that there are waves for every CU, and more where there are enough (4096), since each
-// chunk leaves two rows of parts to be joined; never more than four million waves.  (5,003 x 771: 28 us with 16
-// pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
+// chunk leaves two rows of parts to be joined; and so few that a launch counts its threads with 32 bits.  Waves are
+// counted as if every lane held eight elements and none were idle: four million by this count are at most sixteen
+// (rows of 257 to 264 elements of 32 bits), 2^30 threads beside the 2^31 that zeros take.  (5,003 x 771: 28 us with
+// 16 pairs, 42 with 64; 64 x 64: 7 and 17; 32,768 x 4096, parts and all: 385 us with 16, 366 with 64.)
 unsigned ChunkOf(unsigned m, int dim) {
   const bool wide = dim > kNarrow;
   const unsigned most = wide ? 256 : 1024;
