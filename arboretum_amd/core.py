@@ -181,7 +181,8 @@ def embedding(out, table, tokens, n, vocab, dim, bag=1, scale=1.0, dtype="float3
 
 def embedding_sort_bytes(n, vocab, bag=1):
     """Bytes of device memory embedding_sort works in (AEmbeddingSortBytes; no GPU needed)."""
-    _refuse_wide((bag,), (n, vocab))
+    if bag >> 31 or (n | vocab) >> 63:
+        _refuse_wide((bag,), (n, vocab))
     v = ctypes.c_ulonglong()
     _check(_LIB.AEmbeddingSortBytes(n, bag, vocab, ctypes.byref(v)))
     return v.value
@@ -200,7 +201,8 @@ def embedding_sort(keys, rows, tokens, n, vocab, work, work_bytes, bag=1, token_
 
 def embedding_grad_bytes(n, dim, bag=1):
     """Bytes of device memory embedding_grad works in (AEmbeddingGradBytes; no GPU needed)."""
-    _refuse_wide((bag, dim), (n,))
+    if (bag | dim) >> 31 or n >> 63:
+        _refuse_wide((bag, dim), (n,))
     v = ctypes.c_ulonglong()
     _check(_LIB.AEmbeddingGradBytes(n, bag, dim, ctypes.byref(v)))
     return v.value
@@ -237,7 +239,9 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta
     read instead of lr and step.  Does not wait."""
     lists = (params, grads, exp_avgs, exp_avg_sqs, sizes)
     try:  # the five lists one after the other
-        table = np.array(lists, dtype=np.int64) if all(map(_whole, lists)) else None
+        table = np.array(lists)
+        if table.dtype.char != "l":  # other integers than 64-bit ones, or other than integers
+            table = np.array(lists, dtype=np.int64) if all(map(_whole, lists)) else None
     except (ValueError, TypeError, OverflowError):
         table = None
     if table is None or table.ndim != 2:
