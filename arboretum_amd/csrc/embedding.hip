@@ -136,9 +136,10 @@ __global__ void __launch_bounds__(kThreads) k_embedding_one(const Bags<Token> ba
 
 // Bags of several tokens.  A row of the result is 2^lanes_log lanes wide (kVec elements a lane), and 2^shares_log
 // shares of them take every so many-th token each and meet in the end, by steps of halves.  kAhead tokens of a lane
-// are in flight; where there is no token the last row of the table is read and not added.  Four at a time are summed
-// before they join the sum of those before them: no more additions than one after the other, and a quarter of a
-// chain's error.  (All eight: 89 registers for 63, and 2 % slower.)
+// are in flight; where there is no token the last row of the table is read and not added.  All eight are summed before
+// they join the sum of those before them: no more additions than one after the other, and an eighth of a chain's
+// error.  (Rows of 16 bits, eight elements a lane, four at a time: eight take 89 registers for 63 and 2 % of the time,
+// and the result is rounded to 2^-8 or 2^-11.)
 constexpr int kAhead = 8;
 __device__ __forceinline__ float SumOfFour(const float (&x)[4]) { return (x[0] + x[1]) + (x[2] + x[3]); }
 template <typename T, int kVec, typename Token>
@@ -149,6 +150,7 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
   const unsigned lane = threadIdx.x & ((1u << lanes_log) - 1u);
   const unsigned share = (threadIdx.x >> lanes_log) & ((1u << shares_log) - 1u), shares = 1u << shares_log;
   const int column = ((int)blockIdx.y << lanes_log) * kVec + (int)lane * kVec, d = min(column, r.dim - kVec);
+  constexpr bool kEights = sizeof(T) == 4;
   float sum[kVec];
 #pragma unroll
   for (int c = 0; c < kVec; ++c) sum[c] = 0.0f;
@@ -162,13 +164,15 @@ k_embedding_bag(const Bags<Token> bags, const Rows<T> r, int lanes_log, int shar
         x[k] = *reinterpret_cast<const Pack<T, kVec> *>(table + (long long)min(bags.Row(token[k]), bags.vocab - 1u) * r.table_stride);
 #pragma unroll
       for (int c = 0; c < kVec; ++c) {
+        float part = kEights ? 0.0f : sum[c];
 #pragma unroll
         for (int h = 0; h < kAhead; h += 4) {
           float y[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) y[k] = bags.Row(token[h + k]) < bags.vocab ? static_cast<float>(x[h + k].v[c]) : 0.0f;
-          sum[c] += SumOfFour(y);
+          part = kEights && h == 0 ? SumOfFour(y) : part + SumOfFour(y);
         }
+        sum[c] = kEights ? sum[c] + part : part;
       }
       if (blockIdx.y == 0 && lane == 0) bags.Report(token);
     };
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) k_embedding_columns(const Bags<Token
         if (j + c >= bags.bag) next[c][k] = Token(-1);
     }
   };
-  float sum[kBagsOfThread] = {};
+  float sum[kBagsOfThread] = {}, part[kBagsOfThread] = {};  // of the columns before, of up to sixteen since
   fetch(0);
   for (int j = 0; j < bags.bag; j += kColumns) {
     unsigned t[kColumns][kBagsOfThread];
@@ -256,10 +260,17 @@ __global__ void __launch_bounds__(kThreads) k_embedding_columns(const Bags<Token
       float y[kColumns];
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) y[c] = t[c][k] < bags.vocab ? x[c][k] : 0.0f;
-      sum[k] += SumOfFour(y);
+      part[k] += SumOfFour(y);
+    }
+    if ((j / kColumns) % 4 == 3) {
+#pragma unroll
+      for (int k = 0; k < kBagsOfThread; ++k) {
+        sum[k] += part[k];
+        part[k] = 0.0f;
+      }
     }
   }
-  for (int k = 0; k < held; ++k) r.out[(first + k) * r.out_stride] = Round<T>(sum[k] * r.scale);
+  for (int k = 0; k < held; ++k) r.out[(first + k) * r.out_stride] = Round<T>((sum[k] + part[k]) * r.scale);
 }
 
 int LogAtLeast(long long v) {

@@ -15,17 +15,21 @@ def arb():
     return arboretum_amd
 
 
-# A bag's tokens are summed four at a time, in pairs, and such a sum joins what came before: no element takes part in more
-# than two additions of pairs, bag / 4 + 1 of what came before, and six where lanes share a bag; one rounding more for
-# the scale.  So a sum is off by at most (bag / 4 + 12) u of the sum of magnitudes (a chain of additions: bag u).
+# A bag's tokens are summed eight at a time (rows of 16 bits: four) before such a sum joins what came before; columns of scalars in fours, and
+# four of these.  No element takes part in more than four additions within, bag / 8 + 1 (bag / 4 + 1) of what came before, six where lanes share
+# a bag, and two roundings at the end: a sum is off by at most (bag / 8 + 14) u of the sum of magnitudes, or bag / 4 + 14 (a
+# chain of additions: bag u).
+def additions(bag, dtype):
+    return bag / (8 if dtype == "float32" else 4) + 14
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("n,bag,dim,columns", [(70_000, 200, 1, True), (70_000, 199, 3, True), (64, 200, 512, False), (64, 203, 1100, True),
                                                (5000, 200, 16, False), (3, 2001, 1, False), (MANY // 200 + 5, 200, 1, True)])
 def test_small_numbers_behind_a_large_one_are_not_lost(arb, n, bag, dim, columns, dtype):
-    # 1 and then half of the last place of 1, again and again: added one at a time, each would be rounded away
+    # 1 and then less than half of the last place of 1, again and again: added one at a time, each would be rounded away
     T = TYPES[dtype]
-    small = U / 2 if dtype == "float32" else U
-    for first in (0, bag // 2, bag - 1):
+    for first, small in ((0, U / 2), (0, U / 4), (0, U / 8), (bag // 2, U / 4), (bag - 1, U / 4)):
         tokens = torch.ones((bag, n) if columns else (n, bag), dtype=torch.int32, device="cuda")
         tokens[first if columns else slice(None), slice(None) if columns else first] = 0
         table = torch.full((2, dim), small, device="cuda", dtype=T)
@@ -34,7 +38,7 @@ def test_small_numbers_behind_a_large_one_are_not_lost(arb, n, bag, dim, columns
         arb.embedding(out.data_ptr(), table.data_ptr(), tokens.data_ptr(), n, 2, dim, bag=bag, dtype=dtype,
                       token_stride=1 if columns else bag, bag_stride=n if columns else 1)
         want = torch.full((n, dim), 1 + (bag - 1) * small, dtype=torch.float64)
-        within(out, want, (bag / 4 + 12) * U * want, T)
+        within(out, want, additions(bag, dtype) * U * want, T)
 
 
 # both sides of 512 MB of tokens, and of 2^19 bags, from which on columns of scalars are read four bags a thread
@@ -55,7 +59,7 @@ def test_columns_of_scalars_on_both_sides_of_the_rule(arb, n, bag, bits):
         x = held[one.long()]  # (-1: the zero at the end)
         want += x
         mag += x.abs()
-    within(out[:n], want.cpu(), (bag / 4 + 12) * U * mag.cpu(), torch.float32)
+    within(out[:n], want.cpu(), additions(bag, "float32") * U * mag.cpu(), torch.float32)
     assert out[n].item() == 7.0 and status.item() == 0
 
 
