@@ -206,7 +206,8 @@ struct RefineOptions {
 };
 
 // refine.hip: trains tables[label] (the leaf weights of that label's trees, one after the other), each over its rows of
-// `tokens` (LeavesOnDevice), against the objective of `cfg` and the target of `data`, starting from `init`.
+// `tokens` (LeavesOnDevice), against the objective of `cfg` and the target of `data`, starting from `init`.  Every label
+// has trees.
 void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *tokens, size_t token_ld,
                     const std::vector<size_t> &trees_of, std::vector<std::vector<float>> *tables, float init, const RefineOptions &options);
 

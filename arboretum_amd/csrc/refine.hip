@@ -81,10 +81,8 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
   for (size_t k = 0; k < K; ++k) {
     const size_t leaves = (*tables)[k].size(), pairs = trees_of[k] * n;
     Table &t = of[k];
-    t.bags = TokenBags{tokens + column * token_ld, 32, (long long)n, (int)trees_of[k], 1, (long long)token_ld,
-                       (long long)std::max<size_t>(leaves, 1), nullptr};
+    t.bags = TokenBags{tokens + column * token_ld, 32, (long long)n, (int)trees_of[k], 1, (long long)token_ld, (long long)leaves, nullptr};
     column += trees_of[k];
-    if (leaves == 0) continue;
     t.weight = work.Take<float>(4 * leaves);
     t.grad = t.weight + leaves;
     t.m = t.grad + leaves;
@@ -103,7 +101,6 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
   std::vector<long long> sizes;
   for (size_t k = 0; k < K; ++k) {
     const std::vector<float> &table = (*tables)[k];
-    if (table.empty()) continue;
     const Table &t = of[k];
     HIP_OK(hipMemcpyAsync(t.weight, table.data(), table.size() * sizeof(float), hipMemcpyHostToDevice, work.stream));
     HIP_OK(hipMemsetAsync(t.m, 0, 2 * table.size() * sizeof(float), work.stream));
@@ -118,8 +115,8 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
   const dim3 grid = grid_of(n);
   const float most = std::fabs(cfg.tree.max_leaf_weight * cfg.tree.eta);
   for (int step = 1; step <= options.steps; ++step) {
-    for (size_t k = 0; k < K; ++k)  // (a class without trees has a sum of 0: bags of no tokens)
-      Embedding(EmbeddingArgs{of[k].bags, of[k].weight ? of[k].weight : y_hat, 1, y_hat + k * n, 1, 1, kFloat32, 1.0f, work.stream});
+    for (size_t k = 0; k < K; ++k)
+      Embedding(EmbeddingArgs{of[k].bags, of[k].weight, 1, y_hat + k * n, 1, 1, kFloat32, 1.0f, work.stream});
     if (cfg.objective == kLinearRegression)
       hipLaunchKernelGGL(k_direction_squared, grid, dim3(256), 0, work.stream, y.get(), y_hat, init, n);
     else if (cfg.objective == kLogisticRegression)
@@ -128,7 +125,6 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
       hipLaunchKernelGGL(k_direction_softmax, grid, dim3(256), 0, work.stream, labels.get(), y_hat, n, (int)K);
     HIP_OK(hipGetLastError());
     for (size_t k = 0; k < K; ++k) {
-      if (!of[k].weight) continue;
       EmbeddingGrad(EmbeddingGradArgs{of[k].keys, of[k].rows, (long long)n, of[k].bags.bag, of[k].bags.vocab, y_hat + k * n, 1, of[k].grad, 1,
                                       1, kFloat32, kFloat32, (float)(-1.0 / (double)n), false, scratch, scratch_bytes, work.stream});
     }
@@ -137,12 +133,12 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
                     work.stream});
     if (cfg.tree.max_leaf_weight == 0.0f) continue;
     for (size_t k = 0; k < K; ++k)
-      if (of[k].weight) hipLaunchKernelGGL(k_limit, grid_of((*tables)[k].size()), dim3(256), 0, work.stream, of[k].weight, most, (*tables)[k].size());
+      hipLaunchKernelGGL(k_limit, grid_of((*tables)[k].size()), dim3(256), 0, work.stream, of[k].weight, most, (*tables)[k].size());
     HIP_OK(hipGetLastError());
   }
   for (size_t k = 0; k < K; ++k) {
     std::vector<float> &table = (*tables)[k];
-    if (!table.empty()) HIP_OK(hipMemcpyAsync(table.data(), of[k].weight, table.size() * sizeof(float), hipMemcpyDeviceToHost, work.stream));
+    HIP_OK(hipMemcpyAsync(table.data(), of[k].weight, table.size() * sizeof(float), hipMemcpyDeviceToHost, work.stream));
   }
   HIP_OK(hipStreamSynchronize(work.stream));
 }
