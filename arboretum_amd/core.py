@@ -86,6 +86,18 @@ def _load_lib():
         "AGardenLeafTokens": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p, c_int],
         "AGardenRefineLeaves": [c_void_p, c_void_p, c_int] + [ctypes.c_double] * 5,
         "AAdamW": [c_int] + [c_void_p] * 5 + [c_int, c_int] + [ctypes.c_double] * 6 + [c_long] + [c_void_p] * 3,
+        "ALogProbsBytes": [c_long, c_long, c_int, P(ctypes.c_ulonglong)],
+        "ALogProbs": [c_void_p] * 7 + [c_long, c_long, c_int, c_long, c_long, c_int, c_int, c_float, c_void_p,
+                                       ctypes.c_ulonglong, c_void_p, c_void_p],
+        "ALogProbsGrad": [c_void_p] * 7 + [c_long] * 6 + [c_int, c_int, c_float, c_void_p, c_void_p],
+        "AActivationCheckpoint": [c_void_p] * 3 + [c_long, c_int, c_long, c_int, c_void_p],
+        "AActivationRestore": [c_void_p] * 3 + [c_long, c_int, c_long, c_int, c_void_p],
+        "AGatedBytes": [c_long, c_int, c_int, c_int, P(ctypes.c_ulonglong)],
+        "AGated": [c_void_p] * 8 + [c_long, c_int, c_int] + [c_long] * 4 + [c_int, c_int, c_void_p, ctypes.c_ulonglong,
+                                                                           c_void_p],
+        "AGatedGradBytes": [c_long, c_int, c_int, c_int, P(ctypes.c_ulonglong)],
+        "AGatedGrad": [c_void_p] * 11 + [c_long, c_int, c_int] + [c_long] * 6 + [c_int, c_int, c_void_p, ctypes.c_ulonglong,
+                                                                                c_void_p],
     }
     for name, args in sigs.items():
         fn = getattr(lib, name)
@@ -252,6 +264,124 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, sizes, step, lr, beta1=0.9, beta
     _check(_LIB.AAdamW(count, at, at + 8 * count, at + 16 * count, at + 24 * count, at + 32 * count, _type(dtype),
                        _type(dtype if grad_dtype is None else grad_dtype), lr, beta1, beta2, eps, weight_decay, grad_scale,
                        step, lr_device, step_device, stream))
+
+
+def log_probs_bytes(n, vocab, top=0):
+    """Bytes of device memory log_probs works in (ALogProbsBytes; no GPU needed); may be 0."""
+    if top >> 31 or (n | vocab) >> 63:
+        _refuse_wide((top,), (n, vocab))
+    v = ctypes.c_ulonglong()
+    _check(_LIB.ALogProbsBytes(n, vocab, top, ctypes.byref(v)))
+    return v.value
+
+
+def log_probs(log_probs, logits, tokens, n, vocab, work, work_bytes, entropy=None, stats=None, top=0, top_tokens=None, top_log_probs=None,
+              scale=1.0, dtype="float32", token_bits=32, row_stride=None, class_stride=1, status=None, stream=None):
+    """Log probabilities of one token a row under softmax(scale * logits) on the GPU (ALogProbs), the entropy of each row, and its
+    `top` likeliest tokens in order with theirs.  Array arguments are DEVICE addresses: log_probs, entropy float32 [n], stats
+    float32 [n][2] (for log_probs_grad), top_tokens int32 and top_log_probs float32 [n][top]; class j of row i is at
+    i * row_stride + j * class_stride.  A token of -1 has the log probability 0; tokens and log_probs may both be None.
+    `work`: log_probs_bytes() of device memory.  Does not wait."""
+    row_stride = vocab if row_stride is None else row_stride
+    if (top | token_bits) >> 31 or (n | vocab | row_stride | class_stride) >> 63:
+        _refuse_wide((top, token_bits), (n, vocab, row_stride, class_stride))
+    _check(_LIB.ALogProbs(log_probs, entropy, stats, top_tokens, top_log_probs, logits, tokens, n, vocab, top, row_stride, class_stride,
+                          _type(dtype), token_bits, scale, work, max(work_bytes, 0), status, stream))
+
+
+def log_probs_grad(grad_logits, grad_log_probs, logits, tokens, stats, n, vocab, grad_entropy=None, entropy=None, scale=1.0, dtype="float32",
+                   token_bits=32, row_stride=None, class_stride=1, grad_row_stride=None, grad_class_stride=None, status=None,
+                   stream=None):
+    """Gradient of log_probs()' logits (ALogProbsGrad), of their type: scale * (grad_log_probs * ([j == token] - p_j) -
+    grad_entropy * p_j * (log p_j + entropy)).  stats, entropy: of log_probs(); grad_log_probs, grad_entropy float32 [n].
+    May be written in the place of the logits.  Strides of the gradient are the logits' unless given.  Does not wait."""
+    row_stride = vocab if row_stride is None else row_stride
+    grad_row_stride = row_stride if grad_row_stride is None else grad_row_stride
+    grad_class_stride = class_stride if grad_class_stride is None else grad_class_stride
+    if token_bits >> 31 or (n | vocab | row_stride | class_stride | grad_row_stride | grad_class_stride) >> 63:
+        _refuse_wide((token_bits,), (n, vocab, row_stride, class_stride, grad_row_stride, grad_class_stride))
+    _check(_LIB.ALogProbsGrad(grad_logits, grad_log_probs, grad_entropy, logits, tokens, stats, entropy, n, vocab, grad_row_stride,
+                              grad_class_stride, row_stride, class_stride, _type(dtype), token_bits, scale, status, stream))
+
+
+def activation_checkpoint(codes, scales, x, rows, dim, dtype="float32", x_stride=None, stream=None):
+    """Activations [rows][dim] kept in 8 bits on the GPU (AActivationCheckpoint): codes int8 [rows][dim], scales float32
+    [rows][ceil(dim / 64)], one for every 64 elements of a row.  Array arguments are DEVICE addresses.  Does not wait."""
+    x_stride = dim if x_stride is None else x_stride
+    if dim >> 31 or (rows | x_stride) >> 63:
+        _refuse_wide((dim,), (rows, x_stride))
+    _check(_LIB.AActivationCheckpoint(codes, scales, x, rows, dim, x_stride, _type(dtype), stream))
+
+
+def activation_restore(x, codes, scales, rows, dim, dtype="float32", x_stride=None, stream=None):
+    """What activation_checkpoint() has kept, read back into x (AActivationRestore): code * scale.  Does not wait."""
+    x_stride = dim if x_stride is None else x_stride
+    if dim >> 31 or (rows | x_stride) >> 63:
+        _refuse_wide((dim,), (rows, x_stride))
+    _check(_LIB.AActivationRestore(x, codes, scales, rows, dim, x_stride, _type(dtype), stream))
+
+
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _activation(name):
+    try:
+        return _ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ArboretumError(ValueError("activation %r is not one of %s" % (name, ", ".join(_ACTIVATIONS)))) from None
+
+
+def gated_bytes(rows, dim, hidden, dtype="float32"):
+    """Bytes of device memory gated works in (AGatedBytes; no GPU needed); may be 0."""
+    if (dim | hidden) >> 31 or rows >> 63:
+        _refuse_wide((dim, hidden), (rows,))
+    v = ctypes.c_ulonglong()
+    _check(_LIB.AGatedBytes(rows, dim, hidden, _type(dtype), ctypes.byref(v)))
+    return v.value
+
+
+def gated(out, x, w_gate, w_up, rows, dim, hidden, work, work_bytes, gate=None, up=None, gate_scales=None, up_scales=None,
+          activation="silu", dtype="float32", out_stride=None, kept_stride=None, x_stride=None, w_stride=None, stream=None):
+    """out = act(x w_gate^T) * (x w_up^T) on the GPU (AGated): x [rows][dim], weights [hidden][dim], out [rows][hidden], DEVICE
+    addresses; activation "silu" or "gelu".  gate, up: where both products are kept for gated_grad(), of `dtype`, or, with
+    gate_scales and up_scales, in 8 bits as activation_checkpoint() keeps them.  `work`: gated_bytes() of device memory.
+    Does not wait."""
+    out_stride = hidden if out_stride is None else out_stride
+    kept_stride = hidden if kept_stride is None else kept_stride
+    x_stride = dim if x_stride is None else x_stride
+    w_stride = dim if w_stride is None else w_stride
+    if (dim | hidden) >> 31 or (rows | out_stride | kept_stride | x_stride | w_stride) >> 63:
+        _refuse_wide((dim, hidden), (rows, out_stride, kept_stride, x_stride, w_stride))
+    _check(_LIB.AGated(out, gate, up, gate_scales, up_scales, x, w_gate, w_up, rows, dim, hidden, out_stride, kept_stride, x_stride,
+                       w_stride, _type(dtype), _activation(activation), work, max(work_bytes, 0), stream))
+
+
+def gated_grad_bytes(rows, dim, hidden, dtype="float32"):
+    """Bytes of device memory gated_grad works in (AGatedGradBytes; no GPU needed)."""
+    if (dim | hidden) >> 31 or rows >> 63:
+        _refuse_wide((dim, hidden), (rows,))
+    v = ctypes.c_ulonglong()
+    _check(_LIB.AGatedGradBytes(rows, dim, hidden, _type(dtype), ctypes.byref(v)))
+    return v.value
+
+
+def gated_grad(grad_x, grad_w_gate, grad_w_up, grad_out, x, w_gate, w_up, rows, dim, hidden, work, work_bytes, gate, up,
+               gate_scales=None, up_scales=None, activation="silu", dtype="float32", grad_x_stride=None, grad_w_stride=None,
+               grad_out_stride=None, kept_stride=None, x_stride=None, w_stride=None, stream=None):
+    """Gradients of gated()'s input and weights from that of its output (AGatedGrad), with the gate and up (and scales) that it
+    kept.  grad_x, or both of the weights', may be None.  `work`: gated_grad_bytes() of device memory.  The same from run to
+    run.  Does not wait."""
+    grad_x_stride = dim if grad_x_stride is None else grad_x_stride
+    grad_w_stride = dim if grad_w_stride is None else grad_w_stride
+    grad_out_stride = hidden if grad_out_stride is None else grad_out_stride
+    kept_stride = hidden if kept_stride is None else kept_stride
+    x_stride = dim if x_stride is None else x_stride
+    w_stride = dim if w_stride is None else w_stride
+    strides = (grad_x_stride, grad_w_stride, grad_out_stride, kept_stride, x_stride, w_stride)
+    if (dim | hidden) >> 31 or (rows | grad_x_stride | grad_w_stride | grad_out_stride | kept_stride | x_stride | w_stride) >> 63:
+        _refuse_wide((dim, hidden), (rows,) + strides)
+    _check(_LIB.AGatedGrad(grad_x, grad_w_gate, grad_w_up, grad_out, x, w_gate, w_up, gate, up, gate_scales, up_scales, rows, dim, hidden,
+                           *strides, _type(dtype), _activation(activation), work, max(work_bytes, 0), stream))
 
 
 def _fptr(a):

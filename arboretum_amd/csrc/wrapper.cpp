@@ -493,4 +493,79 @@ const char *AAdamW(int count, void *const *params, const void *const *grads, flo
   });
 }
 
+const char *ALogProbsBytes(long long n, long long vocab, int top, unsigned long long *bytes) {
+  return Guard([&] {
+    if (!bytes) throw std::runtime_error("bad arguments");
+    *bytes = LogProbsBytes(n, vocab, top);
+  });
+}
+
+const char *ALogProbs(float *log_probs, float *entropy, float *stats, int *top_tokens, float *top_log_probs, const void *logits,
+                      const void *tokens, long long n, long long vocab, int top, long long row_stride, long long class_stride,
+                      int type, int token_bits, float scale, void *work, unsigned long long work_bytes, unsigned *status,
+                      void *stream) {
+  return Guard([&] {
+    LogProbs(LogProbsArgs{{logits, n, vocab, row_stride, class_stride, type, scale, tokens, token_bits, status}, log_probs, entropy, stats,
+                          top, top_tokens, top_log_probs, work, work_bytes, stream});
+  });
+}
+
+const char *ALogProbsGrad(void *grad_logits, const float *grad_log_probs, const float *grad_entropy, const void *logits,
+                          const void *tokens, const float *stats, const float *entropy, long long n, long long vocab,
+                          long long grad_row_stride, long long grad_class_stride, long long row_stride, long long class_stride,
+                          int type, int token_bits, float scale, unsigned *status, void *stream) {
+  return Guard([&] {
+    LogProbsGrad(LogProbsGradArgs{{logits, n, vocab, row_stride, class_stride, type, scale, tokens, token_bits, status}, grad_logits,
+                                  grad_row_stride, grad_class_stride, stats, entropy, grad_log_probs, grad_entropy, stream});
+  });
+}
+
+const char *AActivationCheckpoint(signed char *codes, float *scales, const void *x, long long rows, int dim, long long x_stride,
+                                  int type, void *stream) {
+  return Guard([&] { ActivationCheckpoint(CheckpointArgs{codes, scales, const_cast<void *>(x), rows, dim, x_stride, type, stream}); });
+}
+
+const char *AActivationRestore(void *x, const signed char *codes, const float *scales, long long rows, int dim,
+                               long long x_stride, int type, void *stream) {
+  return Guard([&] {
+    ActivationRestore(CheckpointArgs{const_cast<signed char *>(codes), const_cast<float *>(scales), x, rows, dim, x_stride, type, stream});
+  });
+}
+
+const char *AGatedBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes) {
+  return Guard([&] {
+    if (!bytes) throw std::runtime_error("bad arguments");
+    *bytes = GatedBytes(rows, dim, hidden, type);
+  });
+}
+
+const char *AGated(void *out, void *gate, void *up, float *gate_scales, float *up_scales, const void *x, const void *w_gate,
+                   const void *w_up, long long rows, int dim, int hidden, long long out_stride, long long kept_stride,
+                   long long x_stride, long long w_stride, int type, int activation, void *work, unsigned long long work_bytes,
+                   void *stream) {
+  return Guard([&] {
+    Gated(GatedArgs{{x, w_gate, w_up, rows, dim, hidden, x_stride, w_stride, type, activation, gate, up, gate_scales, up_scales, kept_stride,
+                     work, work_bytes, stream}, out, out_stride});
+  });
+}
+
+const char *AGatedGradBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes) {
+  return Guard([&] {
+    if (!bytes) throw std::runtime_error("bad arguments");
+    *bytes = GatedGradBytes(rows, dim, hidden, type);
+  });
+}
+
+const char *AGatedGrad(void *grad_x, void *grad_w_gate, void *grad_w_up, const void *grad_out, const void *x, const void *w_gate,
+                       const void *w_up, const void *gate, const void *up, const float *gate_scales, const float *up_scales,
+                       long long rows, int dim, int hidden, long long grad_x_stride, long long grad_w_stride,
+                       long long grad_out_stride, long long kept_stride, long long x_stride, long long w_stride, int type,
+                       int activation, void *work, unsigned long long work_bytes, void *stream) {
+  return Guard([&] {
+    GatedGrad(GatedGradArgs{{x, w_gate, w_up, rows, dim, hidden, x_stride, w_stride, type, activation, const_cast<void *>(gate),
+                             const_cast<void *>(up), const_cast<float *>(gate_scales), const_cast<float *>(up_scales), kept_stride, work,
+                             work_bytes, stream}, grad_out, grad_out_stride, grad_x, grad_x_stride, grad_w_gate, grad_w_up, grad_w_stride});
+  });
+}
+
 }  // extern "C"

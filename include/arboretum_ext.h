@@ -264,6 +264,76 @@ const char *AAdamW(int count, void *const *params, const void *const *grads, flo
                    double beta2, double eps, double weight_decay, double grad_scale, long long step,
                    const float *lr_device, const long long *step_device, void *stream);
 
+/* ---- The operators of a model on top of embeddings: its loss, its layers, and what they keep for the backward pass.
+ *
+ * As above: EVERY POINTER IS A DEVICE POINTER; the calls enqueue on `stream` of the device that their outputs are on, return
+ * WITHOUT waiting, allocate nothing, may be captured, and hold nothing from one call for the next.  Element types 0
+ * float32, 1 bfloat16, 2 float16, and each result is rounded once, to nearest, from float32.  Strides count elements; rows may
+ * begin at any element.  work: 16-byte aligned, of the size that the call's ...Bytes gives (NULL where that is 0), undefined
+ * before and after; calls that may run at the same time need work memory of their own. */
+
+/* Log probabilities under n rows of `vocab` classes: class j of row i is logits[i * row_stride + j * class_stride], so rows
+ * may be classes side by side (class_stride 1, a model's logits) or class by class (row_stride 1, a booster's scores).
+ * With x = scale * logits (scale > 0: the inverse of a temperature), in float32:
+ *   log_probs[i] = log softmax(x[i])[token i], 0 where the token is -1 (as any other outside [0, vocab), which sets
+ *                  *status to 1); tokens and log_probs are both given or both NULL
+ *   entropy[i]   = -sum softmax(x[i]) log softmax(x[i]); may be NULL
+ *   stats[i]     = (greatest logit, log sum exp(x - scale * it)), two floats for ALogProbsGrad; may be NULL
+ *   top_tokens, top_log_probs [n][top]: the `top` (0 to 64, at most vocab) greatest logits in order, equal ones by their
+ *                  index, and their log probabilities
+ * Logits may be minus infinity: their probability is 0.  A row of nothing else has log probabilities of minus infinity, the
+ * entropy 0 and the first `top` tokens.  A row with a NaN or with plus infinity has NaN for all, and -1 for its top tokens.
+ * n and vocab are below 2^31 (vocab by 65,536). */
+const char *ALogProbsBytes(long long n, long long vocab, int top, unsigned long long *bytes);
+const char *ALogProbs(float *log_probs, float *entropy, float *stats, int *top_tokens, float *top_log_probs, const void *logits,
+                      const void *tokens, long long n, long long vocab, int top, long long row_stride, long long class_stride,
+                      int type, int token_bits, float scale, void *work, unsigned long long work_bytes, unsigned *status,
+                      void *stream);
+
+/* The gradient of ALogProbs' logits (same tokens and scale): with p = softmax(x[i]),
+ *   grad_logits[i][j] = scale * (grad_log_probs[i] * ([j == token i] - p_j)
+ *                                - grad_entropy[i] * p_j * (log p_j + entropy[i]))
+ * grad_entropy and entropy are both given or both NULL.  A row without a token has no part of the first kind, whatever
+ * its grad_log_probs; logits of minus infinity, and rows of nothing else, have the gradient 0.  grad_logits has the logits' type,
+ * and may be the logits themselves (same strides); otherwise the two must not overlap. */
+const char *ALogProbsGrad(void *grad_logits, const float *grad_log_probs, const float *grad_entropy, const void *logits,
+                          const void *tokens, const float *stats, const float *entropy, long long n, long long vocab,
+                          long long grad_row_stride, long long grad_class_stride, long long row_stride, long long class_stride,
+                          int type, int token_bits, float scale, unsigned *status, void *stream);
+
+/* Activations kept in 8 bits for a backward pass, and read back: codes [rows][dim] back to back, a scale for every 64
+ * elements of a row, scales [rows][ceil(dim / 64)] (the last of a row for what is left).
+ *   scale = max |x| / 127 (at least 2^-100),  code = x / scale rounded to nearest;  x is read back as code * scale
+ * An element comes back off by at most half a scale (and the rounding to its type); 64 elements with an infinity or a NaN among
+ * them come back as NaN. */
+const char *AActivationCheckpoint(signed char *codes, float *scales, const void *x, long long rows, int dim, long long x_stride,
+                                  int type, void *stream);
+const char *AActivationRestore(void *x, const signed char *codes, const float *scales, long long rows, int dim,
+                               long long x_stride, int type, void *stream);
+
+/* A gated layer: out = act(x w_gate^T) * (x w_up^T), x [rows][dim], weights [hidden][dim] (w_stride: of both), out
+ * [rows][hidden].  activation: 0 silu, 1 gelu (by the error function).  Products are summed in float32.
+ * gate, up: what the backward pass needs, x w_gate^T and x w_up^T [rows][hidden] (kept_stride: of both) of `type`, or with
+ * gate_scales and up_scales given as codes of 8 bits with scales [rows][ceil(hidden / 64)], as of AActivationCheckpoint.  All may
+ * be NULL.  dim and hidden are 1 to 2^24, rows below 2^31 (0 for none). */
+const char *AGatedBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes);
+const char *AGated(void *out, void *gate, void *up, float *gate_scales, float *up_scales, const void *x, const void *w_gate,
+                   const void *w_up, long long rows, int dim, int hidden, long long out_stride, long long kept_stride,
+                   long long x_stride, long long w_stride, int type, int activation, void *work, unsigned long long work_bytes,
+                   void *stream);
+
+/* Its gradients, given that of out: with the gate and up that AGated kept (and the same scales),
+ *   d_gate = grad_out * up * act'(gate),  d_up = grad_out * act(gate)     (rounded to `type`, as the products take them)
+ *   grad_x = d_gate w_gate + d_up w_up,  grad_w_gate = d_gate^T x,  grad_w_up = d_up^T x
+ * grad_x, or both gradients of the weights, may be NULL; rows == 0 gives weights' gradients of 0.  Results are the same
+ * from run to run. */
+const char *AGatedGradBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes);
+const char *AGatedGrad(void *grad_x, void *grad_w_gate, void *grad_w_up, const void *grad_out, const void *x, const void *w_gate,
+                       const void *w_up, const void *gate, const void *up, const float *gate_scales, const float *up_scales,
+                       long long rows, int dim, int hidden, long long grad_x_stride, long long grad_w_stride,
+                       long long grad_out_stride, long long kept_stride, long long x_stride, long long w_stride, int type,
+                       int activation, void *work, unsigned long long work_bytes, void *stream);
+
 /* The leaf every row of `data` reaches in each of the first n_rounds trees (-1: all): tokens[t * stride + row],
  * DEVICE memory for 32-bit words of which nothing pending may make use, stride >= rows.  The trees of a class
  * stand together (by class, then in the order they grew), and the leaves are numbered through the trees of a
