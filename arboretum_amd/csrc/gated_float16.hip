@@ -1,0 +1,7 @@
+// The gated layer's kernels in float16.
+#include "gated_kernels.h"
+
+namespace arb {
+template void RunGated<_Float16>(const GatedArgs &a, bool large);
+template void RunGatedGrad<_Float16>(const GatedGradArgs &a, const GatedPlan &plan);
+}  // namespace arb

@@ -1,0 +1,585 @@
+// A gated layer and its gradient.  With g = x Wg^T, u = x Wu^T (weights [hidden][dim]),
+//   out = act(g) u,  silu(g) = g / (1 + e^-g),  gelu(g) = g Phi(g);
+//   dg = grad u act'(g),  du = grad act(g),  grad_x = dg Wg + du Wu,  grad_Wg = dg^T x,  grad_Wu = du^T x.
+// Products by matrix instructions, their sums in 32 bits.
+#ifndef ARBORETUM_AMD_GATED_KERNELS_H_
+#define ARBORETUM_AMD_GATED_KERNELS_H_
+#include <algorithm>
+#include <type_traits>
+
+#include "checkpoint.h"
+#include "gated_launch.h"
+#include "operators_device.h"
+
+namespace arb {
+namespace {
+
+typedef float F4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of an operand: what a lane gives to a product.
+template <typename T>
+struct alignas(16) Chunk {
+  T v[16 / sizeof(T)];
+};
+
+// acc[r] += sum over k of a(row 4 (lane / 16) + r, k) b(row lane % 16, k); a lane's chunk is its row lane % 16 at the
+// k's number lane / 16 of as many.
+__device__ __forceinline__ F4 Product(const Chunk<__bf16> &a, const Chunk<__bf16> &b, F4 acc) {
+  typedef __bf16 V __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ F4 Product(const Chunk<_Float16> &a, const Chunk<_Float16> &b, F4 acc) {
+  typedef _Float16 V __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ F4 Product(const Chunk<float> &a, const Chunk<float> &b, F4 acc) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc, 0, 0, 0);
+  return acc;
+}
+
+// ------------------------------------------------------------------ activations
+
+__device__ __forceinline__ float Sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+
+template <int kAct>
+__device__ __forceinline__ float Act(float g) {
+  if (kAct == kSilu) return g * Sigmoid(g);
+  return 0.5f * g * erfcf(-0.70710678118654752f * g);
+}
+
+// act(g) and act'(g)
+template <int kAct>
+__device__ __forceinline__ void ActAndSlope(float g, float *act, float *slope) {
+  if (kAct == kSilu) {
+    const float s = Sigmoid(g);
+    *act = g * s;
+    *slope = s + *act * (1.0f - s);
+  } else {
+    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    *act = g * phi;
+    *slope = phi + g * (0.39894228040143268f * expf(-0.5f * g * g));
+  }
+}
+
+// ------------------------------------------------------------------ matrix products
+
+// C[i][j] = sum over segments and k of A(i, k) B(j, k); a batch of two such products.
+// An operand lies row by row with its k's side by side, or (ACROSS) k by k with its rows side by side.
+struct Operand {
+  const void *at[2];  // of each segment, or of each member of the batch
+  long long stride;   // between rows, or between k's
+};
+struct Products {
+  Operand a, b;
+  long long rows;  // of A
+  int columns;     // of C: rows of B
+  long long inner;  // k's of a segment
+  int segments;    // 1, or 2: C sums over both
+  int batch;       // 1, or 2
+  void *c[2];
+  long long c_stride;
+  // the k's of a tile shared out
+  int splits;
+  long long split_blocks;  // blocks of k's of each
+  float *partial;          // [batch][splits][rows][columns] where there are several
+};
+
+constexpr unsigned kNowhere = 0x80000000u;  // offset beyond every operand: a load from there gives 0
+
+typedef int I4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) unsigned char LdsByte;
+typedef __attribute__((address_space(3))) I4 LdsI4;
+
+// The chunks of an operand's block in the LDS.  Along k: line by line, 8 chunks each; across: k by k, the chunks of all lines.
+// Chunks change places from line to line (from k to k), so that the lanes that read together meet other banks: they
+// read one chunk of 16 lines, of which two make up all banks; or 32 bytes (16 lines of 16 bits) of eight k's, 64 bytes of four k's of 32 bits.
+template <typename T, int kLines, bool kAcross>
+struct Layout {
+  static constexpr int kVec = 16 / sizeof(T), kRowChunks = kAcross ? kLines / kVec : 8;
+  static __device__ __forceinline__ int Swap(int row) {
+    if (!kAcross) return (row >> 1) & 7;
+    if (sizeof(T) == 2) return (((row & 3) | ((row >> 1) & 4)) << 1) & (kRowChunks - 1);
+    return (row & 12) & (kRowChunks - 1);
+  }
+  static __device__ __forceinline__ int At(int row, int chunk) { return (row * kRowChunks + (chunk ^ Swap(row))) * 16; }
+  // The chunk of a product for line `line` (of lane % 16) and the quarter `quarter` of the k's of half `half`.
+  static __device__ __forceinline__ Chunk<T> Read(const LdsByte *block, int first, int half) {
+    const int lane = threadIdx.x & 63, quarter = lane / 16, l = lane % 16;
+    if constexpr (!kAcross) {
+      return __builtin_bit_cast(Chunk<T>, *(const LdsI4 *)(block + At(first + l, half * 4 + quarter)));
+    } else if constexpr (sizeof(T) == 2) {
+      // (16 lanes name the 8-byte pieces of four k's by 16 lines, and each gets the four k's of one line)
+      typedef short S4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) S4 LdsS4;
+      const int k = half * 32 + quarter * 8 + l / 4, chunk = first / 8 + l % 4 / 2, in = l % 2 * 8;
+      const S4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4 *)(block + At(k, chunk) + in));
+      const S4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4 *)(block + At(k + 4, chunk) + in));
+      struct Both {
+        S4 low, high;
+      };
+      return __builtin_bit_cast(Chunk<T>, (Both{low, high}));
+    } else {
+      Chunk<T> c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        c.v[e] = *(const __attribute__((address_space(3))) float *)(block + At(half * 16 + quarter * 4 + e, (first + l) / 4) + (first + l) % 4 * 4);
+      return c;
+    }
+  }
+};
+
+// Rows of an operand, `lines` of which are there from `base` on.
+template <typename T>
+struct PlainRows {
+  const T *base;
+  long long stride, lines;
+  __device__ __forceinline__ const T *Base(int) const { return base; }
+  __device__ __forceinline__ int Number(int row) const { return row; }
+  __device__ __forceinline__ bool Held(int row) const { return row < lines; }
+  __device__ __forceinline__ long long Clamped(int row) const { return min((long long)row, lines - 1); }
+};
+
+// 64 rows of the gate and the same of up, the next 64, ... (what a workgroup loads at once is of one of the two)
+template <typename T>
+struct PairedRows {
+  const T *gate, *up;
+  long long stride, lines;
+  __device__ __forceinline__ const T *Base(int row) const { return row & 64 ? up : gate; }
+  __device__ __forceinline__ int Number(int row) const { return row / 128 * 64 + row % 64; }
+  __device__ __forceinline__ bool Held(int row) const { return Number(row) < lines; }
+  __device__ __forceinline__ long long Clamped(int row) const { return min((long long)Number(row), lines - 1); }
+};
+
+// One operand's block on its way to the LDS.  kDirect: by loads that write there, for operands whose chunks are aligned and
+// whole; else through registers, whatever the alignment.
+template <typename T, int kLines, int kThreads, bool kAcross, bool kDirect>
+struct Loader {
+  typedef Layout<T, kLines, kAcross> L;
+  static constexpr int kVec = L::kVec, kPieces = kLines * 8 / kThreads;
+  Chunk<T> piece[kDirect ? 1 : kPieces];
+
+  // The block that `rows` (of lines along k, or k by k) stand for, `left` of whose k's, and across `lines` of whose lines, are in
+  // the operand.
+  template <typename Rows>
+  __device__ __forceinline__ void Load(const Rows &rows, long long lines, long long left, LdsByte *block) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (kDirect) {
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(rows.Base(p * kThreads / L::kRowChunks)), 0, 0x7FFFFFFF, 0x00020000);
+        const int q = p * kThreads + threadIdx.x, row = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(row);
+        const bool held = kAcross ? row < left && chunk * kVec < lines : rows.Held(row) && chunk * kVec < left;
+        const unsigned at = held ? ((unsigned)rows.Number(row) * (unsigned)rows.stride + chunk * kVec) * (unsigned)sizeof(T) : kNowhere;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(block + (p * kThreads + wave * 64) * 16), 16, at, 0, 0, 0);
+      }
+    } else {
+      // (lines beyond the operand along k: the last one again, whose results are not stored; k's beyond it are 0)
+      const bool whole = left >= kLineBytes / (int)sizeof(T) && (!kAcross || lines >= kLines);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const int q = p * kThreads + threadIdx.x, row = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(row);
+        const T *from = rows.Base(p * kThreads / L::kRowChunks) + (kAcross ? row : rows.Clamped(row)) * rows.stride + chunk * kVec;
+        if (whole) {
+          piece[p] = __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Pack<T, kVec> *>(from));
+        } else {
+          const long long held = !kAcross ? left - chunk * kVec : row < left ? lines - chunk * kVec : 0;
+#pragma unroll
+          for (int c = 0; c < kVec; ++c) piece[p].v[c] = c < held ? from[c] : T(0);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void Store(LdsByte *block) const {
+    if constexpr (!kDirect) {
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+        *(LdsI4 *)(block + (p * kThreads + threadIdx.x) * 16) = __builtin_bit_cast(I4, piece[p]);
+    }
+  }
+};
+
+// What a wave sums: fragments of 16 rows by 16 columns; a lane holds row lane % 16, columns 4 (lane / 16) + 0 .. 3 of each.
+struct Tile {
+  F4 acc[kWaveI / 16][kWaveJ / 16];
+  __device__ __forceinline__ void Clear() {
+#pragma unroll
+    for (int i = 0; i < kWaveI / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < kWaveJ / 16; ++j) acc[i][j] = F4{0, 0, 0, 0};
+  }
+  template <typename T, typename LayoutA, typename LayoutB>
+  __device__ __forceinline__ void Add(const LdsByte *a, const LdsByte *b, int wave_i, int wave_j) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      Chunk<T> x[kWaveI / 16], y[kWaveJ / 16];
+#pragma unroll
+      for (int i = 0; i < kWaveI / 16; ++i) x[i] = LayoutA::Read(a, wave_i * kWaveI + i * 16, half);
+#pragma unroll
+      for (int j = 0; j < kWaveJ / 16; ++j) y[j] = LayoutB::Read(b, wave_j * kWaveJ + j * 16, half);
+#pragma unroll
+      for (int j = 0; j < kWaveJ / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < kWaveI / 16; ++i) acc[i][j] = Product(y[j], x[i], acc[i][j]);
+    }
+  }
+};
+
+// The blocks of a tile, one after the other: while one is multiplied the next is on its way into the other half of the LDS.
+// load(n, half): block n on its way; store(half): what came through registers, to the LDS; add(half).
+template <bool kDirect, typename LoadFn, typename StoreFn, typename AddFn>
+__device__ __forceinline__ void RunBlocks(long long blocks, const LoadFn &load, const StoreFn &store, const AddFn &add) {
+  if (blocks <= 0) return;
+  load(0, 0);
+  store(0);
+  for (long long n = 0; n < blocks; ++n) {
+    const int half = (int)(n & 1);
+    if (kDirect) __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();  // (block n is there, and the half that block n + 1 goes to has been read)
+    if (n + 1 < blocks) load(n + 1, half ^ 1);
+    add(half);
+    if (n + 1 < blocks) store(half ^ 1);
+  }
+  __syncthreads();
+}
+
+// Workgroups that follow each other are on different XCDs: each XCD (its L2) gets tiles that lie together, eight rows of them by
+// as many columns as there are.
+__device__ __forceinline__ long long PlaceOfTile(long long id, long long all) {
+  const long long x = id % 8, each = all / 8, rest = all % 8;
+  return x * each + min(x, rest) + id / 8;
+}
+__device__ __forceinline__ void PlaceInGroup(long long tile, long long tile_rows, int tile_columns, long long *i, int *j) {
+  const long long group = tile / (8ll * tile_columns), first = group * 8, rows = min(tile_rows - first, 8ll);
+  const long long in = tile - group * 8 * tile_columns;
+  *i = first + in % rows;
+  *j = (int)(in / rows);
+}
+
+// Four elements of a row from column `at` on, of `columns`.
+template <typename T>
+__device__ __forceinline__ void StoreFour(T *row, long long at, long long columns, const T (&v)[4]) {
+  if (at + 4 <= columns) {
+    *reinterpret_cast<Pack<T, 4> *>(row + at) = Pack<T, 4>{{v[0], v[1], v[2], v[3]}};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (at + r < columns) row[at + r] = v[r];
+  }
+}
+
+struct Forward {
+  const void *x, *w_gate, *w_up;
+  long long rows;
+  int dim, hidden;
+  long long x_stride, w_stride;
+  void *out;
+  long long out_stride;
+  void *gate, *up;
+  float *gate_scales, *up_scales;
+  long long kept_stride;
+};
+
+// What a lane holds of four values in each of four fragments along a row: 16 of a group of 64, the other lanes of its
+// row the rest.
+template <typename T>
+__device__ __forceinline__ void Keep(void *kept, float *scales, long long stride, long long row, int at, int hidden, const F4 *v) {
+  const int quarter = (threadIdx.x & 63) / 16;
+  if (scales == nullptr) {
+    T *to = static_cast<T *>(kept) + row * stride;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const T four[4] = {Round<T>(v[j][0]), Round<T>(v[j][1]), Round<T>(v[j][2]), Round<T>(v[j][3])};
+      StoreFour<T>(to, at + j * 16 + quarter * 4, hidden, four);
+    }
+    return;
+  }
+  float most = 0.0f;  // (columns beyond the layer hold 0)
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) most = Larger(most, fabsf(v[j][r]));
+  most = Larger(most, __shfl_xor(most, 16));
+  most = Larger(most, __shfl_xor(most, 32));
+  const float scale = ScaleOf(most);
+  if (quarter == 0) scales[row * ((hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup] = scale;
+  signed char *to = static_cast<signed char *>(kept) + row * stride;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float four[4] = {v[j][0], v[j][1], v[j][2], v[j][3]};
+    const Pack<signed char, 4> codes = CodesOf(four, scale);
+    StoreFour<signed char>(to, at + j * 16 + quarter * 4, hidden, codes.v);
+  }
+}
+
+static_assert(kWaveJ == 2 * kScaleGroup, "a wave holds whole groups");
+
+// A tile's columns are the gate's and up's of the same hidden ones: 64 of the gate and 64 of up for each wave.
+template <typename T, int kAct, typename S, bool kDirect>
+__global__ void __launch_bounds__(S::kThreads) k_gated(const Forward a, long long tiles, long long tile_rows, int tile_columns) {
+  __shared__ __align__(16) unsigned char s_blocks[2 * S::kBlockBytes];
+  LdsByte *blocks = (LdsByte *)s_blocks;
+  constexpr int kK = kLineBytes / sizeof(T), kHidden = S::kJ / 2;
+  const T *x = static_cast<const T *>(a.x), *w_gate = static_cast<const T *>(a.w_gate), *w_up = static_cast<const T *>(a.w_up);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
+  for (long long id = blockIdx.x; id < tiles; id += gridDim.x) {
+    long long i0;
+    int j0;
+    PlaceInGroup(PlaceOfTile(id, tiles), tile_rows, tile_columns, &i0, &j0);
+    i0 *= S::kI;
+    const int h0 = j0 * kHidden;
+    Tile t;
+    t.Clear();
+    Loader<T, S::kI, S::kThreads, false, kDirect> xs;
+    Loader<T, S::kJ, S::kThreads, false, kDirect> ws;
+    RunBlocks<kDirect>((a.dim + kK - 1) / kK,
+        [&](long long n, int half) {
+          LdsByte *to = blocks + half * S::kBlockBytes;
+          const long long w_at = h0 * a.w_stride + n * kK;
+          xs.Load(PlainRows<T>{x + i0 * a.x_stride + n * kK, a.x_stride, a.rows - i0}, 0, a.dim - n * kK, to);
+          ws.Load(PairedRows<T>{w_gate + w_at, w_up + w_at, a.w_stride, a.hidden - h0}, 0, a.dim - n * kK, to + S::kI * kLineBytes);
+        },
+        [&](int half) {
+          xs.Store(blocks + half * S::kBlockBytes);
+          ws.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
+        },
+        [&](int half) {
+          const LdsByte *from = blocks + half * S::kBlockBytes;
+          t.Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
+        });
+    const int h = h0 + wave_j * (kWaveJ / 2);
+#pragma unroll
+    for (int i = 0; i < kWaveI / 16; ++i) {
+      const long long row = i0 + wave_i * kWaveI + i * 16 + lane % 16;
+      if (row >= a.rows || h >= a.hidden) continue;  // (all four lanes of a row)
+      T *out = static_cast<T *>(a.out) + row * a.out_stride;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        T four[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) four[r] = Round<T>(Act<kAct>(t.acc[i][j][r]) * t.acc[i][j + 4][r]);
+        StoreFour<T>(out, h + j * 16 + lane / 16 * 4, a.hidden, four);
+      }
+      if (a.gate != nullptr) {
+        Keep<T>(a.gate, a.gate_scales, a.kept_stride, row, h, a.hidden, t.acc[i]);
+        Keep<T>(a.up, a.up_scales, a.kept_stride, row, h, a.hidden, t.acc[i] + 4);
+      }
+    }
+  }
+}
+
+template <typename T, bool kAcrossA, bool kAcrossB, typename S, bool kDirect>
+__global__ void __launch_bounds__(S::kThreads) k_products(const Products p, long long tiles, long long tile_rows, int tile_columns) {
+  __shared__ __align__(16) unsigned char s_blocks[2 * S::kBlockBytes];
+  LdsByte *blocks = (LdsByte *)s_blocks;
+  constexpr int kK = kLineBytes / sizeof(T);
+  const long long segment_blocks = (p.inner + kK - 1) / kK, each = tile_rows * tile_columns;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
+  for (long long id = blockIdx.x; id < tiles; id += gridDim.x) {
+    const long long at = PlaceOfTile(id, tiles), one = at / each;
+    const int member = (int)(one / p.splits), split = (int)(one % p.splits);
+    long long i0;
+    int j0;
+    PlaceInGroup(at - one * each, tile_rows, tile_columns, &i0, &j0);
+    i0 *= S::kI;
+    j0 *= S::kJ;
+    Tile t;
+    t.Clear();
+    Loader<T, S::kI, S::kThreads, kAcrossA, kDirect> as;
+    Loader<T, S::kJ, S::kThreads, kAcrossB, kDirect> bs;
+    const long long first = split * p.split_blocks, end = min(first + p.split_blocks, segment_blocks * p.segments);
+    RunBlocks<kDirect>(end - first,
+        [&](long long n, int half) {
+          const int segment = first + n >= segment_blocks;
+          const long long k0 = (first + n - segment * segment_blocks) * kK;
+          const T *a = static_cast<const T *>(p.a.at[member + segment]), *b = static_cast<const T *>(p.b.at[member + segment]);
+          LdsByte *to = blocks + half * S::kBlockBytes;
+          as.Load(PlainRows<T>{kAcrossA ? a + k0 * p.a.stride + i0 : a + i0 * p.a.stride + k0, p.a.stride, p.rows - i0}, p.rows - i0, p.inner - k0, to);
+          bs.Load(PlainRows<T>{kAcrossB ? b + k0 * p.b.stride + j0 : b + j0 * p.b.stride + k0, p.b.stride, p.columns - j0}, p.columns - j0, p.inner - k0,
+                  to + S::kI * kLineBytes);
+        },
+        [&](int half) {
+          as.Store(blocks + half * S::kBlockBytes);
+          bs.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
+        },
+        [&](int half) {
+          const LdsByte *from = blocks + half * S::kBlockBytes;
+          t.Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
+        });
+#pragma unroll
+    for (int i = 0; i < kWaveI / 16; ++i) {
+      const long long row = i0 + wave_i * kWaveI + i * 16 + lane % 16;
+      if (row >= p.rows) continue;
+#pragma unroll
+      for (int j = 0; j < kWaveJ / 16; ++j) {
+        const int column = j0 + wave_j * kWaveJ + j * 16 + lane / 16 * 4;
+        if (p.splits > 1) {
+          const float four[4] = {t.acc[i][j][0], t.acc[i][j][1], t.acc[i][j][2], t.acc[i][j][3]};
+          StoreFour<float>(p.partial + (one * p.rows + row) * p.columns, column, p.columns, four);
+        } else {
+          const T four[4] = {Round<T>(t.acc[i][j][0]), Round<T>(t.acc[i][j][1]), Round<T>(t.acc[i][j][2]), Round<T>(t.acc[i][j][3])};
+          StoreFour<T>(static_cast<T *>(p.c[member]) + row * p.c_stride, column, p.columns, four);
+        }
+      }
+    }
+  }
+}
+
+constexpr int kThreads = 256;  // of the kernels that go element by element
+
+// The sums of what was shared out, in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_products_join(const Products p) {
+  const long long each = p.rows * p.columns, all = each * p.batch;
+  for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < all; e += (long long)gridDim.x * kThreads) {
+    const long long member = e / each, at = e - member * each, row = at / p.columns;
+    const float *from = p.partial + member * p.splits * each + at;
+    float sum = from[0];
+    for (int s = 1; s < p.splits; ++s) sum += from[s * each];
+    static_cast<T *>(p.c[member])[row * p.c_stride + (at - row * p.columns)] = Round<T>(sum);
+  }
+}
+
+// ------------------------------------------------------------------ the layer's own gradient
+
+struct Slopes {
+  const void *grad_out;
+  long long grad_out_stride;
+  const void *gate, *up;
+  const float *gate_scales, *up_scales;
+  long long kept_stride;
+  void *d_gate, *d_up;  // [rows][d_stride]
+  long long d_stride, rows;
+  int hidden;
+};
+
+constexpr int kSlopeVec = 4;
+
+// d_gate and d_up, rounded to the type of the products they enter; 0 in the columns from the layer's end to the next row.
+template <typename T, int kAct>
+__global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks, unsigned row_blocks) {
+  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const long long row = block / row_blocks;
+    const int at = (int)((unsigned)(block - row * row_blocks) * kThreads + threadIdx.x) * kSlopeVec;
+    if (at >= a.d_stride) continue;
+    const T *grad = static_cast<const T *>(a.grad_out) + row * a.grad_out_stride + at;
+    const long long kept = row * a.kept_stride + at;
+    float gate_scale = 0, up_scale = 0;
+    if (a.gate_scales != nullptr) {
+      const long long group = row * ((a.hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup;  // (d_stride ends with the last group)
+      gate_scale = a.gate_scales[group];
+      up_scale = a.up_scales[group];
+    }
+    T dg[kSlopeVec], du[kSlopeVec];
+#pragma unroll
+    for (int c = 0; c < kSlopeVec; ++c) {
+      const bool held = at + c < a.hidden;
+      const float y = held ? (float)grad[c] : 0.0f;
+      float g, u;
+      if (a.gate_scales != nullptr) {
+        g = held ? Restored(static_cast<const signed char *>(a.gate)[kept + c], gate_scale) : 0.0f;
+        u = held ? Restored(static_cast<const signed char *>(a.up)[kept + c], up_scale) : 0.0f;
+      } else {
+        g = held ? (float)static_cast<const T *>(a.gate)[kept + c] : 0.0f;
+        u = held ? (float)static_cast<const T *>(a.up)[kept + c] : 0.0f;
+      }
+      float act, slope;
+      ActAndSlope<kAct>(g, &act, &slope);
+      dg[c] = Round<T>(y * u * slope);
+      du[c] = Round<T>(y * act);
+    }
+    StoreFour<T>(static_cast<T *>(a.d_gate) + row * a.d_stride, at, a.d_stride, dg);
+    StoreFour<T>(static_cast<T *>(a.d_up) + row * a.d_stride, at, a.d_stride, du);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+
+constexpr long long kMostGrid = 1 << 20;
+
+template <typename Fn>
+void WithActivation(int activation, Fn &&fn) {
+  if (activation == kSilu) fn(std::integral_constant<int, kSilu>());
+  else fn(std::integral_constant<int, kGelu>());
+}
+
+// Whether an operand's chunks are aligned and whole, and its tiles within what a load's offset spans.
+template <typename T>
+bool IsDirect(const void *p, long long stride, long long extent) {
+  const long long item = sizeof(T);
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * item % 16 == 0 && extent * item % 16 == 0 && stride * item * 256 < (1ll << 31) - (1 << 20);
+}
+
+template <typename T, bool kAcrossA, bool kAcrossB>
+void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
+  const auto launch = [&](auto shape, auto is_direct) {
+    typedef decltype(shape) S;
+    const long long tile_rows = Pieces(p.rows, S::kI), tiles = tile_rows * Pieces(p.columns, S::kJ) * p.batch * p.splits;
+    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kMostGrid)), dim3(S::kThreads), 0, stream, p, tiles,
+                       tile_rows, (int)Pieces(p.columns, S::kJ));
+  };
+  if (large && direct) launch(LargeTile(), std::true_type());
+  else if (large) launch(LargeTile(), std::false_type());
+  else if (direct) launch(SmallTile(), std::true_type());
+  else launch(SmallTile(), std::false_type());
+  if (p.splits > 1) {
+    const long long blocks = Pieces(p.rows * p.columns * p.batch, kThreads);
+    hipLaunchKernelGGL((k_products_join<T>), dim3((unsigned)std::min(blocks, kMostGrid)), dim3(kThreads), 0, stream, p);
+  }
+}
+
+}  // namespace
+
+template <typename T>
+void RunGated(const GatedArgs &a, bool large) {
+  const GatedLayer &l = a.layer;
+  const Forward f{l.x, l.w_gate, l.w_up, l.rows, l.dim, l.hidden, l.x_stride, l.w_stride, a.out, a.out_stride, l.gate, l.up, l.gate_scales,
+                  l.up_scales, l.kept_stride};
+  const bool direct = IsDirect<T>(l.x, l.x_stride, l.dim) && IsDirect<T>(l.w_gate, l.w_stride, l.dim) && IsDirect<T>(l.w_up, l.w_stride, l.dim);
+  WithActivation(l.activation, [&](auto act) {
+    const auto launch = [&](auto shape, auto is_direct) {
+      typedef decltype(shape) S;
+      const long long tile_rows = Pieces(l.rows, S::kI), tile_columns = Pieces(l.hidden, S::kJ / 2), tiles = tile_rows * tile_columns;
+      hipLaunchKernelGGL((k_gated<T, decltype(act)::value, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kMostGrid)),
+                         dim3(S::kThreads), 0, static_cast<hipStream_t>(l.stream), f, tiles, tile_rows, (int)tile_columns);
+    };
+    if (large && direct) launch(LargeTile(), std::true_type());
+    else if (large) launch(LargeTile(), std::false_type());
+    else if (direct) launch(SmallTile(), std::true_type());
+    else launch(SmallTile(), std::false_type());
+  });
+  HIP_OK(hipGetLastError());
+}
+
+template <typename T>
+void RunGatedGrad(const GatedGradArgs &a, const GatedPlan &plan) {
+  const GatedLayer &l = a.layer;
+  const hipStream_t stream = static_cast<hipStream_t>(l.stream);
+  unsigned char *work = static_cast<unsigned char *>(l.work);
+  void *d_gate = work, *d_up = work + plan.d_bytes;
+  float *partial = reinterpret_cast<float *>(work + 2 * plan.d_bytes);
+  if (l.rows > 0) {
+    const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden};
+    const unsigned row_blocks = (unsigned)Pieces(plan.d_stride, kThreads * kSlopeVec);
+    const long long blocks = l.rows * row_blocks;
+    WithActivation(l.activation, [&](auto act) {
+      hipLaunchKernelGGL((k_slopes<T, decltype(act)::value>), dim3((unsigned)std::min(blocks, kMostGrid)), dim3(kThreads), 0, stream, s, blocks, row_blocks);
+    });
+  }
+  const Operand d{{d_gate, d_up}, plan.d_stride};
+  const bool d_direct = IsDirect<T>(d_gate, plan.d_stride, plan.d_stride);
+  if (a.grad_x && l.rows > 0) {
+    const Products p{d, {{l.w_gate, l.w_up}, l.w_stride}, l.rows, l.dim, l.hidden, 2, 1, {a.grad_x, nullptr}, a.grad_x_stride,
+                     (int)plan.x.splits, plan.x.split_blocks, partial};
+    Launch<T, false, true>(p, plan.x.large, d_direct && IsDirect<T>(l.w_gate, l.w_stride, l.dim) && IsDirect<T>(l.w_up, l.w_stride, l.dim), stream);
+  }
+  if (a.grad_w_gate) {
+    const Products p{d, {{l.x, l.x}, l.x_stride}, l.hidden, l.dim, l.rows, 1, 2, {a.grad_w_gate, a.grad_w_up}, a.grad_w_stride,
+                     (int)plan.w.splits, plan.w.split_blocks, partial};
+    Launch<T, true, true>(p, plan.w.large, d_direct && IsDirect<T>(l.x, l.x_stride, l.dim), stream);
+  }
+  HIP_OK(hipGetLastError());
+}
+
+}  // namespace arb
+#endif  // ARBORETUM_AMD_GATED_KERNELS_H_

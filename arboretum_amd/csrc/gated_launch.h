@@ -1,0 +1,41 @@
+// What the gated layer's checks (gated.hip) hand to its kernels, which are compiled type by type (gated_float32.hip,
+// gated_bfloat16.hip, gated_float16.hip).
+#ifndef ARBORETUM_AMD_GATED_LAUNCH_H_
+#define ARBORETUM_AMD_GATED_LAUNCH_H_
+#include "operators.h"
+
+namespace arb {
+
+constexpr int kLineBytes = 128;           // of k's in a block: 64 of 16 bits, 32 of 32
+constexpr int kWaveI = 64, kWaveJ = 128;  // a wave's part of a tile: 4 x 8 fragments of 16 x 16
+
+// A workgroup's tile: kWavesI x kWavesJ waves.
+template <int kWavesI, int kWavesJ>
+struct TileShape {
+  static constexpr int kThreads = 64 * kWavesI * kWavesJ, kI = kWaveI * kWavesI, kJ = kWaveJ * kWavesJ;
+  static constexpr int kBlockBytes = (kI + kJ) * kLineBytes;
+};
+typedef TileShape<4, 2> LargeTile;
+typedef TileShape<2, 1> SmallTile;
+
+// How a product is cut up: into which tiles, and how many shares of its k's (blocks of kLineBytes of them).
+struct ProductCut {
+  bool large;
+  long long splits, split_blocks;
+};
+struct GatedPlan {
+  long long d_stride;  // elements between rows of d_gate and of d_up in the work memory
+  ProductCut x, w;     // of grad_x, of the weights' gradients
+  size_t d_bytes, bytes;
+};
+
+inline long long Pieces(long long n, long long of) { return (n + of - 1) / of; }
+
+// (arguments that have passed the checks)
+template <typename T>
+void RunGated(const GatedArgs &a, bool large);
+template <typename T>
+void RunGatedGrad(const GatedGradArgs &a, const GatedPlan &plan);
+
+}  // namespace arb
+#endif  // ARBORETUM_AMD_GATED_LAUNCH_H_

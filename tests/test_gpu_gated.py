@@ -31,6 +31,7 @@ def half_step(dtype):
 
 def close(got, want, err, dtype, what):
     rel, step = half_step(dtype)
+    got, want, err = got.cpu(), want.cpu(), err.cpu()
     bound = err + rel * (want.abs() + err) + step
     off = (got.double().cpu() - want).abs()
     # (rounding to nearest takes what is beyond the type's greatest number by half a step or more to infinity: 1.1e5 is no number of float16)
@@ -133,6 +134,7 @@ class Layer:
         if self.gate is not None:
             for k, (got, want, err) in enumerate(zip(self.kept_values(), (g, u), (eg, eu))):
                 if self.eight:
+                    got, want, err = got.cpu(), want.cpu(), err.cpu()
                     for c in range(0, self.hidden, 64):
                         most = want[:, c:c + 64].abs().max(1).values + err[:, c:c + 64].max(1).values
                         scale = self.scales[k][:self.rows, c // 64].double().cpu()
@@ -472,3 +474,32 @@ def test_a_layer_of_leaf_embeddings_from_lookup_to_step(arb):
         got = got.double().cpu()
         assert (got - want.grad).norm() <= 0.05 * want.grad.norm()
     assert abs(-lp.double().sum().item() - loss.item()) <= 0.02 * loss.item() and (lp[~named.cuda()] == 0).all()
+
+
+class OnDevice(Layer):
+    """The same, its restatement in 64 bits on the GPU."""
+
+    def __init__(self, *args, **more):
+        super().__init__(*args, **more)
+        self.x, self.wg, self.wu, self.grad_out = (v.cuda() for v in (self.x, self.wg, self.wu, self.grad_out))
+
+    def kept_values(self):
+        out = []
+        for k, v in enumerate((self.gate, self.up)):
+            v = v[:, :self.hidden]
+            if self.eight:
+                v = v.float() * self.scales[k][:self.rows].repeat_interleave(64, 1)[:, :self.hidden]
+            out.append(v.double())
+        return out
+
+
+@pytest.mark.parametrize("rows,dim,hidden,dtype,pad,first,kept", [
+    (4000, 136, 2100, "bfloat16", 0, 0, "no"), (4000, 136, 2100, "float16", 8, 8, "as is"), (4100, 129, 1999, "bfloat16", 0, 0, "as is"),
+    (1030, 3600, 4100, "bfloat16", 0, 0, "as is"), (1001, 3601, 4099, "float16", 3, 1, "as is"), (3001, 132, 2300, "float32", 0, 0, "as is"),
+    (260, 7000, 7200, "bfloat16", 0, 0, "as is"), (300, 3700, 3500, "float32", 1, 1, "as is"), (3000, 72, 2200, "bfloat16", 0, 0, "8 bits")])
+def test_sizes_that_fill_the_chip(arb, rows, dim, hidden, dtype, pad, first, kept):
+    layer = OnDevice(arb, rows, dim, hidden, dtype, kept=kept, pad=pad, first=first, activation="gelu" if rows % 2 else "silu").forward()
+    layer.check_forward()
+    if kept != "no":
+        layer.backward().check_backward()
+    layer.check_margins()
