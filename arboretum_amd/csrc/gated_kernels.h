@@ -91,12 +91,24 @@ typedef int I4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char LdsByte;
 typedef __attribute__((address_space(3))) I4 LdsI4;
 
+// 16 bytes a lane from `base` + `at` (beyond 2^31: 0) to the LDS, the wave's 1 KB side by side from `to` on.  By hand: the
+// compiler waits for a load of its own before any read of the LDS, and this one is meant to be on its way meanwhile.  Whoever reads
+// what it writes waits for it first (WaitForLoads and a barrier).
+__device__ __forceinline__ void LoadToLds(const void *base, unsigned at, LdsByte *to) {
+  const unsigned long long address = reinterpret_cast<unsigned long long>(base);
+  const I4 from = {(int)__builtin_amdgcn_readfirstlane((int)address), (int)__builtin_amdgcn_readfirstlane((int)(address >> 32)) & 0xFFFF, 0x7FFFFFFF, 0x00020000};
+  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)to);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void WaitForLoads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // The chunks of an operand's block in the LDS.  Along k: line by line, 8 chunks each; across: k by k, the chunks of all lines.
 // Chunks change places from line to line (from k to k), so that the lanes that read together meet other banks: they
 // read one chunk of 16 lines, of which two make up all banks; or 32 bytes (16 lines of 16 bits) of eight k's, 64 bytes of four k's of 32 bits.
 template <typename T, int kLines, bool kAcross>
 struct Layout {
   static constexpr int kVec = 16 / sizeof(T), kRowChunks = kAcross ? kLines / kVec : 8;
+  static constexpr int kReads = kAcross ? sizeof(T) : 1;  // of the LDS for a chunk of a product
   static __device__ __forceinline__ int Swap(int row) {
     if (!kAcross) return (row >> 1) & 7;
     if (sizeof(T) == 2) return (((row & 3) | ((row >> 1) & 4)) << 1) & (kRowChunks - 1);
@@ -167,11 +179,10 @@ struct Loader {
     if constexpr (kDirect) {
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
-        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(rows.Base(p * kThreads / L::kRowChunks)), 0, 0x7FFFFFFF, 0x00020000);
         const int q = p * kThreads + threadIdx.x, row = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(row);
         const bool held = kAcross ? row < left && chunk * kVec < lines : rows.Held(row) && chunk * kVec < left;
         const unsigned at = held ? ((unsigned)rows.Number(row) * (unsigned)rows.stride + chunk * kVec) * (unsigned)sizeof(T) : kNowhere;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(block + (p * kThreads + wave * 64) * 16), 16, at, 0, 0, 0);
+        LoadToLds(rows.Base(p * kThreads / L::kRowChunks), at, block + (p * kThreads + wave * 64) * 16);
       }
     } else {
       // (lines beyond the operand along k: the last one again, whose results are not stored; k's beyond it are 0)
@@ -208,19 +219,37 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < kWaveJ / 16; ++j) acc[i][j] = F4{0, 0, 0, 0};
   }
+  // Both halves of a block.  What is read for a product is asked for eight products ahead, which the order at the end makes sure of:
+  // left alone the compiler reads a chunk, waits and multiplies, with as few registers as that takes.
   template <typename T, typename LayoutA, typename LayoutB>
   __device__ __forceinline__ void Add(const LdsByte *a, const LdsByte *b, int wave_i, int wave_j) {
+    constexpr int kFragsI = kWaveI / 16, kFragsJ = kWaveJ / 16;
+    Chunk<T> x[2][kFragsI], y[2][kFragsJ];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      Chunk<T> x[kWaveI / 16], y[kWaveJ / 16];
 #pragma unroll
-      for (int i = 0; i < kWaveI / 16; ++i) x[i] = LayoutA::Read(a, wave_i * kWaveI + i * 16, half);
+      for (int i = 0; i < kFragsI; ++i) x[half][i] = LayoutA::Read(a, wave_i * kWaveI + i * 16, half);
 #pragma unroll
-      for (int j = 0; j < kWaveJ / 16; ++j) y[j] = LayoutB::Read(b, wave_j * kWaveJ + j * 16, half);
+      for (int j = 0; j < kFragsJ; ++j) y[half][j] = LayoutB::Read(b, wave_j * kWaveJ + j * 16, half);
 #pragma unroll
-      for (int j = 0; j < kWaveJ / 16; ++j)
+      for (int j = 0; j < kFragsJ; ++j)
 #pragma unroll
-        for (int i = 0; i < kWaveI / 16; ++i) acc[i][j] = Product(y[j], x[i], acc[i][j]);
+        for (int i = 0; i < kFragsI; ++i) acc[i][j] = Product(y[half][j], x[half][i], acc[i][j]);
+    }
+    constexpr int kRead = 0x100, kMultiply = 0x8, kPer = kFragsI * (sizeof(T) == 4 ? 4 : 1);
+    __builtin_amdgcn_sched_group_barrier(kRead, kFragsI * LayoutA::kReads + 2 * LayoutB::kReads, 0);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int j = 0; j < kFragsJ - 2; ++j) {
+        __builtin_amdgcn_sched_group_barrier(kMultiply, kPer, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, LayoutB::kReads, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        __builtin_amdgcn_sched_group_barrier(kMultiply, kPer, 0);
+        if (half == 0) __builtin_amdgcn_sched_group_barrier(kRead, kFragsI / 2 * LayoutA::kReads + LayoutB::kReads, 0);
+      }
     }
   }
 };
@@ -234,7 +263,7 @@ __device__ __forceinline__ void RunBlocks(long long blocks, const LoadFn &load, 
   store(0);
   for (long long n = 0; n < blocks; ++n) {
     const int half = (int)(n & 1);
-    if (kDirect) __builtin_amdgcn_s_waitcnt(0);
+    if (kDirect) WaitForLoads();
     __syncthreads();  // (block n is there, and the half that block n + 1 goes to has been read)
     if (n + 1 < blocks) load(n + 1, half ^ 1);
     add(half);
@@ -316,7 +345,7 @@ static_assert(kWaveJ == 2 * kScaleGroup, "a wave holds whole groups");
 
 // A tile's columns are the gate's and up's of the same hidden ones: 64 of the gate and 64 of up for each wave.
 template <typename T, int kAct, typename S, bool kDirect>
-__global__ void __launch_bounds__(S::kThreads) k_gated(const Forward a, long long tiles, long long tile_rows, int tile_columns) {
+__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_gated(const Forward a, long long tiles, long long tile_rows, int tile_columns) {
   __shared__ __align__(16) unsigned char s_blocks[2 * S::kBlockBytes];
   LdsByte *blocks = (LdsByte *)s_blocks;
   constexpr int kK = kLineBytes / sizeof(T), kHidden = S::kJ / 2;
@@ -369,7 +398,7 @@ __global__ void __launch_bounds__(S::kThreads) k_gated(const Forward a, long lon
 }
 
 template <typename T, bool kAcrossA, bool kAcrossB, typename S, bool kDirect>
-__global__ void __launch_bounds__(S::kThreads) k_products(const Products p, long long tiles, long long tile_rows, int tile_columns) {
+__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_products(const Products p, long long tiles, long long tile_rows, int tile_columns) {
   __shared__ __align__(16) unsigned char s_blocks[2 * S::kBlockBytes];
   LdsByte *blocks = (LdsByte *)s_blocks;
   constexpr int kK = kLineBytes / sizeof(T);

@@ -14,6 +14,7 @@ template <int kWavesI, int kWavesJ>
 struct TileShape {
   static constexpr int kThreads = 64 * kWavesI * kWavesJ, kI = kWaveI * kWavesI, kJ = kWaveJ * kWavesJ;
   static constexpr int kBlockBytes = (kI + kJ) * kLineBytes;
+  static constexpr int kWavesEach = kWavesI * kWavesJ / 4 > 0 ? kWavesI * kWavesJ / 4 : 1;  // waves of a SIMD: the LDS holds one large tile, or two small ones
 };
 typedef TileShape<4, 2> LargeTile;
 typedef TileShape<2, 1> SmallTile;
