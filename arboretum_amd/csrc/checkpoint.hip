@@ -26,65 +26,88 @@ struct Place {
   long long row, group;
   int at, held;  // first value in the row, values of it in the row
 };
-__device__ __forceinline__ bool PlaceOf(const Shape &a, long long block, Place *p) {
+__device__ __forceinline__ Place PlaceOf(const Shape &a, long long block) {
   const long long first = block * (kThreads / kLanes), row = first / a.row_groups;
   const unsigned g = (unsigned)(first - row * a.row_groups) + threadIdx.x / kLanes, more = g / a.row_groups;
-  p->group = first + threadIdx.x / kLanes;
-  p->row = row + more;
-  p->at = (int)((g - more * a.row_groups) * kScaleGroup + threadIdx.x % kLanes * kCodeVec);
-  p->held = max(0, min(a.dim - p->at, kCodeVec));
-  return p->group < a.groups;
+  Place p;
+  p.group = first + threadIdx.x / kLanes;
+  p.row = row + more;
+  p.at = (int)((g - more * a.row_groups) * kScaleGroup + threadIdx.x % kLanes * kCodeVec);
+  p.held = p.group < a.groups ? max(0, min(a.dim - p.at, kCodeVec)) : 0;
+  return p;
 }
+
+constexpr int kEach = 2;  // blocks of groups that a workgroup has in flight
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_checkpoint(const Shape a, long long blocks) {
-  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
-    Place p;
-    const bool live = PlaceOf(a, block, &p);
-    float v[kCodeVec];
-    const T *x = static_cast<const T *>(a.x) + p.row * a.x_stride + p.at;
-    if (live && p.held == kCodeVec) {
-      const Pack<T, kCodeVec> w = *reinterpret_cast<const Pack<T, kCodeVec> *>(x);
+  for (long long block = (long long)blockIdx.x * kEach; block < blocks; block += (long long)gridDim.x * kEach) {
+    Place p[kEach];
+    float v[kEach][kCodeVec];
 #pragma unroll
-      for (int c = 0; c < kCodeVec; ++c) v[c] = (float)w.v[c];
-    } else {
+    for (int e = 0; e < kEach; ++e) {
+      p[e] = PlaceOf(a, block + e);
+      const T *x = static_cast<const T *>(a.x) + p[e].row * a.x_stride + p[e].at;
+      if (p[e].held == kCodeVec) {
+        const Pack<T, kCodeVec> w = *reinterpret_cast<const Pack<T, kCodeVec> *>(x);
 #pragma unroll
-      for (int c = 0; c < kCodeVec; ++c) v[c] = live && c < p.held ? (float)x[c] : 0.0f;
+        for (int c = 0; c < kCodeVec; ++c) v[e][c] = (float)w.v[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < kCodeVec; ++c) v[e][c] = c < p[e].held ? (float)x[c] : 0.0f;
+      }
     }
-    float most = MostOf(v);
 #pragma unroll
-    for (int by = kLanes / 2; by > 0; by /= 2) most = Larger(most, __shfl_xor(most, by));
-    if (!live) continue;  // (a group is whole or not there)
-    const float scale = ScaleOf(most);
-    if (threadIdx.x % kLanes == 0) a.scales[p.group] = scale;
-    const Pack<signed char, kCodeVec> codes = CodesOf(v, scale);
-    signed char *to = a.codes + p.row * a.dim + p.at;
-    if (p.held == kCodeVec) *reinterpret_cast<Pack<signed char, kCodeVec> *>(to) = codes;
-    else
+    for (int e = 0; e < kEach; ++e) {
+      unsigned most = MostOf(v[e]);
 #pragma unroll
-      for (int c = 0; c < kCodeVec; ++c)
-        if (c < p.held) to[c] = codes.v[c];
+      for (int by = kLanes / 2; by > 0; by /= 2) most = max(most, (unsigned)__shfl_xor((int)most, by));
+      const float scale = ScaleOf(most);
+      if (threadIdx.x % kLanes == 0 && p[e].held > 0) a.scales[p[e].group] = scale;
+      const Pack<signed char, kCodeVec> codes = CodesOf(v[e], scale);
+      signed char *to = a.codes + p[e].row * a.dim + p[e].at;
+      if (p[e].held == kCodeVec) {
+        *reinterpret_cast<Pack<signed char, kCodeVec> *>(to) = codes;
+      } else {
+#pragma unroll
+        for (int c = 0; c < kCodeVec; ++c)
+          if (c < p[e].held) to[c] = codes.v[c];
+      }
+    }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_restore(const Shape a, long long blocks) {
-  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
-    Place p;
-    if (!PlaceOf(a, block, &p)) continue;
-    const float scale = a.scales[p.group];
-    const signed char *from = a.codes + p.row * a.dim + p.at;
-    T *x = static_cast<T *>(a.x) + p.row * a.x_stride + p.at;
-    if (p.held == kCodeVec) {
-      const Pack<signed char, kCodeVec> codes = *reinterpret_cast<const Pack<signed char, kCodeVec> *>(from);
+  for (long long block = (long long)blockIdx.x * kEach; block < blocks; block += (long long)gridDim.x * kEach) {
+    Place p[kEach];
+    float scale[kEach];
+    Pack<signed char, kCodeVec> codes[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      p[e] = PlaceOf(a, block + e);
+      const signed char *from = a.codes + p[e].row * a.dim + p[e].at;
+      scale[e] = p[e].held > 0 ? a.scales[p[e].group] : 0.0f;
+      if (p[e].held == kCodeVec) {
+        codes[e] = *reinterpret_cast<const Pack<signed char, kCodeVec> *>(from);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kCodeVec; ++c) codes[e].v[c] = c < p[e].held ? from[c] : (signed char)0;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      T *x = static_cast<T *>(a.x) + p[e].row * a.x_stride + p[e].at;
       Pack<T, kCodeVec> w;
 #pragma unroll
-      for (int c = 0; c < kCodeVec; ++c) w.v[c] = Round<T>(Restored(codes.v[c], scale));
-      *reinterpret_cast<Pack<T, kCodeVec> *>(x) = w;
-    } else {
+      for (int c = 0; c < kCodeVec; ++c) w.v[c] = Round<T>(Restored(codes[e].v[c], scale[e]));
+      if (p[e].held == kCodeVec) {
+        *reinterpret_cast<Pack<T, kCodeVec> *>(x) = w;
+      } else {
 #pragma unroll
-      for (int c = 0; c < kCodeVec; ++c)
-        if (c < p.held) x[c] = Round<T>(Restored(from[c], scale));
+        for (int c = 0; c < kCodeVec; ++c)
+          if (c < p[e].held) x[c] = w.v[c];
+      }
     }
   }
 }
@@ -109,7 +132,7 @@ void ActivationCheckpoint(const CheckpointArgs &a) {
   OnDeviceOf device(a.codes);
   const long long blocks = (s.groups + kThreads / kLanes - 1) / (kThreads / kLanes);
   WithType(a.type, [&](auto type) {
-    hipLaunchKernelGGL((k_checkpoint<decltype(type)>), dim3((unsigned)std::min(blocks, 1ll << 22)), dim3(kThreads), 0,
+    hipLaunchKernelGGL((k_checkpoint<decltype(type)>), dim3((unsigned)std::min((blocks + kEach - 1) / kEach, 1ll << 22)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(a.stream), s, blocks);
   });
   HIP_OK(hipGetLastError());
@@ -122,7 +145,7 @@ void ActivationRestore(const CheckpointArgs &a) {
   OnDeviceOf device(a.x);
   const long long blocks = (s.groups + kThreads / kLanes - 1) / (kThreads / kLanes);
   WithType(a.type, [&](auto type) {
-    hipLaunchKernelGGL((k_restore<decltype(type)>), dim3((unsigned)std::min(blocks, 1ll << 22)), dim3(kThreads), 0,
+    hipLaunchKernelGGL((k_restore<decltype(type)>), dim3((unsigned)std::min((blocks + kEach - 1) / kEach, 1ll << 22)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(a.stream), s, blocks);
   });
   HIP_OK(hipGetLastError());

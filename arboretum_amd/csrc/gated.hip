@@ -12,7 +12,7 @@ ProductCut CutOf(long long rows, long long columns, long long batch, long long b
   ProductCut c;
   c.large = Pieces(rows, LargeTile::kI) * Pieces(columns, LargeTile::kJ) * batch >= 200;
   const long long tiles = c.large ? Pieces(rows, LargeTile::kI) * Pieces(columns, LargeTile::kJ) * batch : Pieces(rows, SmallTile::kI) * Pieces(columns, SmallTile::kJ) * batch;
-  const long long most = std::max<long long>(1, std::min({512 / std::max<long long>(tiles, 1), blocks / 8, 64ll}));
+  const long long most = std::max<long long>(1, std::min({(c.large ? 256 : 512) / std::max<long long>(tiles, 1), blocks / 8, 64ll}));
   c.split_blocks = std::max<long long>(1, Pieces(blocks, most));
   c.splits = std::max<long long>(1, Pieces(blocks, c.split_blocks));
   return c;

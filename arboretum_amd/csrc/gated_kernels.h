@@ -323,13 +323,13 @@ __device__ __forceinline__ void Keep(void *kept, float *scales, long long stride
     }
     return;
   }
-  float most = 0.0f;  // (columns beyond the layer hold 0)
+  unsigned most = 0;  // (columns beyond the layer hold 0, or what the last one holds)
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) most = Larger(most, fabsf(v[j][r]));
-  most = Larger(most, __shfl_xor(most, 16));
-  most = Larger(most, __shfl_xor(most, 32));
+    for (int r = 0; r < 4; ++r) most = max(most, Magnitude(v[j][r]));
+  most = max(most, (unsigned)__shfl_xor((int)most, 16));
+  most = max(most, (unsigned)__shfl_xor((int)most, 32));
   const float scale = ScaleOf(most);
   if (quarter == 0) scales[row * ((hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup] = scale;
   signed char *to = static_cast<signed char *>(kept) + row * stride;
@@ -482,43 +482,61 @@ struct Slopes {
   int hidden;
 };
 
-constexpr int kSlopeVec = 4;
+constexpr int kSlopeVec = 8;
 
-// d_gate and d_up, rounded to the type of the products they enter; 0 in the columns from the layer's end to the next row.
-template <typename T, int kAct>
-__global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks, unsigned row_blocks) {
+// d_gate and d_up, rounded to the type of the products they enter; 0 in the columns from the layer's end to the next row.  A thread
+// has kSlopeVec columns of a row (d_stride is a multiple of 64).
+template <typename T, int kAct, bool kCodes>
+__global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks) {
+  typedef std::conditional_t<kCodes, signed char, T> Kept;
+  const unsigned vectors = (unsigned)(a.d_stride / kSlopeVec);
   for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
-    const long long row = block / row_blocks;
-    const int at = (int)((unsigned)(block - row * row_blocks) * kThreads + threadIdx.x) * kSlopeVec;
-    if (at >= a.d_stride) continue;
+    const long long first = block * kThreads, row0 = first / vectors;
+    const unsigned in = (unsigned)(first - row0 * vectors) + threadIdx.x, more = in / vectors;
+    const long long row = row0 + more;
+    if (row >= a.rows) continue;
+    const int at = (int)(in - more * vectors) * kSlopeVec, held = min(a.hidden - at, kSlopeVec);
     const T *grad = static_cast<const T *>(a.grad_out) + row * a.grad_out_stride + at;
-    const long long kept = row * a.kept_stride + at;
-    float gate_scale = 0, up_scale = 0;
-    if (a.gate_scales != nullptr) {
-      const long long group = row * ((a.hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup;  // (d_stride ends with the last group)
+    const Kept *gate = static_cast<const Kept *>(a.gate) + row * a.kept_stride + at, *up = static_cast<const Kept *>(a.up) + row * a.kept_stride + at;
+    Pack<T, kSlopeVec> y;
+    Pack<Kept, kSlopeVec> g, u;
+    float gate_scale = 0.0f, up_scale = 0.0f;
+    if (kCodes) {
+      const long long group = row * (a.d_stride / kScaleGroup) + at / kScaleGroup;
       gate_scale = a.gate_scales[group];
       up_scale = a.up_scales[group];
     }
-    T dg[kSlopeVec], du[kSlopeVec];
+    if (held == kSlopeVec) {
+      y = *reinterpret_cast<const Pack<T, kSlopeVec> *>(grad);
+      g = *reinterpret_cast<const Pack<Kept, kSlopeVec> *>(gate);
+      u = *reinterpret_cast<const Pack<Kept, kSlopeVec> *>(up);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kSlopeVec; ++c) {
+        y.v[c] = c < held ? grad[c] : T(0);
+        g.v[c] = c < held ? gate[c] : Kept(0);
+        u.v[c] = c < held ? up[c] : Kept(0);
+      }
+    }
+    Pack<T, kSlopeVec> dg, du;
 #pragma unroll
     for (int c = 0; c < kSlopeVec; ++c) {
-      const bool held = at + c < a.hidden;
-      const float y = held ? (float)grad[c] : 0.0f;
-      float g, u;
-      if (a.gate_scales != nullptr) {
-        g = held ? Restored(static_cast<const signed char *>(a.gate)[kept + c], gate_scale) : 0.0f;
-        u = held ? Restored(static_cast<const signed char *>(a.up)[kept + c], up_scale) : 0.0f;
+      float gv, uv;
+      if constexpr (kCodes) {
+        gv = Restored(g.v[c], gate_scale);
+        uv = Restored(u.v[c], up_scale);
       } else {
-        g = held ? (float)static_cast<const T *>(a.gate)[kept + c] : 0.0f;
-        u = held ? (float)static_cast<const T *>(a.up)[kept + c] : 0.0f;
+        gv = (float)g.v[c];
+        uv = (float)u.v[c];
       }
       float act, slope;
-      ActAndSlope<kAct>(g, &act, &slope);
-      dg[c] = Round<T>(y * u * slope);
-      du[c] = Round<T>(y * act);
+      ActAndSlope<kAct>(gv, &act, &slope);
+      const bool there = c < held;
+      dg.v[c] = there ? Round<T>((float)y.v[c] * uv * slope) : T(0);
+      du.v[c] = there ? Round<T>((float)y.v[c] * act) : T(0);
     }
-    StoreFour<T>(static_cast<T *>(a.d_gate) + row * a.d_stride, at, a.d_stride, dg);
-    StoreFour<T>(static_cast<T *>(a.d_up) + row * a.d_stride, at, a.d_stride, du);
+    *reinterpret_cast<Pack<T, kSlopeVec> *>(static_cast<T *>(a.d_gate) + row * a.d_stride + at) = dg;
+    *reinterpret_cast<Pack<T, kSlopeVec> *>(static_cast<T *>(a.d_up) + row * a.d_stride + at) = du;
   }
 }
 
@@ -589,10 +607,12 @@ void RunGatedGrad(const GatedGradArgs &a, const GatedPlan &plan) {
   float *partial = reinterpret_cast<float *>(work + 2 * plan.d_bytes);
   if (l.rows > 0) {
     const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden};
-    const unsigned row_blocks = (unsigned)Pieces(plan.d_stride, kThreads * kSlopeVec);
-    const long long blocks = l.rows * row_blocks;
+    const long long blocks = Pieces(l.rows * (plan.d_stride / kSlopeVec), kThreads);
+    const dim3 grid((unsigned)std::min(blocks, kMostGrid));
     WithActivation(l.activation, [&](auto act) {
-      hipLaunchKernelGGL((k_slopes<T, decltype(act)::value>), dim3((unsigned)std::min(blocks, kMostGrid)), dim3(kThreads), 0, stream, s, blocks, row_blocks);
+      constexpr int kAct = decltype(act)::value;
+      if (l.gate_scales) hipLaunchKernelGGL((k_slopes<T, kAct, true>), grid, dim3(kThreads), 0, stream, s, blocks);
+      else hipLaunchKernelGGL((k_slopes<T, kAct, false>), grid, dim3(kThreads), 0, stream, s, blocks);
     });
   }
   const Operand d{{d_gate, d_up}, plan.d_stride};
