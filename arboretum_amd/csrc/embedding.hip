@@ -71,27 +71,6 @@ __device__ __forceinline__ void Store(T *__restrict__ at, int held, const Pack<T
   }
 }
 
-// Results larger than the L2 caches of all XCDs (32 MB) go past them: nobody would find them there, and the table's
-// rows stay (a lookup of 65,536 x 4096 bf16 152 -> 130 us).
-constexpr size_t kStreamedBytes = (size_t)32 << 20;
-template <typename T, int kVec>
-__device__ __forceinline__ void StorePast(T *__restrict__ at, const Pack<T, kVec> &from) {
-  constexpr int kBytes = sizeof(T) * kVec;
-  if constexpr (kBytes % 16 == 0) {
-    typedef float Part __attribute__((ext_vector_type(4), aligned(2)));  // (of the smallest element)
-    struct Parts {
-      Pack<float, 4> v[kBytes / 16];
-    };
-    const Parts parts = __builtin_bit_cast(Parts, from);
-#pragma unroll
-    for (int k = 0; k < kBytes / 16; ++k)
-      __builtin_nontemporal_store(Part{parts.v[k].v[0], parts.v[k].v[1], parts.v[k].v[2], parts.v[k].v[3]},
-                                  reinterpret_cast<Part *>(at) + k);
-  } else {
-    *reinterpret_cast<Pack<T, kVec> *>(at) = from;
-  }
-}
-
 // Rows of the two matrices of a lookup.
 template <typename T>
 struct Rows {

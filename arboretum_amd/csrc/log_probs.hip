@@ -16,19 +16,19 @@ namespace {
 typedef unsigned long long Key;  // value (in an order of whole numbers) and inverted index: the greater one comes first; 0: none
 
 constexpr int kMostTop = 64;     // of them a wave holds one a lane
-constexpr int kMostParts = 64;   // of a row, joined by a wave
-constexpr long long kPart = 2048;  // a row is not cut into less
-constexpr float kLog2E = 1.44269504088896340736f;
-constexpr float kLowest = -1.0e20f;  // exponents beyond are taken for it where they are factors: their power is 0, and must not meet an infinity
+constexpr int kMostParts = 32;   // of a row, joined by a wave
+constexpr long long kPart = 8192;  // a row is not cut into less: 16 KB, a workgroup's loads in one go
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLowest = -1000.0f;  // exponents (of two) below are taken for it where they are factors: their power is 0, and must not meet an infinity
 
 __device__ __forceinline__ float Infinity() { return __builtin_inff(); }
 __device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ Key KeyOf(float value, unsigned index) {
+__device__ __forceinline__ unsigned OrderOf(float value) {
   const unsigned bits = __float_as_uint(value + 0.0f);  // (-0 and 0 are equal)
-  const unsigned order = bits ^ ((bits >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-  return ((Key)order << 32) | (Key)(~index);
+  return bits ^ ((bits >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
+__device__ __forceinline__ Key KeyOf(float value, unsigned index) { return ((Key)OrderOf(value) << 32) | (Key)(~index); }
 __device__ __forceinline__ float ValueOf(Key key) {
   const unsigned order = (unsigned)(key >> 32);
   return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xFFFFFFFFu));
@@ -38,6 +38,29 @@ __device__ __forceinline__ unsigned IndexOf(Key key) { return ~(unsigned)key; }
 __device__ __forceinline__ Key LaneKey(Key key, int lane) {
   const unsigned low = __builtin_amdgcn_readlane((int)(unsigned)key, lane), high = __builtin_amdgcn_readlane((int)(unsigned)(key >> 32), lane);
   return ((Key)high << 32) | low;
+}
+
+// The greatest word that at least `k` of a wave's words (kEach a lane) are no less than, bit by bit from the top; or, as soon as
+// some word has exactly k on its side, that one.
+template <int kEach, typename Word>
+__device__ __forceinline__ Word Least(const Word (&words)[kEach], int k) {
+  Word least = 0;
+  for (int bit = sizeof(Word) * 8 - 1; bit >= 0; --bit) {
+    const Word tried = least | (Word)1 << bit;
+    int count = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) count += __popcll(__ballot(words[e] >= tried));
+    if (count >= k) least = tried;
+    if (count == k) break;
+  }
+  return least;
+}
+
+// A wave's list of 64 keys in order, one a lane: `one` takes its place, and the last one falls out.
+__device__ __forceinline__ void Insert(Key *held, Key one) {
+  const int lane = threadIdx.x & 63, place = __popcll(__ballot(*held > one));
+  const Key before = ((Key)(unsigned)__shfl_up((int)(unsigned)(*held >> 32), 1) << 32) | (unsigned)__shfl_up((int)(unsigned)*held, 1);
+  *held = lane < place ? *held : lane == place ? one : before;
 }
 
 // Sums of (a part of) a row: the maximum, sum 2^d and sum d 2^d of d = log2(e) scale (x - maximum).
@@ -103,29 +126,34 @@ __device__ __forceinline__ void WriteRow(const RowsArgs &a, const Sums &s, float
   }
   if (a.entropy != nullptr) {
     // (ln 2 takes the moment back to exponents of e)
-    const float h = s.sum == 0.0f ? 0.0f : log_sum - 0.693147180559945309f * (s.moment / s.sum);
+    const float h = s.sum == 0.0f ? 0.0f : log_sum - kLn2 * (s.moment / s.sum);
     a.entropy[i] = h;
   }
   if (a.stats != nullptr) a.stats[i] = make_float2(s.most, log_sum);
 }
 
-__device__ __forceinline__ void WriteTop(const RowsArgs &a, const Sums &s, float log_sum, long long i, int rank, Key key) {
+__device__ __forceinline__ void WriteTop(const RowsArgs &a, const Sums &s, float log_sum, long long i, int rank, float value, unsigned index) {
   const bool none = log_sum != log_sum;  // a row with a NaN, or plus infinity
-  a.top_tokens[i * a.top + rank] = none ? -1 : (int)IndexOf(key);
-  a.top_log_probs[i * a.top + rank] = a.scale * (ValueOf(key) - Base(s.most)) - log_sum;
+  a.top_tokens[i * a.top + rank] = none ? -1 : (int)index;
+  a.top_log_probs[i * a.top + rank] = a.scale * (value - Base(s.most)) - log_sum;
+}
+__device__ __forceinline__ void WriteTop(const RowsArgs &a, const Sums &s, float log_sum, long long i, int rank, Key key) {
+  WriteTop(a, s, log_sum, i, rank, ValueOf(key), IndexOf(key));
 }
 
 // ------------------------------------------------------------------ rows whose classes lie side by side
 
 // A team of kWaves waves reads a row, or a part of one; one wave a row: four teams a workgroup.
-// Every thread keeps the maximum of what it reads.  Of the whole row the k likeliest can only be where the k greatest of
-// these maxima are (whoever is in no such thread is behind k others), so only those threads' share of the row is read again.
+// The likeliest tokens: every thread keeps the maximum of what it reads.  The k-th greatest of these maxima has k elements of the row on
+// its side, so the k likeliest are no less than it, and whatever is no less lies with the threads whose maxima are no less: about k
+// of 256, so that only their share of the row is read again.  (Where many are equal, as in a row of one value, more is.)
 template <typename T, int kWaves, int kUnroll, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const RowsArgs a) {
   constexpr int kVec = 16 / sizeof(T), kTeam = kWaves * 64, kTeams = kWaves == 1 ? 4 : 1, kChunk = kUnroll * kVec;
   __shared__ Sums s_sums[kWaves];
-  __shared__ Key s_lists[kTop ? kTeams * kWaves : 1][kTop ? kMostTop : 1];
-  __shared__ Key s_top[kTop ? kTeams : 1][kTop ? kMostTop : 1];
+  __shared__ unsigned s_most[kTop ? kTeams : 1][kTop ? kTeam : 1];
+  __shared__ unsigned short s_owners[kTop ? kTeams * kWaves : 1][kTop ? 64 : 1];
+  __shared__ Key s_lists[kTop && kWaves > 1 ? kWaves : 1][kTop && kWaves > 1 ? kMostTop : 1];
   const int lane = threadIdx.x & 63, wave = kWaves == 1 ? 0 : threadIdx.x >> 6, team = kWaves == 1 ? threadIdx.x >> 6 : 0;
   const unsigned t = kWaves == 1 ? lane : threadIdx.x;
   const long long items = a.n * a.parts;
@@ -139,13 +167,11 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride + begin;
 
     Sums s = {-Infinity(), 0.0f, 0.0f};
-    unsigned best = 0;  // vector from which on the maximum is found
-    const auto add = [&](const float (&v)[kChunk], unsigned at) {
+    const auto add = [&](const float (&v)[kChunk]) {
       float most = v[0];
 #pragma unroll
       for (int c = 1; c < kChunk; ++c) most = fmaxf(most, v[c]);
       if (most > s.most) {
-        if (kTop) best = at;
         const float d = a.factor * (s.most - most), e = Exp2(d);
         if (kEntropy) s.moment = e * (s.moment + fmaxf(d, kLowest) * s.sum);
         s.sum *= e;
@@ -169,7 +195,7 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
       for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
         for (int c = 0; c < kVec; ++c) v[u * kVec + c] = (float)p[u].v[c];
-      add(v, i);
+      add(v);
     }
     if ((size_t)whole * kTeam + t < vectors) {  // the rest; what is beyond the end counts as minus infinity
       float v[kChunk];
@@ -182,17 +208,9 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
 #pragma unroll
         for (int c = 0; c < kVec; ++c) v[u * kVec + c] = all ? (float)p.v[c] : at < length && c < (int)(length - at) ? (float)x[at + c] : -Infinity();
       }
-      add(v, whole);
+      add(v);
     }
-    // the thread's greatest value, the first of equal ones
-    Key mine = 0;
-    if (kTop && t < vectors) {
-      for (unsigned i = best, end = best + kUnroll; i < end && mine == 0; ++i) {
-        const unsigned at = (i * kTeam + t) * kVec;
-        for (int c = 0; c < kVec; ++c)
-          if (mine == 0 && at < length && (unsigned)c < length - at && (float)x[at + c] == s.most) mine = KeyOf(s.most, begin + at + c);
-      }
-    }
+    const unsigned mine = kTop && t < vectors ? OrderOf(s.most) : 0;
 
     // the sums of the team
 #pragma unroll
@@ -211,80 +229,87 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
     }
 
     if constexpr (kTop) {
-      // Ranks: how many keys of the wave are greater, then how many of each other wave's list.
-      Key(*lists)[kMostTop] = &s_lists[team * kWaves];
-      const auto rank = [&](Key key, Key *to) {  // the team's greatest a.top keys to `to`, in order; whatever else there is: 0
-        int r = 0;
-        for (int l = 0; l < 64; ++l) {
-          const Key other = LaneKey(key, l);
-          r += other > key || (other == key && l < lane);
-        }
-        if (kWaves == 1) {
-          if (r < a.top) to[r] = key;
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-          __builtin_amdgcn_wave_barrier();
-          return;
-        }
-        lists[wave][r] = key;
+      unsigned words[kWaves];
+      if constexpr (kWaves > 1) {
+        s_most[0][t] = mine;
         __syncthreads();
-        int all = r;
-        if (r < a.top && key != 0) {
-          for (int w = 0; w < kWaves; ++w) {
-            if (w == wave) continue;
-            int low = 0, high = kMostTop;  // keys before `low` are greater, those from `high` on are not
-            while (low < high) {
-              const int mid = (low + high) / 2;
-              if (lists[w][mid] > key) low = mid + 1;
-              else high = mid;
-            }
-            all += low;
-          }
-          if (all < a.top) to[all] = key;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) words[w] = s_most[0][w * 64 + lane];
+      } else {
+        words[0] = mine;
+      }
+      const unsigned least = Least<kWaves>(words, a.top);
+      // the wave's own threads of those, and their vectors, shared out over its lanes
+      const unsigned long long owners = __ballot(mine != 0 && mine >= least);
+      unsigned short *list = s_owners[team * kWaves + wave];
+      if (owners >> lane & 1) list[__popcll(owners & ((1ull << lane) - 1))] = (unsigned short)t;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      __builtin_amdgcn_wave_barrier();
+      const unsigned rounds = (vectors + kTeam - 1) / kTeam, count = (unsigned)__popcll(owners) * rounds;
+      Key held = 0;
+      for (unsigned e0 = 0; e0 < count; e0 += 64) {
+        const unsigned e = min(e0 + lane, count - 1), owner = e / rounds, at = ((e - owner * rounds) * kTeam + list[owner]) * kVec;
+        const unsigned there = e0 + lane < count && at < length ? min(length - at, (unsigned)kVec) : 0;
+        Pack<T, kVec> p;
+        if (there == kVec) {
+          p = *reinterpret_cast<const Pack<T, kVec> *>(x + at);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kVec; ++c) p.v[c] = (unsigned)c < there ? x[at + c] : T(0);
         }
-        __syncthreads();
-      };
-      if (t < kMostTop) s_top[team][t] = 0;
-      if (kWaves > 1) __syncthreads();
-      rank(mine, s_top[team]);
-      const Key least = s_top[team][a.top - 1];
-      Key held = 0;  // of the wave, a sorted list, one a lane
-      for (int k = wave; k < a.top; k += kWaves) {
-        const Key owner = s_top[team][k];
-        if (owner == 0) break;
-        const unsigned from = (IndexOf(owner) - begin) / kVec % kTeam;
-        const unsigned rounds = (vectors - from + kTeam - 1) / kTeam;
-        for (unsigned e = lane; e - lane < rounds * kVec; e += 64) {
-          const unsigned at = (e / kVec * kTeam + from) * kVec + e % kVec;
-          const Key key = e < rounds * kVec && at < length ? KeyOf((float)x[at], begin + at) : 0;
-          unsigned long long found = __ballot(key != 0 && key >= least);
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+          const Key key = (unsigned)c < there ? KeyOf((float)p.v[c], begin + at + c) : 0;
+          const Key last = LaneKey(held, a.top - 1);
+          unsigned long long found = __ballot((unsigned)(key >> 32) >= least && key > last);
           while (found != 0) {
-            const Key one = LaneKey(key, __builtin_ctzll(found));
+            Insert(&held, LaneKey(key, __builtin_ctzll(found)));
             found &= found - 1;
-            const int place = __popcll(__ballot(held > one));
-            const Key before = ((Key)(unsigned)__shfl_up((int)(unsigned)(held >> 32), 1) << 32) | (unsigned)__shfl_up((int)(unsigned)held, 1);
-            held = lane < place ? held : lane == place ? one : before;
           }
         }
       }
-      if (kWaves > 1) __syncthreads();
-      if (t < kMostTop) s_top[team][t] = 0;
-      if (kWaves > 1) __syncthreads();
-      rank(held, s_top[team]);
-      if (live && (int)t < a.top) {
-        if (a.parts == 1) WriteTop(a, s, log_sum, row, t, s_top[team][t]);
-        else a.keys[item * a.top + t] = s_top[team][t];
+      // the wave's list meets the others': a key's place is how many are greater, in each of them
+      int place = lane;
+      if constexpr (kWaves > 1) {
+        s_lists[wave][lane] = held;
+        __syncthreads();
+        int greater[kWaves] = {};
+#pragma unroll
+        for (int step = 64; step > 0; step /= 2) {  // (halving, in all lists at once; the last step twice: there may be 64)
+          const int by = max(step / 2, 1);
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w)
+            if (greater[w] + by <= kMostTop && s_lists[w][greater[w] + by - 1] > held) greater[w] += by;
+        }
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) place += w == wave ? 0 : greater[w];
+      }
+      // (with a NaN in it nothing is in order; a part shorter than the list leaves places empty)
+      const bool broken = log_sum != log_sum;
+      if (live && !broken && held != 0 && lane < a.top && place < a.top) {
+        if (a.parts == 1) WriteTop(a, s, log_sum, row, place, held);
+        else a.keys[item * a.top + place] = held;
+      }
+      if (live && wave == 0 && lane < a.top && (broken || (unsigned)lane >= length)) {
+        if (a.parts == 1) WriteTop(a, s, log_sum, row, lane, 0);
+        else a.keys[item * a.top + lane] = 0;
       }
     }
     if (kWaves > 1) __syncthreads();
   }
 }
 
-// The parts of a row, by one wave: a lane holds a part.
-template <typename T>
+// The parts of a row, by one wave: a lane holds a part's sums and kEach of the parts' keys.
+template <typename T, int kEach>
 __global__ void __launch_bounds__(64) k_join(const RowsArgs a) {
+  __shared__ Key s_top[kMostTop];
   const int lane = threadIdx.x;
   for (long long row = blockIdx.x; row < a.n; row += gridDim.x) {
     Sums s = {-Infinity(), 0.0f, 0.0f};
+    Key words[kEach];
+    const Key *keys = a.keys + row * a.parts * a.top;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) words[e] = e * 64 + lane < a.parts * a.top ? keys[e * 64 + lane] : 0;
     if (lane < a.parts) {
       const float4 p = a.sums[row * a.parts + lane];
       s = Sums{p.x, p.y, p.z};
@@ -293,46 +318,55 @@ __global__ void __launch_bounds__(64) k_join(const RowsArgs a) {
     for (int by = 32; by > 0; by /= 2) s = Join(s, Sums{__shfl_xor(s.most, by), __shfl_xor(s.sum, by), __shfl_xor(s.moment, by)}, a.factor);
     const float log_sum = LogSum(s);
     if (lane == 0) WriteRow<T>(a, s, log_sum, row);
-    const Key *keys = a.keys + (row * a.parts + lane) * a.top;
-    int at = 0;  // the heads of the parts' lists; the greatest leaves its list
-    Key head = lane < a.parts && a.top > 0 ? keys[0] : 0;
-    for (int k = 0; k < a.top; ++k) {
-      Key most = head;
-#pragma unroll
-      for (int by = 32; by > 0; by /= 2) {
-        const Key other = ((Key)(unsigned)__shfl_xor((int)(unsigned)(most >> 32), by) << 32) | (unsigned)__shfl_xor((int)(unsigned)most, by);
-        most = max(most, other);
-      }
-      if (lane == 0) WriteTop(a, s, log_sum, row, k, most);
-      if (head == most && lane < a.parts) head = ++at < a.top ? keys[at] : 0;
+    if (a.top == 0) continue;
+    if (log_sum != log_sum) {
+      if (lane < a.top) WriteTop(a, s, log_sum, row, lane, 0);
+      continue;
     }
+    // (keys differ from each other: a.top of them are no less than the least)
+    const Key least = Least<kEach>(words, a.top);
+    int before = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const unsigned long long found = __ballot(words[e] != 0 && words[e] >= least);
+      const int place = before + __popcll(found & ((1ull << lane) - 1));
+      if ((found >> lane & 1) && place < kMostTop) s_top[place] = words[e];
+      before += __popcll(found);
+    }
+    __syncthreads();
+    const Key mine = lane < a.top ? s_top[lane] : 0;
+    int place = 0;
+    for (int l = 0; l < a.top; ++l) place += LaneKey(mine, l) > mine;
+    if (lane < a.top) WriteTop(a, s, log_sum, row, place, mine);
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------ a row a thread
 
-// The greatest kHeld in one pass, in order; `top` beyond that takes further passes, each behind the last one found.
-template <typename T, int kHeld>
+// The greatest kHeld in one pass, in order; `top` beyond that takes further passes, each behind the last one found.  kUnroll classes
+// are asked for at once.
+template <typename T, int kHeld, int kUnroll>
 __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
-  constexpr int kUnroll = 4;
   const long long step = (long long)gridDim.x * 256;
   for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < a.n; row += step) {
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     Sums s = {-Infinity(), 0.0f, 0.0f};
-    float log_sum = 0.0f;
-    Key limit = ~0ull;
+    float log_sum = 0.0f, limit = Infinity();
+    unsigned limit_at = 0;  // the last one found: what comes next is less, or as much and behind it
     for (int from = 0; from == 0 || from < a.top; from += kHeld) {
-      Key held[kHeld];
+      float held[kHeld];  // (NaN: empty)
+      unsigned held_at[kHeld];
 #pragma unroll
-      for (int h = 0; h < kHeld; ++h) held[h] = 0;
+      for (int h = 0; h < kHeld; ++h) held[h] = __builtin_nanf(""), held_at[h] = ~0u;
       for (unsigned j0 = 0; j0 < a.vocab; j0 += kUnroll) {
         float v[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) v[u] = j0 + u < a.vocab ? (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride] : -Infinity();
+        for (int u = 0; u < kUnroll; ++u) v[u] = (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride];
         if (from == 0) {
-          float most = s.most;
+          float most = v[0];
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u) most = fmaxf(most, v[u]);
+          for (int u = 1; u < kUnroll; ++u) most = fmaxf(most, v[u]);  // (the last class again, where there is no other)
           if (most > s.most) {
             const float d = a.factor * (s.most - most), e = Exp2(d);
             s.moment = e * (s.moment + fmaxf(d, kLowest) * s.sum);
@@ -342,6 +376,7 @@ __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
           const float base = Base(s.most);
 #pragma unroll
           for (int u = 0; u < kUnroll; ++u) {
+            if (j0 + u >= a.vocab) break;
             const float d = a.factor * (v[u] - base), e = Exp2(d);
             s.sum += e;
             s.moment = fmaf(fmaxf(d, kLowest), e, s.moment);
@@ -350,13 +385,20 @@ __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
         if (a.top > 0) {
 #pragma unroll
           for (int u = 0; u < kUnroll; ++u) {
-            Key key = KeyOf(v[u], j0 + u);
-            if (j0 + u >= a.vocab || key >= limit) key = 0;
+            if (j0 + u >= a.vocab) break;
+            float value = v[u];
+            unsigned at = j0 + u;
+            bool moves = false;
+            if (from > 0 && !(value < limit || (value == limit && at > limit_at))) continue;
 #pragma unroll
-            for (int h = 0; h < kHeld; ++h) {  // (in order: it takes its place, those behind move on)
-              const Key lower = min(held[h], key);
-              held[h] = max(held[h], key);
-              key = lower;
+            for (int h = 0; h < kHeld; ++h) {  // (it takes its place before the first that is less, or empty, and those from there on move)
+              moves = moves || !(value <= held[h]);
+              const float other = held[h];
+              const unsigned other_at = held_at[h];
+              held[h] = moves ? value : other;
+              held_at[h] = moves ? at : other_at;
+              value = moves ? other : value;
+              at = moves ? other_at : at;
             }
           }
         }
@@ -365,10 +407,23 @@ __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
         log_sum = LogSum(s);
         WriteRow<T>(a, s, log_sum, row);
       }
+      if (kHeld == a.top) {  // (side by side)
+        Pack<int, kHeld> tokens;
+        Pack<float, kHeld> values;
 #pragma unroll
-      for (int h = 0; h < kHeld; ++h)
-        if (from + h < a.top) WriteTop(a, s, log_sum, row, from + h, held[h]);
+        for (int h = 0; h < kHeld; ++h) {
+          tokens.v[h] = log_sum != log_sum ? -1 : (int)held_at[h];
+          values.v[h] = a.scale * (held[h] - Base(s.most)) - log_sum;
+        }
+        *reinterpret_cast<Pack<int, kHeld> *>(a.top_tokens + row * kHeld) = tokens;
+        *reinterpret_cast<Pack<float, kHeld> *>(a.top_log_probs + row * kHeld) = values;
+      } else {
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+          if (from + h < a.top) WriteTop(a, s, log_sum, row, from + h, held[h], held_at[h]);
+      }
       limit = held[kHeld - 1];
+      limit_at = held_at[kHeld - 1];
     }
   }
 }
@@ -389,75 +444,115 @@ struct GradArgs {
   unsigned *status;
 };
 
-// A row's constants.
+// A row's constants.  In powers of two, with d = log2 p,
+//   grad_j = p_j (of_p + of_log d), and with [j = token] the one where p is taken from
 struct RowGrad {
-  float most, log_sum, weight, entropy_weight, entropy;
-  long long token;
-  bool nothing;  // no logit but minus infinity: no gradient
+  float most, log_sum, of_p, of_log, weight, entropy;
+  unsigned token;  // vocab for none
 };
 
+template <bool kEntropy>
 __device__ __forceinline__ RowGrad RowGradOf(const GradArgs &a, long long row) {
   RowGrad r;
   const float2 stats = a.stats[row];
-  r.most = stats.x;
-  r.log_sum = stats.y;
-  r.nothing = stats.x == -Infinity() && stats.y == 0.0f;
-  r.token = a.tokens == nullptr ? -1 : a.token_bits == 32 ? (long long)static_cast<const int *>(a.tokens)[row] : static_cast<const long long *>(a.tokens)[row];
-  if (r.token < 0 || r.token >= (long long)a.vocab) {
-    if (r.token != -1 && a.status != nullptr) *a.status = 1u;
-    r.token = -1;
+  // (a row of nothing but minus infinity: whatever is subtracted from it, its powers are 0)
+  const bool nothing = stats.x == -Infinity() && stats.y == 0.0f;
+  r.most = nothing ? 0.0f : stats.x;
+  r.log_sum = stats.y * kLog2E;
+  const long long token = a.tokens == nullptr ? -1 : a.token_bits == 32 ? (long long)static_cast<const int *>(a.tokens)[row] : static_cast<const long long *>(a.tokens)[row];
+  const bool there = token >= 0 && token < (long long)a.vocab;
+  if (!there && token != -1 && a.status != nullptr) *a.status = 1u;
+  r.token = there && !nothing ? (unsigned)token : a.vocab;
+  r.weight = there ? a.scale * a.grad_log_probs[row] : 0.0f;
+  if (nothing) r.weight = 0.0f;
+  r.entropy = r.of_log = 0.0f;
+  r.of_p = -r.weight;
+  if (kEntropy) {
+    const float h = nothing ? 0.0f : a.scale * a.grad_entropy[row];
+    r.entropy = a.entropy[row];
+    r.of_log = -h * kLn2;
+    r.of_p -= h * r.entropy;
   }
-  r.weight = r.token >= 0 ? a.grad_log_probs[row] : 0.0f;
-  r.entropy_weight = a.grad_entropy != nullptr ? a.grad_entropy[row] : 0.0f;
-  r.entropy = a.grad_entropy != nullptr ? a.entropy[row] : 0.0f;
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ T GradOf(const GradArgs &a, const RowGrad &r, float x, long long j) {
-  const float log_p = a.scale * (x - r.most) - r.log_sum;
-  const float p = Exp2(log_p * kLog2E);
-  float g = r.weight * ((j == r.token ? 1.0f : 0.0f) - p);
-  if (a.grad_entropy != nullptr) g -= r.entropy_weight * (p > 0.0f ? p * (log_p + r.entropy) : p);
-  return Round<T>(r.nothing ? 0.0f : a.scale * g);
+template <typename T, bool kEntropy>
+__device__ __forceinline__ T GradOf(const RowGrad &r, float factor, float x) {
+  const float d = fmaf(factor, x - r.most, -r.log_sum), p = Exp2(d);
+  return Round<T>(kEntropy ? p * fmaf(r.of_log, fmaxf(d, kLowest), r.of_p) : p * r.of_p);
+}
+// The gradient of the token itself: weight (1 - p) as it stands, where its parts would meet with opposite signs.
+template <typename T, bool kEntropy>
+__device__ __forceinline__ T GradOfToken(const RowGrad &r, float factor, float x) {
+  const float d = fmaf(factor, x - r.most, -r.log_sum), p = Exp2(d);
+  float g = r.weight * (1.0f - p);
+  if (kEntropy) g += p * fmaf(r.of_log, fmaxf(d, kLowest), r.of_p + r.weight);
+  return Round<T>(g);
 }
 
 // Classes side by side: `lanes` threads of a workgroup take a row's piece of lanes * kVec * kUnroll classes.
 // (The gradient may take the place of the logits: what a thread writes only it has read.)
-template <typename T, int kUnroll>
+template <typename T, int kUnroll, bool kEntropy, bool kPast>
 __global__ void __launch_bounds__(256) k_grad_rows(const GradArgs a, int lanes, unsigned pieces) {
   constexpr int kVec = 16 / sizeof(T);
   const unsigned of = threadIdx.x / lanes, t = threadIdx.x % lanes, teams = 256 / lanes;
   const long long items = a.n * pieces;
+  const float factor = a.scale * kLog2E;
   for (long long item = (long long)blockIdx.x * teams + of; item < items; item += (long long)gridDim.x * teams) {
     const long long row = pieces == 1 ? item : item / pieces;
     const unsigned begin = (unsigned)(item - row * pieces) * (unsigned)(lanes * kVec * kUnroll);
-    const RowGrad r = RowGradOf(a, row);
+    const RowGrad r = RowGradOf<kEntropy>(a, row);
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     T *grad = static_cast<T *>(a.grad) + row * a.grad_row_stride;
-    if (a.vocab - begin >= (unsigned)(lanes * kVec * kUnroll)) {
-      Pack<T, kVec> p[kUnroll];
+    const bool whole = a.vocab - begin >= (unsigned)(lanes * kVec * kUnroll);
+    Pack<T, kVec> p[kUnroll];
+    int held[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = *reinterpret_cast<const Pack<T, kVec> *>(x + begin + (u * lanes + t) * kVec);
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned at = begin + (u * lanes + t) * kVec;
+      held[u] = whole ? kVec : at < a.vocab ? (int)min(a.vocab - at, (unsigned)kVec) : 0;
+      if (held[u] == kVec) {
+        p[u] = *reinterpret_cast<const Pack<T, kVec> *>(x + at);
+      } else {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const unsigned at = begin + (u * lanes + t) * kVec;
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) p[u].v[c] = GradOf<T>(a, r, (float)p[u].v[c], at + c);
-        *reinterpret_cast<Pack<T, kVec> *>(grad + at) = p[u];
+        for (int c = 0; c < kVec; ++c) p[u].v[c] = c < held[u] ? x[at + c] : T(0);
       }
-    } else {
-      for (unsigned at = begin + t; at < a.vocab; at += lanes) grad[at] = GradOf<T>(a, r, (float)x[at], at);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned at = begin + (u * lanes + t) * kVec, hit = r.token - at;
+      T of_token = T(0);
+      if (hit < (unsigned)kVec) {  // (one lane of a row)
+        float v = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) v = hit == (unsigned)c ? (float)p[u].v[c] : v;
+        of_token = GradOfToken<T, kEntropy>(r, factor, v);
+      }
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) p[u].v[c] = GradOf<T, kEntropy>(r, factor, (float)p[u].v[c]);
+      if (hit < (unsigned)kVec) {
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) p[u].v[c] = hit == (unsigned)c ? of_token : p[u].v[c];
+      }
+      if (held[u] == kVec) {
+        if constexpr (kPast) StorePast(grad + at, p[u]);
+        else *reinterpret_cast<Pack<T, kVec> *>(grad + at) = p[u];
+      } else {
+#pragma unroll
+        for (int c = 0; c < kVec; ++c)
+          if (c < held[u]) grad[at + c] = p[u].v[c];
+      }
     }
   }
 }
 
-template <typename T>
+template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(256) k_grad_columns(const GradArgs a) {
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 8;
   const long long step = (long long)gridDim.x * 256;
+  const float factor = a.scale * kLog2E;
   for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < a.n; row += step) {
-    const RowGrad r = RowGradOf(a, row);
+    const RowGrad r = RowGradOf<kEntropy>(a, row);
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     T *grad = static_cast<T *>(a.grad) + row * a.grad_row_stride;
     for (unsigned j0 = 0; j0 < a.vocab; j0 += kUnroll) {
@@ -465,8 +560,10 @@ __global__ void __launch_bounds__(256) k_grad_columns(const GradArgs a) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) v[u] = (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j0 + u < a.vocab) grad[(long long)(j0 + u) * a.grad_class_stride] = GradOf<T>(a, r, v[u], j0 + u);
+      for (int u = 0; u < kUnroll; ++u) {
+        if (j0 + u >= a.vocab) break;
+        grad[(long long)(j0 + u) * a.grad_class_stride] = j0 + u == r.token ? GradOfToken<T, kEntropy>(r, factor, v[u]) : GradOf<T, kEntropy>(r, factor, v[u]);
+      }
     }
   }
 }
@@ -538,9 +635,13 @@ void LogProbs(const LogProbsArgs &a) {
   WithType(l.type, [&](auto type) {
     typedef decltype(type) T;
     if (!side_by_side || l.vocab <= 32) {
-      const unsigned grid = GridOf((l.n + 255) / 256);
-      if (a.top <= 4) hipLaunchKernelGGL((k_columns<T, 4>), dim3(grid), dim3(256), 0, stream, r);
-      else hipLaunchKernelGGL((k_columns<T, 8>), dim3(grid), dim3(256), 0, stream, r);
+      const dim3 grid(GridOf((l.n + 255) / 256));
+      const auto columns = [&](auto held) { hipLaunchKernelGGL((k_columns<T, decltype(held)::value, 8>), grid, dim3(256), 0, stream, r); };
+      if (a.top <= 1) columns(std::integral_constant<int, 1>());
+      else if (a.top == 2) columns(std::integral_constant<int, 2>());
+      else if (a.top == 3) columns(std::integral_constant<int, 3>());
+      else if (a.top <= 5) columns(std::integral_constant<int, 5>());
+      else columns(std::integral_constant<int, 8>());
       return;
     }
     r.parts = PartsOf(l.n, l.vocab);
@@ -553,8 +654,7 @@ void LogProbs(const LogProbsArgs &a) {
     const auto launch = [&](auto entropy, auto top) {
       constexpr bool kEntropy = decltype(entropy)::value, kTop = decltype(top)::value;
       const long long items = l.n * r.parts;
-      if (r.parts > 1) hipLaunchKernelGGL((k_rows<T, 4, 1, kEntropy, kTop>), dim3(GridOf(items)), dim3(256), 0, stream, r);
-      else if (r.part <= 2048) hipLaunchKernelGGL((k_rows<T, 1, 1, kEntropy, kTop>), dim3(GridOf((items + 3) / 4)), dim3(256), 0, stream, r);
+      if (r.part <= 2048) hipLaunchKernelGGL((k_rows<T, 1, 1, kEntropy, kTop>), dim3(GridOf((items + 3) / 4)), dim3(256), 0, stream, r);
       else hipLaunchKernelGGL((k_rows<T, 4, 4, kEntropy, kTop>), dim3(GridOf(items)), dim3(256), 0, stream, r);
     };
     typedef std::true_type Yes;
@@ -563,7 +663,8 @@ void LogProbs(const LogProbsArgs &a) {
     else if (a.entropy) launch(Yes(), No());
     else if (a.top) launch(No(), Yes());
     else launch(No(), No());
-    if (r.parts > 1) hipLaunchKernelGGL((k_join<T>), dim3(GridOf(l.n)), dim3(64), 0, stream, r);
+    if (r.parts > 1 && r.parts * r.top <= 512) hipLaunchKernelGGL((k_join<T, 8>), dim3(GridOf(l.n)), dim3(64), 0, stream, r);
+    else if (r.parts > 1) hipLaunchKernelGGL((k_join<T, 32>), dim3(GridOf(l.n)), dim3(64), 0, stream, r);
   });
   HIP_OK(hipGetLastError());
 }
@@ -597,16 +698,24 @@ void LogProbsGrad(const LogProbsGradArgs &a) {
   const bool side_by_side = l.vocab == 1 || (l.class_stride == 1 && a.grad_class_stride == 1);
   WithType(l.type, [&](auto type) {
     typedef decltype(type) T;
-    if (!side_by_side) {
-      hipLaunchKernelGGL((k_grad_columns<T>), dim3(GridOf((l.n + 255) / 256)), dim3(256), 0, stream, g);
-      return;
-    }
-    constexpr int kUnroll = 4, kVec = 16 / sizeof(T);
-    int lanes = 256;
-    while (lanes > 4 && lanes / 2 >= l.vocab) lanes /= 2;
-    const unsigned pieces = (unsigned)((l.vocab + lanes * kVec * kUnroll - 1) / (lanes * kVec * kUnroll));
-    const long long items = l.n * pieces, teams = 256 / lanes;
-    hipLaunchKernelGGL((k_grad_rows<T, kUnroll>), dim3(GridOf((items + teams - 1) / teams)), dim3(256), 0, stream, g, lanes, pieces);
+    const auto launch = [&](auto entropy) {
+      constexpr bool kEntropy = decltype(entropy)::value;
+      if (!side_by_side) {
+        hipLaunchKernelGGL((k_grad_columns<T, kEntropy>), dim3(GridOf((l.n + 255) / 256)), dim3(256), 0, stream, g);
+        return;
+      }
+      constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
+      int lanes = 256;
+      while (lanes > 1 && lanes / 2 * kVec * kUnroll >= l.vocab) lanes /= 2;
+      const unsigned pieces = (unsigned)((l.vocab + lanes * kVec * kUnroll - 1) / (lanes * kVec * kUnroll));
+      const long long items = l.n * pieces, teams = 256 / lanes;
+      const dim3 grid(GridOf((items + teams - 1) / teams));
+      // a gradient that the L2 caches do not hold is written past them
+      if ((size_t)l.n * l.vocab * sizeof(T) > kStreamedBytes) hipLaunchKernelGGL((k_grad_rows<T, kUnroll, kEntropy, true>), grid, dim3(256), 0, stream, g, lanes, pieces);
+      else hipLaunchKernelGGL((k_grad_rows<T, kUnroll, kEntropy, false>), grid, dim3(256), 0, stream, g, lanes, pieces);
+    };
+    if (a.grad_entropy) launch(std::true_type());
+    else launch(std::false_type());
   });
   HIP_OK(hipGetLastError());
 }

@@ -6,7 +6,7 @@ distances that end to end are |a|, and two roundings each.  A sum of c steps add
 (a wave shares a row at least), or all of a row that one thread reads.  So
   err(L) = u (4 E|a| + c + 4 + 2 |L|),   err(log_prob) = u (3 |a_t| + |log_prob|) + err(L)
   err(H) = err(L) + u (4 E[a^2] + (c + 16) E|a|) + E|a| err(S) + 4 u (|L| + H),   err(S) the part of err(L) that S is off by
-  err(p) / p = u (2 |a| + 4 |log p| + 4) + err(L)
+  err(p) / p = u (3 |a| + 2 |L| + 4 |log p| + 4) + err(L)   (a difference, a constant of two roundings, L in powers of two, their sum)
 and the gradient's terms with these and a rounding for each operation.  A result's type adds half its step."""
 import itertools
 
@@ -103,8 +103,8 @@ class Want:
         hit = torch.zeros_like(self.p)
         hit[self.named, self.tokens[self.named]] = 1
         log_p, a = torch.where(self.p > 0, self.log_p, 0.0), torch.where(self.p > 0, self.a, 0.0)
-        err_lp = U * (2 * a.abs() + log_p.abs()) + self.err_L[:, None]
-        rel = err_lp + U * (4 * log_p.abs() + 4)
+        err_lp = U * (3 * a.abs() + 2 * self.L[:, None].abs() + log_p.abs()) + self.err_L[:, None]
+        rel = err_lp + U * (3 * log_p.abs() + 4)
         p = torch.where(self.nothing[:, None], 0.0, self.p)
         hit = torch.where(self.nothing[:, None], 0.0, hit)
         g, err = w * (hit - p), w.abs() * (p * rel + 3 * U * (hit - p).abs())
@@ -242,8 +242,6 @@ def test_rows(arb, n, vocab, top, dtype):
 @pytest.mark.parametrize("n,vocab,top", [(7, 3, 3), (9, 32, 17), (8, 40, 40), (6, 700, 64), (4, 3000, 9), (300, 5001, 20), (3, 40_007, 64)])
 @pytest.mark.parametrize("layout", ["rows", "columns"])
 def test_values_that_tie_rise_or_are_masked(arb, n, vocab, top, kind, layout):
-    if layout == "columns" and n * vocab > 1 << 20:
-        pytest.skip("the largest is for rows")
     gen = torch.Generator().manual_seed(vocab)
     dtype = [torch.float32, torch.bfloat16, torch.float16][(vocab + len(kind)) % 3]
     x = make_logits(gen, n, vocab, kind, dtype)
