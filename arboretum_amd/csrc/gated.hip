@@ -7,15 +7,36 @@
 namespace arb {
 namespace {
 
-// Large tiles where they fill the chip; else small ones, and few tiles share out their k's, at least eight blocks to a share.
-ProductCut CutOf(long long rows, long long columns, long long batch, long long blocks) {
+// Large tiles where they fill the chip; else small ones, and few tiles share out their k's, at least `least` blocks to a share.
+ProductCut CutOf(long long large_tiles, long long small_tiles, long long blocks, long long least) {
   ProductCut c;
-  c.large = Pieces(rows, LargeTile::kI) * Pieces(columns, LargeTile::kJ) * batch >= 200;
-  const long long tiles = c.large ? Pieces(rows, LargeTile::kI) * Pieces(columns, LargeTile::kJ) * batch : Pieces(rows, SmallTile::kI) * Pieces(columns, SmallTile::kJ) * batch;
-  const long long most = std::max<long long>(1, std::min({(c.large ? 256 : 512) / std::max<long long>(tiles, 1), blocks / 8, 64ll}));
+  c.large = large_tiles >= 200;
+  const long long most = std::max<long long>(1, std::min({c.large ? 256 / large_tiles : 512 / std::max<long long>(small_tiles, 1), blocks / least, 64ll}));
   c.split_blocks = std::max<long long>(1, Pieces(blocks, most));
   c.splits = std::max<long long>(1, Pieces(blocks, c.split_blocks));
   return c;
+}
+
+// Bytes taken one after the other, each piece on 256.
+struct Room {
+  size_t bytes = 0;
+  size_t Take(size_t more) {
+    const size_t at = bytes;
+    bytes += (more + 255) / 256 * 256;
+    return at;
+  }
+};
+
+// Rows whose chunks are not aligned come through registers into small tiles, at less than half the rate; copies of x and both
+// weights are read and written once.  What the copies cost grows with the weights, what they spare with the rows as well: from about 500 rows on.
+LayerPad PadOf(long long rows, int dim, int hidden, size_t item, Room *room) {
+  LayerPad p{0, 0, 0, 0};
+  if (dim * item % 16 == 0 || rows < 512) return p;
+  p.stride = Pieces(dim, 64) * 64;
+  p.x = room->Take((size_t)rows * p.stride * item);
+  p.w_gate = room->Take((size_t)hidden * p.stride * item);
+  p.w_up = room->Take((size_t)hidden * p.stride * item);
+  return p;
 }
 
 void CheckLayerSizes(long long rows, int dim, int hidden, int type) {
@@ -26,14 +47,33 @@ void CheckLayerSizes(long long rows, int dim, int hidden, int type) {
 }
 
 GatedPlan PlanOf(long long rows, int dim, int hidden, int type) {
-  const long long item = (long long)ElementBytes(type), k = kLineBytes / item;
+  const size_t item = ElementBytes(type);
   GatedPlan p;
+  Room room;
+  p.few = rows <= 16;
+  p.out = CutOf(Pieces(rows, LargeTile::kI) * Pieces(hidden, LargeTile::kJ / 2), Pieces(rows, SmallTile::kI) * Pieces(hidden, SmallTile::kJ / 2),
+                Pieces(dim * item, kLineBytes), 4);
+  p.pad = PadOf(rows, dim, hidden, item, &room);
+  p.partial = room.Take(p.out.splits > 1 ? (size_t)p.out.splits * rows * Pieces(hidden, kScaleGroup) * kWaveJ * sizeof(float) : 0);
+  p.bytes = room.bytes;
+  return p;
+}
+
+GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
+  const size_t item = ElementBytes(type);
+  GatedGradPlan p;
+  Room room;
   p.d_stride = Pieces(hidden, 64) * 64;
-  p.x = CutOf(rows, dim, 1, 2 * Pieces(hidden, k));
-  p.w = CutOf(hidden, dim, 2, Pieces(rows, k));
-  p.d_bytes = (size_t)(rows * p.d_stride * item + 255) / 256 * 256;
-  const size_t partial = std::max<size_t>(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * 4 : 0, p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * 4 : 0);
-  p.bytes = 2 * p.d_bytes + partial;
+  p.x = CutOf(Pieces(rows, LargeTile::kI) * Pieces(dim, LargeTile::kJ), Pieces(rows, SmallTile::kI) * Pieces(dim, SmallTile::kJ),
+              2 * Pieces(hidden * item, kLineBytes), 8);
+  p.w = CutOf(2 * Pieces(hidden, LargeTile::kI) * Pieces(dim, LargeTile::kJ), 2 * Pieces(hidden, SmallTile::kI) * Pieces(dim, SmallTile::kJ),
+              Pieces(rows * item, kLineBytes), 8);
+  p.d_gate = room.Take((size_t)rows * p.d_stride * item);
+  p.d_up = room.Take((size_t)rows * p.d_stride * item);
+  p.pad = PadOf(rows, dim, hidden, item, &room);
+  p.partial = room.Take(std::max<size_t>(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * sizeof(float) : 0,
+                                         p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * sizeof(float) : 0));
+  p.bytes = room.bytes;
   return p;
 }
 
@@ -70,29 +110,29 @@ void CheckLayer(const GatedLayer &l, bool kept, size_t need) {
 
 size_t GatedBytes(long long rows, int dim, int hidden, int type) {
   CheckLayerSizes(rows, dim, hidden, type);
-  return 0;
+  return PlanOf(rows, dim, hidden, type).bytes;
 }
 
 void Gated(const GatedArgs &a) {
   const GatedLayer &l = a.layer;
-  CheckLayer(l, false, GatedBytes(l.rows, l.dim, l.hidden, l.type));
+  const GatedPlan plan = (CheckLayerSizes(l.rows, l.dim, l.hidden, l.type), PlanOf(l.rows, l.dim, l.hidden, l.type));
+  CheckLayer(l, false, plan.bytes);
   CheckStride(a.out_stride, l.hidden, l.rows, "out");
   CheckAligned(a.out, ElementBytes(l.type), "out");
   if (l.rows == 0) return;
   if (!a.out) throw std::runtime_error("null pointer argument");
   OnDeviceOf device(a.out);
-  const bool large = Pieces(l.rows, LargeTile::kI) * Pieces(l.hidden, LargeTile::kJ / 2) >= 200;
-  WithType(l.type, [&](auto type) { RunGated<decltype(type)>(a, large); });
+  WithType(l.type, [&](auto type) { RunGated<decltype(type)>(a, plan); });
 }
 
 size_t GatedGradBytes(long long rows, int dim, int hidden, int type) {
   CheckLayerSizes(rows, dim, hidden, type);
-  return PlanOf(rows, dim, hidden, type).bytes;
+  return GradPlanOf(rows, dim, hidden, type).bytes;
 }
 
 void GatedGrad(const GatedGradArgs &a) {
   const GatedLayer &l = a.layer;
-  const GatedPlan plan = (CheckLayerSizes(l.rows, l.dim, l.hidden, l.type), PlanOf(l.rows, l.dim, l.hidden, l.type));
+  const GatedGradPlan plan = (CheckLayerSizes(l.rows, l.dim, l.hidden, l.type), GradPlanOf(l.rows, l.dim, l.hidden, l.type));
   CheckLayer(l, true, plan.bytes);
   if ((a.grad_w_gate == nullptr) != (a.grad_w_up == nullptr)) throw std::runtime_error("the gradients of both weights go together");
   const size_t item = ElementBytes(l.type);

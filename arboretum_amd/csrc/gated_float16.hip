@@ -2,6 +2,6 @@
 #include "gated_kernels.h"
 
 namespace arb {
-template void RunGated<_Float16>(const GatedArgs &a, bool large);
-template void RunGatedGrad<_Float16>(const GatedGradArgs &a, const GatedPlan &plan);
+template void RunGated<_Float16>(const GatedArgs &a, const GatedPlan &plan);
+template void RunGatedGrad<_Float16>(const GatedGradArgs &a, const GatedGradPlan &plan);
 }  // namespace arb

@@ -2,6 +2,6 @@
 #include "gated_kernels.h"
 
 namespace arb {
-template void RunGated<float>(const GatedArgs &a, bool large);
-template void RunGatedGrad<float>(const GatedGradArgs &a, const GatedPlan &plan);
+template void RunGated<float>(const GatedArgs &a, const GatedPlan &plan);
+template void RunGatedGrad<float>(const GatedGradArgs &a, const GatedGradPlan &plan);
 }  // namespace arb

@@ -40,7 +40,10 @@ __device__ __forceinline__ F4 Product(const Chunk<float> &a, const Chunk<float> 
 
 // ------------------------------------------------------------------ activations
 
-__device__ __forceinline__ float Sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+// (the instructions for powers of two and reciprocals, of a rounding each: a division and expf take three times the time, and an
+// epilogue of nothing but them is what bounds narrow layers)
+__device__ __forceinline__ float PowerOfE(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+__device__ __forceinline__ float Sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + PowerOfE(-g)); }
 
 template <int kAct>
 __device__ __forceinline__ float Act(float g) {
@@ -58,7 +61,7 @@ __device__ __forceinline__ void ActAndSlope(float g, float *act, float *slope) {
   } else {
     const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
     *act = g * phi;
-    *slope = phi + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    *slope = phi + g * (0.39894228040143268f * PowerOfE(-0.5f * g * g));
   }
 }
 
@@ -254,22 +257,40 @@ struct Tile {
   }
 };
 
-// The blocks of a tile, one after the other: while one is multiplied the next is on its way into the other half of the LDS.
-// load(n, half): block n on its way; store(half): what came through registers, to the LDS; add(half).
-template <bool kDirect, typename LoadFn, typename StoreFn, typename AddFn>
-__device__ __forceinline__ void RunBlocks(long long blocks, const LoadFn &load, const StoreFn &store, const AddFn &add) {
-  if (blocks <= 0) return;
-  load(0, 0);
-  store(0);
-  for (long long n = 0; n < blocks; ++n) {
-    const int half = (int)(n & 1);
-    if (kDirect) WaitForLoads();
-    __syncthreads();  // (block n is there, and the half that block n + 1 goes to has been read)
-    if (n + 1 < blocks) load(n + 1, half ^ 1);
-    add(half);
-    if (n + 1 < blocks) store(half ^ 1);
+// The tiles of a workgroup, one after the other, and the blocks of each: while one block is multiplied the next is on its way into the
+// other half of the LDS.  kDirect: so is the first one of the next tile, while this tile's results are written.
+//   tile_of(id): a tile, with its number of blocks;  load(tile, n, half): its block n on its way;  store(half): what came through
+//   registers, to the LDS;  add(half);  end(tile)
+template <bool kDirect, typename TileFn, typename LoadFn, typename StoreFn, typename AddFn, typename EndFn>
+__device__ __forceinline__ void RunTiles(long long tiles, const TileFn &tile_of, const LoadFn &load, const StoreFn &store, const AddFn &add, const EndFn &end) {
+  long long id = blockIdx.x;
+  if (id >= tiles) return;
+  auto tile = tile_of(id);
+  int half = 0;
+  if (kDirect && tile.blocks > 0) load(tile, 0, half);
+  while (true) {
+    const long long next_id = id + gridDim.x;
+    const bool more = next_id < tiles;
+    auto next = tile_of(more ? next_id : id);
+    if (!kDirect && tile.blocks > 0) {
+      load(tile, 0, half);
+      __syncthreads();  // (the tile before has been multiplied)
+      store(half);
+    }
+    for (long long n = 0; n < tile.blocks; ++n) {
+      if (kDirect) WaitForLoads();
+      __syncthreads();  // (block n is there, and the half that what follows goes to has been read)
+      if (n + 1 < tile.blocks) load(tile, n + 1, half ^ 1);
+      else if (kDirect && more && next.blocks > 0) load(next, 0, half ^ 1);
+      add(half);
+      if (!kDirect && n + 1 < tile.blocks) store(half ^ 1);
+      half ^= 1;
+    }
+    end(tile);
+    if (!more) return;
+    id = next_id;
+    tile = next;
   }
-  __syncthreads();
 }
 
 // Workgroups that follow each other are on different XCDs: each XCD (its L2) gets tiles that lie together, eight rows of them by
@@ -307,6 +328,10 @@ struct Forward {
   void *gate, *up;
   float *gate_scales, *up_scales;
   long long kept_stride;
+  // the k's of a tile shared out
+  int splits;
+  long long split_blocks;
+  float *partial;  // [splits][rows][groups of 64 hidden columns][64 of the gate, 64 of up]
 };
 
 // What a lane holds of four values in each of four fragments along a row: 16 of a group of 64, the other lanes of its
@@ -350,37 +375,54 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
   LdsByte *blocks = (LdsByte *)s_blocks;
   constexpr int kK = kLineBytes / sizeof(T), kHidden = S::kJ / 2;
   const T *x = static_cast<const T *>(a.x), *w_gate = static_cast<const T *>(a.w_gate), *w_up = static_cast<const T *>(a.w_up);
+  const long long all_blocks = (a.dim + kK - 1) / kK, each = tile_rows * tile_columns;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
-  for (long long id = blockIdx.x; id < tiles; id += gridDim.x) {
-    long long i0;
-    int j0;
-    PlaceInGroup(PlaceOfTile(id, tiles), tile_rows, tile_columns, &i0, &j0);
-    i0 *= S::kI;
-    const int h0 = j0 * kHidden;
-    Tile t;
-    t.Clear();
-    Loader<T, S::kI, S::kThreads, false, kDirect> xs;
-    Loader<T, S::kJ, S::kThreads, false, kDirect> ws;
-    RunBlocks<kDirect>((a.dim + kK - 1) / kK,
-        [&](long long n, int half) {
-          LdsByte *to = blocks + half * S::kBlockBytes;
-          const long long w_at = h0 * a.w_stride + n * kK;
-          xs.Load(PlainRows<T>{x + i0 * a.x_stride + n * kK, a.x_stride, a.rows - i0}, 0, a.dim - n * kK, to);
-          ws.Load(PairedRows<T>{w_gate + w_at, w_up + w_at, a.w_stride, a.hidden - h0}, 0, a.dim - n * kK, to + S::kI * kLineBytes);
-        },
-        [&](int half) {
-          xs.Store(blocks + half * S::kBlockBytes);
-          ws.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
-        },
-        [&](int half) {
-          const LdsByte *from = blocks + half * S::kBlockBytes;
-          t.Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
-        });
-    const int h = h0 + wave_j * (kWaveJ / 2);
+  struct At {
+    long long i0, split, first, blocks;
+    int h0;
+  };
+  Tile t;
+  t.Clear();
+  Loader<T, S::kI, S::kThreads, false, kDirect> xs;
+  Loader<T, S::kJ, S::kThreads, false, kDirect> ws;
+  const auto tile_of = [&](long long id) {
+    At at;
+    const long long place = PlaceOfTile(id, tiles);
+    int column;
+    at.split = place / each;
+    PlaceInGroup(place - at.split * each, tile_rows, tile_columns, &at.i0, &column);
+    at.i0 *= S::kI;
+    at.h0 = column * kHidden;
+    at.first = at.split * a.split_blocks;
+    at.blocks = min(a.split_blocks, all_blocks - at.first);
+    return at;
+  };
+  const auto load = [&](const At &at, long long n, int half) {
+    LdsByte *to = blocks + half * S::kBlockBytes;
+    const long long k0 = (at.first + n) * kK, w_at = at.h0 * a.w_stride + k0;
+    xs.Load(PlainRows<T>{x + at.i0 * a.x_stride + k0, a.x_stride, a.rows - at.i0}, 0, a.dim - k0, to);
+    ws.Load(PairedRows<T>{w_gate + w_at, w_up + w_at, a.w_stride, a.hidden - at.h0}, 0, a.dim - k0, to + S::kI * kLineBytes);
+  };
+  const auto store = [&](int half) {
+    xs.Store(blocks + half * S::kBlockBytes);
+    ws.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
+  };
+  const auto add = [&](int half) {
+    const LdsByte *from = blocks + half * S::kBlockBytes;
+    t.Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
+  };
+  RunTiles<kDirect>(tiles, tile_of, load, store, add, [&](const At &at) {
+    const int h = at.h0 + wave_j * (kWaveJ / 2);
 #pragma unroll
     for (int i = 0; i < kWaveI / 16; ++i) {
-      const long long row = i0 + wave_i * kWaveI + i * 16 + lane % 16;
+      const long long row = at.i0 + wave_i * kWaveI + i * 16 + lane % 16;
       if (row >= a.rows || h >= a.hidden) continue;  // (all four lanes of a row)
+      if (a.splits > 1) {
+        float *to = a.partial + ((at.split * a.rows + row) * ((a.hidden + 63) / 64) + h / 64) * kWaveJ + lane / 16 * 4;
+#pragma unroll
+        for (int j = 0; j < kWaveJ / 16; ++j) *reinterpret_cast<F4 *>(to + j * 16) = t.acc[i][j];
+        continue;
+      }
       T *out = static_cast<T *>(a.out) + row * a.out_stride;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -394,6 +436,139 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
         Keep<T>(a.up, a.up_scales, a.kept_stride, row, h, a.hidden, t.acc[i] + 4);
       }
     }
+    t.Clear();
+  });
+}
+
+constexpr int kThreads = 256;  // of the kernels that go element by element
+
+// What was shared out: a wave sums 64 hidden columns of a row, in order, and ends as a tile does.
+template <typename T, int kAct>
+__global__ void __launch_bounds__(kThreads) k_gated_join(const Forward a, long long items) {
+  const int lane = threadIdx.x & 63, groups = (a.hidden + 63) / 64;
+  const long long step = a.rows * groups * kWaveJ;
+  for (long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); item < items; item += (long long)gridDim.x * 4) {
+    const long long row = item / groups;
+    const int group = (int)(item - row * groups), h = group * 64 + lane;
+    const float *from = a.partial + item * kWaveJ + lane;
+    float g = from[0], u = from[64];
+    for (int split = 1; split < a.splits; ++split) {
+      g += from[split * step];
+      u += from[split * step + 64];
+    }
+    const bool there = h < a.hidden;
+    if (there) static_cast<T *>(a.out)[row * a.out_stride + h] = Round<T>(Act<kAct>(g) * u);
+    if (a.gate == nullptr) continue;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const float v = which == 0 ? g : u;
+      void *kept = which == 0 ? a.gate : a.up;
+      float *scales = which == 0 ? a.gate_scales : a.up_scales;
+      if (scales == nullptr) {
+        if (there) static_cast<T *>(kept)[row * a.kept_stride + h] = Round<T>(v);
+        continue;
+      }
+      unsigned most = there ? Magnitude(v) : 0;
+#pragma unroll
+      for (int by = 32; by > 0; by /= 2) most = max(most, (unsigned)__shfl_xor((int)most, by));
+      const float scale = ScaleOf(most);
+      if (lane == 0) scales[row * groups + group] = scale;
+      const float one[1] = {v};
+      if (there) static_cast<signed char *>(kept)[row * a.kept_stride + h] = CodesOf(one, scale).v[0];
+    }
+  }
+}
+
+// Few rows (up to 16): 16 hidden columns a workgroup, whose eight waves share out the k's.  The weights are read once, from memory into the
+// registers that the products take them from: a lane's chunk is 16 bytes of a weight row, four steps of 64 bytes a row at once.
+constexpr int kFewRows = 16, kFewWaves = 8;
+template <typename T, int kAct>
+__global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
+  constexpr int kVec = 16 / sizeof(T), kStep = 4 * kVec, kUnroll = 4;
+  __shared__ float s_sums[kFewWaves][2][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h0 = blockIdx.x * 16, quarter = lane / 16;
+  const long long h = min(h0 + lane % 16, a.hidden - 1), i = min(lane % 16ll, a.rows - 1);
+  const T *gate = static_cast<const T *>(a.w_gate) + h * a.w_stride + quarter * kVec, *up = static_cast<const T *>(a.w_up) + h * a.w_stride + quarter * kVec;
+  const T *x = static_cast<const T *>(a.x) + i * a.x_stride + quarter * kVec;
+  F4 g = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+  const int steps = (a.dim + kStep - 1) / kStep, groups = a.dim / kStep / kUnroll;
+  const auto whole = [&](const T *from) { return __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Pack<T, kVec> *>(from)); };
+  for (int group = wave; group < groups; group += kFewWaves) {
+    Chunk<T> gs[kUnroll], us[kUnroll], xs[kUnroll];
+#pragma unroll
+    for (int n = 0; n < kUnroll; ++n) {
+      const int k = (group * kUnroll + n) * kStep;
+      gs[n] = whole(gate + k);
+      us[n] = whole(up + k);
+      xs[n] = whole(x + k);
+    }
+#pragma unroll
+    for (int n = 0; n < kUnroll; ++n) {
+      g = Product(gs[n], xs[n], g);
+      u = Product(us[n], xs[n], u);
+    }
+  }
+  static_assert(kUnroll <= kFewWaves, "a wave for each step that is left");
+  if (const int step = groups * kUnroll + wave; step < steps) {
+    const int k = step * kStep, held = a.dim - k - quarter * kVec;
+    const auto part = [&](const T *from) {
+      Chunk<T> c;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) c.v[e] = e < held ? from[e] : T(0);
+      return c;
+    };
+    const Chunk<T> xs = part(x + k);
+    g = Product(part(gate + k), xs, g);
+    u = Product(part(up + k), xs, u);
+  }
+  *reinterpret_cast<F4 *>(&s_sums[wave][0][lane * 4]) = g;
+  *reinterpret_cast<F4 *>(&s_sums[wave][1][lane * 4]) = u;
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int in = threadIdx.x, of = in / 4, row = of % 16, column = h0 + of / 16 * 4 + in % 4;  // of: the lane that held it
+  if (row >= a.rows || column >= a.hidden) return;
+  float gv = 0.0f, uv = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) {
+    gv += s_sums[w][0][in];
+    uv += s_sums[w][1][in];
+  }
+  static_cast<T *>(a.out)[row * a.out_stride + column] = Round<T>(Act<kAct>(gv) * uv);
+  if (a.gate != nullptr) {
+    static_cast<T *>(a.gate)[row * a.kept_stride + column] = Round<T>(gv);
+    static_cast<T *>(a.up)[row * a.kept_stride + column] = Round<T>(uv);
+  }
+}
+
+// Up to three matrices of rows that begin anywhere, to rows that begin at multiples of 64 elements, 0 behind each row's end.
+struct Padded {
+  const void *from[3];
+  void *to[3];
+  long long rows[3], from_stride[3];
+  int width;
+  long long to_stride;
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_pad(const Padded a, long long blocks) {
+  constexpr int kVec = 8;
+  const unsigned vectors = (unsigned)(a.to_stride / kVec);
+  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const long long first = block * kThreads, row0 = first / vectors;
+    const unsigned in = (unsigned)(first - row0 * vectors) + threadIdx.x, more = in / vectors;
+    long long row = row0 + more;
+    int which = 0;
+    while (which < 3 && row >= a.rows[which]) row -= a.rows[which++];
+    if (which == 3) continue;
+    const int at = (int)(in - more * vectors) * kVec, held = a.width - at;
+    const T *from = static_cast<const T *>(a.from[which]) + row * a.from_stride[which] + at;
+    Pack<T, kVec> p;
+    if (held >= kVec) {
+      p = *reinterpret_cast<const Pack<T, kVec> *>(from);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) p.v[c] = c < held ? from[c] : T(0);
+    }
+    *reinterpret_cast<Pack<T, kVec> *>(static_cast<T *>(a.to[which]) + row * a.to_stride + at) = p;
   }
 }
 
@@ -404,57 +579,63 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
   constexpr int kK = kLineBytes / sizeof(T);
   const long long segment_blocks = (p.inner + kK - 1) / kK, each = tile_rows * tile_columns;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
-  for (long long id = blockIdx.x; id < tiles; id += gridDim.x) {
-    const long long at = PlaceOfTile(id, tiles), one = at / each;
-    const int member = (int)(one / p.splits), split = (int)(one % p.splits);
-    long long i0;
-    int j0;
-    PlaceInGroup(at - one * each, tile_rows, tile_columns, &i0, &j0);
-    i0 *= S::kI;
-    j0 *= S::kJ;
-    Tile t;
-    t.Clear();
-    Loader<T, S::kI, S::kThreads, kAcrossA, kDirect> as;
-    Loader<T, S::kJ, S::kThreads, kAcrossB, kDirect> bs;
-    const long long first = split * p.split_blocks, end = min(first + p.split_blocks, segment_blocks * p.segments);
-    RunBlocks<kDirect>(end - first,
-        [&](long long n, int half) {
-          const int segment = first + n >= segment_blocks;
-          const long long k0 = (first + n - segment * segment_blocks) * kK;
-          const T *a = static_cast<const T *>(p.a.at[member + segment]), *b = static_cast<const T *>(p.b.at[member + segment]);
-          LdsByte *to = blocks + half * S::kBlockBytes;
-          as.Load(PlainRows<T>{kAcrossA ? a + k0 * p.a.stride + i0 : a + i0 * p.a.stride + k0, p.a.stride, p.rows - i0}, p.rows - i0, p.inner - k0, to);
-          bs.Load(PlainRows<T>{kAcrossB ? b + k0 * p.b.stride + j0 : b + j0 * p.b.stride + k0, p.b.stride, p.columns - j0}, p.columns - j0, p.inner - k0,
-                  to + S::kI * kLineBytes);
-        },
-        [&](int half) {
-          as.Store(blocks + half * S::kBlockBytes);
-          bs.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
-        },
-        [&](int half) {
-          const LdsByte *from = blocks + half * S::kBlockBytes;
-          t.Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
-        });
+  struct At {
+    long long i0, one, first, blocks;
+    int j0, member;
+  };
+  Tile t;
+  t.Clear();
+  Loader<T, S::kI, S::kThreads, kAcrossA, kDirect> as;
+  Loader<T, S::kJ, S::kThreads, kAcrossB, kDirect> bs;
+  const auto tile_of = [&](long long id) {
+    At at;
+    const long long place = PlaceOfTile(id, tiles);
+    at.one = place / each;
+    at.member = (int)(at.one / p.splits);
+    PlaceInGroup(place - at.one * each, tile_rows, tile_columns, &at.i0, &at.j0);
+    at.i0 *= S::kI;
+    at.j0 *= S::kJ;
+    at.first = (at.one % p.splits) * p.split_blocks;
+    at.blocks = min(p.split_blocks, segment_blocks * p.segments - at.first);
+    return at;
+  };
+  const auto load = [&](const At &at, long long n, int half) {
+    const int segment = at.first + n >= segment_blocks, which = at.member + segment;
+    const long long k0 = (at.first + n - segment * segment_blocks) * kK;
+    const T *a = static_cast<const T *>(p.a.at[which]), *b = static_cast<const T *>(p.b.at[which]);
+    LdsByte *to = blocks + half * S::kBlockBytes;
+    as.Load(PlainRows<T>{kAcrossA ? a + k0 * p.a.stride + at.i0 : a + at.i0 * p.a.stride + k0, p.a.stride, p.rows - at.i0}, p.rows - at.i0, p.inner - k0, to);
+    bs.Load(PlainRows<T>{kAcrossB ? b + k0 * p.b.stride + at.j0 : b + at.j0 * p.b.stride + k0, p.b.stride, p.columns - at.j0}, p.columns - at.j0, p.inner - k0,
+            to + S::kI * kLineBytes);
+  };
+  const auto store = [&](int half) {
+    as.Store(blocks + half * S::kBlockBytes);
+    bs.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
+  };
+  const auto add = [&](int half) {
+    const LdsByte *from = blocks + half * S::kBlockBytes;
+    t.Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
+  };
+  RunTiles<kDirect>(tiles, tile_of, load, store, add, [&](const At &at) {
 #pragma unroll
     for (int i = 0; i < kWaveI / 16; ++i) {
-      const long long row = i0 + wave_i * kWaveI + i * 16 + lane % 16;
+      const long long row = at.i0 + wave_i * kWaveI + i * 16 + lane % 16;
       if (row >= p.rows) continue;
 #pragma unroll
       for (int j = 0; j < kWaveJ / 16; ++j) {
-        const int column = j0 + wave_j * kWaveJ + j * 16 + lane / 16 * 4;
+        const int column = at.j0 + wave_j * kWaveJ + j * 16 + lane / 16 * 4;
         if (p.splits > 1) {
           const float four[4] = {t.acc[i][j][0], t.acc[i][j][1], t.acc[i][j][2], t.acc[i][j][3]};
-          StoreFour<float>(p.partial + (one * p.rows + row) * p.columns, column, p.columns, four);
+          StoreFour<float>(p.partial + (at.one * p.rows + row) * p.columns, column, p.columns, four);
         } else {
           const T four[4] = {Round<T>(t.acc[i][j][0]), Round<T>(t.acc[i][j][1]), Round<T>(t.acc[i][j][2]), Round<T>(t.acc[i][j][3])};
-          StoreFour<T>(static_cast<T *>(p.c[member]) + row * p.c_stride, column, p.columns, four);
+          StoreFour<T>(static_cast<T *>(p.c[at.member]) + row * p.c_stride, column, p.columns, four);
         }
       }
     }
-  }
+    t.Clear();
+  });
 }
-
-constexpr int kThreads = 256;  // of the kernels that go element by element
 
 // The sums of what was shared out, in order.
 template <typename T>
@@ -542,7 +723,7 @@ __global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long b
 
 // ------------------------------------------------------------------ launches
 
-constexpr long long kMostGrid = 1 << 20;
+constexpr long long kMostGrid = 1 << 20, kCus = 256;
 
 template <typename Fn>
 void WithActivation(int activation, Fn &&fn) {
@@ -562,11 +743,10 @@ void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   const auto launch = [&](auto shape, auto is_direct) {
     typedef decltype(shape) S;
     const long long tile_rows = Pieces(p.rows, S::kI), tiles = tile_rows * Pieces(p.columns, S::kJ) * p.batch * p.splits;
-    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kMostGrid)), dim3(S::kThreads), 0, stream, p, tiles,
+    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, p, tiles,
                        tile_rows, (int)Pieces(p.columns, S::kJ));
   };
   if (large && direct) launch(LargeTile(), std::true_type());
-  else if (large) launch(LargeTile(), std::false_type());
   else if (direct) launch(SmallTile(), std::true_type());
   else launch(SmallTile(), std::false_type());
   if (p.splits > 1) {
@@ -575,36 +755,64 @@ void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   }
 }
 
+// x and the two weights in rows that begin at multiples of 64 elements, where the plan has room for that and any of them needs it.
+template <typename T>
+bool Pad(GatedLayer *l, const LayerPad &pad, bool x, bool weights, unsigned char *work) {
+  if (pad.stride == 0) return false;
+  Padded p{{l->x, l->w_gate, l->w_up}, {work + pad.x, work + pad.w_gate, work + pad.w_up}, {x ? l->rows : 0, weights ? l->hidden : 0, weights ? l->hidden : 0},
+           {l->x_stride, l->w_stride, l->w_stride}, l->dim, pad.stride};
+  const long long blocks = Pieces((p.rows[0] + p.rows[1] + p.rows[2]) * (pad.stride / 8), kThreads);
+  hipLaunchKernelGGL((k_pad<T>), dim3((unsigned)std::min(blocks, kMostGrid)), dim3(kThreads), 0, static_cast<hipStream_t>(l->stream), p, blocks);
+  l->x = p.to[0];
+  l->w_gate = p.to[1];
+  l->w_up = p.to[2];
+  l->x_stride = l->w_stride = pad.stride;
+  return true;
+}
+
 }  // namespace
 
 template <typename T>
-void RunGated(const GatedArgs &a, bool large) {
-  const GatedLayer &l = a.layer;
+void RunGated(const GatedArgs &a, const GatedPlan &plan) {
+  GatedLayer l = a.layer;
+  const hipStream_t stream = static_cast<hipStream_t>(l.stream);
+  unsigned char *work = static_cast<unsigned char *>(l.work);
+  const bool few = plan.few && !l.gate_scales;
+  const bool padded = !few && Pad<T>(&l, plan.pad, true, true, work);
+  const long long extent = padded ? plan.pad.stride : l.dim;
+  const bool direct = IsDirect<T>(l.x, l.x_stride, extent) && IsDirect<T>(l.w_gate, l.w_stride, extent) && IsDirect<T>(l.w_up, l.w_stride, extent);
   const Forward f{l.x, l.w_gate, l.w_up, l.rows, l.dim, l.hidden, l.x_stride, l.w_stride, a.out, a.out_stride, l.gate, l.up, l.gate_scales,
-                  l.up_scales, l.kept_stride};
-  const bool direct = IsDirect<T>(l.x, l.x_stride, l.dim) && IsDirect<T>(l.w_gate, l.w_stride, l.dim) && IsDirect<T>(l.w_up, l.w_stride, l.dim);
+                  l.up_scales, l.kept_stride, (int)plan.out.splits, plan.out.split_blocks, reinterpret_cast<float *>(work + plan.partial)};
   WithActivation(l.activation, [&](auto act) {
+    constexpr int kAct = decltype(act)::value;
+    if (few) {
+      hipLaunchKernelGGL((k_gated_few<T, kAct>), dim3((unsigned)Pieces(l.hidden, 16)), dim3(64 * kFewWaves), 0, stream, f);
+      return;
+    }
     const auto launch = [&](auto shape, auto is_direct) {
       typedef decltype(shape) S;
-      const long long tile_rows = Pieces(l.rows, S::kI), tile_columns = Pieces(l.hidden, S::kJ / 2), tiles = tile_rows * tile_columns;
-      hipLaunchKernelGGL((k_gated<T, decltype(act)::value, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kMostGrid)),
-                         dim3(S::kThreads), 0, static_cast<hipStream_t>(l.stream), f, tiles, tile_rows, (int)tile_columns);
+      const long long tile_rows = Pieces(l.rows, S::kI), tile_columns = Pieces(l.hidden, S::kJ / 2), tiles = tile_rows * tile_columns * f.splits;
+      hipLaunchKernelGGL((k_gated<T, kAct, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, f, tiles,
+                         tile_rows, (int)tile_columns);
     };
-    if (large && direct) launch(LargeTile(), std::true_type());
-    else if (large) launch(LargeTile(), std::false_type());
+    if (plan.out.large && direct) launch(LargeTile(), std::true_type());
     else if (direct) launch(SmallTile(), std::true_type());
     else launch(SmallTile(), std::false_type());
+    if (f.splits > 1) {
+      const long long items = l.rows * Pieces(l.hidden, 64);
+      hipLaunchKernelGGL((k_gated_join<T, kAct>), dim3((unsigned)std::min(Pieces(items, 4), kMostGrid)), dim3(kThreads), 0, stream, f, items);
+    }
   });
   HIP_OK(hipGetLastError());
 }
 
 template <typename T>
-void RunGatedGrad(const GatedGradArgs &a, const GatedPlan &plan) {
-  const GatedLayer &l = a.layer;
+void RunGatedGrad(const GatedGradArgs &a, const GatedGradPlan &plan) {
+  GatedLayer l = a.layer;
   const hipStream_t stream = static_cast<hipStream_t>(l.stream);
   unsigned char *work = static_cast<unsigned char *>(l.work);
-  void *d_gate = work, *d_up = work + plan.d_bytes;
-  float *partial = reinterpret_cast<float *>(work + 2 * plan.d_bytes);
+  void *d_gate = work + plan.d_gate, *d_up = work + plan.d_up;
+  float *partial = reinterpret_cast<float *>(work + plan.partial);
   if (l.rows > 0) {
     const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden};
     const long long blocks = Pieces(l.rows * (plan.d_stride / kSlopeVec), kThreads);
@@ -615,17 +823,19 @@ void RunGatedGrad(const GatedGradArgs &a, const GatedPlan &plan) {
       else hipLaunchKernelGGL((k_slopes<T, kAct, false>), grid, dim3(kThreads), 0, stream, s, blocks);
     });
   }
+  const bool padded = Pad<T>(&l, plan.pad, a.grad_w_gate != nullptr, a.grad_x != nullptr, work);
+  const long long extent = padded ? plan.pad.stride : l.dim;
   const Operand d{{d_gate, d_up}, plan.d_stride};
   const bool d_direct = IsDirect<T>(d_gate, plan.d_stride, plan.d_stride);
   if (a.grad_x && l.rows > 0) {
     const Products p{d, {{l.w_gate, l.w_up}, l.w_stride}, l.rows, l.dim, l.hidden, 2, 1, {a.grad_x, nullptr}, a.grad_x_stride,
                      (int)plan.x.splits, plan.x.split_blocks, partial};
-    Launch<T, false, true>(p, plan.x.large, d_direct && IsDirect<T>(l.w_gate, l.w_stride, l.dim) && IsDirect<T>(l.w_up, l.w_stride, l.dim), stream);
+    Launch<T, false, true>(p, plan.x.large, d_direct && IsDirect<T>(l.w_gate, l.w_stride, extent) && IsDirect<T>(l.w_up, l.w_stride, extent), stream);
   }
   if (a.grad_w_gate) {
     const Products p{d, {{l.x, l.x}, l.x_stride}, l.hidden, l.dim, l.rows, 1, 2, {a.grad_w_gate, a.grad_w_up}, a.grad_w_stride,
                      (int)plan.w.splits, plan.w.split_blocks, partial};
-    Launch<T, true, true>(p, plan.w.large, d_direct && IsDirect<T>(l.x, l.x_stride, l.dim), stream);
+    Launch<T, true, true>(p, plan.w.large, d_direct && IsDirect<T>(l.x, l.x_stride, extent), stream);
   }
   HIP_OK(hipGetLastError());
 }

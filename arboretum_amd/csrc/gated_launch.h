@@ -14,7 +14,8 @@ template <int kWavesI, int kWavesJ>
 struct TileShape {
   static constexpr int kThreads = 64 * kWavesI * kWavesJ, kI = kWaveI * kWavesI, kJ = kWaveJ * kWavesJ;
   static constexpr int kBlockBytes = (kI + kJ) * kLineBytes;
-  static constexpr int kWavesEach = kWavesI * kWavesJ / 4 > 0 ? kWavesI * kWavesJ / 4 : 1;  // waves of a SIMD: the LDS holds one large tile, or two small ones
+  static constexpr int kEach = kBlockBytes > 40 * 1024 ? 1 : 2;             // workgroups of a CU: its LDS holds two blocks of each
+  static constexpr int kWavesEach = (kWavesI * kWavesJ * kEach + 3) / 4;  // waves of a SIMD
 };
 typedef TileShape<4, 2> LargeTile;
 typedef TileShape<2, 1> SmallTile;
@@ -24,19 +25,32 @@ struct ProductCut {
   bool large;
   long long splits, split_blocks;
 };
+// Where in the work memory (bytes from its start) copies of x and the weights lie whose rows begin at multiples of 64 elements;
+// stride 0: there are none.
+struct LayerPad {
+  long long stride;
+  size_t x, w_gate, w_up;
+};
 struct GatedPlan {
-  long long d_stride;  // elements between rows of d_gate and of d_up in the work memory
+  bool few;
+  ProductCut out;
+  LayerPad pad;
+  size_t partial, bytes;
+};
+struct GatedGradPlan {
+  long long d_stride;  // elements between rows of d_gate and of d_up
   ProductCut x, w;     // of grad_x, of the weights' gradients
-  size_t d_bytes, bytes;
+  LayerPad pad;
+  size_t d_gate, d_up, partial, bytes;
 };
 
 inline long long Pieces(long long n, long long of) { return (n + of - 1) / of; }
 
 // (arguments that have passed the checks)
 template <typename T>
-void RunGated(const GatedArgs &a, bool large);
+void RunGated(const GatedArgs &a, const GatedPlan &plan);
 template <typename T>
-void RunGatedGrad(const GatedGradArgs &a, const GatedPlan &plan);
+void RunGatedGrad(const GatedGradArgs &a, const GatedGradPlan &plan);
 
 }  // namespace arb
 #endif  // ARBORETUM_AMD_GATED_LAUNCH_H_
