@@ -96,14 +96,18 @@ typedef __attribute__((address_space(3))) I4 LdsI4;
 
 // 16 bytes a lane from `base` + `at` (beyond 2^31: 0) to the LDS, the wave's 1 KB side by side from `to` on.  By hand: the
 // compiler waits for a load of its own before any read of the LDS, and this one is meant to be on its way meanwhile.  Whoever reads
-// what it writes waits for it first (WaitForLoads and a barrier).
-__device__ __forceinline__ void LoadToLds(const void *base, unsigned at, LdsByte *to) {
-  const unsigned long long address = reinterpret_cast<unsigned long long>(base);
-  const I4 from = {(int)__builtin_amdgcn_readfirstlane((int)address), (int)__builtin_amdgcn_readfirstlane((int)(address >> 32)) & 0xFFFF, 0x7FFFFFFF, 0x00020000};
-  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)to);
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(lds) : "memory");
+// what it writes waits for it first (WaitAndMeet, which nothing that touches memory moves across).
+__device__ __forceinline__ void LoadToLds(unsigned long long base, unsigned at, unsigned to) {
+  const I4 from = {(int)(unsigned)base, (int)(unsigned)(base >> 32), 0x7FFFFFFF, 0x00020000};
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(to));
 }
-__device__ __forceinline__ void WaitForLoads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Until no more than kLast of the wave's loads are on their way (they arrive in the order they were issued in), what it has read of the LDS is there,
+// and all waves of the workgroup are as far.
+template <int kLast>
+__device__ __forceinline__ void WaitAndMeet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLast) : "memory");
+}
 
 // The chunks of an operand's block in the LDS.  Along k: line by line, 8 chunks each; across: k by k, the chunks of all lines.
 // Chunks change places from line to line (from k to k), so that the lanes that read together meet other banks: they
@@ -144,72 +148,124 @@ struct Layout {
   }
 };
 
-// Rows of an operand, `lines` of which are there from `base` on.
-template <typename T>
-struct PlainRows {
-  const T *base;
-  long long stride, lines;
-  __device__ __forceinline__ const T *Base(int) const { return base; }
-  __device__ __forceinline__ int Number(int row) const { return row; }
-  __device__ __forceinline__ bool Held(int row) const { return row < lines; }
-  __device__ __forceinline__ long long Clamped(int row) const { return min((long long)row, lines - 1); }
+__device__ __forceinline__ unsigned long long Uniform(unsigned long long v) {
+  return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)v);
+}
+
+// The k's of a tile's lines that lie one after the other: `blocks` blocks of them from `base` on (kPaired: 64 lines from there, 64 from `second`, the next
+// 64 of each ...), `left` k's and `lines` lines (of each) from there to the operand's end.
+struct Run {
+  const void *base, *second;
+  long long lines, left;
+  int blocks;
 };
 
-// 64 rows of the gate and the same of up, the next 64, ... (what a workgroup loads at once is of one of the two)
-template <typename T>
-struct PairedRows {
-  const T *gate, *up;
-  long long stride, lines;
-  __device__ __forceinline__ const T *Base(int row) const { return row & 64 ? up : gate; }
-  __device__ __forceinline__ int Number(int row) const { return row / 128 * 64 + row % 64; }
-  __device__ __forceinline__ bool Held(int row) const { return Number(row) < lines; }
-  __device__ __forceinline__ long long Clamped(int row) const { return min((long long)Number(row), lines - 1); }
-};
+// The row of a block's line (k, across): kPaired, of the gate or of up.
+template <bool kPaired>
+__device__ __forceinline__ int RowOf(int line) {
+  return kPaired ? line / 128 * 64 + line % 64 : line;
+}
 
-// One operand's block on its way to the LDS.  kDirect: by loads that write there, for operands whose chunks are aligned and
-// whole; else through registers, whatever the alignment.
-template <typename T, int kLines, int kThreads, bool kAcross, bool kDirect>
-struct Loader {
+// An operand's blocks, run after run and tile after tile, each by loads that write to the LDS: for operands whose chunks are aligned and
+// whole.  A block costs its loads and next to nothing else: where a lane reads is worked out once a run.
+template <typename T, int kLines, int kThreads, bool kAcross, bool kPaired>
+struct Stream {
   typedef Layout<T, kLines, kAcross> L;
-  static constexpr int kVec = L::kVec, kPieces = kLines * 8 / kThreads;
-  Chunk<T> piece[kDirect ? 1 : kPieces];
+  static constexpr int kVec = L::kVec, kPieces = kLines * 8 / kThreads, kK = kLineBytes / sizeof(T);
+  static_assert(!kPaired || kThreads / 8 <= 64, "what is loaded at once is of one of the two");
+  unsigned at[kPieces];
+  unsigned long long base, second, step;
+  int left, blocks, part;  // left: k's to the operand's end (2^30: or more)
+  unsigned id, lds;
+  bool live;
 
-  // The block that `rows` (of lines along k, or k by k) stand for, `left` of whose k's, and across `lines` of whose lines, are in
-  // the operand.
-  template <typename Rows>
-  __device__ __forceinline__ void Load(const Rows &rows, long long lines, long long left, LdsByte *block) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if constexpr (kDirect) {
-#pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
-        const int q = p * kThreads + threadIdx.x, row = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(row);
-        const bool held = kAcross ? row < left && chunk * kVec < lines : rows.Held(row) && chunk * kVec < left;
-        const unsigned at = held ? ((unsigned)rows.Number(row) * (unsigned)rows.stride + chunk * kVec) * (unsigned)sizeof(T) : kNowhere;
-        LoadToLds(rows.Base(p * kThreads / L::kRowChunks), at, block + (p * kThreads + wave * 64) * 16);
+  template <typename RunOf>
+  __device__ __forceinline__ void Start(const RunOf &run_of, unsigned tiles, int parts, long long stride) {
+    step = kAcross ? (unsigned long long)kK * stride * sizeof(T) : kLineBytes;
+    id = blockIdx.x - gridDim.x;
+    part = parts - 1;
+    Next(run_of, tiles, parts, stride);
+  }
+  template <typename RunOf>
+  __device__ __forceinline__ void Next(const RunOf &run_of, unsigned tiles, int parts, long long stride) {
+    Run run;
+    do {
+      if (++part == parts) {
+        part = 0;
+        id += gridDim.x;
       }
-    } else {
-      // (lines beyond the operand along k: the last one again, whose results are not stored; k's beyond it are 0)
-      const bool whole = left >= kLineBytes / (int)sizeof(T) && (!kAcross || lines >= kLines);
+      live = id < tiles;
+      if (!live) return;
+      run = run_of(id, part);
+    } while (run.blocks <= 0);
+    base = Uniform(reinterpret_cast<unsigned long long>(run.base));
+    second = Uniform(reinterpret_cast<unsigned long long>(run.second));
+    left = (int)min(run.left, 1ll << 30);
+    blocks = run.blocks;
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
-        const int q = p * kThreads + threadIdx.x, row = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(row);
-        const T *from = rows.Base(p * kThreads / L::kRowChunks) + (kAcross ? row : rows.Clamped(row)) * rows.stride + chunk * kVec;
-        if (whole) {
-          piece[p] = __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Pack<T, kVec> *>(from));
-        } else {
-          const long long held = !kAcross ? left - chunk * kVec : row < left ? lines - chunk * kVec : 0;
+    for (int p = 0; p < kPieces; ++p) {
+      const int q = p * kThreads + threadIdx.x, line = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(line);
+      const bool held = kAcross ? chunk * kVec < run.lines : RowOf<kPaired>(line) < run.lines;
+      at[p] = held ? ((unsigned)RowOf<kPaired>(line) * (unsigned)stride + chunk * kVec) * (unsigned)sizeof(T) : kNowhere;
+    }
+  }
+  // The next block, if there is one, goes to `to`: its loads one by one (Piece), then Done.
+  template <typename RunOf>
+  __device__ __forceinline__ void Prepare(unsigned to, const RunOf &run_of, unsigned tiles, int parts, long long stride) {
+    if (blocks == 0 && live) Next(run_of, tiles, parts, stride);
+    lds = to + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+  }
+  __device__ __forceinline__ void Piece(int p) const {
+    // (k's beyond the operand's end: from nowhere)
+    const int q = p * kThreads + threadIdx.x, line = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(line);
+    const unsigned from = (kAcross ? line : chunk * kVec) < left ? at[p] : kNowhere;
+    LoadToLds(kPaired && (p * kThreads / 8 & 64) ? second : base, from, lds + p * kThreads * 16);
+  }
+  __device__ __forceinline__ void Done() {
+    if (!live) return;
+    base += step;
+    second += step;
+    left -= kK;
+    --blocks;
+  }
+  template <typename RunOf>
+  __device__ __forceinline__ void Issue(unsigned to, const RunOf &run_of, unsigned tiles, int parts, long long stride) {
+    Prepare(to, run_of, tiles, parts, stride);
+    if (!live) return;
 #pragma unroll
-          for (int c = 0; c < kVec; ++c) piece[p].v[c] = c < held ? from[c] : T(0);
-        }
+    for (int p = 0; p < kPieces; ++p) Piece(p);
+    Done();
+  }
+};
+
+// An operand's block through registers, whatever its alignment.  (Lines beyond the operand along k: the last one again, whose results are not stored; k's
+// beyond it are 0.)
+template <typename T, int kLines, int kThreads, bool kAcross, bool kPaired>
+struct Stage {
+  typedef Layout<T, kLines, kAcross> L;
+  static constexpr int kVec = L::kVec, kPieces = kLines * 8 / kThreads, kK = kLineBytes / sizeof(T);
+  Chunk<T> piece[kPieces];
+
+  __device__ __forceinline__ void Load(const Run &run, long long n, long long stride) {
+    const long long left = run.left - n * kK, skip = n * kK * (kAcross ? stride : 1);
+    const bool whole = left >= kK && (!kAcross || run.lines >= kLines);
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int q = p * kThreads + threadIdx.x, line = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(line);
+      const T *base = static_cast<const T *>(kPaired && (p * kThreads / 8 & 64) ? run.second : run.base) + skip;
+      const T *from = base + (kAcross ? line : min((long long)RowOf<kPaired>(line), run.lines - 1)) * stride + chunk * kVec;
+      if (whole) {
+        piece[p] = __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Pack<T, kVec> *>(from));
+      } else {
+        const long long held = !kAcross ? left - chunk * kVec : line < left ? run.lines - chunk * kVec : 0;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) piece[p].v[c] = c < held ? from[c] : T(0);
       }
     }
   }
   __device__ __forceinline__ void Store(LdsByte *block) const {
-    if constexpr (!kDirect) {
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p)
-        *(LdsI4 *)(block + (p * kThreads + threadIdx.x) * 16) = __builtin_bit_cast(I4, piece[p]);
-    }
+    for (int p = 0; p < kPieces; ++p) *(LdsI4 *)(block + (p * kThreads + threadIdx.x) * 16) = __builtin_bit_cast(I4, piece[p]);
   }
 };
 
@@ -222,88 +278,126 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < kWaveJ / 16; ++j) acc[i][j] = F4{0, 0, 0, 0};
   }
-  // Both halves of a block.  What is read for a product is asked for eight products ahead, which the order at the end makes sure of:
-  // left alone the compiler reads a chunk, waits and multiplies, with as few registers as that takes.
-  template <typename T, typename LayoutA, typename LayoutB>
-  __device__ __forceinline__ void Add(const LdsByte *a, const LdsByte *b, int wave_i, int wave_j) {
+  // Both halves of a block, in 16 steps of four products; between(step) after each.  What is read for a product is asked for kAhead steps ahead, and
+  // steps stay as they are written: left alone the compiler reads a chunk, waits and multiplies, with as few registers as that takes.
+  static constexpr int kSteps = 2 * (kWaveJ / 16), kAhead = 4;
+  template <typename T, typename LayoutA, typename LayoutB, typename Between>
+  __device__ __forceinline__ void Add(const LdsByte *a, const LdsByte *b, int wave_i, int wave_j, const Between &between) {
     constexpr int kFragsI = kWaveI / 16, kFragsJ = kWaveJ / 16;
     Chunk<T> x[2][kFragsI], y[2][kFragsJ];
+    const auto read_x = [&](int half, int i) { x[half][i] = LayoutA::Read(a, wave_i * kWaveI + i * 16, half); };
+    const auto read_y = [&](int half, int j) { y[half][j] = LayoutB::Read(b, wave_j * kWaveJ + j * 16, half); };
+#pragma unroll
+    for (int i = 0; i < kFragsI; ++i) read_x(0, i);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) read_y(0, j);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int i = 0; i < kFragsI; ++i) x[half][i] = LayoutA::Read(a, wave_i * kWaveI + i * 16, half);
-#pragma unroll
-      for (int j = 0; j < kFragsJ; ++j) y[half][j] = LayoutB::Read(b, wave_j * kWaveJ + j * 16, half);
-#pragma unroll
-      for (int j = 0; j < kFragsJ; ++j)
+      for (int j = 0; j < kFragsJ; ++j) {
+        const int soon = j + kAhead - kFragsJ;  // of the next half
+        if (soon < 0) {
+          read_y(half, j + kAhead);
+        } else if (half == 0) {
+          read_y(1, soon);
+          if (soon < kFragsI) read_x(1, soon);
+        }
 #pragma unroll
         for (int i = 0; i < kFragsI; ++i) acc[i][j] = Product(y[half][j], x[half][i], acc[i][j]);
-    }
-    constexpr int kRead = 0x100, kMultiply = 0x8, kPer = kFragsI * (sizeof(T) == 4 ? 4 : 1);
-    __builtin_amdgcn_sched_group_barrier(kRead, kFragsI * LayoutA::kReads + 2 * LayoutB::kReads, 0);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int j = 0; j < kFragsJ - 2; ++j) {
-        __builtin_amdgcn_sched_group_barrier(kMultiply, kPer, 0);
-        __builtin_amdgcn_sched_group_barrier(kRead, LayoutB::kReads, 0);
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        __builtin_amdgcn_sched_group_barrier(kMultiply, kPer, 0);
-        if (half == 0) __builtin_amdgcn_sched_group_barrier(kRead, kFragsI / 2 * LayoutA::kReads + LayoutB::kReads, 0);
+        between(half * kFragsJ + j);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 };
 
-// The tiles of a workgroup, one after the other, and the blocks of each: while one block is multiplied the next is on its way into the
-// other half of the LDS.  kDirect: so is the first one of the next tile, while this tile's results are written.
-//   tile_of(id): a tile, with its number of blocks;  load(tile, n, half): its block n on its way;  store(half): what came through
-//   registers, to the LDS;  add(half);  end(tile)
-template <bool kDirect, typename TileFn, typename LoadFn, typename StoreFn, typename AddFn, typename EndFn>
-__device__ __forceinline__ void RunTiles(long long tiles, const TileFn &tile_of, const LoadFn &load, const StoreFn &store, const AddFn &add, const EndFn &end) {
-  long long id = blockIdx.x;
-  if (id >= tiles) return;
-  auto tile = tile_of(id);
-  int half = 0;
-  if (kDirect && tile.blocks > 0) load(tile, 0, half);
-  while (true) {
-    const long long next_id = id + gridDim.x;
-    const bool more = next_id < tiles;
-    auto next = tile_of(more ? next_id : id);
-    if (!kDirect && tile.blocks > 0) {
-      load(tile, 0, half);
-      __syncthreads();  // (the tile before has been multiplied)
-      store(half);
+// The blocks of a workgroup's tiles, one after the other.  kDirect: while one is multiplied, the next one of A and the next two of B are on their
+// way (as far as the LDS holds: two of A, three of B), those of the tiles that follow too while a tile's results are written.
+//   run_a(id, part), run_b: the runs of a tile, `parts` of them;  add(a, b);  end(id)
+template <bool kDirect, typename StreamA, typename StreamB, typename StageA, typename StageB, typename S, typename RunA, typename RunB, typename AddFn, typename EndFn>
+__device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts, long long stride_a, long long stride_b, const RunA &run_a, const RunB &run_b,
+                                         const AddFn &add, const EndFn &end) {
+  constexpr int kA = S::kI * kLineBytes, kB = S::kJ * kLineBytes;
+  if constexpr (kDirect) {
+    const unsigned first = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)lds);
+    StreamA a;
+    StreamB b;
+    a.Start(run_a, tiles, parts, stride_a);
+    b.Start(run_b, tiles, parts, stride_b);
+    unsigned a0 = first, a1 = first + kA, b0 = first + 2 * kA, b1 = b0 + kB, b2 = b1 + kB;
+    a.Issue(a0, run_a, tiles, parts, stride_a);
+    b.Issue(b0, run_b, tiles, parts, stride_b);
+    b.Issue(b1, run_b, tiles, parts, stride_b);
+    bool pending = b.live;  // whether the last loads are of a block that is not asked for yet, and nothing was stored since
+    for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
+      for (int part = 0; part < parts; ++part) {
+        for (int n = run_b(id, part).blocks; n > 0; --n) {
+          if (pending) WaitAndMeet<StreamB::kPieces>();
+          else WaitAndMeet<0>();
+          // (the block is there, and what follows goes where the one before was, which has been read)
+          a.Prepare(a1, run_a, tiles, parts, stride_a);
+          b.Prepare(b2, run_b, tiles, parts, stride_b);
+          // Loads one by one between the products: all at once they fill the queue of the memory pipeline, which takes 16 cycles for each, and
+          // the waves wait to issue them while nothing is multiplied.
+          add((const LdsByte *)(uintptr_t)a0, (const LdsByte *)(uintptr_t)b0, [&](int step) {
+            constexpr int kLoads = StreamA::kPieces + StreamB::kPieces, kGap = Tile::kSteps / kLoads;
+            static_assert(kGap >= 1, "a load after every step at most");
+            if (step % kGap != 0) return;
+            const int p = step / kGap;
+            if (p < StreamA::kPieces) {
+              if (a.live) a.Piece(p);
+            } else if (p < kLoads) {
+              if (b.live) b.Piece(p - StreamA::kPieces);
+            }
+          });
+          a.Done();
+          b.Done();
+          pending = b.live;
+          const unsigned a_was = a0, b_was = b0;
+          a0 = a1;
+          a1 = a_was;
+          b0 = b1;
+          b1 = b2;
+          b2 = b_was;
+        }
+      }
+      end(id);
+      pending = false;
     }
-    for (long long n = 0; n < tile.blocks; ++n) {
-      if (kDirect) WaitForLoads();
-      __syncthreads();  // (block n is there, and the half that what follows goes to has been read)
-      if (n + 1 < tile.blocks) load(tile, n + 1, half ^ 1);
-      else if (kDirect && more && next.blocks > 0) load(next, 0, half ^ 1);
-      add(half);
-      if (!kDirect && n + 1 < tile.blocks) store(half ^ 1);
-      half ^= 1;
+  } else {
+    LdsByte *const to_b = lds + kA;
+    for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
+      for (int part = 0; part < parts; ++part) {
+        const Run of_a = run_a(id, part), of_b = run_b(id, part);
+        StageA a;
+        StageB b;
+        if (of_b.blocks > 0) a.Load(of_a, 0, stride_a), b.Load(of_b, 0, stride_b);
+        for (int n = 0; n < of_b.blocks; ++n) {
+          __syncthreads();  // (the block before has been read)
+          a.Store(lds);
+          b.Store(to_b);
+          __syncthreads();
+          if (n + 1 < of_b.blocks) a.Load(of_a, n + 1, stride_a), b.Load(of_b, n + 1, stride_b);
+          add(lds, to_b, [](int) {});
+        }
+      }
+      end(id);
     }
-    end(tile);
-    if (!more) return;
-    id = next_id;
-    tile = next;
   }
 }
 
 // Workgroups that follow each other are on different XCDs: each XCD (its L2) gets tiles that lie together, eight rows of them by
 // as many columns as there are.
-__device__ __forceinline__ long long PlaceOfTile(long long id, long long all) {
-  const long long x = id % 8, each = all / 8, rest = all % 8;
+__device__ __forceinline__ unsigned PlaceOfTile(unsigned id, unsigned all) {
+  const unsigned x = id % 8, each = all / 8, rest = all % 8;
   return x * each + min(x, rest) + id / 8;
 }
-__device__ __forceinline__ void PlaceInGroup(long long tile, long long tile_rows, int tile_columns, long long *i, int *j) {
-  const long long group = tile / (8ll * tile_columns), first = group * 8, rows = min(tile_rows - first, 8ll);
-  const long long in = tile - group * 8 * tile_columns;
+__device__ __forceinline__ void PlaceInGroup(unsigned tile, unsigned tile_rows, unsigned tile_columns, unsigned *i, unsigned *j) {
+  const unsigned group = tile / (8 * tile_columns), first = group * 8, rows = min(tile_rows - first, 8u);
+  const unsigned in = tile - group * 8 * tile_columns;
   *i = first + in % rows;
-  *j = (int)(in / rows);
+  *j = in / rows;
 }
 
 // Four elements of a row from column `at` on, of `columns`.
@@ -370,48 +464,44 @@ static_assert(kWaveJ == 2 * kScaleGroup, "a wave holds whole groups");
 
 // A tile's columns are the gate's and up's of the same hidden ones: 64 of the gate and 64 of up for each wave.
 template <typename T, int kAct, typename S, bool kDirect>
-__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_gated(const Forward a, long long tiles, long long tile_rows, int tile_columns) {
-  __shared__ __align__(16) unsigned char s_blocks[2 * S::kBlockBytes];
-  LdsByte *blocks = (LdsByte *)s_blocks;
+__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_gated(const Forward a, unsigned tiles, unsigned tile_rows, unsigned tile_columns) {
+  __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
   constexpr int kK = kLineBytes / sizeof(T), kHidden = S::kJ / 2;
-  const T *x = static_cast<const T *>(a.x), *w_gate = static_cast<const T *>(a.w_gate), *w_up = static_cast<const T *>(a.w_up);
-  const long long all_blocks = (a.dim + kK - 1) / kK, each = tile_rows * tile_columns;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
   struct At {
-    long long i0, split, first, blocks;
+    long long i0, split, first;
     int h0;
+  };
+  const auto at_of = [&](unsigned id) {
+    At at;
+    const unsigned each = tile_rows * tile_columns, place = PlaceOfTile(id, tiles), split = a.splits == 1 ? 0 : place / each;
+    unsigned i, j;
+    PlaceInGroup(place - split * each, tile_rows, tile_columns, &i, &j);
+    at.i0 = (long long)i * S::kI;
+    at.h0 = j * kHidden;
+    at.split = split;
+    at.first = split * a.split_blocks;
+    return at;
+  };
+  const auto blocks_of = [&](const At &at) { return (int)min(a.split_blocks, (a.dim + kK - 1) / kK - at.first); };
+  const auto run_x = [&](unsigned id, int) {
+    const At at = at_of(id);
+    const T *x = static_cast<const T *>(a.x) + at.i0 * a.x_stride + at.first * kK;
+    return Run{x, x, a.rows - at.i0, a.dim - at.first * kK, blocks_of(at)};
+  };
+  const auto run_w = [&](unsigned id, int) {
+    const At at = at_of(id);
+    const long long from = at.h0 * a.w_stride + at.first * kK;
+    return Run{static_cast<const T *>(a.w_gate) + from, static_cast<const T *>(a.w_up) + from, a.hidden - at.h0, a.dim - at.first * kK, blocks_of(at)};
   };
   Tile t;
   t.Clear();
-  Loader<T, S::kI, S::kThreads, false, kDirect> xs;
-  Loader<T, S::kJ, S::kThreads, false, kDirect> ws;
-  const auto tile_of = [&](long long id) {
-    At at;
-    const long long place = PlaceOfTile(id, tiles);
-    int column;
-    at.split = place / each;
-    PlaceInGroup(place - at.split * each, tile_rows, tile_columns, &at.i0, &column);
-    at.i0 *= S::kI;
-    at.h0 = column * kHidden;
-    at.first = at.split * a.split_blocks;
-    at.blocks = min(a.split_blocks, all_blocks - at.first);
-    return at;
+  const auto add = [&](const LdsByte *x, const LdsByte *w, const auto &between) {
+    t.Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(x, w, wave_i, wave_j, between);
   };
-  const auto load = [&](const At &at, long long n, int half) {
-    LdsByte *to = blocks + half * S::kBlockBytes;
-    const long long k0 = (at.first + n) * kK, w_at = at.h0 * a.w_stride + k0;
-    xs.Load(PlainRows<T>{x + at.i0 * a.x_stride + k0, a.x_stride, a.rows - at.i0}, 0, a.dim - k0, to);
-    ws.Load(PairedRows<T>{w_gate + w_at, w_up + w_at, a.w_stride, a.hidden - at.h0}, 0, a.dim - k0, to + S::kI * kLineBytes);
-  };
-  const auto store = [&](int half) {
-    xs.Store(blocks + half * S::kBlockBytes);
-    ws.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
-  };
-  const auto add = [&](int half) {
-    const LdsByte *from = blocks + half * S::kBlockBytes;
-    t.Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
-  };
-  RunTiles<kDirect>(tiles, tile_of, load, store, add, [&](const At &at) {
+  RunTiles<kDirect, Stream<T, S::kI, S::kThreads, false, false>, Stream<T, S::kJ, S::kThreads, false, true>, Stage<T, S::kI, S::kThreads, false, false>,
+           Stage<T, S::kJ, S::kThreads, false, true>, S>((LdsByte *)s_blocks, tiles, 1, a.x_stride, a.w_stride, run_x, run_w, add, [&](unsigned id) {
+    const At at = at_of(id);
     const int h = at.h0 + wave_j * (kWaveJ / 2);
 #pragma unroll
     for (int i = 0; i < kWaveI / 16; ++i) {
@@ -573,50 +663,50 @@ __global__ void __launch_bounds__(kThreads) k_pad(const Padded a, long long bloc
 }
 
 template <typename T, bool kAcrossA, bool kAcrossB, typename S, bool kDirect>
-__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_products(const Products p, long long tiles, long long tile_rows, int tile_columns) {
-  __shared__ __align__(16) unsigned char s_blocks[2 * S::kBlockBytes];
-  LdsByte *blocks = (LdsByte *)s_blocks;
+__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_products(const Products p, unsigned tiles, unsigned tile_rows, unsigned tile_columns) {
+  __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
   constexpr int kK = kLineBytes / sizeof(T);
-  const long long segment_blocks = (p.inner + kK - 1) / kK, each = tile_rows * tile_columns;
+  const long long segment_blocks = (p.inner + kK - 1) / kK;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
   struct At {
-    long long i0, one, first, blocks;
+    long long i0, one, first;
     int j0, member;
+  };
+  const auto at_of = [&](unsigned id) {
+    At at;
+    const unsigned each = tile_rows * tile_columns, place = PlaceOfTile(id, tiles), one = place / each, member = one / (unsigned)p.splits;
+    unsigned i, j;
+    PlaceInGroup(place - one * each, tile_rows, tile_columns, &i, &j);
+    at.i0 = (long long)i * S::kI;
+    at.j0 = j * S::kJ;
+    at.one = one;
+    at.member = member;
+    at.first = (one - member * p.splits) * p.split_blocks;
+    return at;
+  };
+  // A tile's blocks of k's in each segment.
+  const auto run_of = [&](const At &at, int segment, const Operand &of, bool across, long long row0, long long rows) {
+    const long long begin = max(at.first, segment * segment_blocks), end = min(at.first + p.split_blocks, (segment + 1) * segment_blocks);
+    const long long k0 = (begin - segment * segment_blocks) * kK;
+    const T *base = static_cast<const T *>(of.at[at.member + segment]) + (across ? k0 * of.stride + row0 : row0 * of.stride + k0);
+    return Run{base, base, rows - row0, p.inner - k0, (int)max(end - begin, 0ll)};
+  };
+  const auto run_a = [&](unsigned id, int segment) {
+    const At at = at_of(id);
+    return run_of(at, segment, p.a, kAcrossA, at.i0, p.rows);
+  };
+  const auto run_b = [&](unsigned id, int segment) {
+    const At at = at_of(id);
+    return run_of(at, segment, p.b, kAcrossB, at.j0, p.columns);
   };
   Tile t;
   t.Clear();
-  Loader<T, S::kI, S::kThreads, kAcrossA, kDirect> as;
-  Loader<T, S::kJ, S::kThreads, kAcrossB, kDirect> bs;
-  const auto tile_of = [&](long long id) {
-    At at;
-    const long long place = PlaceOfTile(id, tiles);
-    at.one = place / each;
-    at.member = (int)(at.one / p.splits);
-    PlaceInGroup(place - at.one * each, tile_rows, tile_columns, &at.i0, &at.j0);
-    at.i0 *= S::kI;
-    at.j0 *= S::kJ;
-    at.first = (at.one % p.splits) * p.split_blocks;
-    at.blocks = min(p.split_blocks, segment_blocks * p.segments - at.first);
-    return at;
+  const auto add = [&](const LdsByte *of_a, const LdsByte *of_b, const auto &between) {
+    t.Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(of_a, of_b, wave_i, wave_j, between);
   };
-  const auto load = [&](const At &at, long long n, int half) {
-    const int segment = at.first + n >= segment_blocks, which = at.member + segment;
-    const long long k0 = (at.first + n - segment * segment_blocks) * kK;
-    const T *a = static_cast<const T *>(p.a.at[which]), *b = static_cast<const T *>(p.b.at[which]);
-    LdsByte *to = blocks + half * S::kBlockBytes;
-    as.Load(PlainRows<T>{kAcrossA ? a + k0 * p.a.stride + at.i0 : a + at.i0 * p.a.stride + k0, p.a.stride, p.rows - at.i0}, p.rows - at.i0, p.inner - k0, to);
-    bs.Load(PlainRows<T>{kAcrossB ? b + k0 * p.b.stride + at.j0 : b + at.j0 * p.b.stride + k0, p.b.stride, p.columns - at.j0}, p.columns - at.j0, p.inner - k0,
-            to + S::kI * kLineBytes);
-  };
-  const auto store = [&](int half) {
-    as.Store(blocks + half * S::kBlockBytes);
-    bs.Store(blocks + half * S::kBlockBytes + S::kI * kLineBytes);
-  };
-  const auto add = [&](int half) {
-    const LdsByte *from = blocks + half * S::kBlockBytes;
-    t.Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(from, from + S::kI * kLineBytes, wave_i, wave_j);
-  };
-  RunTiles<kDirect>(tiles, tile_of, load, store, add, [&](const At &at) {
+  RunTiles<kDirect, Stream<T, S::kI, S::kThreads, kAcrossA, false>, Stream<T, S::kJ, S::kThreads, kAcrossB, false>, Stage<T, S::kI, S::kThreads, kAcrossA, false>,
+           Stage<T, S::kJ, S::kThreads, kAcrossB, false>, S>((LdsByte *)s_blocks, tiles, p.segments, p.a.stride, p.b.stride, run_a, run_b, add, [&](unsigned id) {
+    const At at = at_of(id);
 #pragma unroll
     for (int i = 0; i < kWaveI / 16; ++i) {
       const long long row = at.i0 + wave_i * kWaveI + i * 16 + lane % 16;
@@ -738,13 +828,18 @@ bool IsDirect(const void *p, long long stride, long long extent) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * item % 16 == 0 && extent * item % 16 == 0 && stride * item * 256 < (1ll << 31) - (1 << 20);
 }
 
+inline unsigned CheckedTiles(long long tiles) {
+  if (tiles >= (1ll << 30)) throw std::runtime_error("the layer is too large");
+  return (unsigned)tiles;
+}
+
 template <typename T, bool kAcrossA, bool kAcrossB>
 void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   const auto launch = [&](auto shape, auto is_direct) {
     typedef decltype(shape) S;
     const long long tile_rows = Pieces(p.rows, S::kI), tiles = tile_rows * Pieces(p.columns, S::kJ) * p.batch * p.splits;
-    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, p, tiles,
-                       tile_rows, (int)Pieces(p.columns, S::kJ));
+    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, p,
+                       CheckedTiles(tiles), (unsigned)tile_rows, (unsigned)Pieces(p.columns, S::kJ));
   };
   if (large && direct) launch(LargeTile(), std::true_type());
   else if (direct) launch(SmallTile(), std::true_type());
@@ -792,8 +887,8 @@ void RunGated(const GatedArgs &a, const GatedPlan &plan) {
     const auto launch = [&](auto shape, auto is_direct) {
       typedef decltype(shape) S;
       const long long tile_rows = Pieces(l.rows, S::kI), tile_columns = Pieces(l.hidden, S::kJ / 2), tiles = tile_rows * tile_columns * f.splits;
-      hipLaunchKernelGGL((k_gated<T, kAct, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, f, tiles,
-                         tile_rows, (int)tile_columns);
+      hipLaunchKernelGGL((k_gated<T, kAct, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, f,
+                         CheckedTiles(tiles), (unsigned)tile_rows, (unsigned)tile_columns);
     };
     if (plan.out.large && direct) launch(LargeTile(), std::true_type());
     else if (direct) launch(SmallTile(), std::true_type());

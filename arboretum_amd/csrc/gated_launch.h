@@ -13,8 +13,8 @@ constexpr int kWaveI = 64, kWaveJ = 128;  // a wave's part of a tile: 4 x 8 frag
 template <int kWavesI, int kWavesJ>
 struct TileShape {
   static constexpr int kThreads = 64 * kWavesI * kWavesJ, kI = kWaveI * kWavesI, kJ = kWaveJ * kWavesJ;
-  static constexpr int kBlockBytes = (kI + kJ) * kLineBytes;
-  static constexpr int kEach = kBlockBytes > 40 * 1024 ? 1 : 2;             // workgroups of a CU: its LDS holds two blocks of each
+  static constexpr int kLdsBytes = (2 * kI + 3 * kJ) * kLineBytes;  // two blocks of A, three of B
+  static constexpr int kEach = 160 * 1024 / kLdsBytes;              // workgroups of a CU
   static constexpr int kWavesEach = (kWavesI * kWavesJ * kEach + 3) / 4;  // waves of a SIMD
 };
 typedef TileShape<4, 2> LargeTile;
