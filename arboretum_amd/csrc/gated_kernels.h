@@ -6,6 +6,7 @@
 #define ARBORETUM_AMD_GATED_KERNELS_H_
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "checkpoint.h"
 #include "gated_launch.h"
@@ -94,12 +95,13 @@ typedef int I4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char LdsByte;
 typedef __attribute__((address_space(3))) I4 LdsI4;
 
-// 16 bytes a lane from `base` + `at` (beyond 2^31: 0) to the LDS, the wave's 1 KB side by side from `to` on.  By hand: the
+// 16 bytes a lane from `base` + `at` (beyond 2^31: 0) to the LDS, the wave's 1 KB side by side from `to` + kOffset on.  By hand: the
 // compiler waits for a load of its own before any read of the LDS, and this one is meant to be on its way meanwhile.  Whoever reads
 // what it writes waits for it first (WaitAndMeet, which nothing that touches memory moves across).
+template <int kOffset>
 __device__ __forceinline__ void LoadToLds(unsigned long long base, unsigned at, unsigned to) {
   const I4 from = {(int)(unsigned)base, (int)(unsigned)(base >> 32), 0x7FFFFFFF, 0x00020000};
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(to));
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(to), "n"(kOffset) : "scc");
 }
 
 // Until no more than kLast of the wave's loads are on their way (they arrive in the order they were issued in), what it has read of the LDS is there,
@@ -108,6 +110,9 @@ template <int kLast>
 __device__ __forceinline__ void WaitAndMeet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLast) : "memory");
 }
+
+__device__ __forceinline__ void WaitForLoads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void Meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The chunks of an operand's block in the LDS.  Along k: line by line, 8 chunks each; across: k by k, the chunks of all lines.
 // Chunks change places from line to line (from k to k), so that the lanes that read together meet other banks: they
@@ -195,11 +200,21 @@ struct Stream {
         id += gridDim.x;
       }
       live = id < tiles;
-      if (!live) return;
+      if (!live) {  // what is asked for from here on is from nowhere
+        base = second = 0;
+        left = 1 << 30;
+        blocks = 0;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) at[p] = kNowhere;
+        return;
+      }
       run = run_of(id, part);
     } while (run.blocks <= 0);
     base = Uniform(reinterpret_cast<unsigned long long>(run.base));
     second = Uniform(reinterpret_cast<unsigned long long>(run.second));
+    // (a load may read a scalar register that a vector instruction wrote, as Uniform does, five instructions later at the earliest; the compiler, which sees to
+    // that elsewhere, does not know what LoadToLds is)
+    asm volatile("s_nop 4" : "+s"(base), "+s"(second));
     left = (int)min(run.left, 1ll << 30);
     blocks = run.blocks;
 #pragma unroll
@@ -209,17 +224,22 @@ struct Stream {
       at[p] = held ? ((unsigned)RowOf<kPaired>(line) * (unsigned)stride + chunk * kVec) * (unsigned)sizeof(T) : kNowhere;
     }
   }
-  // The next block, if there is one, goes to `to`: its loads one by one (Piece), then Done.
+  // The next block goes to `to`: its loads one by one (Piece), then Done.  (Where no block is left they are from nowhere.)
   template <typename RunOf>
   __device__ __forceinline__ void Prepare(unsigned to, const RunOf &run_of, unsigned tiles, int parts, long long stride) {
     if (blocks == 0 && live) Next(run_of, tiles, parts, stride);
+    if (left < kK) {  // the operand's end, and that of the run
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const int q = p * kThreads + threadIdx.x, line = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(line);
+        if ((kAcross ? line : chunk * kVec) >= left) at[p] = kNowhere;
+      }
+    }
     lds = to + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
   }
-  __device__ __forceinline__ void Piece(int p) const {
-    // (k's beyond the operand's end: from nowhere)
-    const int q = p * kThreads + threadIdx.x, line = q / L::kRowChunks, chunk = q % L::kRowChunks ^ L::Swap(line);
-    const unsigned from = (kAcross ? line : chunk * kVec) < left ? at[p] : kNowhere;
-    LoadToLds(kPaired && (p * kThreads / 8 & 64) ? second : base, from, lds + p * kThreads * 16);
+  template <int p>
+  __device__ __forceinline__ void Piece() const {
+    LoadToLds<p * kThreads * 16>(kPaired && (p * kThreads / 8 & 64) ? second : base, at[p], lds);
   }
   __device__ __forceinline__ void Done() {
     if (!live) return;
@@ -228,13 +248,15 @@ struct Stream {
     left -= kK;
     --blocks;
   }
+  template <typename RunOf, int... p>
+  __device__ __forceinline__ void Issue(unsigned to, const RunOf &run_of, unsigned tiles, int parts, long long stride, std::integer_sequence<int, p...>) {
+    Prepare(to, run_of, tiles, parts, stride);
+    (Piece<p>(), ...);
+    Done();
+  }
   template <typename RunOf>
   __device__ __forceinline__ void Issue(unsigned to, const RunOf &run_of, unsigned tiles, int parts, long long stride) {
-    Prepare(to, run_of, tiles, parts, stride);
-    if (!live) return;
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p) Piece(p);
-    Done();
+    Issue(to, run_of, tiles, parts, stride, std::make_integer_sequence<int, kPieces>());
   }
 };
 
@@ -292,23 +314,23 @@ struct Tile {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) read_y(0, j);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int j = 0; j < kFragsJ; ++j) {
-        const int soon = j + kAhead - kFragsJ;  // of the next half
-        if (soon < 0) {
-          read_y(half, j + kAhead);
-        } else if (half == 0) {
-          read_y(1, soon);
-          if (soon < kFragsI) read_x(1, soon);
-        }
-#pragma unroll
-        for (int i = 0; i < kFragsI; ++i) acc[i][j] = Product(y[half][j], x[half][i], acc[i][j]);
-        between(half * kFragsJ + j);
-        __builtin_amdgcn_sched_barrier(0);
+    ForEach([&](auto step) {
+      constexpr int half = step.value / kFragsJ, j = step.value % kFragsJ, soon = j + kAhead - kFragsJ;  // soon: of the next half
+      if constexpr (soon < 0) {
+        read_y(half, j + kAhead);
+      } else if constexpr (half == 0) {
+        read_y(1, soon);
+        if constexpr (soon < kFragsI) read_x(1, soon);
       }
-    }
+#pragma unroll
+      for (int i = 0; i < kFragsI; ++i) acc[i][j] = Product(y[half][j], x[half][i], acc[i][j]);
+      between(step);
+      __builtin_amdgcn_sched_barrier(0);
+    }, std::make_integer_sequence<int, kSteps>());
+  }
+  template <typename Fn, int... step>
+  static __device__ __forceinline__ void ForEach(const Fn &fn, std::integer_sequence<int, step...>) {
+    (fn(std::integral_constant<int, step>()), ...);
   }
 };
 
@@ -329,31 +351,26 @@ __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts
     a.Issue(a0, run_a, tiles, parts, stride_a);
     b.Issue(b0, run_b, tiles, parts, stride_b);
     b.Issue(b1, run_b, tiles, parts, stride_b);
-    bool pending = b.live;  // whether the last loads are of a block that is not asked for yet, and nothing was stored since
+    bool landed = false;  // whether all loads have arrived (else those of A and B asked for last, as far as B goes ahead, have not)
     for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
       for (int part = 0; part < parts; ++part) {
         for (int n = run_b(id, part).blocks; n > 0; --n) {
-          if (pending) WaitAndMeet<StreamB::kPieces>();
-          else WaitAndMeet<0>();
+          if (landed) Meet();
+          else WaitAndMeet<StreamB::kPieces>();
           // (the block is there, and what follows goes where the one before was, which has been read)
+          landed = false;
           a.Prepare(a1, run_a, tiles, parts, stride_a);
           b.Prepare(b2, run_b, tiles, parts, stride_b);
           // Loads one by one between the products: all at once they fill the queue of the memory pipeline, which takes 16 cycles for each, and
           // the waves wait to issue them while nothing is multiplied.
-          add((const LdsByte *)(uintptr_t)a0, (const LdsByte *)(uintptr_t)b0, [&](int step) {
-            constexpr int kLoads = StreamA::kPieces + StreamB::kPieces, kGap = Tile::kSteps / kLoads;
+          add((const LdsByte *)(uintptr_t)a0, (const LdsByte *)(uintptr_t)b0, [&](auto step) {
+            constexpr int kLoads = StreamA::kPieces + StreamB::kPieces, kGap = Tile::kSteps / kLoads, p = step.value / kGap;
             static_assert(kGap >= 1, "a load after every step at most");
-            if (step % kGap != 0) return;
-            const int p = step / kGap;
-            if (p < StreamA::kPieces) {
-              if (a.live) a.Piece(p);
-            } else if (p < kLoads) {
-              if (b.live) b.Piece(p - StreamA::kPieces);
-            }
+            if constexpr (step.value % kGap == 0 && p < StreamA::kPieces) a.template Piece<p>();
+            else if constexpr (step.value % kGap == 0 && p < kLoads) b.template Piece<p - StreamA::kPieces>();
           });
           a.Done();
           b.Done();
-          pending = b.live;
           const unsigned a_was = a0, b_was = b0;
           a0 = a1;
           a1 = a_was;
@@ -362,8 +379,10 @@ __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts
           b2 = b_was;
         }
       }
+      // (before the tile's results are stored: a wait for loads issued before them would be one for the stores as well)
+      WaitForLoads();
+      landed = true;
       end(id);
-      pending = false;
     }
   } else {
     LdsByte *const to_b = lds + kA;
@@ -379,7 +398,7 @@ __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts
           b.Store(to_b);
           __syncthreads();
           if (n + 1 < of_b.blocks) a.Load(of_a, n + 1, stride_a), b.Load(of_b, n + 1, stride_b);
-          add(lds, to_b, [](int) {});
+          add(lds, to_b, [](auto) {});
         }
       }
       end(id);
