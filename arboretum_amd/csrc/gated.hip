@@ -7,11 +7,14 @@
 namespace arb {
 namespace {
 
-// Large tiles where they fill the chip; else small ones, and few tiles share out their k's, at least `least` blocks to a share.
-ProductCut CutOf(long long large_tiles, long long small_tiles, long long blocks, long long least) {
+// A product of `rows` x `columns` (`batch` of them) over `blocks` blocks of k's: large tiles where they fill the chip and are not mostly beyond its columns; else
+// small ones, and few tiles share out their k's, at least `least` blocks to a share.  half: a tile has half as many columns.
+ProductCut CutOf(long long rows, long long columns, int half, long long batch, long long blocks, long long least) {
+  const auto tiles = [&](long long i, long long j) { return Pieces(rows, i) * Pieces(columns, j / half) * batch; };
+  const long long large = tiles(LargeTile::kI, LargeTile::kJ), small = tiles(SmallTile::kI, SmallTile::kJ);
   ProductCut c;
-  c.large = large_tiles >= 200;
-  const long long most = std::max<long long>(1, std::min({c.large ? 256 / large_tiles : 512 / std::max<long long>(small_tiles, 1), blocks / least, 64ll}));
+  c.large = large >= 200 && columns > SmallTile::kJ / half;
+  const long long most = std::max<long long>(1, std::min({c.large ? 256 / large : 512 / std::max<long long>(small, 1), blocks / least, 64ll}));
   c.split_blocks = std::max<long long>(1, Pieces(blocks, most));
   c.splits = std::max<long long>(1, Pieces(blocks, c.split_blocks));
   return c;
@@ -51,8 +54,7 @@ GatedPlan PlanOf(long long rows, int dim, int hidden, int type) {
   GatedPlan p;
   Room room;
   p.few = rows <= 16;
-  p.out = CutOf(Pieces(rows, LargeTile::kI) * Pieces(hidden, LargeTile::kJ / 2), Pieces(rows, SmallTile::kI) * Pieces(hidden, SmallTile::kJ / 2),
-                Pieces(dim * item, kLineBytes), 4);
+  p.out = CutOf(rows, hidden, 2, 1, Pieces(dim * item, kLineBytes), 4);
   p.pad = PadOf(rows, dim, hidden, item, &room);
   p.partial = room.Take(p.out.splits > 1 ? (size_t)p.out.splits * rows * Pieces(hidden, kScaleGroup) * kWaveJ * sizeof(float) : 0);
   p.bytes = room.bytes;
@@ -64,10 +66,8 @@ GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
   GatedGradPlan p;
   Room room;
   p.d_stride = Pieces(hidden, 64) * 64;
-  p.x = CutOf(Pieces(rows, LargeTile::kI) * Pieces(dim, LargeTile::kJ), Pieces(rows, SmallTile::kI) * Pieces(dim, SmallTile::kJ),
-              2 * Pieces(hidden * item, kLineBytes), 8);
-  p.w = CutOf(2 * Pieces(hidden, LargeTile::kI) * Pieces(dim, LargeTile::kJ), 2 * Pieces(hidden, SmallTile::kI) * Pieces(dim, SmallTile::kJ),
-              Pieces(rows * item, kLineBytes), 8);
+  p.x = CutOf(rows, dim, 1, 1, 2 * Pieces(hidden * item, kLineBytes), 8);
+  p.w = CutOf(hidden, dim, 1, 2, Pieces(rows * item, kLineBytes), 8);
   p.d_gate = room.Take((size_t)rows * p.d_stride * item);
   p.d_up = room.Take((size_t)rows * p.d_stride * item);
   p.pad = PadOf(rows, dim, hidden, item, &room);

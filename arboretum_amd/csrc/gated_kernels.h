@@ -419,16 +419,58 @@ __device__ __forceinline__ void PlaceInGroup(unsigned tile, unsigned tile_rows, 
   *j = in / rows;
 }
 
-// Four elements of a row from column `at` on, of `columns`.
-template <typename T>
-__device__ __forceinline__ void StoreFour(T *row, long long at, long long columns, const T (&v)[4]) {
-  if (at + 4 <= columns) {
-    *reinterpret_cast<Pack<T, 4> *>(row + at) = Pack<T, 4>{{v[0], v[1], v[2], v[3]}};
+// N elements of a row from column `at` on, of `columns`.
+template <typename T, int N>
+__device__ __forceinline__ void StoreSome(T *row, long long at, long long columns, const Pack<T, N> &v) {
+  if (at + N <= columns) {
+    *reinterpret_cast<Pack<T, N> *>(row + at) = v;
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (at + r < columns) row[at + r] = v[r];
+    for (int r = 0; r < N; ++r)
+      if (at + r < columns) row[at + r] = v.v[r];
   }
+}
+
+// A lane's four values of each of four fragments that follow each other along a row: 64 columns from `at` on, between the four lanes of the row.  Elements of 16 and 8
+// bits: the four lanes first exchange what they have of two fragments, so that each has eight columns side by side, 64 (32) bytes of the row
+// between them in one store (100,003 x 64 x 256 kept as it is: 61 us with stores of four columns a lane).
+template <typename T>
+__device__ __forceinline__ void StoreColumns(T *row, long long at, long long columns, const Pack<T, 4> (&v)[4]) {
+  const int quarter = (threadIdx.x & 63) / 16;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) StoreSome(row, at + j * 16 + quarter * 4, columns, v[j]);
+  } else {
+    struct Words {
+      unsigned w[sizeof(T)];
+    };
+    struct Both {
+      Words low, high;
+    };
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      // lanes' quarters 0 1 2 3 of the fragments a and b:  a0 a1 a2 a3, b0 b1 b2 b3  ->  a0 a1 b0 b1, a2 a3 b2 b3  ->  a0 a2 b0 b2, a1 a3 b1 b3
+      Both p = {__builtin_bit_cast(Words, v[j]), __builtin_bit_cast(Words, v[j + 1])};
+#pragma unroll
+      for (int w = 0; w < (int)sizeof(T); ++w) {
+        const auto halves = __builtin_amdgcn_permlane32_swap(p.low.w[w], p.high.w[w], false, false);
+        const auto quarters = __builtin_amdgcn_permlane16_swap(halves[0], halves[1], false, false);
+        p.low.w[w] = quarters[0];
+        p.high.w[w] = quarters[1];
+      }
+      StoreSome(row, at + j * 16 + quarter * 8, columns, __builtin_bit_cast(Pack<T, 8>, p));
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void StoreRounded(T *row, long long at, long long columns, const F4 *v) {
+  Pack<T, 4> rounded[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) rounded[j].v[r] = Round<T>(v[j][r]);
+  StoreColumns(row, at, columns, rounded);
 }
 
 struct Forward {
@@ -451,14 +493,8 @@ struct Forward {
 // row the rest.
 template <typename T>
 __device__ __forceinline__ void Keep(void *kept, float *scales, long long stride, long long row, int at, int hidden, const F4 *v) {
-  const int quarter = (threadIdx.x & 63) / 16;
   if (scales == nullptr) {
-    T *to = static_cast<T *>(kept) + row * stride;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const T four[4] = {Round<T>(v[j][0]), Round<T>(v[j][1]), Round<T>(v[j][2]), Round<T>(v[j][3])};
-      StoreFour<T>(to, at + j * 16 + quarter * 4, hidden, four);
-    }
+    StoreRounded(static_cast<T *>(kept) + row * stride, at, hidden, v);
     return;
   }
   unsigned most = 0;  // (columns beyond the layer hold 0, or what the last one holds)
@@ -469,14 +505,14 @@ __device__ __forceinline__ void Keep(void *kept, float *scales, long long stride
   most = max(most, (unsigned)__shfl_xor((int)most, 16));
   most = max(most, (unsigned)__shfl_xor((int)most, 32));
   const float scale = ScaleOf(most);
-  if (quarter == 0) scales[row * ((hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup] = scale;
-  signed char *to = static_cast<signed char *>(kept) + row * stride;
+  if ((threadIdx.x & 63) < 16) scales[row * ((hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup] = scale;
+  Pack<signed char, 4> codes[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float four[4] = {v[j][0], v[j][1], v[j][2], v[j][3]};
-    const Pack<signed char, 4> codes = CodesOf(four, scale);
-    StoreFour<signed char>(to, at + j * 16 + quarter * 4, hidden, codes.v);
+    codes[j] = CodesOf(four, scale);
   }
+  StoreColumns(static_cast<signed char *>(kept) + row * stride, at, hidden, codes);
 }
 
 static_assert(kWaveJ == 2 * kScaleGroup, "a wave holds whole groups");
@@ -532,14 +568,12 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
         for (int j = 0; j < kWaveJ / 16; ++j) *reinterpret_cast<F4 *>(to + j * 16) = t.acc[i][j];
         continue;
       }
-      T *out = static_cast<T *>(a.out) + row * a.out_stride;
+      F4 out[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        T four[4];
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) four[r] = Round<T>(Act<kAct>(t.acc[i][j][r]) * t.acc[i][j + 4][r]);
-        StoreFour<T>(out, h + j * 16 + lane / 16 * 4, a.hidden, four);
-      }
+        for (int r = 0; r < 4; ++r) out[j][r] = Act<kAct>(t.acc[i][j][r]) * t.acc[i][j + 4][r];
+      StoreRounded(static_cast<T *>(a.out) + row * a.out_stride, h, a.hidden, out);
       if (a.gate != nullptr) {
         Keep<T>(a.gate, a.gate_scales, a.kept_stride, row, h, a.hidden, t.acc[i]);
         Keep<T>(a.up, a.up_scales, a.kept_stride, row, h, a.hidden, t.acc[i] + 4);
@@ -731,30 +765,41 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
       const long long row = at.i0 + wave_i * kWaveI + i * 16 + lane % 16;
       if (row >= p.rows) continue;
 #pragma unroll
-      for (int j = 0; j < kWaveJ / 16; ++j) {
-        const int column = at.j0 + wave_j * kWaveJ + j * 16 + lane / 16 * 4;
-        if (p.splits > 1) {
-          const float four[4] = {t.acc[i][j][0], t.acc[i][j][1], t.acc[i][j][2], t.acc[i][j][3]};
-          StoreFour<float>(p.partial + (at.one * p.rows + row) * p.columns, column, p.columns, four);
-        } else {
-          const T four[4] = {Round<T>(t.acc[i][j][0]), Round<T>(t.acc[i][j][1]), Round<T>(t.acc[i][j][2]), Round<T>(t.acc[i][j][3])};
-          StoreFour<T>(static_cast<T *>(p.c[at.member]) + row * p.c_stride, column, p.columns, four);
-        }
+      for (int j = 0; j < kWaveJ / 16; j += 4) {
+        const int column = at.j0 + wave_j * kWaveJ + j * 16;
+        if (p.splits > 1) StoreRounded(p.partial + (at.one * p.rows + row) * p.columns, column, p.columns, &t.acc[i][j]);
+        else StoreRounded(static_cast<T *>(p.c[at.member]) + row * p.c_stride, column, p.columns, &t.acc[i][j]);
       }
     }
     t.Clear();
   });
 }
 
-// The sums of what was shared out, in order.
-template <typename T>
+// The sums of what was shared out, in an order that depends on the sizes alone: kShares threads an element, each with every kShares-th of the
+// shares.  (Many shares mean few elements: 63 of 2 x 256 x 64 by a thread each take 17.7 us, 8 threads each 6.)
+template <typename T, int kShares>
 __global__ void __launch_bounds__(kThreads) k_products_join(const Products p) {
+  constexpr int kElements = kThreads / kShares;
+  __shared__ float s_sums[kShares][kElements];
   const long long each = p.rows * p.columns, all = each * p.batch;
-  for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < all; e += (long long)gridDim.x * kThreads) {
-    const long long member = e / each, at = e - member * each, row = at / p.columns;
+  const int in = threadIdx.x % kElements, share = threadIdx.x / kElements;
+  for (long long first = (long long)blockIdx.x * kElements; first < all; first += (long long)gridDim.x * kElements) {
+    const long long e = first + in;
+    const bool there = e < all;
+    const long long member = e >= each, at = e - member * each;
     const float *from = p.partial + member * p.splits * each + at;
-    float sum = from[0];
-    for (int s = 1; s < p.splits; ++s) sum += from[s * each];
+    float sum = 0.0f;
+    for (int s = share; s < p.splits; s += kShares) sum += there ? from[s * each] : 0.0f;
+    if constexpr (kShares > 1) {
+      s_sums[share][in] = sum;
+      __syncthreads();
+      sum = s_sums[0][in];
+#pragma unroll
+      for (int s = 1; s < kShares; ++s) sum += s_sums[s][in];
+      __syncthreads();
+    }
+    if (!there || share != 0) continue;
+    const long long row = at / p.columns;
     static_cast<T *>(p.c[member])[row * p.c_stride + (at - row * p.columns)] = Round<T>(sum);
   }
 }
@@ -863,10 +908,10 @@ void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   if (large && direct) launch(LargeTile(), std::true_type());
   else if (direct) launch(SmallTile(), std::true_type());
   else launch(SmallTile(), std::false_type());
-  if (p.splits > 1) {
-    const long long blocks = Pieces(p.rows * p.columns * p.batch, kThreads);
-    hipLaunchKernelGGL((k_products_join<T>), dim3((unsigned)std::min(blocks, kMostGrid)), dim3(kThreads), 0, stream, p);
-  }
+  if (p.splits <= 1) return;
+  const long long elements = p.rows * p.columns * p.batch;
+  if (p.splits >= 16) hipLaunchKernelGGL((k_products_join<T, 8>), dim3((unsigned)std::min(Pieces(elements, kThreads / 8), kMostGrid)), dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((k_products_join<T, 1>), dim3((unsigned)std::min(Pieces(elements, kThreads), kMostGrid)), dim3(kThreads), 0, stream, p);
 }
 
 // x and the two weights in rows that begin at multiples of 64 elements, where the plan has room for that and any of them needs it.
