@@ -84,6 +84,7 @@ def _load_lib():
         "AEmbeddingGrad": [c_void_p] * 4 + [c_long, c_int, c_long, c_int, c_long, c_long, c_int, c_int, c_float, c_int,
                                             c_void_p, ctypes.c_ulonglong, c_void_p],
         "AGardenLeafTokens": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p, c_int],
+        "AGardenLogProbs": [c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 4,
         "AGardenRefineLeaves": [c_void_p, c_void_p, c_int] + [ctypes.c_double] * 5,
         "AAdamW": [c_int] + [c_void_p] * 5 + [c_int, c_int] + [ctypes.c_double] * 6 + [c_long] + [c_void_p] * 3,
         "ALogProbsBytes": [c_long, c_long, c_int, P(ctypes.c_ulonglong)],
@@ -576,6 +577,26 @@ class Garden(object):
         leaves = np.zeros(int(self.config.get('tree', {}).get('labels_count', 1)), dtype=np.int64)
         _check(_LIB.AGardenLeafTokens(self.handle, data.handle, tokens, stride, n_rounds, leaves.ctypes.data, leaves.size))
         return leaves.tolist()
+
+    def log_probs(self, data, top=0, of_labels=True, n_rounds=-1):
+        """Under a booster of several classes (AGardenLogProbs): {"log_probs": of each row's label (not with
+        of_labels=False, for matrices without labels), "entropy": over the classes, "top", "top_log_probs": the `top` likeliest
+        classes of each row in order [rows][top] (with top > 0)}."""
+        self._ensure()
+        _refuse_wide((int(top), int(n_rounds)), ())
+        if top > self.config.get('tree', {}).get('labels_count', 1):
+            raise ArboretumError(ValueError("top must be 0 to the number of classes"))
+        rows = int(data.rows)
+        out = {"entropy": np.empty(rows, dtype=np.float32)}
+        if of_labels:
+            out["log_probs"] = np.empty(rows, dtype=np.float32)
+        if top > 0:
+            out["top"] = np.empty((rows, top), dtype=np.int32)
+            out["top_log_probs"] = np.empty((rows, top), dtype=np.float32)
+        at = {name: v.ctypes.data for name, v in out.items()}
+        _check(_LIB.AGardenLogProbs(self.handle, data.handle, int(n_rounds), int(top), at.get("log_probs"), at["entropy"], at.get("top"),
+                                    at.get("top_log_probs")))
+        return out
 
     def refine_leaves(self, data=None, steps=100, lr=0.01, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0):
         """Trains the leaf weights of all trees together, the splits as they are, by AdamW on the objective's mean over

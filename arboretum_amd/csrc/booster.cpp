@@ -276,6 +276,39 @@ void Garden::LeafTokens(const DataMatrix *data, int *tokens, size_t token_ld, in
   LeavesOnDevice(predictor_.get(), *data, trees_, use, K, tokens, token_ld);
 }
 
+// Loaded trees all have the label 0, as in the reference: what class they were of is not known.  (Every round grows
+// a tree of each class, so a booster of several classes has as many of each if and only if it grew them all.)
+std::vector<size_t> Garden::TreesOfClasses(const char *what) const {
+  const size_t K = cfg.tree.labels_count;
+  std::vector<size_t> trees_of(K, 0);
+  for (const RegTree &t : trees_)
+    if (t.label < K) ++trees_of[t.label];
+  for (size_t count : trees_of)
+    if (count != trees_of[0]) throw std::runtime_error(std::string(what) + " needs as many trees of each class: the trees of a loaded model have none");
+  return trees_of;
+}
+
+void Garden::LogProbs(DataMatrix *data, int n_trees, const ClassLogProbs &out) const {
+  const size_t K = cfg.tree.labels_count;
+  if (cfg.objective < kSoftMaxOneVsAll || K < 2) throw std::runtime_error("log probabilities need a soft-max objective of two classes or more");
+  if (out.top < 0 || (size_t)out.top > K) throw std::runtime_error("top must be 0 to the number of classes");
+  if (out.top > 0 && (!out.top_classes || !out.top_log_probs)) throw std::runtime_error("null pointer argument");
+  if (out.log_probs) CheckTarget(data);
+  SyncTrees();
+  TreesOfClasses("a log probability");
+  const size_t use = CheckLeafWalk(data, n_trees);
+  struct Sums {
+    float *p;
+    ~Sums() { DevicePoolGive(p); }  // (nothing is pending: both calls below wait)
+  } sums{static_cast<float *>(DevicePoolTake(K * data->rows * sizeof(float)))};
+  {
+    std::lock_guard<std::mutex> lock(predictor_mutex_);
+    if (!predictor_) predictor_.reset(CreateDevicePredictor());
+    SumsOnDevice(predictor_.get(), *data, trees_, use, K, IntoInternal(cfg.tree.initial_y), sums.p);
+  }
+  ClassLogProbsOnDevice(data, sums.p, K, out);
+}
+
 void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
   if (options.steps < 0) throw std::runtime_error("bad number of steps");
   if (cfg.objective < kSoftMaxOneVsAll && cfg.tree.labels_count > 1) throw std::runtime_error("several classes need a soft-max objective");
@@ -285,13 +318,7 @@ void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
   if (cfg.objective >= kSoftMaxOneVsAll && K < 2) throw std::runtime_error("soft-max needs labels_count >= 2");
   if (!(cfg.tree.max_leaf_weight >= 0.0f)) throw std::runtime_error("max_leaf_weight must not be negative");
   SyncTrees();
-  // Loaded trees all have the label 0, as in the reference: what class they were of is not known.  (Every round grows
-  // a tree of each class, so a booster of several classes has as many of each if and only if it grew them all.)
-  std::vector<size_t> trees_of(K, 0);
-  for (const RegTree &t : trees_)
-    if (t.label < K) ++trees_of[t.label];
-  for (size_t count : trees_of)
-    if (count != trees_of[0]) throw std::runtime_error("refinement needs as many trees of each class: the trees of a loaded model have none");
+  const std::vector<size_t> trees_of = TreesOfClasses("refinement");
   const size_t use = CheckLeafWalk(data, -1);
   std::vector<std::vector<float>> tables(K);
   for (size_t k = 0; k < K; ++k)

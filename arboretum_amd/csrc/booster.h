@@ -195,6 +195,9 @@ const float *PredictOnDevice(DevicePredictor *p, const DataMatrix &data, const s
 // of labels (stable), leaves numbered through the trees of a label.  Waits for the result.
 void LeavesOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees, size_t end, size_t labels,
                     int *tokens, size_t token_ld);
+// PredictOnDevice's sums left on the device: sums[label * rows + row].  Waits for the result.
+void SumsOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees, size_t end, size_t labels, float init,
+                  float *sums);
 // False for what only the host walks: 2 GB of trees and more, and rows on the host of which not even one fits a
 // staging block (a million features).
 bool DeviceWalkFits(const DataMatrix &data, const std::vector<RegTree> &trees, size_t begin, size_t end);
@@ -210,6 +213,17 @@ struct RefineOptions {
 // has trees.
 void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *tokens, size_t token_ld,
                     const std::vector<size_t> &trees_of, std::vector<std::vector<float>> *tables, float init, const RefineOptions &options);
+
+// What Garden::LogProbs gives, host arrays of a row each (of `top` a row); any may be null.
+struct ClassLogProbs {
+  int top;
+  float *log_probs, *entropy;
+  int *top_classes;
+  float *top_log_probs;
+};
+
+// class_log_probs.hip: the same of sums[label * rows + row] in device memory, the label of `data` being a row's token.
+void ClassLogProbsOnDevice(DataMatrix *data, const float *sums, size_t classes, const ClassLogProbs &out);
 
 class Garden {
  public:
@@ -227,6 +241,8 @@ class Garden {
   void LeafTokens(const DataMatrix *data, int *tokens, size_t token_ld, int n_trees, long long *leaves_of) const;
   // Trains the leaf weights of all trees together, the splits as they are.  The booster grows no tree afterwards.
   void RefineLeaves(DataMatrix *data, const RefineOptions &options);
+  // The log probability of each row's label under the soft-max of its classes' sums, their entropy and the likeliest classes.
+  void LogProbs(DataMatrix *data, int n_trees, const ClassLogProbs &out) const;
   const char *GetModel();                                    // :659-665
   void Restore(const char *json_model);                      // :667-677
 
@@ -265,6 +281,8 @@ class Garden {
   bool refined_ = false;
   // What LeafTokens and RefineLeaves ask of a matrix; the number of trees of the first n_trees (negative: all).
   size_t CheckLeafWalk(const DataMatrix *data, int n_trees) const;
+  // How many trees each class has; an error (`what` needs them) unless all have as many.
+  std::vector<size_t> TreesOfClasses(const char *what) const;
   void CheckTarget(const DataMatrix *data) const;
   bool WalksOnDevice(const DataMatrix *data) const;
   mutable std::mutex predictor_mutex_;  // the predictors' results are read under it

@@ -464,9 +464,10 @@ struct DevicePredictor {
 #undef ARB_WALK
   }
 
-  // The sums; with `tokens` (device memory, [trees][token_ld]) the leaves instead, and no sums.
+  // The sums, in pinned memory, or with `sums` (device memory, [labels][n]) there; with `tokens` (device memory, [trees][token_ld]) the
+  // leaves instead, and no sums.
   const float *Run(const DataMatrix &data, const std::vector<RegTree> &trees, size_t first, size_t use, size_t labels,
-                   float init, size_t row_begin, size_t row_end, int *tokens = nullptr, size_t token_ld = 0) {
+                   float init, size_t row_begin, size_t row_end, int *tokens = nullptr, size_t token_ld = 0, float *sums = nullptr) {
     const size_t n = std::min(row_end, data.rows) - row_begin, F = data.columns_dense;
     if (n == 0 || F == 0) throw std::runtime_error("empty data matrix");
     // only the block-wise walk of a streamed matrix indexes rows with 64 bits
@@ -477,14 +478,14 @@ struct DevicePredictor {
     LayOut(trees, first, use, F, labels);
     // Kernels write the sums where the host reads them: stores of 256 bytes a wave, at the rate of a copy
     // and beside the walk.
-    if (!tokens && labels * n > result_floats) {
+    if (!tokens && !sums && labels * n > result_floats) {
       PinnedPoolGive(result);
       result = nullptr;
       result_floats = 0;
       result = static_cast<float *>(PinnedPoolTake(labels * n * sizeof(float)));
       result_floats = labels * n;
     }
-    float *const out = tokens ? reinterpret_cast<float *>(tokens) : result;
+    float *const out = tokens ? reinterpret_cast<float *>(tokens) : sums ? sums : result;
     const size_t out_ld = tokens ? token_ld : n;
     // rows on the host: piece by piece through pinned memory into one device block (the stream keeps
     // a piece's copy behind the walk of the one before)
@@ -552,6 +553,11 @@ const float *PredictOnDevice(DevicePredictor *p, const DataMatrix &data, const s
 void LeavesOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees, size_t end, size_t labels,
                     int *tokens, size_t token_ld) {
   p->Run(data, trees, 0, end, labels, 0.0f, 0, SIZE_MAX, tokens, token_ld);
+}
+
+void SumsOnDevice(DevicePredictor *p, const DataMatrix &data, const std::vector<RegTree> &trees, size_t end, size_t labels, float init,
+                  float *sums) {
+  p->Run(data, trees, 0, end, labels, init, 0, SIZE_MAX, nullptr, 0, sums);
 }
 
 bool DeviceWalkFits(const DataMatrix &data, const std::vector<RegTree> &trees, size_t begin, size_t end) {

@@ -9,6 +9,7 @@
 
 #include "booster.h"
 #include "device_common.h"
+#include "device_work.h"
 #include "gain.h"
 #include "memory_pool.h"
 #include "operators.h"
@@ -48,29 +49,12 @@ __global__ void k_limit(float *__restrict__ weight, float most, size_t n) {
     weight[i] = weight[i] > most ? most : weight[i] < -most ? -most : weight[i];  // (a NaN stays one)
 }
 
-// Device memory and the stream of one call, given back when nothing is pending.
-struct Work {
-  hipStream_t stream = StreamPoolTake();
-  std::vector<void *> blocks;
-  template <typename T>
-  T *Take(size_t count) {
-    void *p = DevicePoolTake(std::max<size_t>(count, 1) * sizeof(T));
-    blocks.push_back(p);
-    return static_cast<T *>(p);
-  }
-  ~Work() {
-    (void)hipStreamSynchronize(stream);
-    for (void *p : blocks) DevicePoolGive(p);
-    StreamPoolGive(stream);
-  }
-};
-
 }  // namespace
 
 void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *tokens, size_t token_ld,
                     const std::vector<size_t> &trees_of, std::vector<std::vector<float>> *tables, float init, const RefineOptions &options) {
   const size_t n = data->rows, K = trees_of.size();
-  Work work;
+  DeviceWork work;
   struct Table {
     float *weight, *grad, *m, *v;
     unsigned *keys, *rows;

@@ -441,6 +441,13 @@ const char *AGardenRefineLeaves(VoidPointer garden, VoidPointer data, int steps,
   });
 }
 
+const char *AGardenLogProbs(VoidPointer garden, VoidPointer data, int n_rounds, int top, float *log_probs, float *entropy,
+                            int *top_classes, float *top_log_probs) {
+  return Guard([&] {
+    AsGarden(garden)->garden.LogProbs(AsData(data), n_rounds, ClassLogProbs{top, log_probs, entropy, top_classes, top_log_probs});
+  });
+}
+
 const char *AEmbedding(void *out, const void *table, const void *tokens, long long n, int bag, long long vocab, int dim,
                        long long out_stride, long long table_stride, long long token_stride, long long bag_stride,
                        int type, int token_bits, float scale, unsigned *status, void *stream) {

@@ -343,6 +343,14 @@ const char *AGatedGrad(void *grad_x, void *grad_w_gate, void *grad_w_up, const v
 const char *AGardenLeafTokens(VoidPointer garden, VoidPointer data, int *tokens, long long stride, int n_rounds,
                               long long *leaves, int classes);
 
+/* Log probabilities under a booster of several classes (soft-max objective), by ALogProbs on the device: HOST arrays of
+ * data's rows, log_probs of each row's label (NULL: none, the matrix then needs no labels), entropy over the classes (may be NULL), and
+ * the `top` (0 to the number of classes, at most 64) likeliest classes in order with their log probabilities [rows][top].  n_rounds: how many
+ * trees are summed, the first ones (-1: all).  A booster that was loaded does not know which class a tree is of, and is
+ * refused. */
+const char *AGardenLogProbs(VoidPointer garden, VoidPointer data, int n_rounds, int top, float *log_probs, float *entropy,
+                            int *top_classes, float *top_log_probs);
+
 /* Trains the leaf weights of all trees of the booster together, the splits as they are, against its objective on
  * `data` (any matrix with a target): `steps` AdamW steps on the mean over all rows of half the squared error, or
  * of the cross-entropy.  lambda and alpha, which a grown leaf's weight answers to, have no part in it (weight_decay
