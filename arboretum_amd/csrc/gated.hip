@@ -30,11 +30,13 @@ struct Room {
   }
 };
 
-// Rows whose chunks are not aligned come through registers into small tiles, at less than half the rate; copies of x and both
-// weights are read and written once.  What the copies cost grows with the weights, what they spare with the rows as well: from about 500 rows on.
-LayerPad PadOf(long long rows, int dim, int hidden, size_t item, Room *room) {
+// Rows whose chunks are not aligned come through registers into small tiles, which takes four times as long; copies of x and both
+// weights are read and written once.  For the gradient (300 x 4095 x 4097: 153 us for grad_x without, 63 with copies) that is always less, for
+// the layer itself, which reads its weights along k, from about 256 rows on (40 rows of 4095 x 16383: 103 us without, 175 with; 300 of
+// 4095 x 4097: 79 and 68).
+LayerPad PadOf(long long rows, int dim, int hidden, size_t item, long long least_rows, Room *room) {
   LayerPad p{0, 0, 0, 0};
-  if (dim * item % 16 == 0 || rows < 512) return p;
+  if (dim * item % 16 == 0 || rows < least_rows) return p;
   p.stride = Pieces(dim, 64) * 64;
   p.x = room->Take((size_t)rows * p.stride * item);
   p.w_gate = room->Take((size_t)hidden * p.stride * item);
@@ -55,7 +57,7 @@ GatedPlan PlanOf(long long rows, int dim, int hidden, int type) {
   Room room;
   p.few = rows <= 16;
   p.out = CutOf(rows, hidden, 2, 1, Pieces(dim * item, kLineBytes), 4);
-  p.pad = PadOf(rows, dim, hidden, item, &room);
+  p.pad = PadOf(rows, dim, hidden, item, 256, &room);
   p.partial = room.Take(p.out.splits > 1 ? (size_t)p.out.splits * rows * Pieces(hidden, kScaleGroup) * kWaveJ * sizeof(float) : 0);
   p.bytes = room.bytes;
   return p;
@@ -70,7 +72,7 @@ GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
   p.w = CutOf(hidden, dim, 1, 2, Pieces(rows * item, kLineBytes), 8);
   p.d_gate = room.Take((size_t)rows * p.d_stride * item);
   p.d_up = room.Take((size_t)rows * p.d_stride * item);
-  p.pad = PadOf(rows, dim, hidden, item, &room);
+  p.pad = PadOf(rows, dim, hidden, item, 1, &room);
   p.partial = room.Take(std::max<size_t>(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * sizeof(float) : 0,
                                          p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * sizeof(float) : 0));
   p.bytes = room.bytes;

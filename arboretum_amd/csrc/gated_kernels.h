@@ -775,32 +775,56 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
   });
 }
 
-// The sums of what was shared out, in an order that depends on the sizes alone: kShares threads an element, each with every kShares-th of the
-// shares.  (Many shares mean few elements: 63 of 2 x 256 x 64 by a thread each take 17.7 us, 8 threads each 6.)
+// The sums of what was shared out, in an order that depends on the sizes alone: four elements side by side a thread, or many shares by kShares threads,
+// each with every kShares-th of them.  (Many shares mean few elements: 63 of 2 x 256 x 64 by a thread each take 17.7 us, by eight 5.)
 template <typename T, int kShares>
 __global__ void __launch_bounds__(kThreads) k_products_join(const Products p) {
-  constexpr int kElements = kThreads / kShares;
-  __shared__ float s_sums[kShares][kElements];
-  const long long each = p.rows * p.columns, all = each * p.batch;
-  const int in = threadIdx.x % kElements, share = threadIdx.x / kElements;
-  for (long long first = (long long)blockIdx.x * kElements; first < all; first += (long long)gridDim.x * kElements) {
-    const long long e = first + in;
-    const bool there = e < all;
-    const long long member = e >= each, at = e - member * each;
-    const float *from = p.partial + member * p.splits * each + at;
-    float sum = 0.0f;
-    for (int s = share; s < p.splits; s += kShares) sum += there ? from[s * each] : 0.0f;
-    if constexpr (kShares > 1) {
-      s_sums[share][in] = sum;
-      __syncthreads();
-      sum = s_sums[0][in];
+  constexpr int kVec = kShares == 1 ? 4 : 1, kElements = kThreads / kShares * kVec;
+  __shared__ float s_sums[kShares][kShares == 1 ? 1 : kElements];
+  const long long each = p.rows * p.columns, step = (long long)gridDim.x * kElements;
+  const int in = threadIdx.x % (kThreads / kShares) * kVec, share = threadIdx.x / (kThreads / kShares);
+  for (int member = 0; member < p.batch; ++member) {
+    T *c = static_cast<T *>(p.c[member]);
+    for (long long first = (long long)blockIdx.x * kElements; first < each; first += step) {
+      const long long at = first + in;
+      const float *from = p.partial + (long long)member * p.splits * each + at;
+      const int held = (int)max(0ll, min(each - at, (long long)kVec));
+      float sum[kVec] = {};
+      for (int s = share; s < p.splits; s += kShares) {
+        if (held == kVec) {
+          const Pack<float, kVec> v = *reinterpret_cast<const Pack<float, kVec> *>(from + s * each);
 #pragma unroll
-      for (int s = 1; s < kShares; ++s) sum += s_sums[s][in];
-      __syncthreads();
+          for (int e = 0; e < kVec; ++e) sum[e] += v.v[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) sum[e] += e < held ? from[s * each + e] : 0.0f;
+        }
+      }
+      if constexpr (kShares > 1) {
+        s_sums[share][in] = sum[0];
+        __syncthreads();
+        sum[0] = s_sums[0][in];
+#pragma unroll
+        for (int s = 1; s < kShares; ++s) sum[0] += s_sums[s][in];
+        __syncthreads();
+      }
+      if (held == 0 || share != 0) continue;
+      const long long row = each < (1ll << 32) ? (long long)((unsigned)at / (unsigned)p.columns) : at / p.columns;
+      const int column = (int)(at - row * p.columns);
+      if (column + kVec <= p.columns) {
+        Pack<T, kVec> rounded;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) rounded.v[e] = Round<T>(sum[e]);
+        *reinterpret_cast<Pack<T, kVec> *>(c + row * p.c_stride + column) = rounded;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          if (e >= held) break;
+          const int over = (column + e) / p.columns;  // rows further on
+          c[(row + over) * p.c_stride + column + e - over * p.columns] = Round<T>(sum[e]);
+        }
+      }
     }
-    if (!there || share != 0) continue;
-    const long long row = at / p.columns;
-    static_cast<T *>(p.c[member])[row * p.c_stride + (at - row * p.columns)] = Round<T>(sum);
   }
 }
 
@@ -909,9 +933,9 @@ void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   else if (direct) launch(SmallTile(), std::true_type());
   else launch(SmallTile(), std::false_type());
   if (p.splits <= 1) return;
-  const long long elements = p.rows * p.columns * p.batch;
+  const long long elements = p.rows * p.columns;
   if (p.splits >= 16) hipLaunchKernelGGL((k_products_join<T, 8>), dim3((unsigned)std::min(Pieces(elements, kThreads / 8), kMostGrid)), dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((k_products_join<T, 1>), dim3((unsigned)std::min(Pieces(elements, kThreads), kMostGrid)), dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((k_products_join<T, 1>), dim3((unsigned)std::min(Pieces(elements, kThreads * 4), kMostGrid)), dim3(kThreads), 0, stream, p);
 }
 
 // x and the two weights in rows that begin at multiples of 64 elements, where the plan has room for that and any of them needs it.

@@ -196,6 +196,17 @@ def test_layer_and_gradient(arb, rows, dim, hidden, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kept", ["as is", "no"])
+@pytest.mark.parametrize("rows,dim,hidden,pad,first", [(1, 4095, 33, 0, 0), (16, 1027, 40, 0, 0), (7, 1024, 50, 1, 0), (9, 2048, 31, 0, 1), (16, 513, 17, 2, 1), (3, 130, 16, 0, 0),
+                                                        (5, 4097, 70, 3, 3), (17, 1027, 40, 0, 0)])
+def test_few_rows_that_begin_anywhere(arb, rows, dim, hidden, pad, first, kept, dtype):
+    layer = Layer(arb, rows, dim, hidden, dtype, kept=kept, pad=pad, first=first).forward().check_forward()
+    if kept != "no":
+        layer.backward().check_backward()
+    layer.check_margins()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
 @pytest.mark.parametrize("rows,dim,hidden", [(1, 40, 200), (3, 8, 7), (70, 64, 64), (130, 96, 129), (257, 30, 320), (5, 512, 1024)])
 def test_kept_in_8_bits(arb, rows, dim, hidden, activation, dtype):
