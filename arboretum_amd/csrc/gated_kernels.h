@@ -292,22 +292,23 @@ struct Stage {
 };
 
 // What a wave sums: fragments of 16 rows by 16 columns; a lane holds row lane % 16, columns 4 (lane / 16) + 0 .. 3 of each.
+template <int kFragsI>
 struct Tile {
-  F4 acc[kWaveI / 16][kWaveJ / 16];
+  static constexpr int kFragsJ = kWaveJ / 16;
+  F4 acc[kFragsI][kFragsJ];
   __device__ __forceinline__ void Clear() {
 #pragma unroll
-    for (int i = 0; i < kWaveI / 16; ++i)
+    for (int i = 0; i < kFragsI; ++i)
 #pragma unroll
-      for (int j = 0; j < kWaveJ / 16; ++j) acc[i][j] = F4{0, 0, 0, 0};
+      for (int j = 0; j < kFragsJ; ++j) acc[i][j] = F4{0, 0, 0, 0};
   }
-  // Both halves of a block, in 16 steps of four products; between(step) after each.  What is read for a product is asked for kAhead steps ahead, and
+  // Both halves of a block, in 16 steps of kFragsI products; between(step) after each.  What is read for a product is asked for kAhead steps ahead, and
   // steps stay as they are written: left alone the compiler reads a chunk, waits and multiplies, with as few registers as that takes.
-  static constexpr int kSteps = 2 * (kWaveJ / 16), kAhead = 4;
+  static constexpr int kSteps = 2 * kFragsJ, kAhead = 4;
   template <typename T, typename LayoutA, typename LayoutB, typename Between>
   __device__ __forceinline__ void Add(const LdsByte *a, const LdsByte *b, int wave_i, int wave_j, const Between &between) {
-    constexpr int kFragsI = kWaveI / 16, kFragsJ = kWaveJ / 16;
     Chunk<T> x[2][kFragsI], y[2][kFragsJ];
-    const auto read_x = [&](int half, int i) { x[half][i] = LayoutA::Read(a, wave_i * kWaveI + i * 16, half); };
+    const auto read_x = [&](int half, int i) { x[half][i] = LayoutA::Read(a, wave_i * kFragsI * 16 + i * 16, half); };
     const auto read_y = [&](int half, int j) { y[half][j] = LayoutB::Read(b, wave_j * kWaveJ + j * 16, half); };
 #pragma unroll
     for (int i = 0; i < kFragsI; ++i) read_x(0, i);
@@ -334,49 +335,56 @@ struct Tile {
   }
 };
 
-// The blocks of a workgroup's tiles, one after the other.  kDirect: while one is multiplied, the next one of A and the next two of B are on their
-// way (as far as the LDS holds: two of A, three of B), those of the tiles that follow too while a tile's results are written.
+// The blocks of a workgroup's tiles, one after the other.  kDirect: while one is multiplied, the next ones are on their way as far as the LDS holds them,
+// those of the tiles that follow too while a tile's results are written.
 //   run_a(id, part), run_b: the runs of a tile, `parts` of them;  add(a, b);  end(id)
 template <bool kDirect, typename StreamA, typename StreamB, typename StageA, typename StageB, typename S, typename RunA, typename RunB, typename AddFn, typename EndFn>
 __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts, long long stride_a, long long stride_b, const RunA &run_a, const RunB &run_b,
                                          const AddFn &add, const EndFn &end) {
   constexpr int kA = S::kI * kLineBytes, kB = S::kJ * kLineBytes;
   if constexpr (kDirect) {
-    const unsigned first = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)lds);
+    constexpr int kAheadA = S::kBlocksA - 1, kAheadB = S::kBlocksB - 1;
+    static_assert(kAheadB == kAheadA || kAheadB == kAheadA + 1, "the order of loads that follows");
+    // Loads that may be on their way when a block is multiplied: those issued after its own (a block's time issues A's, then B's, of blocks further on).
+    constexpr int kLater = (kAheadA - 1) * (StreamA::kPieces + StreamB::kPieces) + (kAheadB - kAheadA) * StreamB::kPieces;
+    const unsigned first = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)lds), first_b = first + S::kBlocksA * kA;
     StreamA a;
     StreamB b;
     a.Start(run_a, tiles, parts, stride_a);
     b.Start(run_b, tiles, parts, stride_b);
-    unsigned a0 = first, a1 = first + kA, b0 = first + 2 * kA, b1 = b0 + kB, b2 = b1 + kB;
-    a.Issue(a0, run_a, tiles, parts, stride_a);
-    b.Issue(b0, run_b, tiles, parts, stride_b);
-    b.Issue(b1, run_b, tiles, parts, stride_b);
-    bool landed = false;  // whether all loads have arrived (else those of A and B asked for last, as far as B goes ahead, have not)
+    if constexpr (kAheadB > kAheadA) b.Issue(first_b, run_b, tiles, parts, stride_b);
+#pragma unroll
+    for (int n = 0; n < kAheadA; ++n) {
+      a.Issue(first + n * kA, run_a, tiles, parts, stride_a);
+      b.Issue(first_b + (n + kAheadB - kAheadA) * kB, run_b, tiles, parts, stride_b);
+    }
+    unsigned at_a = first, at_b = first_b, to_a = first + kAheadA * kA, to_b = first_b + kAheadB * kB;
+    const auto next_a = [&](unsigned at) { return at == first + kAheadA * kA ? first : at + kA; };
+    const auto next_b = [&](unsigned at) { return at == first_b + kAheadB * kB ? first_b : at + kB; };
+    bool landed = false;  // whether all loads have arrived
     for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
       for (int part = 0; part < parts; ++part) {
         for (int n = run_b(id, part).blocks; n > 0; --n) {
           if (landed) Meet();
-          else WaitAndMeet<StreamB::kPieces>();
+          else WaitAndMeet<kLater>();
           // (the block is there, and what follows goes where the one before was, which has been read)
           landed = false;
-          a.Prepare(a1, run_a, tiles, parts, stride_a);
-          b.Prepare(b2, run_b, tiles, parts, stride_b);
+          a.Prepare(to_a, run_a, tiles, parts, stride_a);
+          b.Prepare(to_b, run_b, tiles, parts, stride_b);
           // Loads one by one between the products: all at once they fill the queue of the memory pipeline, which takes 16 cycles for each, and
           // the waves wait to issue them while nothing is multiplied.
-          add((const LdsByte *)(uintptr_t)a0, (const LdsByte *)(uintptr_t)b0, [&](auto step) {
-            constexpr int kLoads = StreamA::kPieces + StreamB::kPieces, kGap = Tile::kSteps / kLoads, p = step.value / kGap;
+          add((const LdsByte *)(uintptr_t)at_a, (const LdsByte *)(uintptr_t)at_b, [&](auto step) {
+            constexpr int kLoads = StreamA::kPieces + StreamB::kPieces, kGap = Tile<1>::kSteps / kLoads, p = step.value / kGap;
             static_assert(kGap >= 1, "a load after every step at most");
             if constexpr (step.value % kGap == 0 && p < StreamA::kPieces) a.template Piece<p>();
             else if constexpr (step.value % kGap == 0 && p < kLoads) b.template Piece<p - StreamA::kPieces>();
           });
           a.Done();
           b.Done();
-          const unsigned a_was = a0, b_was = b0;
-          a0 = a1;
-          a1 = a_was;
-          b0 = b1;
-          b1 = b2;
-          b2 = b_was;
+          at_a = next_a(at_a);
+          at_b = next_b(at_b);
+          to_a = next_a(to_a);
+          to_b = next_b(to_b);
         }
       }
       // (before the tile's results are stored: a wait for loads issued before them would be one for the stores as well)
@@ -522,7 +530,7 @@ template <typename T, int kAct, typename S, bool kDirect>
 __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_gated(const Forward a, unsigned tiles, unsigned tile_rows, unsigned tile_columns) {
   __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
   constexpr int kK = kLineBytes / sizeof(T), kHidden = S::kJ / 2;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / S::kWaveI), wave_j = wave / (S::kI / S::kWaveI);
   struct At {
     long long i0, split, first;
     int h0;
@@ -549,18 +557,18 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
     const long long from = at.h0 * a.w_stride + at.first * kK;
     return Run{static_cast<const T *>(a.w_gate) + from, static_cast<const T *>(a.w_up) + from, a.hidden - at.h0, a.dim - at.first * kK, blocks_of(at)};
   };
-  Tile t;
+  Tile<S::kWaveI / 16> t;
   t.Clear();
   const auto add = [&](const LdsByte *x, const LdsByte *w, const auto &between) {
-    t.Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(x, w, wave_i, wave_j, between);
+    t.template Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(x, w, wave_i, wave_j, between);
   };
   RunTiles<kDirect, Stream<T, S::kI, S::kThreads, false, false>, Stream<T, S::kJ, S::kThreads, false, true>, Stage<T, S::kI, S::kThreads, false, false>,
            Stage<T, S::kJ, S::kThreads, false, true>, S>((LdsByte *)s_blocks, tiles, 1, a.x_stride, a.w_stride, run_x, run_w, add, [&](unsigned id) {
     const At at = at_of(id);
     const int h = at.h0 + wave_j * (kWaveJ / 2);
 #pragma unroll
-    for (int i = 0; i < kWaveI / 16; ++i) {
-      const long long row = at.i0 + wave_i * kWaveI + i * 16 + lane % 16;
+    for (int i = 0; i < S::kWaveI / 16; ++i) {
+      const long long row = at.i0 + wave_i * S::kWaveI + i * 16 + lane % 16;
       if (row >= a.rows || h >= a.hidden) continue;  // (all four lanes of a row)
       if (a.splits > 1) {
         float *to = a.partial + ((at.split * a.rows + row) * ((a.hidden + 63) / 64) + h / 64) * kWaveJ + lane / 16 * 4;
@@ -720,7 +728,7 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
   __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
   constexpr int kK = kLineBytes / sizeof(T);
   const long long segment_blocks = (p.inner + kK - 1) / kK;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / kWaveI), wave_j = wave / (S::kI / kWaveI);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / S::kWaveI), wave_j = wave / (S::kI / S::kWaveI);
   struct At {
     long long i0, one, first;
     int j0, member;
@@ -752,17 +760,17 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
     const At at = at_of(id);
     return run_of(at, segment, p.b, kAcrossB, at.j0, p.columns);
   };
-  Tile t;
+  Tile<S::kWaveI / 16> t;
   t.Clear();
   const auto add = [&](const LdsByte *of_a, const LdsByte *of_b, const auto &between) {
-    t.Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(of_a, of_b, wave_i, wave_j, between);
+    t.template Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(of_a, of_b, wave_i, wave_j, between);
   };
   RunTiles<kDirect, Stream<T, S::kI, S::kThreads, kAcrossA, false>, Stream<T, S::kJ, S::kThreads, kAcrossB, false>, Stage<T, S::kI, S::kThreads, kAcrossA, false>,
            Stage<T, S::kJ, S::kThreads, kAcrossB, false>, S>((LdsByte *)s_blocks, tiles, p.segments, p.a.stride, p.b.stride, run_a, run_b, add, [&](unsigned id) {
     const At at = at_of(id);
 #pragma unroll
-    for (int i = 0; i < kWaveI / 16; ++i) {
-      const long long row = at.i0 + wave_i * kWaveI + i * 16 + lane % 16;
+    for (int i = 0; i < S::kWaveI / 16; ++i) {
+      const long long row = at.i0 + wave_i * S::kWaveI + i * 16 + lane % 16;
       if (row >= p.rows) continue;
 #pragma unroll
       for (int j = 0; j < kWaveJ / 16; j += 4) {

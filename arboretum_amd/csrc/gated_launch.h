@@ -7,18 +7,21 @@
 namespace arb {
 
 constexpr int kLineBytes = 128;           // of k's in a block: 64 of 16 bits, 32 of 32
-constexpr int kWaveI = 64, kWaveJ = 128;  // a wave's part of a tile: 4 x 8 fragments of 16 x 16
+constexpr int kWaveJ = 128;       // columns of a wave's part of a tile
 
-// A workgroup's tile: kWavesI x kWavesJ waves.
-template <int kWavesI, int kWavesJ>
+// A workgroup's tile: kWavesI x kWavesJ waves, kWaveI rows by kWaveJ columns each.  The LDS holds kBlocksA blocks of A and kBlocksB of B: one that is multiplied, the
+// others on their way.
+template <int kWavesI, int kWavesJ, int kWaveI_, int kBlocksA_, int kBlocksB_>
 struct TileShape {
-  static constexpr int kThreads = 64 * kWavesI * kWavesJ, kI = kWaveI * kWavesI, kJ = kWaveJ * kWavesJ;
-  static constexpr int kLdsBytes = (2 * kI + 3 * kJ) * kLineBytes;  // two blocks of A, three of B
+  static constexpr int kWaveI = kWaveI_, kThreads = 64 * kWavesI * kWavesJ, kI = kWaveI * kWavesI, kJ = kWaveJ * kWavesJ;
+  static constexpr int kBlocksA = kBlocksA_, kBlocksB = kBlocksB_;
+  static constexpr int kLdsBytes = (kBlocksA * kI + kBlocksB * kJ) * kLineBytes;
   static constexpr int kEach = 160 * 1024 / kLdsBytes;              // workgroups of a CU
-  static constexpr int kWavesEach = (kWavesI * kWavesJ * kEach + 3) / 4;  // waves of a SIMD
+  static constexpr int kWavesEach = kWavesI * kWavesJ * kEach / 4;  // waves of a SIMD
 };
-typedef TileShape<4, 2> LargeTile;
-typedef TileShape<2, 1> SmallTile;
+typedef TileShape<4, 2, 64, 2, 3> LargeTile;  // 256 x 256
+typedef TileShape<4, 1, 32, 2, 3> SmallTile;  // 128 x 128, two to a CU.  Four waves, one for each SIMD where a CU has only one tile, read 1.7 times as much of
+                                              // the LDS as two of 64 rows did, and took 20.4 us for 1003 x 771 x 2055 (22.3), 15.7 for 200000 x 16 x 64 (21.0)
 
 // How a product is cut up: into which tiles, and how many shares of its k's (blocks of kLineBytes of them).
 struct ProductCut {
