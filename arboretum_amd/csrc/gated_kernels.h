@@ -46,10 +46,25 @@ __device__ __forceinline__ F4 Product(const Chunk<float> &a, const Chunk<float> 
 __device__ __forceinline__ float PowerOfE(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ __forceinline__ float Sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + PowerOfE(-g)); }
 
+// Phi(g), and e^(-g^2/2) in two factors (which reach below 2^-126 together).  From -|g| on it is e^(-g^2/2) times Mills' ratio, here t P(t) with
+// t = 1 / (1 + 0.35 |g|): P has the least greatest relative error that a polynomial of its degree has for 0 <= |g| <= 16 (3e-8; summed in 32 bits 4e-7),
+// beyond which the other factor is 0.  (erfcf has a branch for either end, of which a wave runs both: 1003 x 771 x 2055 took 20.2 us.)
+__device__ __forceinline__ float Phi(float g, float *root) {
+  const float a = fminf(fabsf(g), 16.0f), t = __builtin_amdgcn_rcpf(1.0f + 0.35f * a);
+  constexpr float kP[9] = {0.13962124f, 0.13986452f, 0.11981419f, 0.10557979f, -0.023275260f, 0.15940905f, -0.25591564f, 0.14406730f, -0.029165233f};
+  float p = kP[8];
+#pragma unroll
+  for (int n = 7; n >= 0; --n) p = fmaf(p, t, kP[n]);
+  *root = __builtin_amdgcn_exp2f(-0.36067376022224085f * (a * a));
+  const float tail = *root * (p * t) * *root;
+  return g < 0.0f ? tail : 1.0f - tail;
+}
+
 template <int kAct>
 __device__ __forceinline__ float Act(float g) {
   if (kAct == kSilu) return g * Sigmoid(g);
-  return 0.5f * g * erfcf(-0.70710678118654752f * g);
+  float root;
+  return g * Phi(g, &root);
 }
 
 // act(g) and act'(g)
@@ -60,9 +75,10 @@ __device__ __forceinline__ void ActAndSlope(float g, float *act, float *slope) {
     *act = g * s;
     *slope = s + *act * (1.0f - s);
   } else {
-    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    float root;
+    const float phi = Phi(g, &root);
     *act = g * phi;
-    *slope = phi + g * (0.39894228040143268f * PowerOfE(-0.5f * g * g));
+    *slope = phi + g * (0.39894228040143268f * root * root);
   }
 }
 

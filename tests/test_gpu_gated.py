@@ -45,7 +45,7 @@ def act_64(name, g):
     if name == "silu":
         s = torch.sigmoid(g)
         return g * s, s + g * s * (1 - s), s + (g * s * (1 - s)).abs()
-    phi = torch.special.ndtr(g)
+    phi = 0.5 * torch.special.erfc(-g * 0.5 ** 0.5)  # (ndtr forms 1 + erf: 0 at -12.5 instead of 3.7e-36)
     bell = torch.exp(-g * g / 2) / (2 * np.pi) ** 0.5
     return g * phi, phi + g * bell, phi + (g * bell).abs()
 
@@ -259,6 +259,29 @@ def test_large_gates(arb, activation, dtype):
     # gates of hundreds on both sides: the activation is the identity, or nothing
     layer = Layer(arb, 40, 64, 64, dtype, activation=activation, size=60.0).forward().check_forward()
     layer.backward().check_backward()
+
+
+@pytest.mark.parametrize("rows", [7, 5000])
+@pytest.mark.parametrize("activation,most", [("silu", 80.0), ("gelu", 12.5)])
+def test_activations_over_their_range(arb, activation, most, rows):
+    # one product with 1 is exact: gates from end to end of what normal numbers of float32 tell from the identity and from nothing, by the kernels for few rows
+    # and for many
+    x = torch.linspace(-most, most, rows, dtype=torch.float32)[:, None].cuda()
+    one = torch.ones(1, 1, device="cuda")
+    out, gate, up, dx = (torch.full_like(x, 7) for _ in range(4))
+    dw = torch.empty(2, 1, 1, device="cuda")
+    grad = torch.ones_like(x)
+    work = torch.empty(max(arb.gated_bytes(rows, 1, 1), arb.gated_grad_bytes(rows, 1, 1)), dtype=torch.uint8, device="cuda")
+    kept = dict(gate=gate.data_ptr(), up=up.data_ptr(), activation=activation)
+    both = (x.data_ptr(), one.data_ptr(), one.data_ptr(), rows, 1, 1, work.data_ptr(), work.numel())
+    arb.gated(out.data_ptr(), *both, **kept)
+    arb.gated_grad(dx.data_ptr(), dw[0].data_ptr(), dw[1].data_ptr(), grad.data_ptr(), *both, **kept)
+    torch.cuda.synchronize()
+    g = x.double().cpu()
+    act, slope, slope_sum = act_64(activation, g)
+    close(out, act * g, 18 * U * (1 + g * g) * (act * g).abs(), torch.float32, "out")
+    want = g * slope + act
+    close(dx, want, 24 * U * (1 + g * g) * (g.abs() * slope_sum + act.abs()), torch.float32, "grad_x")
 
 
 def test_infinities_and_nan_stay_in_their_rows(arb):
