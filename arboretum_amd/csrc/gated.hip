@@ -7,13 +7,15 @@
 namespace arb {
 namespace {
 
-// A product of `rows` x `columns` (`batch` of them) over `blocks` blocks of k's: large tiles where they fill the chip and are not mostly beyond its columns; else
-// small ones, and few tiles share out their k's, at least `least` blocks to a share.  half: a tile has half as many columns.
+// A product of `rows` x `columns` (`batch` of them) over `blocks` blocks of k's; half: a tile has half as many columns.  Large tiles, which read the LDS less for
+// each product, where they fill the chip, are not mostly beyond its columns, and have k's enough that their results are not most of the work (the layer
+// itself, small and large: 50000 x 100 x 300 27.9 and 31.4 us, 100000 x 256 x 512 77.5 and 78.1, 20000 x 1024 x 2048 173 and 151).  Else small ones, and few of them share out
+// their k's, at least `least` blocks to a share, until each half of a CU has one.
 ProductCut CutOf(long long rows, long long columns, int half, long long batch, long long blocks, long long least) {
   const auto tiles = [&](long long i, long long j) { return Pieces(rows, i) * Pieces(columns, j / half) * batch; };
   const long long large = tiles(LargeTile::kI, LargeTile::kJ), small = tiles(SmallTile::kI, SmallTile::kJ);
   ProductCut c;
-  c.large = large >= 200 && columns > SmallTile::kJ / half;
+  c.large = large >= 200 && columns > SmallTile::kJ / half && blocks > 2;
   const long long most = std::max<long long>(1, std::min({c.large ? 256 / large : 512 / std::max<long long>(small, 1), blocks / least, 64ll}));
   c.split_blocks = std::max<long long>(1, Pieces(blocks, most));
   c.splits = std::max<long long>(1, Pieces(blocks, c.split_blocks));
@@ -30,10 +32,9 @@ struct Room {
   }
 };
 
-// Rows whose chunks are not aligned come through registers into small tiles, which takes four times as long; copies of x and both
-// weights are read and written once.  For the gradient (300 x 4095 x 4097: 153 us for grad_x without, 63 with copies) that is always less, for
-// the layer itself, which reads its weights along k, from about 256 rows on (40 rows of 4095 x 16383: 103 us without, 175 with; 300 of
-// 4095 x 4097: 79 and 68).
+// Rows whose chunks are not aligned come through registers into small tiles, a block at a time; copies of x and both weights are read and written once, a
+// launch of its own.  For the gradient (300 x 4095 x 4097: 153 us for grad_x without, 63 with copies) that is always less, for the layer itself, which reads
+// its weights along k, from some 400 rows on (300 of 4095 x 4097: 66.3 us without, 69.5 with; 500 of 1001 x 1003: 19.8 and 18.0; 8191: 57 and 41.6).
 LayerPad PadOf(long long rows, int dim, int hidden, size_t item, long long least_rows, Room *room) {
   LayerPad p{0, 0, 0, 0};
   if (dim * item % 16 == 0 || rows < least_rows) return p;
@@ -55,9 +56,9 @@ GatedPlan PlanOf(long long rows, int dim, int hidden, int type) {
   const size_t item = ElementBytes(type);
   GatedPlan p;
   Room room;
-  p.few = rows <= 16;
+  p.few = rows <= kFewRows;
   p.out = CutOf(rows, hidden, 2, 1, Pieces(dim * item, kLineBytes), 4);
-  p.pad = PadOf(rows, dim, hidden, item, 256, &room);
+  p.pad = PadOf(rows, dim, hidden, item, 400, &room);
   p.partial = room.Take(p.out.splits > 1 ? (size_t)p.out.splits * rows * Pieces(hidden, kScaleGroup) * kWaveJ * sizeof(float) : 0);
   p.bytes = room.bytes;
   return p;

@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_join(const Forward a, long l
 
 // Few rows (up to 16): 16 hidden columns a workgroup, whose eight waves share out the k's.  The weights are read once, from memory into the
 // registers that the products take them from: a lane's chunk is 16 bytes of a weight row, four steps of 64 bytes a row at once.
-constexpr int kFewRows = 16, kFewWaves = 8;
+constexpr int kFewWaves = 8;
 template <typename T, int kAct>
 __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
   constexpr int kVec = 16 / sizeof(T), kStep = 4 * kVec, kUnroll = 4;

@@ -6,8 +6,9 @@
 
 namespace arb {
 
-constexpr int kLineBytes = 128;           // of k's in a block: 64 of 16 bits, 32 of 32
-constexpr int kWaveJ = 128;       // columns of a wave's part of a tile
+constexpr int kLineBytes = 128;  // of k's in a block: 64 of 16 bits, 32 of 32
+constexpr int kWaveJ = 128;      // columns of a wave's part of a tile
+constexpr int kFewRows = 16;     // up to here a product's sixteen rows hold all of x
 
 // A workgroup's tile: kWavesI x kWavesJ waves, kWaveI rows by kWaveJ columns each.  The LDS holds kBlocksA blocks of A and kBlocksB of B: one that is multiplied, the
 // others on their way.
