@@ -8,36 +8,41 @@ namespace {
 
 constexpr int kCodeVec = 8;  // values a lane codes at a time
 
-// Magnitudes as whole numbers: their order is that of the floats, with NaN above infinity.
-__device__ __forceinline__ unsigned Magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-template <int N>
-__device__ __forceinline__ unsigned MostOf(const float (&v)[N]) {
-  unsigned most = Magnitude(v[0]);
-#pragma unroll
-  for (int c = 1; c < N; ++c) most = max(most, Magnitude(v[c]));
-  return most;
-}
+// The greater of `most` and the magnitude of v; a NaN where either is one.
+__device__ __forceinline__ float MostOf(float most, float v) { return __builtin_elementwise_maximum(most, fabsf(v)); }
 
 // The scale of a group whose greatest magnitude is `most`.  Steps are no smaller than 2^-100, so that their reciprocal is a
 // number; an infinity or a NaN in a group makes the scale a NaN, and with it all that is read back of the group.
-__device__ __forceinline__ float ScaleOf(unsigned most) {
-  return most < 0x7F800000u ? fmaxf(__uint_as_float(most) / 127.0f, 0x1p-100f) : __builtin_nanf("");
-}
+__device__ __forceinline__ float ScaleOf(float most) { return most < __builtin_inff() ? fmaxf(most / 127.0f, 0x1p-100f) : __builtin_nanf(""); }
 
 // rint(v / scale).  With y = 1 / scale correctly rounded, q = v y is off by no more than a rounding or two and v - q scale is exact,
 // so that q + (v - q scale) y, rounded, is the quotient correctly rounded (Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000"): three operations, where a division takes about ten and bound the kernel (297 us for 65,536 x 4096, now 190).
+// System/6000"): three operations, where a division takes about ten and bound the kernel (297 us for 65,536 x 4096, now 190).  Quotients are within
+// 127 and a rounding: the sum with 1.5 2^23, whose last bit is worth 1, rounds them to nearest, ties to even, with the code in its low eight bits.
 // (What a NaN becomes does not matter: the scale tells of it.)
 template <int N>
 __device__ __forceinline__ Pack<signed char, N> CodesOf(const float (&v)[N], float scale) {
   Pack<signed char, N> codes;
   const float y = 1.0f / scale;
+  unsigned sum[N];
 #pragma unroll
   for (int c = 0; c < N; ++c) {
     const float q = v[c] * y;
-    const float quotient = fmaf(fmaf(-q, scale, v[c]), y, q);
-    codes.v[c] = (signed char)(int)rintf(__builtin_amdgcn_fmed3f(quotient, -127.0f, 127.0f));
+    sum[c] = __float_as_uint(fmaf(fmaf(-q, scale, v[c]), y, q) + 12582912.0f);
+  }
+  if constexpr (N % 4 == 0) {
+    struct Words {
+      unsigned w[N / 4];
+    } words;
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+      const unsigned low = __builtin_amdgcn_perm(sum[4 * w + 1], sum[4 * w], 0x0C0C0400), high = __builtin_amdgcn_perm(sum[4 * w + 3], sum[4 * w + 2], 0x0C0C0400);
+      words.w[w] = high << 16 | low;
+    }
+    codes = __builtin_bit_cast(Pack<signed char, N>, words);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) codes.v[c] = (signed char)(sum[c] & 0xFF);
   }
   return codes;
 }

@@ -59,9 +59,11 @@ __global__ void __launch_bounds__(kThreads) k_checkpoint(const Shape a, long lon
     }
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      unsigned most = MostOf(v[e]);
+      float most = 0.0f;
 #pragma unroll
-      for (int by = kLanes / 2; by > 0; by /= 2) most = max(most, (unsigned)__shfl_xor((int)most, by));
+      for (int c = 0; c < kCodeVec; ++c) most = MostOf(most, v[e][c]);
+#pragma unroll
+      for (int by = kLanes / 2; by > 0; by /= 2) most = MostOf(most, __shfl_xor(most, by));
       const float scale = ScaleOf(most);
       if (threadIdx.x % kLanes == 0 && p[e].held > 0) a.scales[p[e].group] = scale;
       const Pack<signed char, kCodeVec> codes = CodesOf(v[e], scale);

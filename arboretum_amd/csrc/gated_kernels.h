@@ -521,13 +521,13 @@ __device__ __forceinline__ void Keep(void *kept, float *scales, long long stride
     StoreRounded(static_cast<T *>(kept) + row * stride, at, hidden, v);
     return;
   }
-  unsigned most = 0;  // (columns beyond the layer hold 0, or what the last one holds)
+  float most = 0.0f;  // (columns beyond the layer hold 0, or what the last one holds)
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) most = max(most, Magnitude(v[j][r]));
-  most = max(most, (unsigned)__shfl_xor((int)most, 16));
-  most = max(most, (unsigned)__shfl_xor((int)most, 32));
+    for (int r = 0; r < 4; ++r) most = MostOf(most, v[j][r]);
+  most = MostOf(most, __shfl_xor(most, 16));
+  most = MostOf(most, __shfl_xor(most, 32));
   const float scale = ScaleOf(most);
   if ((threadIdx.x & 63) < 16) scales[row * ((hidden + kScaleGroup - 1) / kScaleGroup) + at / kScaleGroup] = scale;
   Pack<signed char, 4> codes[4];
@@ -635,9 +635,9 @@ __global__ void __launch_bounds__(kThreads) k_gated_join(const Forward a, long l
         if (there) static_cast<T *>(kept)[row * a.kept_stride + h] = Round<T>(v);
         continue;
       }
-      unsigned most = there ? Magnitude(v) : 0;
+      float most = there ? fabsf(v) : 0.0f;
 #pragma unroll
-      for (int by = 32; by > 0; by /= 2) most = max(most, (unsigned)__shfl_xor((int)most, by));
+      for (int by = 32; by > 0; by /= 2) most = MostOf(most, __shfl_xor(most, by));
       const float scale = ScaleOf(most);
       if (lane == 0) scales[row * groups + group] = scale;
       const float one[1] = {v};
