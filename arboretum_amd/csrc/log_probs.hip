@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <limits>
+#include <type_traits>
 
 #include "operators_device.h"
 
@@ -59,7 +60,8 @@ __device__ __forceinline__ Word Least(const Word (&words)[kEach], int k) {
 // A wave's list of 64 keys in order, one a lane: `one` takes its place, and the last one falls out.
 __device__ __forceinline__ void Insert(Key *held, Key one) {
   const int lane = threadIdx.x & 63, place = __popcll(__ballot(*held > one));
-  const Key before = ((Key)(unsigned)__shfl_up((int)(unsigned)(*held >> 32), 1) << 32) | (unsigned)__shfl_up((int)(unsigned)*held, 1);
+  const auto lane_before = [](unsigned word) { return (unsigned)__builtin_amdgcn_update_dpp((int)word, (int)word, 0x138, 0xF, 0xF, false); };
+  const Key before = ((Key)lane_before((unsigned)(*held >> 32)) << 32) | lane_before((unsigned)*held);
   *held = lane < place ? *held : lane == place ? one : before;
 }
 
@@ -79,6 +81,36 @@ __device__ __forceinline__ Sums Join(const Sums &a, const Sums &b, float factor)
   r.most = most;
   r.sum = ea * a.sum + eb * b.sum;
   r.moment = ea * (a.moment + fmaxf(da, kLowest) * a.sum) + eb * (b.moment + fmaxf(db, kLowest) * b.sum);
+  return r;
+}
+
+// All lanes' values by op, whose order does not matter to it but for rounding (which is the same in every lane): neighbours, pairs, then mirrored halves of 16
+// lanes by instructions that take an operand from another lane, then the halves of 32 and of all.  (__shfl_xor goes through the LDS each time.)
+template <typename Op>
+__device__ __forceinline__ float OfLanes(float v, const Op &op) {
+  const auto other = [](float x, auto how) {
+    const int w = __float_as_int(x);
+    return __int_as_float(__builtin_amdgcn_update_dpp(w, w, decltype(how)::value, 0xF, 0xF, false));
+  };
+  v = op(v, other(v, std::integral_constant<int, 0xB1>()));   // lanes 1 0 3 2 of four
+  v = op(v, other(v, std::integral_constant<int, 0x4E>()));   // lanes 2 3 0 1
+  v = op(v, other(v, std::integral_constant<int, 0x141>()));  // eight mirrored
+  v = op(v, other(v, std::integral_constant<int, 0x140>()));  // sixteen mirrored
+  const auto sixteens = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(sixteens[0]), __uint_as_float(sixteens[1]));
+  const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+
+// The lanes' sums joined: their maximum first, to which each takes its own.
+template <bool kMoment>
+__device__ __forceinline__ Sums JoinLanes(const Sums &s, float factor) {
+  Sums r;
+  r.most = OfLanes(s.most, [](float a, float b) { return fmaxf(a, b); });
+  const float d = factor * (s.most - Base(r.most)), e = Exp2(d);
+  const auto add = [](float a, float b) { return a + b; };
+  r.sum = OfLanes(e * s.sum, add);
+  r.moment = kMoment ? OfLanes(e * (s.moment + fmaxf(d, kLowest) * s.sum), add) : 0.0f;
   return r;
 }
 
@@ -147,7 +179,7 @@ __device__ __forceinline__ void WriteTop(const RowsArgs &a, const Sums &s, float
 // The likeliest tokens: every thread keeps the maximum of what it reads.  The k-th greatest of these maxima has k elements of the row on
 // its side, so the k likeliest are no less than it, and whatever is no less lies with the threads whose maxima are no less: about k
 // of 256, so that only their share of the row is read again.  (Where many are equal, as in a row of one value, more is.)
-template <typename T, int kWaves, int kUnroll, bool kEntropy, bool kTop>
+template <typename T, int kWaves, int kUnroll, bool kSide, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const RowsArgs a) {
   constexpr int kVec = 16 / sizeof(T), kTeam = kWaves * 64, kTeams = kWaves == 1 ? 4 : 1, kChunk = kUnroll * kVec;
   __shared__ Sums s_sums[kWaves];
@@ -164,7 +196,18 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
     const long long row = live ? item / a.parts : 0;
     const unsigned part = live ? (unsigned)(item - row * a.parts) : 0;
     const unsigned begin = part * a.part, length = live ? min(a.part, a.vocab - begin) : 0;
-    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride + begin;
+    const long long apart = kSide ? 1 : a.class_stride;
+    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride + begin * apart;
+    const auto vector_at = [&](unsigned at) {
+      if constexpr (kSide) {
+        return *reinterpret_cast<const Pack<T, kVec> *>(x + at);
+      } else {
+        Pack<T, kVec> p;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) p.v[c] = x[(at + c) * apart];
+        return p;
+      }
+    };
 
     Sums s = {-Infinity(), 0.0f, 0.0f};
     const auto add = [&](const float (&v)[kChunk]) {
@@ -189,7 +232,7 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
     for (unsigned i = 0; i < whole; i += kUnroll) {
       Pack<T, kVec> p[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = *reinterpret_cast<const Pack<T, kVec> *>(x + (size_t)((i + u) * kTeam + t) * kVec);
+      for (int u = 0; u < kUnroll; ++u) p[u] = vector_at(((i + u) * kTeam + t) * kVec);
       float v[kChunk];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
@@ -204,17 +247,16 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
         const unsigned at = ((whole + u) * kTeam + t) * kVec;
         const bool all = at < length && length - at >= kVec;
         Pack<T, kVec> p;
-        if (all) p = *reinterpret_cast<const Pack<T, kVec> *>(x + at);
+        if (all) p = vector_at(at);
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) v[u * kVec + c] = all ? (float)p.v[c] : at < length && c < (int)(length - at) ? (float)x[at + c] : -Infinity();
+        for (int c = 0; c < kVec; ++c) v[u * kVec + c] = all ? (float)p.v[c] : at < length && c < (int)(length - at) ? (float)x[(at + c) * apart] : -Infinity();
       }
       add(v);
     }
     const unsigned mine = kTop && t < vectors ? OrderOf(s.most) : 0;
 
     // the sums of the team
-#pragma unroll
-    for (int by = 32; by > 0; by /= 2) s = Join(s, Sums{__shfl_xor(s.most, by), __shfl_xor(s.sum, by), __shfl_xor(s.moment, by)}, a.factor);
+    s = JoinLanes<kEntropy>(s, a.factor);
     if (kWaves > 1) {
       if (lane == 0) s_sums[wave] = s;
       __syncthreads();
@@ -252,10 +294,10 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
         const unsigned there = e0 + lane < count && at < length ? min(length - at, (unsigned)kVec) : 0;
         Pack<T, kVec> p;
         if (there == kVec) {
-          p = *reinterpret_cast<const Pack<T, kVec> *>(x + at);
+          p = vector_at(at);
         } else {
 #pragma unroll
-          for (int c = 0; c < kVec; ++c) p.v[c] = (unsigned)c < there ? x[at + c] : T(0);
+          for (int c = 0; c < kVec; ++c) p.v[c] = (unsigned)c < there ? x[(at + c) * apart] : T(0);
         }
 #pragma unroll
         for (int c = 0; c < kVec; ++c) {
@@ -314,8 +356,7 @@ __global__ void __launch_bounds__(64) k_join(const RowsArgs a) {
       const float4 p = a.sums[row * a.parts + lane];
       s = Sums{p.x, p.y, p.z};
     }
-#pragma unroll
-    for (int by = 32; by > 0; by /= 2) s = Join(s, Sums{__shfl_xor(s.most, by), __shfl_xor(s.sum, by), __shfl_xor(s.moment, by)}, a.factor);
+    s = JoinLanes<true>(s, a.factor);
     const float log_sum = LogSum(s);
     if (lane == 0) WriteRow<T>(a, s, log_sum, row);
     if (a.top == 0) continue;
@@ -346,7 +387,7 @@ __global__ void __launch_bounds__(64) k_join(const RowsArgs a) {
 
 // The greatest kHeld in one pass, in order; `top` beyond that takes further passes, each behind the last one found.  kUnroll classes
 // are asked for at once.
-template <typename T, int kHeld, int kUnroll>
+template <typename T, bool kSide, int kHeld, int kUnroll>
 __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
   const long long step = (long long)gridDim.x * 256;
   for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < a.n; row += step) {
@@ -361,8 +402,14 @@ __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
       for (int h = 0; h < kHeld; ++h) held[h] = __builtin_nanf(""), held_at[h] = ~0u;
       for (unsigned j0 = 0; j0 < a.vocab; j0 += kUnroll) {
         float v[kUnroll];
+        if (kSide && a.vocab - j0 >= kUnroll) {
+          const Pack<T, kUnroll> p = *reinterpret_cast<const Pack<T, kUnroll> *>(x + j0);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) v[u] = (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride];
+          for (int u = 0; u < kUnroll; ++u) v[u] = (float)p.v[u];
+        } else {
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) v[u] = (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride];
+        }
         if (from == 0) {
           float most = v[0];
 #pragma unroll
@@ -546,22 +593,25 @@ __global__ void __launch_bounds__(256) k_grad_rows(const GradArgs a, int lanes, 
   }
 }
 
+// A row a thread, `part` classes of it (a multiple of kUnroll) by each row of workgroups.
+constexpr unsigned kColumnsUnroll = 8;
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(256) k_grad_columns(const GradArgs a) {
-  constexpr int kUnroll = 8;
+__global__ void __launch_bounds__(256) k_grad_columns(const GradArgs a, unsigned part) {
+  constexpr unsigned kUnroll = kColumnsUnroll;
+  const unsigned begin = blockIdx.y * part, end = min(a.vocab, begin + part);
   const long long step = (long long)gridDim.x * 256;
   const float factor = a.scale * kLog2E;
   for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < a.n; row += step) {
     const RowGrad r = RowGradOf<kEntropy>(a, row);
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride;
     T *grad = static_cast<T *>(a.grad) + row * a.grad_row_stride;
-    for (unsigned j0 = 0; j0 < a.vocab; j0 += kUnroll) {
+    for (unsigned j0 = begin; j0 < end; j0 += kUnroll) {
       float v[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride];
+      for (unsigned u = 0; u < kUnroll; ++u) v[u] = (float)x[(long long)min(j0 + u, a.vocab - 1) * a.class_stride];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (j0 + u >= a.vocab) break;
+      for (unsigned u = 0; u < kUnroll; ++u) {
+        if (j0 + u >= end) break;
         grad[(long long)(j0 + u) * a.grad_class_stride] = j0 + u == r.token ? GradOfToken<T, kEntropy>(r, factor, v[u]) : GradOf<T, kEntropy>(r, factor, v[u]);
       }
     }
@@ -634,9 +684,12 @@ void LogProbs(const LogProbsArgs &a) {
              a.entropy, reinterpret_cast<float2 *>(a.stats), a.top, a.top_tokens, a.top_log_probs, l.status, 1, (unsigned)l.vocab, nullptr, nullptr};
   WithType(l.type, [&](auto type) {
     typedef decltype(type) T;
-    if (!side_by_side || l.vocab <= 32) {
+    if ((!side_by_side || l.vocab <= 128) && l.n / 32 >= l.vocab * std::max(a.top, 1)) {
       const dim3 grid(GridOf((l.n + 255) / 256));
-      const auto columns = [&](auto held) { hipLaunchKernelGGL((k_columns<T, decltype(held)::value, 8>), grid, dim3(256), 0, stream, r); };
+      const auto columns = [&](auto held) {
+        if (side_by_side) hipLaunchKernelGGL((k_columns<T, true, decltype(held)::value, 8>), grid, dim3(256), 0, stream, r);
+        else hipLaunchKernelGGL((k_columns<T, false, decltype(held)::value, 8>), grid, dim3(256), 0, stream, r);
+      };
       if (a.top <= 1) columns(std::integral_constant<int, 1>());
       else if (a.top == 2) columns(std::integral_constant<int, 2>());
       else if (a.top == 3) columns(std::integral_constant<int, 3>());
@@ -651,18 +704,22 @@ void LogProbs(const LogProbsArgs &a) {
       r.sums = static_cast<float4 *>(a.work);
       r.keys = reinterpret_cast<Key *>(r.sums + l.n * r.parts);
     }
-    const auto launch = [&](auto entropy, auto top) {
-      constexpr bool kEntropy = decltype(entropy)::value, kTop = decltype(top)::value;
-      const long long items = l.n * r.parts;
-      if (r.part <= 2048) hipLaunchKernelGGL((k_rows<T, 1, 1, kEntropy, kTop>), dim3(GridOf((items + 3) / 4)), dim3(256), 0, stream, r);
-      else hipLaunchKernelGGL((k_rows<T, 4, 4, kEntropy, kTop>), dim3(GridOf(items)), dim3(256), 0, stream, r);
-    };
     typedef std::true_type Yes;
     typedef std::false_type No;
-    if (a.entropy && a.top) launch(Yes(), Yes());
-    else if (a.entropy) launch(Yes(), No());
-    else if (a.top) launch(No(), Yes());
-    else launch(No(), No());
+    const auto launch = [&](auto side, auto entropy, auto top) {
+      constexpr bool kSide = decltype(side)::value, kEntropy = decltype(entropy)::value, kTop = decltype(top)::value;
+      const long long items = l.n * r.parts;
+      if (r.part <= 2048) hipLaunchKernelGGL((k_rows<T, 1, 1, kSide, kEntropy, kTop>), dim3(GridOf((items + 3) / 4)), dim3(256), 0, stream, r);
+      else hipLaunchKernelGGL((k_rows<T, 4, 4, kSide, kEntropy, kTop>), dim3(GridOf(items)), dim3(256), 0, stream, r);
+    };
+    const auto launch_as = [&](auto side) {
+      if (a.entropy && a.top) launch(side, Yes(), Yes());
+      else if (a.entropy) launch(side, Yes(), No());
+      else if (a.top) launch(side, No(), Yes());
+      else launch(side, No(), No());
+    };
+    if (side_by_side) launch_as(Yes());
+    else launch_as(No());
     if (r.parts > 1 && r.parts * r.top <= 512) hipLaunchKernelGGL((k_join<T, 8>), dim3(GridOf(l.n)), dim3(64), 0, stream, r);
     else if (r.parts > 1) hipLaunchKernelGGL((k_join<T, 32>), dim3(GridOf(l.n)), dim3(64), 0, stream, r);
   });
@@ -701,18 +758,28 @@ void LogProbsGrad(const LogProbsGradArgs &a) {
     const auto launch = [&](auto entropy) {
       constexpr bool kEntropy = decltype(entropy)::value;
       if (!side_by_side) {
-        hipLaunchKernelGGL((k_grad_columns<T, kEntropy>), dim3(GridOf((l.n + 255) / 256)), dim3(256), 0, stream, g);
+        // few rows share out their classes, at least 64 to a part, until there are threads for the chip
+        const long long parts = std::max(1ll, std::min({(1ll << 18) / l.n, l.vocab / 64, 32768ll}));
+        const unsigned part = (unsigned)((l.vocab + parts - 1) / parts + kColumnsUnroll - 1) / kColumnsUnroll * kColumnsUnroll;
+        hipLaunchKernelGGL((k_grad_columns<T, kEntropy>), dim3(GridOf((l.n + 255) / 256), (unsigned)((l.vocab + part - 1) / part)), dim3(256), 0, stream, g, part);
         return;
       }
-      constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
-      int lanes = 256;
-      while (lanes > 1 && lanes / 2 * kVec * kUnroll >= l.vocab) lanes /= 2;
-      const unsigned pieces = (unsigned)((l.vocab + lanes * kVec * kUnroll - 1) / (lanes * kVec * kUnroll));
-      const long long items = l.n * pieces, teams = 256 / lanes;
-      const dim3 grid(GridOf((items + teams - 1) / teams));
+      // threads of a row, or of as much of one as a workgroup takes: vectors of up to 32 threads one each, or four each
+      const auto rows = [&](auto unroll, auto past) {
+        constexpr int kUnroll = decltype(unroll)::value, kEach = 16 / sizeof(T) * kUnroll;
+        int lanes = kUnroll == 1 ? 32 : 256;
+        while (lanes > 1 && lanes / 2 * kEach >= l.vocab) lanes /= 2;
+        const unsigned pieces = (unsigned)((l.vocab + lanes * kEach - 1) / (lanes * kEach));
+        const long long items = l.n * pieces, teams = 256 / lanes;
+        hipLaunchKernelGGL((k_grad_rows<T, kUnroll, kEntropy, decltype(past)::value>), dim3(GridOf((items + teams - 1) / teams)), dim3(256), 0, stream, g, lanes, pieces);
+      };
+      const auto rows_of = [&](auto past) {
+        if (l.vocab <= 32 * 16 / (long long)sizeof(T)) rows(std::integral_constant<int, 1>(), past);
+        else rows(std::integral_constant<int, 4>(), past);
+      };
       // a gradient that the L2 caches do not hold is written past them
-      if ((size_t)l.n * l.vocab * sizeof(T) > kStreamedBytes) hipLaunchKernelGGL((k_grad_rows<T, kUnroll, kEntropy, true>), grid, dim3(256), 0, stream, g, lanes, pieces);
-      else hipLaunchKernelGGL((k_grad_rows<T, kUnroll, kEntropy, false>), grid, dim3(256), 0, stream, g, lanes, pieces);
+      if ((size_t)l.n * l.vocab * sizeof(T) > kStreamedBytes) rows_of(std::true_type());
+      else rows_of(std::false_type());
     };
     if (a.grad_entropy) launch(std::true_type());
     else launch(std::false_type());
