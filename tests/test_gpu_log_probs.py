@@ -191,7 +191,7 @@ class Held:
 def check(arb, x, tokens, layout, scale=1.0, top=0, bits=32, h=True):
     n, vocab = x.shape
     scale = float(np.float32(scale))
-    chain = vocab + 64 if layout in ("columns", "spread") or vocab <= 32 else vocab / 64 + 64
+    chain = vocab + 64 if layout in ("columns", "spread") or vocab <= 128 else vocab / 64 + 64
     want = Want(x, tokens, scale, chain)
     held = Held(arb, x, tokens, layout, bits=bits, scale=scale, top=top).forward()
     close(held.log_probs[:n], want.log_prob, want.err_log_prob, "log_probs")
@@ -257,7 +257,37 @@ def test_strides_and_starts_of_any_alignment(arb, n, vocab, top, layout, dtype):
     check(arb, x, some_tokens(gen, n, vocab), layout, scale=1.3, top=top, bits=64)
 
 
-@pytest.mark.parametrize("n,vocab", [(5, 12), (4, 600), (6, 3000), (300, 9000), (2, 30_000)])
+# many rows of few classes: a thread a row, and top in passes of eight
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("layout", ["rows", "padded", "columns", "spread"])
+@pytest.mark.parametrize("n,vocab,top", [(40, 1, 1), (500, 4, 3), (2600, 10, 8), (5200, 16, 10), (18_000, 61, 9), (9000, 128, 2), (4200, 127, 0)])
+def test_many_rows_of_few_classes(arb, n, vocab, top, layout, dtype):
+    gen = torch.Generator().manual_seed(n + vocab)
+    x = make_logits(gen, n, vocab, "normal", TYPES[dtype])
+    check(arb, x, some_tokens(gen, n, vocab), layout, scale=1.1, top=top)
+
+
+@pytest.mark.parametrize("kind", ["ties", "rising", "falling", "constant", "masked", "one", "lowest"])
+@pytest.mark.parametrize("layout", ["rows", "columns"])
+@pytest.mark.parametrize("n,vocab,top", [(2000, 7, 5), (6000, 17, 11)])
+def test_many_rows_that_tie_rise_or_are_masked(arb, n, vocab, top, kind, layout):
+    gen = torch.Generator().manual_seed(vocab + n)
+    dtype = [torch.float32, torch.bfloat16, torch.float16][(vocab + len(kind)) % 3]
+    x = make_logits(gen, n, vocab, kind, dtype)
+    check(arb, x, some_tokens(gen, n, vocab), layout, scale=0.8 if kind != "lowest" else 1.0, top=top)
+
+
+# few rows class by class: teams whose loads lie apart, rows in parts, gradients whose classes are shared out
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("layout", ["columns", "spread"])
+@pytest.mark.parametrize("n,vocab,top", [(1, 2000, 64), (2, 40_007, 20), (260, 2049, 3), (10, 16_385, 0), (3, 131, 9)])
+def test_few_rows_class_by_class(arb, n, vocab, top, layout, dtype):
+    gen = torch.Generator().manual_seed(n + vocab)
+    x = make_logits(gen, n, vocab, "normal", TYPES[dtype])
+    check(arb, x, some_tokens(gen, n, vocab), layout, scale=0.9, top=top)
+
+
+@pytest.mark.parametrize("n,vocab", [(5, 12), (4, 600), (6, 3000), (300, 9000), (2, 30_000), (3000, 12), (9000, 50)])
 @pytest.mark.parametrize("bad", [float("nan"), INF])
 def test_rows_with_a_nan_or_plus_infinity_say_so_and_others_do_not(arb, n, vocab, bad):
     gen = torch.Generator().manual_seed(vocab)
