@@ -648,23 +648,28 @@ __global__ void __launch_bounds__(kThreads) k_gated_join(const Forward a, long l
 
 // Few rows (up to 16): 16 hidden columns a workgroup, whose eight waves share out the k's.  The weights are read once, from memory into the
 // registers that the products take them from: a lane's chunk is 16 bytes of a weight row, four steps of 64 bytes a row at once.
+// kApart: rows that begin anywhere.  Every eighth of them begins alike within 16 bytes, and the workgroup takes sixteen of those; behind as many k's as
+// the row's first 16 bytes hold its chunks are aligned.
 constexpr int kFewWaves = 8;
-template <typename T, int kAct>
+template <typename T, int kAct, bool kApart>
 __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
-  constexpr int kVec = 16 / sizeof(T), kStep = 4 * kVec, kUnroll = 4;
+  constexpr int kVec = 16 / sizeof(T), kStep = 4 * kVec, kUnroll = 4, kEach = kApart ? 8 : 1;  // kEach: rows from one to the next
   __shared__ float s_sums[kFewWaves][2][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h0 = blockIdx.x * 16, quarter = lane / 16;
-  const long long h = min(h0 + lane % 16, a.hidden - 1), i = min(lane % 16ll, a.rows - 1);
-  const T *gate = static_cast<const T *>(a.w_gate) + h * a.w_stride + quarter * kVec, *up = static_cast<const T *>(a.w_up) + h * a.w_stride + quarter * kVec;
-  const T *x = static_cast<const T *>(a.x) + i * a.x_stride + quarter * kVec;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane / 16;
+  const int h0 = kApart ? blockIdx.x / 8 * 128 + blockIdx.x % 8 : blockIdx.x * 16;
+  if (h0 >= a.hidden) return;
+  const long long h = h0 + lane % 16 * kEach < a.hidden ? h0 + lane % 16 * kEach : h0, i = min(lane % 16ll, a.rows - 1);
+  const T *gate = static_cast<const T *>(a.w_gate) + h * a.w_stride, *up = static_cast<const T *>(a.w_up) + h * a.w_stride, *x = static_cast<const T *>(a.x) + i * a.x_stride;
+  int head = 0;
+  if (kApart) head = min((int)((16 - reinterpret_cast<uintptr_t>(static_cast<const T *>(a.w_gate) + h0 * a.w_stride) % 16) % 16 / sizeof(T)), a.dim);
   F4 g = {0, 0, 0, 0}, u = {0, 0, 0, 0};
-  const int steps = (a.dim + kStep - 1) / kStep, groups = a.dim / kStep / kUnroll;
+  const int steps = (a.dim - head + kStep - 1) / kStep, groups = (a.dim - head) / kStep / kUnroll;
   const auto whole = [&](const T *from) { return __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Pack<T, kVec> *>(from)); };
   for (int group = wave; group < groups; group += kFewWaves) {
     Chunk<T> gs[kUnroll], us[kUnroll], xs[kUnroll];
 #pragma unroll
     for (int n = 0; n < kUnroll; ++n) {
-      const int k = (group * kUnroll + n) * kStep;
+      const int k = head + (group * kUnroll + n) * kStep + quarter * kVec;
       gs[n] = whole(gate + k);
       us[n] = whole(up + k);
       xs[n] = whole(x + k);
@@ -675,9 +680,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
       u = Product(us[n], xs[n], u);
     }
   }
-  static_assert(kUnroll <= kFewWaves, "a wave for each step that is left");
-  if (const int step = groups * kUnroll + wave; step < steps) {
-    const int k = step * kStep, held = a.dim - k - quarter * kVec;
+  // what is left, a step a wave: up to four at the end, and the k's before `head`
+  static_assert(kUnroll < kFewWaves, "a wave for each step that is left, and one for the head");
+  const bool first = kApart && wave == kFewWaves - 1;
+  const int step = groups * kUnroll + wave;
+  if (first ? head > 0 : step < steps) {
+    const int k = first ? 0 : head + step * kStep + quarter * kVec, held = !first ? a.dim - k : quarter == 0 ? head : 0;
     const auto part = [&](const T *from) {
       Chunk<T> c;
 #pragma unroll
@@ -692,7 +700,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
   *reinterpret_cast<F4 *>(&s_sums[wave][1][lane * 4]) = u;
   __syncthreads();
   if (threadIdx.x >= 256) return;
-  const int in = threadIdx.x, of = in / 4, row = of % 16, column = h0 + of / 16 * 4 + in % 4;  // of: the lane that held it
+  const int in = threadIdx.x, of = in / 4, row = of % 16, column = h0 + (of / 16 * 4 + in % 4) * kEach;  // of: the lane that held it
   if (row >= a.rows || column >= a.hidden) return;
   float gv = 0.0f, uv = 0.0f;
 #pragma unroll
@@ -993,7 +1001,15 @@ void RunGated(const GatedArgs &a, const GatedPlan &plan) {
   WithActivation(l.activation, [&](auto act) {
     constexpr int kAct = decltype(act)::value;
     if (few) {
-      hipLaunchKernelGGL((k_gated_few<T, kAct>), dim3((unsigned)Pieces(l.hidden, 16)), dim3(64 * kFewWaves), 0, stream, f);
+      if constexpr (sizeof(T) == 2) {
+        // Rows that begin at odd elements, in both weights alike: loads at less than four bytes' alignment take twice as long (bf16, 1 row of 4095 x 16383 102 us,
+        // apart 61; of 4094 x 16383, whose rows lie on four bytes, 65, apart 67).
+        if (l.w_stride % 2 != 0 && (reinterpret_cast<uintptr_t>(l.w_gate) - reinterpret_cast<uintptr_t>(l.w_up)) % 16 == 0) {
+          hipLaunchKernelGGL((k_gated_few<T, kAct, true>), dim3((unsigned)Pieces(l.hidden, 128) * 8), dim3(64 * kFewWaves), 0, stream, f);
+          return;
+        }
+      }
+      hipLaunchKernelGGL((k_gated_few<T, kAct, false>), dim3((unsigned)Pieces(l.hidden, 16)), dim3(64 * kFewWaves), 0, stream, f);
       return;
     }
     const auto launch = [&](auto shape, auto is_direct) {

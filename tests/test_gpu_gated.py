@@ -198,7 +198,8 @@ def test_layer_and_gradient(arb, rows, dim, hidden, dtype):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("kept", ["as is", "no"])
 @pytest.mark.parametrize("rows,dim,hidden,pad,first", [(1, 4095, 33, 0, 0), (16, 1027, 40, 0, 0), (7, 1024, 50, 1, 0), (9, 2048, 31, 0, 1), (16, 513, 17, 2, 1), (3, 130, 16, 0, 0),
-                                                        (5, 4097, 70, 3, 3), (17, 1027, 40, 0, 0)])
+                                                        (5, 4097, 70, 3, 3), (17, 1027, 40, 0, 0), (2, 1, 300, 0, 0), (4, 5, 259, 0, 1),
+                                                        (16, 7, 131, 0, 0), (1, 771, 1000, 0, 0), (3, 9, 15, 2, 5), (1, 256, 129, 1, 3)])
 def test_few_rows_that_begin_anywhere(arb, rows, dim, hidden, pad, first, kept, dtype):
     layer = Layer(arb, rows, dim, hidden, dtype, kept=kept, pad=pad, first=first).forward().check_forward()
     if kept != "no":
