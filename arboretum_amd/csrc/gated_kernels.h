@@ -659,9 +659,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
   const int h0 = kApart ? blockIdx.x / 8 * 128 + blockIdx.x % 8 : blockIdx.x * 16;
   if (h0 >= a.hidden) return;
   const long long h = h0 + lane % 16 * kEach < a.hidden ? h0 + lane % 16 * kEach : h0, i = min(lane % 16ll, a.rows - 1);
-  const T *gate = static_cast<const T *>(a.w_gate) + h * a.w_stride, *up = static_cast<const T *>(a.w_up) + h * a.w_stride, *x = static_cast<const T *>(a.x) + i * a.x_stride;
   int head = 0;
   if (kApart) head = min((int)((16 - reinterpret_cast<uintptr_t>(static_cast<const T *>(a.w_gate) + h0 * a.w_stride) % 16) % 16 / sizeof(T)), a.dim);
+  const int at = head + quarter * kVec;
+  const T *gate = static_cast<const T *>(a.w_gate) + h * a.w_stride + at, *up = static_cast<const T *>(a.w_up) + h * a.w_stride + at;
+  const T *x = static_cast<const T *>(a.x) + i * a.x_stride + at;
   F4 g = {0, 0, 0, 0}, u = {0, 0, 0, 0};
   const int steps = (a.dim - head + kStep - 1) / kStep, groups = (a.dim - head) / kStep / kUnroll;
   const auto whole = [&](const T *from) { return __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const Pack<T, kVec> *>(from)); };
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
     Chunk<T> gs[kUnroll], us[kUnroll], xs[kUnroll];
 #pragma unroll
     for (int n = 0; n < kUnroll; ++n) {
-      const int k = head + (group * kUnroll + n) * kStep + quarter * kVec;
+      const int k = (group * kUnroll + n) * kStep;
       gs[n] = whole(gate + k);
       us[n] = whole(up + k);
       xs[n] = whole(x + k);
@@ -685,7 +687,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
   const bool first = kApart && wave == kFewWaves - 1;
   const int step = groups * kUnroll + wave;
   if (first ? head > 0 : step < steps) {
-    const int k = first ? 0 : head + step * kStep + quarter * kVec, held = !first ? a.dim - k : quarter == 0 ? head : 0;
+    const int k = first ? -at : step * kStep, held = !first ? a.dim - at - k : quarter == 0 ? head : 0;
     const auto part = [&](const T *from) {
       Chunk<T> c;
 #pragma unroll
