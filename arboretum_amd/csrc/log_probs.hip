@@ -706,11 +706,16 @@ void LogProbs(const LogProbsArgs &a) {
     }
     typedef std::true_type Yes;
     typedef std::false_type No;
+    // A wave a row, or four.  One has no barriers, four have more on its way and keep the likeliest among more maxima (bf16, us, one and four:
+    // 50,000 x 1000 top 10 63 and 294; 4000 x 8000 top 10 22 and 35, top 64 82 and 47; 4000 x 50,021 75 and 90, 1000 x 50,021 45 and 25; the parts of
+    // 1 x 131,072 top 20 22 and 18).
+    const size_t bytes = r.part * sizeof(T);
+    const bool wave = r.parts == 1 && (a.top > 32 ? bytes <= 2048 : bytes <= 16384 || (bytes <= 65536 && a.top <= 5 && l.n >= 4096));
     const auto launch = [&](auto side, auto entropy, auto top) {
       constexpr bool kSide = decltype(side)::value, kEntropy = decltype(entropy)::value, kTop = decltype(top)::value;
       const long long items = l.n * r.parts;
-      if (r.part <= 2048) hipLaunchKernelGGL((k_rows<T, 1, 1, kSide, kEntropy, kTop>), dim3(GridOf((items + 3) / 4)), dim3(256), 0, stream, r);
-      else hipLaunchKernelGGL((k_rows<T, 4, 4, kSide, kEntropy, kTop>), dim3(GridOf(items)), dim3(256), 0, stream, r);
+      if (wave) hipLaunchKernelGGL((k_rows<T, 1, 2, kSide, kEntropy, kTop>), dim3(GridOf((items + 3) / 4)), dim3(256), 0, stream, r);
+      else hipLaunchKernelGGL((k_rows<T, 4, 2, kSide, kEntropy, kTop>), dim3(GridOf(items)), dim3(256), 0, stream, r);
     };
     const auto launch_as = [&](auto side) {
       if (a.entropy && a.top) launch(side, Yes(), Yes());
