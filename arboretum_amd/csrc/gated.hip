@@ -10,13 +10,15 @@ namespace {
 // A product of `rows` x `columns` (`batch` of them) over `blocks` blocks of k's; half: a tile has half as many columns.  Large tiles, which read the LDS less for
 // each product, where they fill the chip, are not mostly beyond its columns, and have k's enough that their results are not most of the work (the layer
 // itself, small and large: 50000 x 100 x 300 27.9 and 31.4 us, 100000 x 256 x 512 77.5 and 78.1, 20000 x 1024 x 2048 173 and 151).  Else small ones, and few of them share out
-// their k's, at least `least` blocks to a share, until each half of a CU has one.
+// their k's until each half of a CU has one: at least `least` blocks to a share, and 24 where there are more than 64 shares, whose sums are written and read
+// again (200000 x 16 x 64, the gradient's last product in 64 and 128 shares: 114 and 105 us in all, float32 375 and 279; 100003 x 64 x 256 150 and 154).
 ProductCut CutOf(long long rows, long long columns, int half, long long batch, long long blocks, long long least) {
   const auto tiles = [&](long long i, long long j) { return Pieces(rows, i) * Pieces(columns, j / half) * batch; };
   const long long large = tiles(LargeTile::kI, LargeTile::kJ), small = tiles(SmallTile::kI, SmallTile::kJ);
   ProductCut c;
   c.large = large >= 200 && columns > SmallTile::kJ / half && blocks > 2;
-  const long long most = std::max<long long>(1, std::min({c.large ? 256 / large : 512 / std::max<long long>(small, 1), blocks / least, 64ll}));
+  const long long free = c.large ? 256 / large : 512 / std::max<long long>(small, 1);
+  const long long most = std::max<long long>(1, std::min(free, std::max(std::min(blocks / least, 64ll), std::min(blocks / 24, 128ll))));
   c.split_blocks = std::max<long long>(1, Pieces(blocks, most));
   c.splits = std::max<long long>(1, Pieces(blocks, c.split_blocks));
   return c;
@@ -33,7 +35,7 @@ struct Room {
 };
 
 // Rows whose chunks are not aligned come through registers into small tiles, a block at a time; copies of x and both weights are read and written once, a
-// launch of its own.  For the gradient (300 x 4095 x 4097: 153 us for grad_x without, 63 with copies) that is always less, for the layer itself, which reads
+// launch of its own.  For the gradient (300 x 4094 x 4098 with the layer itself: 251 us without, 186 with copies; 100 x 1002 x 1004 68 and 44) that is always less, for the layer itself, which reads
 // its weights along k, from some 400 rows on (300 of 4095 x 4097: 66.3 us without, 69.5 with; 500 of 1001 x 1003: 19.8 and 18.0; 8191: 57 and 41.6).
 LayerPad PadOf(long long rows, int dim, int hidden, size_t item, long long least_rows, Room *room) {
   LayerPad p{0, 0, 0, 0};
@@ -70,7 +72,7 @@ GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
   Room room;
   p.d_stride = Pieces(hidden, 64) * 64;
   p.x = CutOf(rows, dim, 1, 1, 2 * Pieces(hidden * item, kLineBytes), 8);
-  p.w = CutOf(hidden, dim, 1, 2, Pieces(rows * item, kLineBytes), 8);
+  p.w = CutOf(hidden, dim, 1, 2, Pieces(rows * item, kLineBytes), 4);
   p.d_gate = room.Take((size_t)rows * p.d_stride * item);
   p.d_up = room.Take((size_t)rows * p.d_stride * item);
   p.pad = PadOf(rows, dim, hidden, item, 1, &room);
