@@ -457,7 +457,7 @@ __device__ __forceinline__ void StoreSome(T *row, long long at, long long column
 
 // A lane's four values of each of four fragments that follow each other along a row: 64 columns from `at` on, between the four lanes of the row.  Elements of 16 and 8
 // bits: the four lanes first exchange what they have of two fragments, so that each has eight columns side by side, 64 (32) bytes of the row
-// between them in one store (100,003 x 64 x 256 kept as it is: 61 us with stores of four columns a lane).
+// between them in one store (100,003 x 64 x 256 kept as it is: 61 us with stores of four columns a lane, 46 so).
 template <typename T>
 __device__ __forceinline__ void StoreColumns(T *row, long long at, long long columns, const Pack<T, 4> (&v)[4]) {
   const int quarter = (threadIdx.x & 63) / 16;
@@ -541,7 +541,10 @@ __device__ __forceinline__ void Keep(void *kept, float *scales, long long stride
 
 static_assert(kWaveJ == 2 * kScaleGroup, "a wave holds whole groups");
 
-// A tile's columns are the gate's and up's of the same hidden ones: 64 of the gate and 64 of up for each wave.
+// A tile's columns are the gate's and up's of the same hidden ones: 64 of the gate and 64 of up for each wave, so that a lane ends with both of an element.
+// The matrix instructions and the power that they take bound large layers: 8192 x 4096 x 16384 bf16 in 1662 us, 1.32 PFLOP/s (a library's plain product of that
+// many operations 1.42), at 1.6 to 1.8 GHz, with the matrix units at work 60 to 66 % of the cycles; instructions of 32 x 32 x 16 took no less time and
+// lowered the clock further.  Narrow ones are bound by what ends a tile: 100,003 x 64 x 256 bf16 25 us (0.064 GB, 2.6 TB/s), keeping both in 8 bits 45.
 template <typename T, int kAct, typename S, bool kDirect>
 __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_gated(const Forward a, unsigned tiles, unsigned tile_rows, unsigned tile_columns) {
   __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_join(const Forward a, long l
 // Few rows (up to 16): 16 hidden columns a workgroup, whose eight waves share out the k's.  The weights are read once, from memory into the
 // registers that the products take them from: a lane's chunk is 16 bytes of a weight row, four steps of 64 bytes a row at once.
 // kApart: rows that begin anywhere.  Every eighth of them begins alike within 16 bytes, and the workgroup takes sixteen of those; behind as many k's as
-// the row's first 16 bytes hold its chunks are aligned.
+// the row's first 16 bytes hold its chunks are aligned.  Reading the weights bounds it: 1 x 4096 x 16384 bf16 48 us, 5.6 TB/s.
 constexpr int kFewWaves = 8;
 template <typename T, int kAct, bool kApart>
 __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
@@ -717,7 +720,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
   }
 }
 
-// Up to three matrices of rows that begin anywhere, to rows that begin at multiples of 64 elements, 0 behind each row's end.
+// Up to three matrices of rows that begin anywhere, to rows that begin at multiples of 64 elements, 0 behind each row's end.  (12 MB in rows of 771 fp16: 8 us; 290 MB
+// in rows of 3033 57, 5.1 TB/s.)
 struct Padded {
   const void *from[3];
   void *to[3];
@@ -749,6 +753,8 @@ __global__ void __launch_bounds__(kThreads) k_pad(const Padded a, long long bloc
   }
 }
 
+// Products of the gradient.  Operands that lie across are turned on their way from the LDS to the registers, by reads made for that, so neither is copied first.  The
+// matrix instructions and their power bound it as they do the layer: 4096 x 4096 x 16384 bf16, d_gate Wg + d_up Wu 840 us, 1.31 PFLOP/s, and both weights' 870, 1.26.
 template <typename T, bool kAcrossA, bool kAcrossB, typename S, bool kDirect>
 __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_products(const Products p, unsigned tiles, unsigned tile_rows, unsigned tile_columns) {
   __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
@@ -877,8 +883,11 @@ struct Slopes {
 
 constexpr int kSlopeVec = 8;
 
-// d_gate and d_up, rounded to the type of the products they enter; 0 in the columns from the layer's end to the next row.  A thread
-// has kSlopeVec columns of a row (d_stride is a multiple of 64).
+// d_gate and d_up; 0 in the columns from the layer's end to the next row.  A thread has kSlopeVec columns of a row (d_stride is a multiple of 64).
+// Both are rounded to the layer's type, which the matrix instructions of the products they enter take: half a step of each term, on top of the half
+// step that gate and up were kept at, which is what sets the gradients of 16-bit layers off (rms 3e-3 of their size in bf16, where products of float32
+// operands, rounded at the end, are off by 1.7e-3).  A second part for what rounding leaves would double the products' work.
+// Memory bounds it: 4096 x 16384 bf16, 0.67 GB, 121 us, 5.6 TB/s; from 8 bits, 100,003 x 256, 0.21 GB, 39 us.
 template <typename T, int kAct, bool kCodes>
 __global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks) {
   typedef std::conditional_t<kCodes, signed char, T> Kept;

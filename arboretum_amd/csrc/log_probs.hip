@@ -3,7 +3,9 @@
 //   log_prob = a_token - log S,   entropy = log S - (sum a_j exp a_j) / S,
 //   grad_j   = scale (g ([j = token] - p_j) - h p_j (log p_j + entropy)),   p_j = exp(a_j - log S).
 // A row is read once: maximum, S and sum a exp a run along it, and a new maximum scales what was summed before
-// (sum (a + d) exp (a + d) = exp d (sum a exp a + d sum exp a)).
+// (sum (a + d) exp (a + d) = exp d (sum a exp a + d sum exp a)).  The gradient reads the row once more: what must be known of all of it, the maximum and
+// log S, is kept in 8 bytes a row.  Reading and writing the logits bounds both (4096 x 131,072 bf16: 1 GiB read in 190 us, read and written in 360, 5.7 and 6.0
+// TB/s); with the likeliest tokens the search for them, where rows are short.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -173,12 +175,15 @@ __device__ __forceinline__ void WriteTop(const RowsArgs &a, const Sums &s, float
   WriteTop(a, s, log_sum, i, rank, ValueOf(key), IndexOf(key));
 }
 
-// ------------------------------------------------------------------ rows whose classes lie side by side
+// ------------------------------------------------------------------ a row a team
 
-// A team of kWaves waves reads a row, or a part of one; one wave a row: four teams a workgroup.
+// A team of kWaves waves reads a row, or a part of one; one wave a row: four teams a workgroup.  kSide: classes side by side, read 16 bytes a lane (777 x 50,021
+// fp16 20.4 us, 3.8 TB/s; rows of an odd length begin anywhere, and loads at less than four bytes' alignment take longer: 8192 x 50,021 bf16 171 us, x 50,024 145;
+// vectors from where 16 bytes begin would make a row's last bits depend on where it lies).
 // The likeliest tokens: every thread keeps the maximum of what it reads.  The k-th greatest of these maxima has k elements of the row on
 // its side, so the k likeliest are no less than it, and whatever is no less lies with the threads whose maxima are no less: about k
-// of 256, so that only their share of the row is read again.  (Where many are equal, as in a row of one value, more is.)
+// of 256, so that only their share of the row is read again.  (Where many are equal, as in a row of one value, more is.)  777 x 50,021 fp16 top 5: 26.7 us, 6
+// of them for this.
 template <typename T, int kWaves, int kUnroll, bool kSide, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const RowsArgs a) {
   constexpr int kVec = 16 / sizeof(T), kTeam = kWaves * 64, kTeams = kWaves == 1 ? 4 : 1, kChunk = kUnroll * kVec;
@@ -341,7 +346,8 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : kWaves * 64) k_rows(const 
   }
 }
 
-// The parts of a row, by one wave: a lane holds a part's sums and kEach of the parts' keys.
+// The parts of a row, by one wave: a lane holds a part's sums and kEach of the parts' keys.  (5 us for 16 parts of 20 keys: a launch and one chain of loads, sums
+// and choices, whatever the row.)
 template <typename T, int kEach>
 __global__ void __launch_bounds__(64) k_join(const RowsArgs a) {
   __shared__ Key s_top[kMostTop];
@@ -386,7 +392,7 @@ __global__ void __launch_bounds__(64) k_join(const RowsArgs a) {
 // ------------------------------------------------------------------ a row a thread
 
 // The greatest kHeld in one pass, in order; `top` beyond that takes further passes, each behind the last one found.  kUnroll classes
-// are asked for at once.
+// are asked for at once (kSide: side by side, in vectors).  Memory bounds it where the top is short: 1,000,003 x 10 fp32 class by class, top 3, 76 MB in 17.5 us, 4.3 TB/s.
 template <typename T, bool kSide, int kHeld, int kUnroll>
 __global__ void __launch_bounds__(256) k_columns(const RowsArgs a) {
   const long long step = (long long)gridDim.x * 256;
@@ -537,7 +543,7 @@ __device__ __forceinline__ T GradOfToken(const RowGrad &r, float factor, float x
   return Round<T>(g);
 }
 
-// Classes side by side: `lanes` threads of a workgroup take a row's piece of lanes * kVec * kUnroll classes.
+// Classes side by side: `lanes` threads of a workgroup take a row's piece of lanes * kVec * kUnroll classes.  4096 x 131,072 bf16, 2 GiB: 360 us, 6.0 TB/s.
 // (The gradient may take the place of the logits: what a thread writes only it has read.)
 template <typename T, int kUnroll, bool kEntropy, bool kPast>
 __global__ void __launch_bounds__(256) k_grad_rows(const GradArgs a, int lanes, unsigned pieces) {
@@ -620,7 +626,8 @@ __global__ void __launch_bounds__(256) k_grad_columns(const GradArgs a, unsigned
 
 // ------------------------------------------------------------------ the host
 
-// Few rows are cut into parts that fill the chip.
+// Few rows are cut into parts, two workgroups for a CU, of 16 KB of bf16 at least (bf16, us: 1 x 131,072 top 20 in 16 parts 17.7, in 4 20.5, in 32 31.7, whose keys
+// the join waits for; 100 x 131,072 top 5 in 5 parts 25.5, whole 28.2; 300 rows whole 32.0, in 3 parts 37.1).
 int PartsOf(long long n, long long vocab) {
   if (n <= 0 || n >= 256) return 1;
   return (int)std::max<long long>(1, std::min({(long long)kMostParts, 512 / n, (vocab + kPart - 1) / kPart}));
@@ -684,6 +691,9 @@ void LogProbs(const LogProbsArgs &a) {
              a.entropy, reinterpret_cast<float2 *>(a.stats), a.top, a.top_tokens, a.top_log_probs, l.status, 1, (unsigned)l.vocab, nullptr, nullptr};
   WithType(l.type, [&](auto type) {
     typedef decltype(type) T;
+    // A thread a row where they are many for what each does, and where rows side by side are short enough for lines to stay in the L1; else teams (fp32, us, a thread
+    // and teams: 64,000 x 10 top 5 14.9 and 55, 64,000 x 100 top 5 28 and 46, 16,000 x 100 top 5 25 and 14, 4000 x 100 top 20 92 and 14; 500,000 x 200
+    // side by side 261 and 185).
     if ((!side_by_side || l.vocab <= 128) && l.n / 32 >= l.vocab * std::max(a.top, 1)) {
       const dim3 grid(GridOf((l.n + 255) / 256));
       const auto columns = [&](auto held) {
@@ -769,7 +779,8 @@ void LogProbsGrad(const LogProbsGradArgs &a) {
         hipLaunchKernelGGL((k_grad_columns<T, kEntropy>), dim3(GridOf((l.n + 255) / 256), (unsigned)((l.vocab + part - 1) / part)), dim3(256), 0, stream, g, part);
         return;
       }
-      // threads of a row, or of as much of one as a workgroup takes: vectors of up to 32 threads one each, or four each
+      // threads of a row, or of as much of one as a workgroup takes: vectors of up to 32 threads one each, or four each (1,000,003 x 10 fp32 with the forward pass
+      // 39 us, with four a thread, which is a row a thread, 57)
       const auto rows = [&](auto unroll, auto past) {
         constexpr int kUnroll = decltype(unroll)::value, kEach = 16 / sizeof(T) * kUnroll;
         int lanes = kUnroll == 1 ? 32 : 256;
@@ -782,7 +793,7 @@ void LogProbsGrad(const LogProbsGradArgs &a) {
         if (l.vocab <= 32 * 16 / (long long)sizeof(T)) rows(std::integral_constant<int, 1>(), past);
         else rows(std::integral_constant<int, 4>(), past);
       };
-      // a gradient that the L2 caches do not hold is written past them
+      // a gradient that the L2 caches do not hold is written past them (4096 x 131,072 bf16: 491 us through them, 358 past)
       if ((size_t)l.n * l.vocab * sizeof(T) > kStreamedBytes) rows_of(std::true_type());
       else rows_of(std::false_type());
     };
