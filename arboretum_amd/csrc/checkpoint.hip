@@ -131,6 +131,7 @@ Shape ShapeOf(const CheckpointArgs &a) {
 void ActivationCheckpoint(const CheckpointArgs &a) {
   const Shape s = ShapeOf(a);
   if (a.rows == 0) return;
+  CheckApart({{a.codes, a.rows * a.dim}, {a.scales, s.groups * 4}}, {{a.x, a.rows, a.x_stride, a.dim, ElementBytes(a.type)}});
   OnDeviceOf device(a.codes);
   const long long blocks = (s.groups + kThreads / kLanes - 1) / (kThreads / kLanes);
   WithType(a.type, [&](auto type) {
@@ -144,6 +145,7 @@ void ActivationRestore(const CheckpointArgs &a) {
   const Shape s = ShapeOf(a);
   if (a.x_stride < a.dim && a.rows > 1) throw std::runtime_error("rows of x overlap");
   if (a.rows == 0) return;
+  CheckApart({{a.x, a.rows, a.x_stride, a.dim, ElementBytes(a.type)}}, {{a.codes, a.rows * a.dim}, {a.scales, s.groups * 4}});
   OnDeviceOf device(a.x);
   const long long blocks = (s.groups + kThreads / kLanes - 1) / (kThreads / kLanes);
   WithType(a.type, [&](auto type) {

@@ -126,6 +126,11 @@ void Gated(const GatedArgs &a) {
   CheckAligned(a.out, ElementBytes(l.type), "out");
   if (l.rows == 0) return;
   if (!a.out) throw std::runtime_error("null pointer argument");
+  const size_t item = ElementBytes(l.type), kept = l.gate_scales ? 1 : item;
+  const long long scales = l.rows * Pieces(l.hidden, kScaleGroup) * 4;
+  CheckApart({{a.out, l.rows, a.out_stride, l.hidden, item}, {l.gate, l.rows, l.kept_stride, l.hidden, kept}, {l.up, l.rows, l.kept_stride, l.hidden, kept},
+              {l.gate_scales, scales}, {l.up_scales, scales}, {l.work, (long long)plan.bytes}},
+             {{l.x, l.rows, l.x_stride, l.dim, item}, {l.w_gate, l.hidden, l.w_stride, l.dim, item}, {l.w_up, l.hidden, l.w_stride, l.dim, item}});
   OnDeviceOf device(a.out);
   WithType(l.type, [&](auto type) { RunGated<decltype(type)>(a, plan); });
 }
@@ -150,6 +155,13 @@ void GatedGrad(const GatedGradArgs &a) {
   if (a.grad_w_gate) CheckStride(a.grad_w_stride, l.dim, l.hidden, "the weights' gradients");
   if (l.rows > 0 && !a.grad_out) throw std::runtime_error("null pointer argument");
   if (!a.grad_w_gate && (!a.grad_x || l.rows == 0)) return;
+  const size_t kept = l.gate_scales ? 1 : item;
+  const long long scales = l.rows * Pieces(l.hidden, kScaleGroup) * 4;
+  CheckApart({{a.grad_x, l.rows, a.grad_x_stride, l.dim, item}, {a.grad_w_gate, l.hidden, a.grad_w_stride, l.dim, item},
+              {a.grad_w_up, l.hidden, a.grad_w_stride, l.dim, item}, {l.work, (long long)plan.bytes}},
+             {{a.grad_out, l.rows, a.grad_out_stride, l.hidden, item}, {l.x, l.rows, l.x_stride, l.dim, item}, {l.w_gate, l.hidden, l.w_stride, l.dim, item},
+              {l.w_up, l.hidden, l.w_stride, l.dim, item}, {l.gate, l.rows, l.kept_stride, l.hidden, kept}, {l.up, l.rows, l.kept_stride, l.hidden, kept},
+              {l.gate_scales, scales}, {l.up_scales, scales}});
   OnDeviceOf device(a.grad_w_gate ? a.grad_w_gate : a.grad_x);
   WithType(l.type, [&](auto type) { RunGatedGrad<decltype(type)>(a, plan); });
 }

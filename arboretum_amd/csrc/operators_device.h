@@ -63,6 +63,35 @@ inline void CheckAligned(const void *p, size_t bytes, const char *what) {
   if (reinterpret_cast<uintptr_t>(p) % bytes != 0) throw std::runtime_error(std::string(what) + " is not aligned to its elements");
 }
 
+// Memory of a call: `rows` pieces of `width` bytes, `stride` bytes from one to the next; nullptr: none.
+struct Extent {
+  const void *at;
+  long long rows, stride, width;
+  Extent(const void *p, long long bytes) : at(p), rows(bytes > 0), stride(bytes), width(bytes) {}
+  Extent(const void *p, long long n, long long elements, long long of, size_t item) : at(p), rows(of > 0 ? n : 0), stride(elements * (long long)item), width(of * (long long)item) {
+    if (stride < width) width += (rows - 1) * stride, rows = rows > 0, stride = width;  // (rows that share elements are one piece)
+  }
+};
+// Whether two places meet.  Rows as far apart in both may lie between each other, as the columns of one matrix do.
+inline bool DoMeet(const Extent &a, const Extent &b) {
+  if (!a.at || !b.at || a.rows == 0 || b.rows == 0) return false;
+  const long long pa = (long long)reinterpret_cast<uintptr_t>(a.at), pb = (long long)reinterpret_cast<uintptr_t>(b.at);
+  if (pb >= pa + (a.rows - 1) * a.stride + a.width || pa >= pb + (b.rows - 1) * b.stride + b.width) return false;
+  if (a.stride != b.stride || (a.rows == 1 && b.rows == 1)) return true;
+  const long long apart = ((pb - pa) % a.stride + a.stride) % a.stride;
+  return apart < a.width || apart + b.width > a.stride;
+}
+// What a call writes is apart from all else that it writes or reads: others' elements would be read before or after they are written, as it happens.
+template <size_t kWritten, size_t kRead>
+void CheckApart(const Extent (&written)[kWritten], const Extent (&read)[kRead]) {
+  for (size_t i = 0; i < kWritten; ++i) {
+    for (size_t j = 0; j < i; ++j)
+      if (DoMeet(written[i], written[j])) throw std::runtime_error("two outputs overlap");
+    for (const Extent &r : read)
+      if (DoMeet(written[i], r)) throw std::runtime_error("an output and an input overlap");
+  }
+}
+
 // Makes the device that `pointer` is on the current one for the length of a call.
 class OnDeviceOf {
  public:

@@ -191,3 +191,45 @@ def test_work_memory_of_ordinary_sizes(arb):
     assert arb.log_probs_bytes(1, 131_072, top=20) < 1 << 20
     # both rounded factors, rows apart by whole tiles, and shares of the products of at most a few outputs
     assert 2 * 8192 * 16384 * 2 <= arb.gated_grad_bytes(8192, 4096, 16384, dtype="bfloat16") < 3 * 8192 * 16384 * 2
+
+
+def test_outputs_that_meet_inputs_or_each_other(arb):
+    for name in ("logits", "tokens"):
+        refused(arb, logits, "an output and an input overlap", **{name: 5 * A})
+    refused(arb, logits, "two outputs overlap", entropy=A + 12)
+    refused(arb, logits, "two outputs overlap", top_tokens=8 * A - 44)
+    refused(arb, logits, "an output and an input overlap", logits=2 * A, log_probs=2 * A + 1596)
+    refused(arb, logits, "an output and an input overlap", logits=2 * A, row_stride=1, class_stride=4, log_probs=2 * A + 1584)
+    refused(arb, logits, "an output and an input overlap", status=3 * A + 4)
+    refused(arb, logits_grad, "an output and an input overlap", grad_logits=3 * A + 400)
+    for name in ("tokens", "stats", "grad_log_probs"):
+        refused(arb, logits_grad, "an output and an input overlap", **{name: A + 4 * 392})
+    refused(arb, keep, "an output and an input overlap", codes=3 * A + 1596)
+    refused(arb, keep, "two outputs overlap", codes=2 * A + 28)
+    refused(arb, read_back, "an output and an input overlap", x=2 * A - 1596)
+    for name in ("x", "w_gate", "w_up"):
+        refused(arb, layer, "an output and an input overlap", **{name: A})
+    refused(arb, layer, "two outputs overlap", gate=9 * A, up=9 * A)
+    refused(arb, layer, "two outputs overlap", gate=9 * A, up=A + 476)
+    refused(arb, layer, "two outputs overlap", gate=9 * A, up=10 * A, gate_scales=11 * A, up_scales=11 * A + 16)
+    for name in ("grad_out", "x", "w_gate", "w_up", "gate", "up"):
+        for output in (A, 2 * A, 3 * A, 8 * A):
+            refused(arb, layer_grad, "an output and an input overlap", **{name: output})
+    refused(arb, layer_grad, "two outputs overlap", grad_w_gate=3 * A)
+
+
+def test_rows_that_lie_between_each_other_do_not_meet(arb):
+    # the columns of one matrix: gate beside up, a result beside its input
+    if arb.device_count() == 0:
+        for call, change in [
+                (layer, dict(gate=9 * A, up=9 * A + 96, kept_stride=48)),
+                (layer, dict(out=2 * A + 64, out_stride=40, x_stride=40)),
+                (layer_grad, dict(grad_w_gate=2 * A, grad_w_up=2 * A + 64, grad_w_stride=32)),
+                (layer_grad, dict(x=A + 64, x_stride=32, grad_x_stride=32)),
+                (logits_grad, dict(grad_logits=3 * A + 400, row_stride=200)),
+                (logits_grad, dict(grad_logits=3 * A + 16, row_stride=1, class_stride=8)),
+                (keep, dict(codes=3 * A + 400 * 4)),
+                (read_back, dict(codes=A + 400 * 4))]:
+            refused(arb, call, "no HIP device", **change)
+        refused(arb, layer, "two outputs overlap", gate=9 * A, up=9 * A + 92, kept_stride=48)
+        refused(arb, layer, "two outputs overlap", gate=9 * A, up=9 * A + 100, kept_stride=48)
