@@ -538,3 +538,26 @@ def test_sizes_that_fill_the_chip(arb, rows, dim, hidden, dtype, pad, first, kep
     if kept != "no":
         layer.backward().check_backward()
     layer.check_margins()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,dim,hidden", [(3, 515, 200), (16, 77, 129), (40, 515, 70), (450, 65, 70)])
+def test_weights_that_begin_differently(arb, rows, dim, hidden, dtype):
+    layer = Layer(arb, rows, dim, hidden, dtype)
+    wu_buffer, layer.d_wu, _ = spread(layer.wu, 0, 3, float("nan"))
+    layer.forward().check_forward().backward().check_backward()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,dim,hidden", [(5, 48, 70), (300, 64, 128)])
+def test_gate_beside_up_in_one_matrix(arb, rows, dim, hidden, dtype):
+    alone, beside = (Layer(arb, rows, dim, hidden, dtype) for _ in range(2))
+    kept = torch.full((rows, 2 * hidden + 1), 7.0, dtype=TYPES[dtype], device="cuda")
+    grads = torch.full((hidden, 2 * dim + 3), 7.0, dtype=TYPES[dtype], device="cuda")
+    beside.gate, beside.up, beside.kept_stride = kept[:, :hidden], kept[:, hidden:2 * hidden], 2 * hidden + 1
+    beside.grad_wg, beside.grad_wu, beside.grad_w_stride = grads[:, :dim], grads[:, dim:2 * dim], 2 * dim + 3
+    for layer in (alone, beside):
+        layer.forward().backward()
+    for name in ("out", "gate", "up", "grad_x", "grad_wg", "grad_wu"):
+        assert torch.equal(getattr(alone, name), getattr(beside, name)), name
+    assert (kept[:, 2 * hidden:] == 7).all() and (grads[:, 2 * dim:] == 7).all()
