@@ -7,20 +7,23 @@
 namespace arb {
 namespace {
 
+constexpr int kPlaces = 256 * SmallTile::kEach;
+
 // A product of `rows` x `columns` (`batch` of them) over `blocks` blocks of k's; half: a tile has half as many columns.  Large tiles, which read the LDS less for
 // each product, where they fill the chip, are not mostly beyond its columns, and have k's enough that their results are not most of the work (the layer
 // itself, small and large: 50000 x 100 x 300 27.9 and 31.4 us, 100000 x 256 x 512 77.5 and 78.1, 20000 x 1024 x 2048 173 and 151).  Else small ones, and few of them share out
-// their k's until each half of a CU has one: at least `least` blocks to a share, and 24 where there are more than 64 shares, whose sums are written and read
+// their k's until `places` have one (of kPlaces, the halves of the CUs): at least `least` blocks to a share, and 24 where there are more than 64 shares, whose sums are written and read
 // again (200000 x 16 x 64, the gradient's last product in 64 and 128 shares: 114 and 105 us in all, float32 375 and 279; 100003 x 64 x 256 150 and 154).
-ProductCut CutOf(long long rows, long long columns, int half, long long batch, long long blocks, long long least) {
+ProductCut CutOf(long long rows, long long columns, int half, long long batch, long long blocks, long long least, int places) {
   const auto tiles = [&](long long i, long long j) { return Pieces(rows, i) * Pieces(columns, j / half) * batch; };
   const long long large = tiles(LargeTile::kI, LargeTile::kJ), small = tiles(SmallTile::kI, SmallTile::kJ);
   ProductCut c;
   c.large = large >= 200 && columns > SmallTile::kJ / half && blocks > 2;
-  const long long free = c.large ? 256 / large : 512 / std::max<long long>(small, 1);
+  const long long free = c.large ? 256 / large : places / std::max<long long>(small, 1);
   const long long most = std::max<long long>(1, std::min(free, std::max(std::min(blocks / least, 64ll), std::min(blocks / 24, 128ll))));
   c.split_blocks = std::max<long long>(1, Pieces(blocks, most));
   c.splits = std::max<long long>(1, Pieces(blocks, c.split_blocks));
+  c.tiles = (c.large ? large : small) * c.splits;
   return c;
 }
 
@@ -59,7 +62,7 @@ GatedPlan PlanOf(long long rows, int dim, int hidden, int type) {
   GatedPlan p;
   Room room;
   p.few = rows <= kFewRows;
-  p.out = CutOf(rows, hidden, 2, 1, Pieces(dim * item, kLineBytes), 4);
+  p.out = CutOf(rows, hidden, 2, 1, Pieces(dim * item, kLineBytes), 4, kPlaces);
   p.pad = PadOf(rows, dim, hidden, item, 400, &room);
   p.partial = room.Take(p.out.splits > 1 ? (size_t)p.out.splits * rows * Pieces(hidden, kScaleGroup) * kWaveJ * sizeof(float) : 0);
   p.bytes = room.bytes;
@@ -71,13 +74,18 @@ GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
   GatedGradPlan p;
   Room room;
   p.d_stride = Pieces(hidden, 64) * 64;
-  p.x = CutOf(rows, dim, 1, 1, 2 * Pieces(hidden * item, kLineBytes), 8);
-  p.w = CutOf(hidden, dim, 1, 2, Pieces(rows * item, kLineBytes), 4);
+  // Both products at once where a half of the places is enough for each, one after the other elsewhere.
+  for (const int places : {kPlaces / 2, kPlaces}) {
+    p.x = CutOf(rows, dim, 1, 1, 2 * Pieces(hidden * item, kLineBytes), 8, places);
+    p.w = CutOf(hidden, dim, 1, 2, Pieces(rows * item, kLineBytes), 4, places);
+    p.together = !p.x.large && !p.w.large && p.x.tiles + p.w.tiles <= kPlaces;
+    if (p.together) break;
+  }
   p.d_gate = room.Take((size_t)rows * p.d_stride * item);
   p.d_up = room.Take((size_t)rows * p.d_stride * item);
   p.pad = PadOf(rows, dim, hidden, item, 1, &room);
-  p.partial = room.Take(std::max<size_t>(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * sizeof(float) : 0,
-                                         p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * sizeof(float) : 0));
+  p.x_partial = room.Take(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * sizeof(float) : 0);
+  p.w_partial = room.Take(p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * sizeof(float) : 0);
   p.bytes = room.bytes;
   return p;
 }

@@ -187,6 +187,11 @@ __device__ __forceinline__ int RowOf(int line) {
   return kPaired ? line / 128 * 64 + line % 64 : line;
 }
 
+// Which tiles a workgroup takes: `first`, and every `of`th from there.
+struct Share {
+  unsigned first, of;
+};
+
 // An operand's blocks, run after run and tile after tile, each by loads that write to the LDS: for operands whose chunks are aligned and
 // whole.  A block costs its loads and next to nothing else: where a lane reads is worked out once a run.
 template <typename T, int kLines, int kThreads, bool kAcross, bool kPaired>
@@ -197,13 +202,14 @@ struct Stream {
   unsigned at[kPieces];
   unsigned long long base, second, step;
   int left, blocks, part;  // left: k's to the operand's end (2^30: or more)
-  unsigned id, lds;
+  unsigned id, further, lds;
   bool live;
 
   template <typename RunOf>
-  __device__ __forceinline__ void Start(const RunOf &run_of, unsigned tiles, int parts, long long stride) {
+  __device__ __forceinline__ void Start(const Share &share, const RunOf &run_of, unsigned tiles, int parts, long long stride) {
     step = kAcross ? (unsigned long long)kK * stride * sizeof(T) : kLineBytes;
-    id = blockIdx.x - gridDim.x;
+    further = share.of;
+    id = share.first - share.of;
     part = parts - 1;
     Next(run_of, tiles, parts, stride);
   }
@@ -213,7 +219,7 @@ struct Stream {
     do {
       if (++part == parts) {
         part = 0;
-        id += gridDim.x;
+        id += further;
       }
       live = id < tiles;
       if (!live) {  // what is asked for from here on is from nowhere
@@ -355,7 +361,7 @@ struct Tile {
 // those of the tiles that follow too while a tile's results are written.
 //   run_a(id, part), run_b: the runs of a tile, `parts` of them;  add(a, b);  end(id)
 template <bool kDirect, typename StreamA, typename StreamB, typename StageA, typename StageB, typename S, typename RunA, typename RunB, typename AddFn, typename EndFn>
-__device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts, long long stride_a, long long stride_b, const RunA &run_a, const RunB &run_b,
+__device__ __forceinline__ void RunTiles(LdsByte *lds, const Share &share, unsigned tiles, int parts, long long stride_a, long long stride_b, const RunA &run_a, const RunB &run_b,
                                          const AddFn &add, const EndFn &end) {
   constexpr int kA = S::kI * kLineBytes, kB = S::kJ * kLineBytes;
   if constexpr (kDirect) {
@@ -366,8 +372,8 @@ __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts
     const unsigned first = __builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)lds), first_b = first + S::kBlocksA * kA;
     StreamA a;
     StreamB b;
-    a.Start(run_a, tiles, parts, stride_a);
-    b.Start(run_b, tiles, parts, stride_b);
+    a.Start(share, run_a, tiles, parts, stride_a);
+    b.Start(share, run_b, tiles, parts, stride_b);
     if constexpr (kAheadB > kAheadA) b.Issue(first_b, run_b, tiles, parts, stride_b);
 #pragma unroll
     for (int n = 0; n < kAheadA; ++n) {
@@ -378,7 +384,7 @@ __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts
     const auto next_a = [&](unsigned at) { return at == first + kAheadA * kA ? first : at + kA; };
     const auto next_b = [&](unsigned at) { return at == first_b + kAheadB * kB ? first_b : at + kB; };
     bool landed = false;  // whether all loads have arrived
-    for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
+    for (unsigned id = share.first; id < tiles; id += share.of) {
       for (int part = 0; part < parts; ++part) {
         for (int n = run_b(id, part).blocks; n > 0; --n) {
           if (landed) Meet();
@@ -410,7 +416,7 @@ __device__ __forceinline__ void RunTiles(LdsByte *lds, unsigned tiles, int parts
     }
   } else {
     LdsByte *const to_b = lds + kA;
-    for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
+    for (unsigned id = share.first; id < tiles; id += share.of) {
       for (int part = 0; part < parts; ++part) {
         const Run of_a = run_a(id, part), of_b = run_b(id, part);
         StageA a;
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
     t.template Add<T, Layout<T, S::kI, false>, Layout<T, S::kJ, false>>(x, w, wave_i, wave_j, between);
   };
   RunTiles<kDirect, Stream<T, S::kI, S::kThreads, false, false>, Stream<T, S::kJ, S::kThreads, false, true>, Stage<T, S::kI, S::kThreads, false, false>,
-           Stage<T, S::kJ, S::kThreads, false, true>, S>((LdsByte *)s_blocks, tiles, 1, a.x_stride, a.w_stride, run_x, run_w, add, [&](unsigned id) {
+           Stage<T, S::kJ, S::kThreads, false, true>, S>((LdsByte *)s_blocks, Share{blockIdx.x, gridDim.x}, tiles, 1, a.x_stride, a.w_stride, run_x, run_w, add, [&](unsigned id) {
     const At at = at_of(id);
     const int h = at.h0 + wave_j * (kWaveJ / 2);
 #pragma unroll
@@ -753,11 +759,15 @@ __global__ void __launch_bounds__(kThreads) k_pad(const Padded a, long long bloc
   }
 }
 
+// What a product's tiles are, and how many.
+struct TilesOf {
+  unsigned all, rows, columns;
+};
+
 // Products of the gradient.  Operands that lie across are turned on their way from the LDS to the registers, by reads made for that, so neither is copied first.  The
 // matrix instructions and their power bound it as they do the layer: 4096 x 4096 x 16384 bf16, d_gate Wg + d_up Wu 840 us, 1.31 PFLOP/s, and both weights' 870, 1.26.
 template <typename T, bool kAcrossA, bool kAcrossB, typename S, bool kDirect>
-__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_products(const Products p, unsigned tiles, unsigned tile_rows, unsigned tile_columns) {
-  __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
+__device__ __forceinline__ void RunProducts(LdsByte *lds, const Share &share, const Products &p, const TilesOf &tiles) {
   constexpr int kK = kLineBytes / sizeof(T);
   const long long segment_blocks = (p.inner + kK - 1) / kK;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_i = wave % (S::kI / S::kWaveI), wave_j = wave / (S::kI / S::kWaveI);
@@ -767,9 +777,9 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
   };
   const auto at_of = [&](unsigned id) {
     At at;
-    const unsigned each = tile_rows * tile_columns, place = PlaceOfTile(id, tiles), one = place / each, member = one / (unsigned)p.splits;
+    const unsigned each = tiles.rows * tiles.columns, place = PlaceOfTile(id, tiles.all), one = place / each, member = one / (unsigned)p.splits;
     unsigned i, j;
-    PlaceInGroup(place - one * each, tile_rows, tile_columns, &i, &j);
+    PlaceInGroup(place - one * each, tiles.rows, tiles.columns, &i, &j);
     at.i0 = (long long)i * S::kI;
     at.j0 = j * S::kJ;
     at.one = one;
@@ -798,7 +808,7 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
     t.template Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(of_a, of_b, wave_i, wave_j, between);
   };
   RunTiles<kDirect, Stream<T, S::kI, S::kThreads, kAcrossA, false>, Stream<T, S::kJ, S::kThreads, kAcrossB, false>, Stage<T, S::kI, S::kThreads, kAcrossA, false>,
-           Stage<T, S::kJ, S::kThreads, kAcrossB, false>, S>((LdsByte *)s_blocks, tiles, p.segments, p.a.stride, p.b.stride, run_a, run_b, add, [&](unsigned id) {
+           Stage<T, S::kJ, S::kThreads, kAcrossB, false>, S>(lds, share, tiles.all, p.segments, p.a.stride, p.b.stride, run_a, run_b, add, [&](unsigned id) {
     const At at = at_of(id);
 #pragma unroll
     for (int i = 0; i < S::kWaveI / 16; ++i) {
@@ -815,17 +825,34 @@ __global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_e
   });
 }
 
+template <typename T, bool kAcrossA, bool kAcrossB, typename S, bool kDirect>
+__global__ void __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(S::kWavesEach, S::kWavesEach))) k_products(const Products p, const TilesOf tiles) {
+  __shared__ __align__(16) unsigned char s_blocks[kDirect ? S::kLdsBytes : (S::kI + S::kJ) * kLineBytes];
+  RunProducts<T, kAcrossA, kAcrossB, S, kDirect>((LdsByte *)s_blocks, Share{blockIdx.x, gridDim.x}, p, tiles);
+}
+
+// grad_x and the weights' gradients side by side, `x_groups` workgroups for the first, where all tiles of both have a place on the chip at once: a layer that
+// small waits for its loads, not for what it shares with the other (bf16, forward and gradient, one after the other and so: 1003 x 771 x 2055 93 and 71 us,
+// 2000 x 300 x 500 53 and 41, 3000 x 1000 x 1000 88 and 68).
+template <typename T>
+__global__ void __launch_bounds__(SmallTile::kThreads) __attribute__((amdgpu_waves_per_eu(SmallTile::kWavesEach, SmallTile::kWavesEach)))
+k_both_products(const Products x, const TilesOf x_tiles, unsigned x_groups, const Products w, const TilesOf w_tiles) {
+  __shared__ __align__(16) unsigned char s_blocks[SmallTile::kLdsBytes];
+  if (blockIdx.x < x_groups) RunProducts<T, false, true, SmallTile, true>((LdsByte *)s_blocks, Share{blockIdx.x, x_groups}, x, x_tiles);
+  else RunProducts<T, true, true, SmallTile, true>((LdsByte *)s_blocks, Share{blockIdx.x - x_groups, gridDim.x - x_groups}, w, w_tiles);
+}
+
 // The sums of what was shared out, in an order that depends on the sizes alone: four elements side by side a thread, or many shares by kShares threads,
 // each with every kShares-th of them.  (Many shares mean few elements: 63 of 2 x 256 x 64 by a thread each take 17.7 us, by eight 5.)
 template <typename T, int kShares>
-__global__ void __launch_bounds__(kThreads) k_products_join(const Products p) {
+__device__ __forceinline__ void JoinProducts(const Share &share_of, const Products &p) {
   constexpr int kVec = kShares == 1 ? 4 : 1, kElements = kThreads / kShares * kVec;
   __shared__ float s_sums[kShares][kShares == 1 ? 1 : kElements];
-  const long long each = p.rows * p.columns, step = (long long)gridDim.x * kElements;
+  const long long each = p.rows * p.columns, step = (long long)share_of.of * kElements;
   const int in = threadIdx.x % (kThreads / kShares) * kVec, share = threadIdx.x / (kThreads / kShares);
   for (int member = 0; member < p.batch; ++member) {
     T *c = static_cast<T *>(p.c[member]);
-    for (long long first = (long long)blockIdx.x * kElements; first < each; first += step) {
+    for (long long first = (long long)share_of.first * kElements; first < each; first += step) {
       const long long at = first + in;
       const float *from = p.partial + (long long)member * p.splits * each + at;
       const int held = (int)max(0ll, min(each - at, (long long)kVec));
@@ -866,6 +893,19 @@ __global__ void __launch_bounds__(kThreads) k_products_join(const Products p) {
       }
     }
   }
+}
+
+constexpr int kManyShares = 16;
+
+// Of one product, or of two: `groups` workgroups for the first.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_products_join(const Products first, unsigned groups, const Products second) {
+  const auto join = [](const Share &share, const Products &p) {
+    if (p.splits >= kManyShares) JoinProducts<T, 8>(share, p);
+    else JoinProducts<T, 1>(share, p);
+  };
+  if (blockIdx.x < groups) join(Share{blockIdx.x, groups}, first);
+  else join(Share{blockIdx.x - groups, gridDim.x - groups}, second);
 }
 
 // ------------------------------------------------------------------ the layer's own gradient
@@ -964,21 +1004,29 @@ inline unsigned CheckedTiles(long long tiles) {
   return (unsigned)tiles;
 }
 
+template <typename S>
+TilesOf TilesFor(const Products &p) {
+  const long long rows = Pieces(p.rows, S::kI), columns = Pieces(p.columns, S::kJ);
+  return TilesOf{CheckedTiles(rows * columns * p.batch * p.splits), (unsigned)rows, (unsigned)columns};
+}
+
+// Workgroups for the joining of a product's shares; 0 where there are none.
+inline unsigned JoinGroups(const Products &p) {
+  if (p.splits <= 1) return 0;
+  return (unsigned)std::min(Pieces(p.rows * p.columns, p.splits >= kManyShares ? kThreads / 8 : kThreads * 4), kMostGrid);
+}
+
 template <typename T, bool kAcrossA, bool kAcrossB>
 void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   const auto launch = [&](auto shape, auto is_direct) {
     typedef decltype(shape) S;
-    const long long tile_rows = Pieces(p.rows, S::kI), tiles = tile_rows * Pieces(p.columns, S::kJ) * p.batch * p.splits;
-    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3((unsigned)std::min(tiles, kCus * S::kEach)), dim3(S::kThreads), 0, stream, p,
-                       CheckedTiles(tiles), (unsigned)tile_rows, (unsigned)Pieces(p.columns, S::kJ));
+    const TilesOf tiles = TilesFor<S>(p);
+    hipLaunchKernelGGL((k_products<T, kAcrossA, kAcrossB, S, decltype(is_direct)::value>), dim3(std::min(tiles.all, (unsigned)(kCus * S::kEach))), dim3(S::kThreads), 0, stream, p, tiles);
   };
   if (large && direct) launch(LargeTile(), std::true_type());
   else if (direct) launch(SmallTile(), std::true_type());
   else launch(SmallTile(), std::false_type());
-  if (p.splits <= 1) return;
-  const long long elements = p.rows * p.columns;
-  if (p.splits >= 16) hipLaunchKernelGGL((k_products_join<T, 8>), dim3((unsigned)std::min(Pieces(elements, kThreads / 8), kMostGrid)), dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((k_products_join<T, 1>), dim3((unsigned)std::min(Pieces(elements, kThreads * 4), kMostGrid)), dim3(kThreads), 0, stream, p);
+  if (const unsigned groups = JoinGroups(p)) hipLaunchKernelGGL((k_products_join<T>), dim3(groups), dim3(kThreads), 0, stream, p, groups, p);
 }
 
 // x and the two weights in rows that begin at multiples of 64 elements, where the plan has room for that and any of them needs it.
@@ -1046,7 +1094,6 @@ void RunGatedGrad(const GatedGradArgs &a, const GatedGradPlan &plan) {
   const hipStream_t stream = static_cast<hipStream_t>(l.stream);
   unsigned char *work = static_cast<unsigned char *>(l.work);
   void *d_gate = work + plan.d_gate, *d_up = work + plan.d_up;
-  float *partial = reinterpret_cast<float *>(work + plan.partial);
   if (l.rows > 0) {
     const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden};
     const long long blocks = Pieces(l.rows * (plan.d_stride / kSlopeVec), kThreads);
@@ -1061,15 +1108,20 @@ void RunGatedGrad(const GatedGradArgs &a, const GatedGradPlan &plan) {
   const long long extent = padded ? plan.pad.stride : l.dim;
   const Operand d{{d_gate, d_up}, plan.d_stride};
   const bool d_direct = IsDirect<T>(d_gate, plan.d_stride, plan.d_stride);
-  if (a.grad_x && l.rows > 0) {
-    const Products p{d, {{l.w_gate, l.w_up}, l.w_stride}, l.rows, l.dim, l.hidden, 2, 1, {a.grad_x, nullptr}, a.grad_x_stride,
-                     (int)plan.x.splits, plan.x.split_blocks, partial};
-    Launch<T, false, true>(p, plan.x.large, d_direct && IsDirect<T>(l.w_gate, l.w_stride, extent) && IsDirect<T>(l.w_up, l.w_stride, extent), stream);
-  }
-  if (a.grad_w_gate) {
-    const Products p{d, {{l.x, l.x}, l.x_stride}, l.hidden, l.dim, l.rows, 1, 2, {a.grad_w_gate, a.grad_w_up}, a.grad_w_stride,
-                     (int)plan.w.splits, plan.w.split_blocks, partial};
-    Launch<T, true, true>(p, plan.w.large, d_direct && IsDirect<T>(l.x, l.x_stride, extent), stream);
+  const Products x{d, {{l.w_gate, l.w_up}, l.w_stride}, l.rows, l.dim, l.hidden, 2, 1, {a.grad_x, nullptr}, a.grad_x_stride,
+                   (int)plan.x.splits, plan.x.split_blocks, reinterpret_cast<float *>(work + plan.x_partial)};
+  const Products w{d, {{l.x, l.x}, l.x_stride}, l.hidden, l.dim, l.rows, 1, 2, {a.grad_w_gate, a.grad_w_up}, a.grad_w_stride,
+                   (int)plan.w.splits, plan.w.split_blocks, reinterpret_cast<float *>(work + plan.w_partial)};
+  const bool x_direct = d_direct && IsDirect<T>(l.w_gate, l.w_stride, extent) && IsDirect<T>(l.w_up, l.w_stride, extent);
+  const bool w_direct = d_direct && IsDirect<T>(l.x, l.x_stride, extent), wants_x = a.grad_x && l.rows > 0;
+  if (plan.together && wants_x && a.grad_w_gate && x_direct && w_direct) {
+    const TilesOf x_tiles = TilesFor<SmallTile>(x), w_tiles = TilesFor<SmallTile>(w);
+    hipLaunchKernelGGL((k_both_products<T>), dim3(x_tiles.all + w_tiles.all), dim3(SmallTile::kThreads), 0, stream, x, x_tiles, x_tiles.all, w, w_tiles);
+    const unsigned x_groups = JoinGroups(x), w_groups = JoinGroups(w);
+    if (x_groups + w_groups > 0) hipLaunchKernelGGL((k_products_join<T>), dim3(x_groups + w_groups), dim3(kThreads), 0, stream, x, x_groups, w);
+  } else {
+    if (wants_x) Launch<T, false, true>(x, plan.x.large, x_direct, stream);
+    if (a.grad_w_gate) Launch<T, true, true>(w, plan.w.large, w_direct, stream);
   }
   HIP_OK(hipGetLastError());
 }

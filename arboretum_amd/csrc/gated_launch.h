@@ -27,7 +27,7 @@ typedef TileShape<4, 1, 32, 2, 3> SmallTile;  // 128 x 128, two to a CU.  Four w
 // How a product is cut up: into which tiles, and how many shares of its k's (blocks of kLineBytes of them).
 struct ProductCut {
   bool large;
-  long long splits, split_blocks;
+  long long splits, split_blocks, tiles;  // tiles: of all shares
 };
 // Where in the work memory (bytes from its start) copies of x and the weights lie whose rows begin at multiples of 64 elements;
 // stride 0: there are none.
@@ -44,8 +44,9 @@ struct GatedPlan {
 struct GatedGradPlan {
   long long d_stride;  // elements between rows of d_gate and of d_up
   ProductCut x, w;     // of grad_x, of the weights' gradients
+  bool together;       // all tiles of both have a place on the chip at once
   LayerPad pad;
-  size_t d_gate, d_up, partial, bytes;
+  size_t d_gate, d_up, x_partial, w_partial, bytes;
 };
 
 inline long long Pieces(long long n, long long of) { return (n + of - 1) / of; }
