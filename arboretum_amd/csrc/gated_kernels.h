@@ -733,21 +733,25 @@ struct Padded {
   void *to[3];
   long long rows[3], from_stride[3];
   int width;
-  long long to_stride;
+  long long to_stride, blocks;  // blocks: of kThreads vectors
 };
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_pad(const Padded a, long long blocks) {
+__device__ __forceinline__ void PadRows(const Share &share, const Padded &a) {
   constexpr int kVec = 8;
   const unsigned vectors = (unsigned)(a.to_stride / kVec);
-  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
+  for (long long block = share.first; block < a.blocks; block += share.of) {
     const long long first = block * kThreads, row0 = first / vectors;
     const unsigned in = (unsigned)(first - row0 * vectors) + threadIdx.x, more = in / vectors;
     long long row = row0 + more;
-    int which = 0;
-    while (which < 3 && row >= a.rows[which]) row -= a.rows[which++];
-    if (which == 3) continue;
+    // (no index that is not a constant: such a one puts the arguments into scratch memory)
+    const void *of = a.from[0];
+    void *to = a.to[0];
+    long long stride = a.from_stride[0];
+    if (row >= a.rows[0]) row -= a.rows[0], of = a.from[1], to = a.to[1], stride = a.from_stride[1];
+    if (to == a.to[1] && row >= a.rows[1]) row -= a.rows[1], of = a.from[2], to = a.to[2], stride = a.from_stride[2];
+    if (to == a.to[2] && row >= a.rows[2]) continue;
     const int at = (int)(in - more * vectors) * kVec, held = a.width - at;
-    const T *from = static_cast<const T *>(a.from[which]) + row * a.from_stride[which] + at;
+    const T *from = static_cast<const T *>(of) + row * stride + at;
     Pack<T, kVec> p;
     if (held >= kVec) {
       p = *reinterpret_cast<const Pack<T, kVec> *>(from);
@@ -755,8 +759,12 @@ __global__ void __launch_bounds__(kThreads) k_pad(const Padded a, long long bloc
 #pragma unroll
       for (int c = 0; c < kVec; ++c) p.v[c] = c < held ? from[c] : T(0);
     }
-    *reinterpret_cast<Pack<T, kVec> *>(static_cast<T *>(a.to[which]) + row * a.to_stride + at) = p;
+    *reinterpret_cast<Pack<T, kVec> *>(static_cast<T *>(to) + row * a.to_stride + at) = p;
   }
+}
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_pad(const Padded a) {
+  PadRows<T>(Share{blockIdx.x, gridDim.x}, a);
 }
 
 // What a product's tiles are, and how many.
@@ -928,11 +936,16 @@ constexpr int kSlopeVec = 8;
 // step that gate and up were kept at, which is what sets the gradients of 16-bit layers off (rms 3e-3 of their size in bf16, where products of float32
 // operands, rounded at the end, are off by 1.7e-3).  A second part for what rounding leaves would double the products' work.
 // Memory bounds it: 4096 x 16384 bf16, 0.67 GB, 121 us, 5.6 TB/s; from 8 bits, 100,003 x 256, 0.21 GB, 39 us.
+// Workgroups from `groups` on copy to aligned rows what the products need there.
 template <typename T, int kAct, bool kCodes>
-__global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks) {
+__global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks, unsigned groups, const Padded pad) {
   typedef std::conditional_t<kCodes, signed char, T> Kept;
   const unsigned vectors = (unsigned)(a.d_stride / kSlopeVec);
-  for (long long block = blockIdx.x; block < blocks; block += gridDim.x) {
+  if (blockIdx.x >= groups) {
+    PadRows<T>(Share{blockIdx.x - groups, gridDim.x - groups}, pad);
+    return;
+  }
+  for (long long block = blockIdx.x; block < blocks; block += groups) {
     const long long first = block * kThreads, row0 = first / vectors;
     const unsigned in = (unsigned)(first - row0 * vectors) + threadIdx.x, more = in / vectors;
     const long long row = row0 + more;
@@ -1029,20 +1042,20 @@ void Launch(const Products &p, bool large, bool direct, hipStream_t stream) {
   if (const unsigned groups = JoinGroups(p)) hipLaunchKernelGGL((k_products_join<T>), dim3(groups), dim3(kThreads), 0, stream, p, groups, p);
 }
 
-// x and the two weights in rows that begin at multiples of 64 elements, where the plan has room for that and any of them needs it.
-template <typename T>
-bool Pad(GatedLayer *l, const LayerPad &pad, bool x, bool weights, unsigned char *work) {
-  if (pad.stride == 0) return false;
+// x and the two weights in rows that begin at multiples of 64 elements, where the plan has room for that: how they get there, with the layer's pointers set to
+// them.  (No blocks: nowhere.)
+inline Padded PadOf(GatedLayer *l, const LayerPad &pad, bool x, bool weights, unsigned char *work) {
+  if (pad.stride == 0) return Padded{};
   Padded p{{l->x, l->w_gate, l->w_up}, {work + pad.x, work + pad.w_gate, work + pad.w_up}, {x ? l->rows : 0, weights ? l->hidden : 0, weights ? l->hidden : 0},
-           {l->x_stride, l->w_stride, l->w_stride}, l->dim, pad.stride};
-  const long long blocks = Pieces((p.rows[0] + p.rows[1] + p.rows[2]) * (pad.stride / 8), kThreads);
-  hipLaunchKernelGGL((k_pad<T>), dim3((unsigned)std::min(blocks, kMostGrid)), dim3(kThreads), 0, static_cast<hipStream_t>(l->stream), p, blocks);
+           {l->x_stride, l->w_stride, l->w_stride}, l->dim, pad.stride, 0};
+  p.blocks = Pieces((p.rows[0] + p.rows[1] + p.rows[2]) * (pad.stride / 8), kThreads);
   l->x = p.to[0];
   l->w_gate = p.to[1];
   l->w_up = p.to[2];
   l->x_stride = l->w_stride = pad.stride;
-  return true;
+  return p;
 }
+inline unsigned GroupsOf(const Padded &p) { return (unsigned)std::min(p.blocks, kMostGrid); }
 
 }  // namespace
 
@@ -1052,8 +1065,9 @@ void RunGated(const GatedArgs &a, const GatedPlan &plan) {
   const hipStream_t stream = static_cast<hipStream_t>(l.stream);
   unsigned char *work = static_cast<unsigned char *>(l.work);
   const bool few = plan.few && !l.gate_scales;
-  const bool padded = !few && Pad<T>(&l, plan.pad, true, true, work);
-  const long long extent = padded ? plan.pad.stride : l.dim;
+  const Padded pad = few ? Padded{} : PadOf(&l, plan.pad, true, true, work);
+  if (pad.blocks > 0) hipLaunchKernelGGL((k_pad<T>), dim3(GroupsOf(pad)), dim3(kThreads), 0, stream, pad);
+  const long long extent = pad.blocks > 0 ? plan.pad.stride : l.dim;
   const bool direct = IsDirect<T>(l.x, l.x_stride, extent) && IsDirect<T>(l.w_gate, l.w_stride, extent) && IsDirect<T>(l.w_up, l.w_stride, extent);
   const Forward f{l.x, l.w_gate, l.w_up, l.rows, l.dim, l.hidden, l.x_stride, l.w_stride, a.out, a.out_stride, l.gate, l.up, l.gate_scales,
                   l.up_scales, l.kept_stride, (int)plan.out.splits, plan.out.split_blocks, reinterpret_cast<float *>(work + plan.partial)};
@@ -1094,18 +1108,19 @@ void RunGatedGrad(const GatedGradArgs &a, const GatedGradPlan &plan) {
   const hipStream_t stream = static_cast<hipStream_t>(l.stream);
   unsigned char *work = static_cast<unsigned char *>(l.work);
   void *d_gate = work + plan.d_gate, *d_up = work + plan.d_up;
+  const Padded pad = PadOf(&l, plan.pad, a.grad_w_gate != nullptr, a.grad_x != nullptr, work);
+  const long long extent = pad.blocks > 0 ? plan.pad.stride : l.dim;
   if (l.rows > 0) {
     const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden};
     const long long blocks = Pieces(l.rows * (plan.d_stride / kSlopeVec), kThreads);
-    const dim3 grid((unsigned)std::min(blocks, kMostGrid));
+    const unsigned groups = (unsigned)std::min(blocks, kMostGrid);
+    const dim3 grid(groups + GroupsOf(pad));
     WithActivation(l.activation, [&](auto act) {
       constexpr int kAct = decltype(act)::value;
-      if (l.gate_scales) hipLaunchKernelGGL((k_slopes<T, kAct, true>), grid, dim3(kThreads), 0, stream, s, blocks);
-      else hipLaunchKernelGGL((k_slopes<T, kAct, false>), grid, dim3(kThreads), 0, stream, s, blocks);
+      if (l.gate_scales) hipLaunchKernelGGL((k_slopes<T, kAct, true>), grid, dim3(kThreads), 0, stream, s, blocks, groups, pad);
+      else hipLaunchKernelGGL((k_slopes<T, kAct, false>), grid, dim3(kThreads), 0, stream, s, blocks, groups, pad);
     });
   }
-  const bool padded = Pad<T>(&l, plan.pad, a.grad_w_gate != nullptr, a.grad_x != nullptr, work);
-  const long long extent = padded ? plan.pad.stride : l.dim;
   const Operand d{{d_gate, d_up}, plan.d_stride};
   const bool d_direct = IsDirect<T>(d_gate, plan.d_stride, plan.d_stride);
   const Products x{d, {{l.w_gate, l.w_up}, l.w_stride}, l.rows, l.dim, l.hidden, 2, 1, {a.grad_x, nullptr}, a.grad_x_stride,
