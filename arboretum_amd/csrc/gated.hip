@@ -37,17 +37,24 @@ struct Room {
   }
 };
 
-// Rows whose chunks are not aligned come through registers into small tiles, a block at a time; copies of x and both weights are read and written once, a
-// launch of its own.  For the gradient (300 x 4094 x 4098 with the layer itself: 251 us without, 186 with copies; 100 x 1002 x 1004 68 and 44) that is always less, for the layer itself, which reads
-// its weights along k, from some 400 rows on (300 of 4095 x 4097: 66.3 us without, 69.5 with; 500 of 1001 x 1003: 19.8 and 18.0; 8191: 57 and 41.6).
-LayerPad PadOf(long long rows, int dim, int hidden, size_t item, long long least_rows, Room *room) {
+// Rows whose chunks are not aligned come through registers into small tiles, a block at a time; copies of x and both weights are read and written once.  For the
+// gradient (300 x 4094 x 4098 with the layer itself: 251 us without, 186 with copies; 100 x 1002 x 1004 68 and 44) the copies are always less.
+LayerPad PadOf(long long rows, int dim, int hidden, size_t item, Room *room) {
   LayerPad p{0, 0, 0, 0};
-  if (dim * item % 16 == 0 || rows < least_rows) return p;
+  if (dim * item % 16 == 0 || rows == 0) return p;
   p.stride = Pieces(dim, 64) * 64;
   p.x = room->Take((size_t)rows * p.stride * item);
   p.w_gate = room->Take((size_t)hidden * p.stride * item);
   p.w_up = room->Take((size_t)hidden * p.stride * item);
   return p;
+}
+
+// Whether the layer itself, which reads its weights along k, copies too: a block through registers takes 1.3 us more, the last one of a row three times that, copies a launch of
+// 5 us and their bytes at 5 TB/s (us without and with: 40 x 4095 x 16383 92 and 175, 300 x 4095 x 4097 66 and 69, 500 x 1001 x 1003 20 and 18, 8191 x 1001 x 1003
+// 57 and 42, 100,003 x 63 x 255 70 and 49, 280 x 7353 x 11442 380 and 297).
+bool CopiesForward(const ProductCut &c, long long rows, int dim, int hidden, size_t item) {
+  const long long turns = Pieces(Pieces(rows, SmallTile::kI) * Pieces(hidden, SmallTile::kJ / 2) * c.splits, kPlaces);
+  return 1.3 * turns * (c.split_blocks + 2) > 5.0 + 2.0 * (rows + 2.0 * hidden) * dim * item / 5.0e6;
 }
 
 void CheckLayerSizes(long long rows, int dim, int hidden, int type) {
@@ -63,7 +70,7 @@ GatedPlan PlanOf(long long rows, int dim, int hidden, int type) {
   Room room;
   p.few = rows <= kFewRows;
   p.out = CutOf(rows, hidden, 2, 1, Pieces(dim * item, kLineBytes), 4, kPlaces);
-  p.pad = PadOf(rows, dim, hidden, item, 400, &room);
+  p.pad = CopiesForward(p.out, rows, dim, hidden, item) ? PadOf(rows, dim, hidden, item, &room) : LayerPad{0, 0, 0, 0};
   p.partial = room.Take(p.out.splits > 1 ? (size_t)p.out.splits * rows * Pieces(hidden, kScaleGroup) * kWaveJ * sizeof(float) : 0);
   p.bytes = room.bytes;
   return p;
@@ -83,7 +90,7 @@ GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
   }
   p.d_gate = room.Take((size_t)rows * p.d_stride * item);
   p.d_up = room.Take((size_t)rows * p.d_stride * item);
-  p.pad = PadOf(rows, dim, hidden, item, 1, &room);
+  p.pad = PadOf(rows, dim, hidden, item, &room);
   p.x_partial = room.Take(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * sizeof(float) : 0);
   p.w_partial = room.Take(p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * sizeof(float) : 0);
   p.bytes = room.bytes;
