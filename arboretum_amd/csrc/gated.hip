@@ -90,6 +90,7 @@ GatedGradPlan GradPlanOf(long long rows, int dim, int hidden, int type) {
   }
   p.d_gate = room.Take((size_t)rows * p.d_stride * item);
   p.d_up = room.Take((size_t)rows * p.d_stride * item);
+  p.range = room.Take(type == kFloat16 && rows > 0 ? (1 + kRangeGroups) * sizeof(float) : 0);
   p.pad = PadOf(rows, dim, hidden, item, &room);
   p.x_partial = room.Take(p.x.splits > 1 ? (size_t)p.x.splits * rows * dim * sizeof(float) : 0);
   p.w_partial = room.Take(p.w.splits > 1 ? (size_t)p.w.splits * 2 * hidden * dim * sizeof(float) : 0);

@@ -103,7 +103,12 @@ struct Products {
   int splits;
   long long split_blocks;  // blocks of k's of each
   float *partial;          // [batch][splits][rows][columns] where there are several
+  const float *undo;       // what sums are multiplied with (a power of two), float16 only; may be null
 };
+template <typename T>
+__device__ __forceinline__ float UndoOf(const Products &p) {
+  return std::is_same_v<T, _Float16> && p.undo != nullptr ? *p.undo : 1.0f;
+}
 
 constexpr unsigned kNowhere = 0x80000000u;  // offset beyond every operand: a load from there gives 0
 
@@ -812,6 +817,7 @@ __device__ __forceinline__ void RunProducts(LdsByte *lds, const Share &share, co
   };
   Tile<S::kWaveI / 16> t;
   t.Clear();
+  const float undo = UndoOf<T>(p);
   const auto add = [&](const LdsByte *of_a, const LdsByte *of_b, const auto &between) {
     t.template Add<T, Layout<T, S::kI, kAcrossA>, Layout<T, S::kJ, kAcrossB>>(of_a, of_b, wave_i, wave_j, between);
   };
@@ -825,8 +831,15 @@ __device__ __forceinline__ void RunProducts(LdsByte *lds, const Share &share, co
 #pragma unroll
       for (int j = 0; j < kWaveJ / 16; j += 4) {
         const int column = at.j0 + wave_j * kWaveJ + j * 16;
-        if (p.splits > 1) StoreRounded(p.partial + (at.one * p.rows + row) * p.columns, column, p.columns, &t.acc[i][j]);
-        else StoreRounded(static_cast<T *>(p.c[at.member]) + row * p.c_stride, column, p.columns, &t.acc[i][j]);
+        if (p.splits > 1) {
+          StoreRounded(p.partial + (at.one * p.rows + row) * p.columns, column, p.columns, &t.acc[i][j]);
+          continue;
+        }
+        if constexpr (std::is_same_v<T, _Float16>) {
+#pragma unroll
+          for (int f = 0; f < 4; ++f) t.acc[i][j + f] *= undo;
+        }
+        StoreRounded(static_cast<T *>(p.c[at.member]) + row * p.c_stride, column, p.columns, &t.acc[i][j]);
       }
     }
     t.Clear();
@@ -857,6 +870,7 @@ __device__ __forceinline__ void JoinProducts(const Share &share_of, const Produc
   constexpr int kVec = kShares == 1 ? 4 : 1, kElements = kThreads / kShares * kVec;
   __shared__ float s_sums[kShares][kShares == 1 ? 1 : kElements];
   const long long each = p.rows * p.columns, step = (long long)share_of.of * kElements;
+  const float undo = UndoOf<T>(p);
   const int in = threadIdx.x % (kThreads / kShares) * kVec, share = threadIdx.x / (kThreads / kShares);
   for (int member = 0; member < p.batch; ++member) {
     T *c = static_cast<T *>(p.c[member]);
@@ -884,6 +898,10 @@ __device__ __forceinline__ void JoinProducts(const Share &share_of, const Produc
         __syncthreads();
       }
       if (held == 0 || share != 0) continue;
+      if constexpr (std::is_same_v<T, _Float16>) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) sum[e] *= undo;
+      }
       const long long row = each < (1ll << 32) ? (long long)((unsigned)at / (unsigned)p.columns) : at / p.columns;
       const int column = (int)(at - row * p.columns);
       if (column + kVec <= p.columns) {
@@ -927,9 +945,28 @@ struct Slopes {
   void *d_gate, *d_up;  // [rows][d_stride]
   long long d_stride, rows;
   int hidden;
+  float *range;  // float16: [1 + workgroup] the greatest finite magnitude of what it formed; [0] what undoes the factor
 };
 
 constexpr int kSlopeVec = 8;
+
+// The greatest of a workgroup's values, to all of its threads.
+__device__ __forceinline__ float MostOfGroup(float most) {
+  __shared__ float s_most[kThreads / 64];
+#pragma unroll
+  for (int by = 32; by > 0; by /= 2) most = fmaxf(most, __shfl_xor(most, by));
+  if ((threadIdx.x & 63) == 0) s_most[threadIdx.x >> 6] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) most = fmaxf(most, s_most[w]);
+  return most;
+}
+
+// The power of two that factors of which `most` is the greatest are taken times in float16 (as far as its reciprocal is a normal number).
+__device__ __forceinline__ float FactorFor(float most) {
+  if (most == 0.0f || (most >= 1.0f && most < 65504.0f)) return 1.0f;
+  return ldexpf(1.0f, min(14 - ilogbf(most), 126));
+}
 
 // d_gate and d_up; 0 in the columns from the layer's end to the next row.  A thread has kSlopeVec columns of a row (d_stride is a multiple of 64).
 // Both are rounded to the layer's type, which the matrix instructions of the products they enter take: half a step of each term, on top of the half
@@ -937,13 +974,26 @@ constexpr int kSlopeVec = 8;
 // operands, rounded at the end, are off by 1.7e-3).  A second part for what rounding leaves would double the products' work.
 // Memory bounds it: 4096 x 16384 bf16, 0.67 GB, 121 us, 5.6 TB/s; from 8 bits, 100,003 x 256, 0.21 GB, 39 us.
 // Workgroups from `groups` on copy to aligned rows what the products need there.
-template <typename T, int kAct, bool kCodes>
+// float16 does not hold what float32 forms of its numbers: 2^11 times 64 is infinite in it, 2^-20 times 2^-8 is 0, while the sums over them may well be numbers of
+// it.  So this pass also finds the greatest (finite) magnitude, and a second one (kAgain) takes both times a power of two that brings it to 2^14 or more, undone where
+// the products end, unless it lies from 1 to float16's greatest number: there what is taken as it is loses no more than 2^-25 of the greatest, as much as
+// float32 sums with it would.  The second pass then ends as it has seen that.  (fp16, us, in one pass and so: 100,003 x 256 from 8 bits 37 and 46 + 5,
+// 4096 x 16384 123 and 135 + 6, 1003 x 2055 9 and 11 + 4.  A pass for the magnitudes alone, before, would read all that this one reads.)
+template <typename T, int kAct, bool kCodes, bool kAgain>
 __global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long blocks, unsigned groups, const Padded pad) {
   typedef std::conditional_t<kCodes, signed char, T> Kept;
   const unsigned vectors = (unsigned)(a.d_stride / kSlopeVec);
   if (blockIdx.x >= groups) {
     PadRows<T>(Share{blockIdx.x - groups, gridDim.x - groups}, pad);
     return;
+  }
+  constexpr bool kRange = std::is_same_v<T, _Float16>;
+  float most = 0.0f, factor = 1.0f;
+  if constexpr (kAgain) {
+    for (unsigned g = threadIdx.x; g < groups; g += kThreads) most = fmaxf(most, a.range[1 + g]);
+    factor = FactorFor(MostOfGroup(most));
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.range[0] = 1.0f / factor;
+    if (factor == 1.0f) return;
   }
   for (long long block = blockIdx.x; block < blocks; block += groups) {
     const long long first = block * kThreads, row0 = first / vectors;
@@ -987,11 +1037,23 @@ __global__ void __launch_bounds__(kThreads) k_slopes(const Slopes a, long long b
       float act, slope;
       ActAndSlope<kAct>(gv, &act, &slope);
       const bool there = c < held;
-      dg.v[c] = there ? Round<T>((float)y.v[c] * uv * slope) : T(0);
-      du.v[c] = there ? Round<T>((float)y.v[c] * act) : T(0);
+      if constexpr (kRange && !kAgain) {
+        // (products of its own: the instruction that rounds those below to 16 bits multiplies as well, where nothing else needs them, and rounds once)
+        float of[2] = {slope, act};
+        asm("" : "+v"(of[0]), "+v"(of[1]));
+        const float d[2] = {fabsf((float)y.v[c] * uv * of[0]), fabsf((float)y.v[c] * of[1])};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) most = there && d[w] < __builtin_inff() ? fmaxf(most, d[w]) : most;
+      }
+      dg.v[c] = there ? Round<T>(kAgain ? (float)y.v[c] * uv * slope * factor : (float)y.v[c] * uv * slope) : T(0);
+      du.v[c] = there ? Round<T>(kAgain ? (float)y.v[c] * act * factor : (float)y.v[c] * act) : T(0);
     }
     *reinterpret_cast<Pack<T, kSlopeVec> *>(static_cast<T *>(a.d_gate) + row * a.d_stride + at) = dg;
     *reinterpret_cast<Pack<T, kSlopeVec> *>(static_cast<T *>(a.d_up) + row * a.d_stride + at) = du;
+  }
+  if constexpr (kRange && !kAgain) {
+    most = MostOfGroup(most);
+    if (threadIdx.x == 0) a.range[1 + blockIdx.x] = most;
   }
 }
 
@@ -1108,25 +1170,33 @@ void RunGatedGrad(const GatedGradArgs &a, const GatedGradPlan &plan) {
   const hipStream_t stream = static_cast<hipStream_t>(l.stream);
   unsigned char *work = static_cast<unsigned char *>(l.work);
   void *d_gate = work + plan.d_gate, *d_up = work + plan.d_up;
+  constexpr bool kRange = std::is_same_v<T, _Float16>;
+  float *range = kRange && l.rows > 0 ? reinterpret_cast<float *>(work + plan.range) : nullptr;
   const Padded pad = PadOf(&l, plan.pad, a.grad_w_gate != nullptr, a.grad_x != nullptr, work);
   const long long extent = pad.blocks > 0 ? plan.pad.stride : l.dim;
   if (l.rows > 0) {
-    const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden};
+    const Slopes s{a.grad_out, a.grad_out_stride, l.gate, l.up, l.gate_scales, l.up_scales, l.kept_stride, d_gate, d_up, plan.d_stride, l.rows, l.hidden, range};
     const long long blocks = Pieces(l.rows * (plan.d_stride / kSlopeVec), kThreads);
-    const unsigned groups = (unsigned)std::min(blocks, kMostGrid);
-    const dim3 grid(groups + GroupsOf(pad));
+    const unsigned groups = (unsigned)(kRange ? Pieces(blocks, Pieces(blocks, kRangeGroups)) : std::min(blocks, kMostGrid));
+    const auto launch = [&](auto act, auto codes, auto again, const Padded &copies) {
+      hipLaunchKernelGGL((k_slopes<T, decltype(act)::value, decltype(codes)::value, decltype(again)::value>), dim3(groups + GroupsOf(copies)), dim3(kThreads), 0, stream, s,
+                         blocks, groups, copies);
+    };
     WithActivation(l.activation, [&](auto act) {
-      constexpr int kAct = decltype(act)::value;
-      if (l.gate_scales) hipLaunchKernelGGL((k_slopes<T, kAct, true>), grid, dim3(kThreads), 0, stream, s, blocks, groups, pad);
-      else hipLaunchKernelGGL((k_slopes<T, kAct, false>), grid, dim3(kThreads), 0, stream, s, blocks, groups, pad);
+      if (l.gate_scales) launch(act, std::true_type(), std::false_type(), pad);
+      else launch(act, std::false_type(), std::false_type(), pad);
+      if constexpr (kRange) {
+        if (l.gate_scales) launch(act, std::true_type(), std::true_type(), Padded{});
+        else launch(act, std::false_type(), std::true_type(), Padded{});
+      }
     });
   }
   const Operand d{{d_gate, d_up}, plan.d_stride};
   const bool d_direct = IsDirect<T>(d_gate, plan.d_stride, plan.d_stride);
   const Products x{d, {{l.w_gate, l.w_up}, l.w_stride}, l.rows, l.dim, l.hidden, 2, 1, {a.grad_x, nullptr}, a.grad_x_stride,
-                   (int)plan.x.splits, plan.x.split_blocks, reinterpret_cast<float *>(work + plan.x_partial)};
+                   (int)plan.x.splits, plan.x.split_blocks, reinterpret_cast<float *>(work + plan.x_partial), range};
   const Products w{d, {{l.x, l.x}, l.x_stride}, l.hidden, l.dim, l.rows, 1, 2, {a.grad_w_gate, a.grad_w_up}, a.grad_w_stride,
-                   (int)plan.w.splits, plan.w.split_blocks, reinterpret_cast<float *>(work + plan.w_partial)};
+                   (int)plan.w.splits, plan.w.split_blocks, reinterpret_cast<float *>(work + plan.w_partial), range};
   const bool x_direct = d_direct && IsDirect<T>(l.w_gate, l.w_stride, extent) && IsDirect<T>(l.w_up, l.w_stride, extent);
   const bool w_direct = d_direct && IsDirect<T>(l.x, l.x_stride, extent), wants_x = a.grad_x && l.rows > 0;
   if (plan.together && wants_x && a.grad_w_gate && x_direct && w_direct) {

@@ -9,6 +9,7 @@ namespace arb {
 constexpr int kLineBytes = 128;  // of k's in a block: 64 of 16 bits, 32 of 32
 constexpr int kWaveJ = 128;      // columns of a wave's part of a tile
 constexpr int kFewRows = 16;     // up to here a product's sixteen rows hold all of x
+constexpr int kRangeGroups = 2048;  // workgroups that form d_gate and d_up in float16: each of the second pass reads what all of the first have found
 
 // A workgroup's tile: kWavesI x kWavesJ waves, kWaveI rows by kWaveJ columns each.  The LDS holds kBlocksA blocks of A and kBlocksB of B: one that is multiplied, the
 // others on their way.
@@ -46,7 +47,7 @@ struct GatedGradPlan {
   ProductCut x, w;     // of grad_x, of the weights' gradients
   bool together;       // all tiles of both have a place on the chip at once
   LayerPad pad;
-  size_t d_gate, d_up, x_partial, w_partial, bytes;
+  size_t d_gate, d_up, range, x_partial, w_partial, bytes;
 };
 
 inline long long Pieces(long long n, long long of) { return (n + of - 1) / of; }

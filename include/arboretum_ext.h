@@ -316,7 +316,8 @@ const char *AActivationRestore(void *x, const signed char *codes, const float *s
  * [rows][hidden].  activation: 0 silu, 1 gelu (by the error function).  Products are summed in float32.
  * gate, up: what the backward pass needs, x w_gate^T and x w_up^T [rows][hidden] (kept_stride: of both) of `type`, or with
  * gate_scales and up_scales given as codes of 8 bits with scales [rows][ceil(hidden / 64)], as of AActivationCheckpoint.  All may
- * be NULL.  dim and hidden are 1 to 2^24, rows below 2^31 (0 for none). */
+ * be NULL.  A gate or up beyond float16 is kept as an infinity in float16, and its gradients are infinite or NaN; codes hold float32's range.
+ * dim and hidden are 1 to 2^24, rows below 2^31 (0 for none). */
 const char *AGatedBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes);
 const char *AGated(void *out, void *gate, void *up, float *gate_scales, float *up_scales, const void *x, const void *w_gate,
                    const void *w_up, long long rows, int dim, int hidden, long long out_stride, long long kept_stride,
@@ -326,6 +327,8 @@ const char *AGated(void *out, void *gate, void *up, float *gate_scales, float *u
 /* Its gradients, given that of out: with the gate and up that AGated kept (and the same scales),
  *   d_gate = grad_out * up * act'(gate),  d_up = grad_out * act(gate)     (rounded to `type`, as the products take them)
  *   grad_x = d_gate w_gate + d_up w_up,  grad_w_gate = d_gate^T x,  grad_w_up = d_up^T x
+ * In float16 d_gate and d_up are taken times a power of two, undone in the results, where their greatest magnitude is below 1 or beyond
+ * float16: none overflows, and beside its rounding none is off by more than 2^-25 of the greatest.
  * grad_x, or both gradients of the weights, may be NULL; rows == 0 gives weights' gradients of 0.  Results are the same
  * from run to run. */
 const char *AGatedGradBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes);
