@@ -119,11 +119,15 @@ typedef __attribute__((address_space(3))) I4 LdsI4;
 // 16 bytes a lane from `base` + `at` (beyond 2^31: 0) to the LDS, the wave's 1 KB side by side from `to` + kOffset on.  By hand: the
 // compiler waits for a load of its own before any read of the LDS, and this one is meant to be on its way meanwhile.  Whoever reads
 // what it writes waits for it first (WaitAndMeet, which nothing that touches memory moves across).
+// (The compiler itself keeps nothing in m0, and says so of the clobber; where it passes an index there, nothing of this comes in between.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int kOffset>
 __device__ __forceinline__ void LoadToLds(unsigned long long base, unsigned at, unsigned to) {
   const I4 from = {(int)(unsigned)base, (int)(unsigned)(base >> 32), 0x7FFFFFFF, 0x00020000};
-  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(to), "n"(kOffset) : "scc");
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(from), "s"(to), "n"(kOffset) : "m0", "scc");
 }
+#pragma clang diagnostic pop
 
 // Until no more than kLast of the wave's loads are on their way (they arrive in the order they were issued in), what it has read of the LDS is there,
 // and all waves of the workgroup are as far.
