@@ -299,7 +299,7 @@ void Garden::LogProbs(DataMatrix *data, int n_trees, const ClassLogProbs &out) c
   const size_t use = CheckLeafWalk(data, n_trees);
   struct Sums {
     float *p;
-    ~Sums() { DevicePoolGive(p); }  // (nothing is pending: both calls below wait)
+    ~Sums() { DevicePoolGive(p); }  // (nothing is pending: both calls below wait, for what they launched before an error too)
   } sums{static_cast<float *>(DevicePoolTake(K * data->rows * sizeof(float)))};
   {
     std::lock_guard<std::mutex> lock(predictor_mutex_);
@@ -331,7 +331,7 @@ void Garden::RefineLeaves(DataMatrix *data, const RefineOptions &options) {
   const size_t token_ld = (n + 63) / 64 * 64;
   struct Tokens {
     int *p;
-    ~Tokens() { DevicePoolGive(p); }  // (nothing is pending: both calls below wait)
+    ~Tokens() { DevicePoolGive(p); }  // (nothing is pending: both calls below wait, for what they launched before an error too)
   } tokens{static_cast<int *>(DevicePoolTake(use * token_ld * sizeof(int)))};
   LeafTokens(data, tokens.p, token_ld, -1, nullptr);
   RefineOnDevice(cfg, data, tokens.p, token_ld, trees_of, &tables, IntoInternal(cfg.tree.initial_y), options);

@@ -475,6 +475,14 @@ struct DevicePredictor {
     if (n >= (1ull << 31) && !blocks) throw std::runtime_error("too many rows");
     if (data.is_prebinned && data.prebinned.empty() && !blocks) throw std::runtime_error("pre-quantised matrix without bins");
     if (!stream) stream = StreamPoolTake();
+    // An error leaves nothing pending either: the caller gives back the memory that the walks write.
+    struct Settled {
+      const hipStream_t stream;
+      bool waited = false;
+      ~Settled() {
+        if (!waited) (void)hipStreamSynchronize(stream);
+      }
+    } settled{stream};
     LayOut(trees, first, use, F, labels);
     // Kernels write the sums where the host reads them: stores of 256 bytes a wave, at the rate of a copy
     // and beside the walk.
@@ -494,7 +502,7 @@ struct DevicePredictor {
       if (piece == 0) throw std::runtime_error("too many features for device prediction");
       struct Block {
         void *p;
-        ~Block() { DevicePoolGive(p); }  // (the staging has waited for the stream's copies, Run waits for its walks)
+        ~Block() { DevicePoolGive(p); }  // (the stream has been waited for: below, or by the staging where that fails)
       };
       const size_t pieces = (n + piece - 1) / piece, group = std::max<size_t>(kBlockBytes / kStageBytes, 1);
       Block block{DevicePoolTake(group * piece * row_bytes)};
@@ -539,6 +547,7 @@ struct DevicePredictor {
       DevicePoolGive(block);
     }
     HIP_OK(hipStreamSynchronize(stream));
+    settled.waited = true;
     return result;
   }
 };
