@@ -18,14 +18,15 @@ __global__ void k_label_tokens(const uint8_t *__restrict__ labels, int *__restri
 void ClassLogProbsOnDevice(DataMatrix *data, const float *sums, size_t classes, const ClassLogProbs &out) {
   const size_t n = data->rows;
   const int top = std::min(out.top, (int)classes);
+  const std::shared_ptr<const unsigned char> labels = out.log_probs ? data->DeviceLabels() : nullptr;  // (these are let go behind `work`, which waits)
+  unsigned outside = 0;
   DeviceWork work;
   const size_t bytes = LogProbsBytes((long long)n, (long long)classes, top);
   void *scratch = work.Take<unsigned char>(bytes);
   float *log_probs = out.log_probs ? work.Take<float>(n) : nullptr, *entropy = out.entropy ? work.Take<float>(n) : nullptr;
   int *tokens = out.log_probs ? work.Take<int>(n) : nullptr, *top_classes = top ? work.Take<int>(n * top) : nullptr;
   float *top_log_probs = top ? work.Take<float>(n * top) : nullptr;
-  unsigned *status = work.Take<unsigned>(1), outside = 0;
-  const std::shared_ptr<const unsigned char> labels = out.log_probs ? data->DeviceLabels() : nullptr;
+  unsigned *status = work.Take<unsigned>(1);
   HIP_OK(hipMemsetAsync(status, 0, sizeof(unsigned), work.stream));
   if (tokens) {
     hipLaunchKernelGGL(k_label_tokens, dim3((unsigned)std::min<size_t>((n + 255) / 256, 4096)), dim3(256), 0, work.stream, labels.get(), tokens, n);

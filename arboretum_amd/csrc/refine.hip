@@ -54,6 +54,8 @@ __global__ void k_limit(float *__restrict__ weight, float most, size_t n) {
 void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *tokens, size_t token_ld,
                     const std::vector<size_t> &trees_of, std::vector<std::vector<float>> *tables, float init, const RefineOptions &options) {
   const size_t n = data->rows, K = trees_of.size();
+  const std::shared_ptr<const float> y = data->DeviceY();  // (both let go behind `work`, which waits)
+  const std::shared_ptr<const unsigned char> labels = data->DeviceLabels();
   DeviceWork work;
   struct Table {
     float *weight, *grad, *m, *v;
@@ -77,8 +79,6 @@ void RefineOnDevice(const Configuration &cfg, DataMatrix *data, const int *token
   }
   float *y_hat = work.Take<float>(K * n);
   unsigned char *scratch = work.Take<unsigned char>(scratch_bytes);
-  const std::shared_ptr<const float> y = data->DeviceY();
-  const std::shared_ptr<const unsigned char> labels = data->DeviceLabels();
   std::vector<void *> weights;
   std::vector<const void *> grads;
   std::vector<float *> ms, vs;

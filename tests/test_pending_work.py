@@ -28,7 +28,7 @@ def program(tmp_path_factory):
     return out
 
 
-@pytest.mark.parametrize("check", ["walk"])
+@pytest.mark.parametrize("check", ["walk", "labels"])
 def test_nothing_is_pending_on_what_is_given_back(program, check):
     r = subprocess.run([program, check], stdout=subprocess.PIPE, timeout=60)
     assert r.returncode == 0, r.stdout.decode()
