@@ -655,14 +655,6 @@ void CheckLogits(const Logits &l) {
   CheckAligned(l.status, 4, "status");
 }
 
-// Rows of classes, or the other way round; where both lie apart nothing is said of them (what lies between may be another's).
-Extent ExtentOf(const Logits &l, const void *at, long long row_stride, long long class_stride) {
-  const size_t item = ElementBytes(l.type);
-  if (class_stride <= 1 || l.vocab == 1) return Extent(at, l.n, l.n == 1 ? l.vocab : row_stride, class_stride == 0 ? 1 : l.vocab, item);
-  if (row_stride <= 1 || l.n == 1) return Extent(at, l.vocab, class_stride, row_stride == 0 ? 1 : l.n, item);
-  return Extent(nullptr, 0);
-}
-
 unsigned GridOf(long long workgroups) { return (unsigned)std::min<long long>(workgroups, 1 << 20); }
 
 }  // namespace
@@ -695,7 +687,7 @@ void LogProbs(const LogProbsArgs &a) {
   if (!a.log_probs && !a.entropy && !a.stats && a.top == 0) return;
   CheckApart({{a.log_probs, l.n * 4}, {a.entropy, l.n * 4}, {a.stats, l.n * 8}, {a.top_tokens, l.n * a.top * 4}, {a.top_log_probs, l.n * a.top * 4},
               {a.work, (long long)need}, {l.status, 4}},
-             {ExtentOf(l, l.logits, l.row_stride, l.class_stride), {l.tokens, l.n * l.token_bits / 8}});
+             {Extent(l.logits, l.n, l.row_stride, l.vocab, l.class_stride, ElementBytes(l.type)), {l.tokens, l.n * l.token_bits / 8}});
   OnDeviceOf device(l.logits);
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
   RowsArgs r{l.logits, l.row_stride, l.class_stride, l.n, (unsigned)l.vocab, l.scale, l.scale * kLog2E, l.tokens, l.token_bits, a.log_probs,
@@ -774,9 +766,9 @@ void LogProbsGrad(const LogProbsGradArgs &a) {
   CheckAligned(a.grad_entropy, 4, "grad_entropy");
   CheckAligned(a.entropy, 4, "entropy");
   CheckAligned(a.stats, 8, "stats");
-  const Extent none(nullptr, 0), grad = ExtentOf(l, a.grad_logits, a.grad_row_stride, a.grad_class_stride);
+  const Extent none(nullptr, 0), grad = Extent(a.grad_logits, l.n, a.grad_row_stride, l.vocab, a.grad_class_stride, ElementBytes(l.type));
   CheckApart({grad, {l.status, 4}},
-             {a.grad_logits == l.logits ? none : ExtentOf(l, l.logits, l.row_stride, l.class_stride), {l.tokens, l.n * l.token_bits / 8}, {a.stats, l.n * 8},
+             {a.grad_logits == l.logits ? none : Extent(l.logits, l.n, l.row_stride, l.vocab, l.class_stride, ElementBytes(l.type)), {l.tokens, l.n * l.token_bits / 8}, {a.stats, l.n * 8},
               {a.grad_log_probs, l.n * 4}, {a.grad_entropy, l.n * 4}, {a.entropy, l.n * 4}});
   OnDeviceOf device(a.grad_logits);
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);

@@ -3,9 +3,11 @@
 #define ARBORETUM_AMD_OPERATORS_DEVICE_H_
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
 
 #include "operators.h"
 
@@ -63,24 +65,65 @@ inline void CheckAligned(const void *p, size_t bytes, const char *what) {
   if (reinterpret_cast<uintptr_t>(p) % bytes != 0) throw std::runtime_error(std::string(what) + " is not aligned to its elements");
 }
 
-// Memory of a call: `rows` pieces of `width` bytes, `stride` bytes from one to the next; nullptr: none.
+// Memory of a call: `rows` by `columns` pieces of `width` bytes, `stride` bytes from a row to the next and `step`, which is less, from a column to the next;
+// nullptr: none.  (Bytes in 128 bits: strides and sizes that no memory has do not wrap around.)
 struct Extent {
+  typedef __int128 Bytes;
   const void *at;
-  long long rows, stride, width;
+  Bytes rows, stride, columns = 1, step = 0, width;
+  bool tangled = false;  // rows that lie between each other's columns
   Extent(const void *p, long long bytes) : at(p), rows(bytes > 0), stride(bytes), width(bytes) {}
-  Extent(const void *p, long long n, long long elements, long long of, size_t item) : at(p), rows(of > 0 ? n : 0), stride(elements * (long long)item), width(of * (long long)item) {
-    if (stride < width) width += (rows - 1) * stride, rows = rows > 0, stride = width;  // (rows that share elements are one piece)
+  // `n` by `of` elements, of `item` bytes each
+  Extent(const void *p, long long n, long long n_stride, long long of, long long of_stride, size_t item)
+      : at(p), rows(n), stride((Bytes)n_stride * item), columns(of), step((Bytes)of_stride * item), width(item) {
+    if (n <= 0 || of <= 0) {
+      rows = 0;
+      return;
+    }
+    if (columns > 1 && (rows == 1 || stride < step)) std::swap(rows, columns), std::swap(stride, step);
+    // (what lies side by side, or shares elements, is one piece)
+    if (columns > 1 && step <= width) width += (columns - 1) * step, columns = 1;
+    if (columns == 1 && rows > 1 && stride <= width) width += (rows - 1) * stride, rows = 1;
+    tangled = columns > 1 && stride < Row();
   }
+  Extent(const void *p, long long n, long long n_stride, long long of, size_t item) : Extent(p, n, n_stride, of, 1, item) {}
+  Bytes Begin() const { return (Bytes) reinterpret_cast<uintptr_t>(at); }
+  Bytes Row() const { return (columns - 1) * step + width; }
+  Bytes All() const { return (rows - 1) * stride + Row(); }
+  bool IsOnePiece() const { return rows == 1 && columns == 1; }
 };
-// Whether two places meet.  Rows as far apart in both may lie between each other, as the columns of one matrix do.
-inline bool DoMeet(const Extent &a, const Extent &b) {
-  if (!a.at || !b.at || a.rows == 0 || b.rows == 0) return false;
-  const long long pa = (long long)reinterpret_cast<uintptr_t>(a.at), pb = (long long)reinterpret_cast<uintptr_t>(b.at);
-  if (pb >= pa + (a.rows - 1) * a.stride + a.width || pa >= pb + (b.rows - 1) * b.stride + b.width) return false;
-  if (a.stride != b.stride || (a.rows == 1 && b.rows == 1)) return true;
-  const long long apart = ((pb - pa) % a.stride + a.stride) % a.stride;
-  return apart < a.width || apart + b.width > a.stride;
+
+// Whether a whole number k from `least` to `most` has low < k by < high.
+inline bool HasMultiple(Extent::Bytes low, Extent::Bytes high, Extent::Bytes by, Extent::Bytes least, Extent::Bytes most, Extent::Bytes *first, Extent::Bytes *last) {
+  const auto floor = [&](Extent::Bytes v) { return v >= 0 ? v / by : -((by - 1 - v) / by); };
+  *first = std::max(floor(low) + 1, least);
+  *last = std::min(floor(high - 1), most);
+  return *first <= *last;
 }
+
+// Whether two places meet.  Pieces between the rows, or columns, of another do not, nor do rows (and columns) as far apart in both that lie between each other,
+// as the columns of one matrix.  Of different distances they are taken to meet where their ends do.
+inline bool DoMeet(const Extent &a, const Extent &b) {
+  typedef Extent::Bytes Bytes;
+  if (!a.at || !b.at || a.rows == 0 || b.rows == 0) return false;
+  const Bytes apart = b.Begin() - a.Begin();
+  if (apart >= a.All() || -apart >= b.All()) return false;
+  if (b.IsOnePiece() && !a.IsOnePiece()) return DoMeet(b, a);
+  if (a.IsOnePiece() && b.IsOnePiece()) return true;
+  if (a.tangled || b.tangled) return true;
+  // (one piece is a row and a column at whatever distances the other has)
+  if (!a.IsOnePiece() && (a.stride != b.stride || (a.columns > 1 || b.columns > 1 ? a.step != b.step : false))) return true;
+  // One of b's pieces begins `apart` - (i stride + j step) behind one of a's that is i rows and j columns further on than it: they meet if that is more than
+  // -(b's width) and less than a's.
+  Bytes i, i_last, j, j_last;
+  if (!HasMultiple(apart - a.width - (a.columns - 1) * b.step, apart + b.width + (b.columns - 1) * b.step, b.stride, 1 - b.rows, a.rows - 1, &i, &i_last)) return false;
+  if (a.columns == 1 && b.columns == 1) return true;
+  if (a.IsOnePiece() && i_last - i > 1) return true;  // (all of a row)
+  for (; i <= i_last; ++i)
+    if (HasMultiple(apart - i * b.stride - a.width, apart - i * b.stride + b.width, b.step, 1 - b.columns, a.columns - 1, &j, &j_last)) return true;
+  return false;
+}
+
 // What a call writes is apart from all else that it writes or reads: others' elements would be read before or after they are written, as it happens.
 template <size_t kWritten, size_t kRead>
 void CheckApart(const Extent (&written)[kWritten], const Extent (&read)[kRead]) {

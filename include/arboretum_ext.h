@@ -269,8 +269,9 @@ const char *AAdamW(int count, void *const *params, const void *const *grads, flo
  * As above: EVERY POINTER IS A DEVICE POINTER; the calls enqueue on `stream` of the device that their outputs are on, return
  * WITHOUT waiting, allocate nothing, may be captured, and hold nothing from one call for the next.  Element types 0
  * float32, 1 bfloat16, 2 float16, and each result is rounded once, to nearest, from float32.  Strides count elements; rows may
- * begin at any element.  Outputs and work are apart from each other and from inputs (rows of one may lie between another's):
- * calls in which they meet are refused.  work: 16-byte aligned, of the size that the call's ...Bytes gives (NULL where that is 0), undefined
+ * begin at any element.  Outputs and work are apart from each other and from inputs: calls in which they meet are
+ * refused.  An array, or one row, may lie between another's rows (or classes), and rows between rows of the same stride; of different strides
+ * they count as meeting where one begins before the other's end.  work: 16-byte aligned, of the size that the call's ...Bytes gives (NULL where that is 0), undefined
  * before and after; calls that may run at the same time need work memory of their own. */
 
 /* Log probabilities under n rows of `vocab` classes: class j of row i is logits[i * row_stride + j * class_stride], so rows
