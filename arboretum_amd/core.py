@@ -345,8 +345,8 @@ def gated(out, x, w_gate, w_up, rows, dim, hidden, work, work_bytes, gate=None, 
           activation="silu", dtype="float32", out_stride=None, kept_stride=None, x_stride=None, w_stride=None, stream=None):
     """out = act(x w_gate^T) * (x w_up^T) on the GPU (AGated): x [rows][dim], weights [hidden][dim], out [rows][hidden], DEVICE
     addresses; activation "silu" or "gelu".  gate, up: where both products are kept for gated_grad(), of `dtype`, or, with
-    gate_scales and up_scales, in 8 bits as activation_checkpoint() keeps them.  `work`: gated_bytes() of device memory.
-    Does not wait."""
+    gate_scales and up_scales, in 8 bits as activation_checkpoint() keeps them.  `work`: gated_bytes() of device memory (up to
+    16 rows without scales: None and 0).  Does not wait."""
     out_stride = hidden if out_stride is None else out_stride
     kept_stride = hidden if kept_stride is None else kept_stride
     x_stride = dim if x_stride is None else x_stride

@@ -137,7 +137,8 @@ size_t GatedBytes(long long rows, int dim, int hidden, int type) {
 void Gated(const GatedArgs &a) {
   const GatedLayer &l = a.layer;
   const GatedPlan plan = (CheckLayerSizes(l.rows, l.dim, l.hidden, l.type), PlanOf(l.rows, l.dim, l.hidden, l.type));
-  CheckLayer(l, false, plan.bytes);
+  const size_t need = plan.few && !l.gate_scales ? 0 : plan.bytes;  // (few rows go without, but for codes, whose scales stand for 64 columns)
+  CheckLayer(l, false, need);
   CheckStride(a.out_stride, l.hidden, l.rows, "out");
   CheckAligned(a.out, ElementBytes(l.type), "out");
   if (l.rows == 0) return;
@@ -145,7 +146,7 @@ void Gated(const GatedArgs &a) {
   const size_t item = ElementBytes(l.type), kept = l.gate_scales ? 1 : item;
   const long long scales = l.rows * Pieces(l.hidden, kScaleGroup) * 4;
   CheckApart({{a.out, l.rows, a.out_stride, l.hidden, item}, {l.gate, l.rows, l.kept_stride, l.hidden, kept}, {l.up, l.rows, l.kept_stride, l.hidden, kept},
-              {l.gate_scales, scales}, {l.up_scales, scales}, {l.work, (long long)plan.bytes}},
+              {l.gate_scales, scales}, {l.up_scales, scales}, {l.work, (long long)need}},
              {{l.x, l.rows, l.x_stride, l.dim, item}, {l.w_gate, l.hidden, l.w_stride, l.dim, item}, {l.w_up, l.hidden, l.w_stride, l.dim, item}});
   OnDeviceOf device(a.out);
   WithType(l.type, [&](auto type) { RunGated<decltype(type)>(a, plan); });
