@@ -703,11 +703,19 @@ void LogProbs(const LogProbsArgs &a) {
         if (side_by_side) hipLaunchKernelGGL((k_columns<T, true, decltype(held)::value, 8>), grid, dim3(256), 0, stream, r);
         else hipLaunchKernelGGL((k_columns<T, false, decltype(held)::value, 8>), grid, dim3(256), 0, stream, r);
       };
-      if (a.top <= 1) columns(std::integral_constant<int, 1>());
-      else if (a.top == 2) columns(std::integral_constant<int, 2>());
-      else if (a.top == 3) columns(std::integral_constant<int, 3>());
-      else if (a.top <= 5) columns(std::integral_constant<int, 5>());
-      else columns(std::integral_constant<int, 8>());
+      // A list of each length to 8, whose rows are then stored side by side; longer ones eight at a time.  (1,000,003 x 10 fp32 class by class, us, by the next longer
+      // list and by their own: top 4 26.8 and 24.5, top 6 36.6 and 27.8, top 7 44.9 and 29.4; top 8 31.)
+      switch (std::min(a.top, 8)) {
+        case 0:
+        case 1: columns(std::integral_constant<int, 1>()); break;
+        case 2: columns(std::integral_constant<int, 2>()); break;
+        case 3: columns(std::integral_constant<int, 3>()); break;
+        case 4: columns(std::integral_constant<int, 4>()); break;
+        case 5: columns(std::integral_constant<int, 5>()); break;
+        case 6: columns(std::integral_constant<int, 6>()); break;
+        case 7: columns(std::integral_constant<int, 7>()); break;
+        default: columns(std::integral_constant<int, 8>());
+      }
       return;
     }
     r.parts = PartsOf(l.n, l.vocab);
