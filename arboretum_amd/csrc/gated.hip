@@ -39,6 +39,8 @@ struct Room {
 
 // Rows whose chunks are not aligned come through registers into small tiles, a block at a time; copies of x and both weights are read and written once.  For the
 // gradient (300 x 4094 x 4098 with the layer itself: 251 us without, 186 with copies; 100 x 1002 x 1004 68 and 44) the copies are always less.
+// There is room for them by the width alone, since whoever asks for the bytes says no more: rows of whole chunks that lie between the places of such go through registers
+// whatever their number (8192 x 4096 x 16384 bf16, one element between rows and none: layer 3576 and 1883 us, gradient 5657 and 3686; 1000 x 768 x 2048 35 and 34, 63 and 40).
 LayerPad PadOf(long long rows, int dim, int hidden, size_t item, Room *room) {
   LayerPad p{0, 0, 0, 0};
   if (dim * item % 16 == 0 || rows == 0) return p;
@@ -49,7 +51,7 @@ LayerPad PadOf(long long rows, int dim, int hidden, size_t item, Room *room) {
   return p;
 }
 
-// Whether the layer itself, which reads its weights along k, copies too: a block through registers takes 1.3 us more, the last one of a row three times that, copies a launch of
+// Whether the layer itself, which reads its weights along k, copies too, by a line through the times that follow: a block through registers takes 1.3 us more, the last one of a row three times that, copies a launch of
 // 5 us and their bytes at 5 TB/s (us without and with: 40 x 4095 x 16383 92 and 175, 300 x 4095 x 4097 66 and 69, 500 x 1001 x 1003 20 and 18, 8191 x 1001 x 1003
 // 57 and 42, 100,003 x 63 x 255 70 and 49, 280 x 7353 x 11442 380 and 297).
 bool CopiesForward(const ProductCut &c, long long rows, int dim, int hidden, size_t item) {

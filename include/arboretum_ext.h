@@ -318,7 +318,8 @@ const char *AActivationRestore(void *x, const signed char *codes, const float *s
  * gate, up: what the backward pass needs, x w_gate^T and x w_up^T [rows][hidden] (kept_stride: of both) of `type`, or with
  * gate_scales and up_scales given as codes of 8 bits with scales [rows][ceil(hidden / 64)], as of AActivationCheckpoint.  All may
  * be NULL.  A gate or up beyond float16 is kept as an infinity in float16, and its gradients are infinite or NaN; codes hold float32's range.
- * dim and hidden are 1 to 2^24, rows below 2^31 (0 for none).  Up to 16 rows take work only where scales are given (NULL else). */
+ * dim and hidden are 1 to 2^24, rows below 2^31 (0 for none).  Up to 16 rows take work only where scales are given (NULL else).
+ * Rows may begin anywhere; where dim is a multiple of 16 bytes and they begin between such, large layers take up to twice as long. */
 const char *AGatedBytes(long long rows, int dim, int hidden, int type, unsigned long long *bytes);
 const char *AGated(void *out, void *gate, void *up, float *gate_scales, float *up_scales, const void *x, const void *w_gate,
                    const void *w_up, long long rows, int dim, int hidden, long long out_stride, long long kept_stride,
