@@ -502,6 +502,7 @@ struct GradArgs {
 struct RowGrad {
   float most, log_sum, of_p, of_log, weight, entropy;
   unsigned token;  // vocab for none
+  bool live;       // false: a row of padding, whose gradient is 0 whatever its logits (and what they make of its sums)
 };
 
 template <bool kEntropy>
@@ -520,8 +521,10 @@ __device__ __forceinline__ RowGrad RowGradOf(const GradArgs &a, long long row) {
   if (nothing) r.weight = 0.0f;
   r.entropy = r.of_log = 0.0f;
   r.of_p = -r.weight;
+  r.live = there;
   if (kEntropy) {
     const float h = nothing ? 0.0f : a.scale * a.grad_entropy[row];
+    r.live = there || h != 0.0f;
     r.entropy = a.entropy[row];
     r.of_log = -h * kLn2;
     r.of_p -= h * r.entropy;
@@ -529,18 +532,18 @@ __device__ __forceinline__ RowGrad RowGradOf(const GradArgs &a, long long row) {
   return r;
 }
 
-template <typename T, bool kEntropy>
-__device__ __forceinline__ T GradOf(const RowGrad &r, float factor, float x) {
+template <bool kEntropy>
+__device__ __forceinline__ float GradOf(const RowGrad &r, float factor, float x) {
   const float d = fmaf(factor, x - r.most, -r.log_sum), p = Exp2(d);
-  return Round<T>(kEntropy ? p * fmaf(r.of_log, fmaxf(d, kLowest), r.of_p) : p * r.of_p);
+  return kEntropy ? p * fmaf(r.of_log, fmaxf(d, kLowest), r.of_p) : p * r.of_p;
 }
 // The gradient of the token itself: weight (1 - p) as it stands, where its parts would meet with opposite signs.
-template <typename T, bool kEntropy>
-__device__ __forceinline__ T GradOfToken(const RowGrad &r, float factor, float x) {
+template <bool kEntropy>
+__device__ __forceinline__ float GradOfToken(const RowGrad &r, float factor, float x) {
   const float d = fmaf(factor, x - r.most, -r.log_sum), p = Exp2(d);
   float g = r.weight * (1.0f - p);
   if (kEntropy) g += p * fmaf(r.of_log, fmaxf(d, kLowest), r.of_p + r.weight);
-  return Round<T>(g);
+  return g;
 }
 
 // Classes side by side: `lanes` threads of a workgroup take a row's piece of lanes * kVec * kUnroll classes.  4096 x 131,072 bf16, 2 GiB: 360 us, 6.0 TB/s.
@@ -560,10 +563,30 @@ __global__ void __launch_bounds__(256) k_grad_rows(const GradArgs a, int lanes, 
     const bool whole = a.vocab - begin >= (unsigned)(lanes * kVec * kUnroll);
     Pack<T, kVec> p[kUnroll];
     int held[kUnroll];
+    const auto store = [&](int u, const Pack<T, kVec> &v) {
+      T *to = grad + begin + (u * lanes + t) * kVec;
+      if (held[u] == kVec) {
+        if constexpr (kPast) StorePast(to, v);
+        else *reinterpret_cast<Pack<T, kVec> *>(to) = v;
+      } else {
+#pragma unroll
+        for (int c = 0; c < kVec; ++c)
+          if (c < held[u]) to[c] = v.v[c];
+      }
+    };
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const unsigned at = begin + (u * lanes + t) * kVec;
       held[u] = whole ? kVec : at < a.vocab ? (int)min(a.vocab - at, (unsigned)kVec) : 0;
+    }
+    if (!r.live) {  // (written and not read: 4096 x 131,072 bf16, 30 % padding, 563 -> 522 us with the forward pass)
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) store(u, Pack<T, kVec>{});
+      continue;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned at = begin + (u * lanes + t) * kVec;
       if (held[u] == kVec) {
         p[u] = *reinterpret_cast<const Pack<T, kVec> *>(x + at);
       } else {
@@ -579,22 +602,15 @@ __global__ void __launch_bounds__(256) k_grad_rows(const GradArgs a, int lanes, 
         float v = 0.0f;
 #pragma unroll
         for (int c = 0; c < kVec; ++c) v = hit == (unsigned)c ? (float)p[u].v[c] : v;
-        of_token = GradOfToken<T, kEntropy>(r, factor, v);
+        of_token = Round<T>(GradOfToken<kEntropy>(r, factor, v));
       }
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) p[u].v[c] = GradOf<T, kEntropy>(r, factor, (float)p[u].v[c]);
+      for (int c = 0; c < kVec; ++c) p[u].v[c] = Round<T>(GradOf<kEntropy>(r, factor, (float)p[u].v[c]));
       if (hit < (unsigned)kVec) {
 #pragma unroll
         for (int c = 0; c < kVec; ++c) p[u].v[c] = hit == (unsigned)c ? of_token : p[u].v[c];
       }
-      if (held[u] == kVec) {
-        if constexpr (kPast) StorePast(grad + at, p[u]);
-        else *reinterpret_cast<Pack<T, kVec> *>(grad + at) = p[u];
-      } else {
-#pragma unroll
-        for (int c = 0; c < kVec; ++c)
-          if (c < held[u]) grad[at + c] = p[u].v[c];
-      }
+      store(u, p[u]);
     }
   }
 }
@@ -618,7 +634,8 @@ __global__ void __launch_bounds__(256) k_grad_columns(const GradArgs a, unsigned
 #pragma unroll
       for (unsigned u = 0; u < kUnroll; ++u) {
         if (j0 + u >= end) break;
-        grad[(long long)(j0 + u) * a.grad_class_stride] = j0 + u == r.token ? GradOfToken<T, kEntropy>(r, factor, v[u]) : GradOf<T, kEntropy>(r, factor, v[u]);
+        const float g = j0 + u == r.token ? GradOfToken<kEntropy>(r, factor, v[u]) : GradOf<kEntropy>(r, factor, v[u]);
+        grad[(long long)(j0 + u) * a.grad_class_stride] = Round<T>(r.live ? g : 0.0f);
       }
     }
   }

@@ -284,7 +284,7 @@ const char *AAdamW(int count, void *const *params, const void *const *grads, flo
  *   top_tokens, top_log_probs [n][top]: the `top` (0 to 64, at most vocab) greatest logits in order, equal ones by their
  *                  index, and their log probabilities
  * Logits may be minus infinity: their probability is 0.  A row of nothing else has log probabilities of minus infinity, the
- * entropy 0 and the first `top` tokens.  A row with a NaN or with plus infinity has NaN for all, and -1 for its top tokens.
+ * entropy 0 and the first `top` tokens.  A row with a NaN or with plus infinity has NaN for all (but 0 for no token), and -1 for its top tokens.
  * n and vocab are below 2^31 (vocab by 65,536). */
 const char *ALogProbsBytes(long long n, long long vocab, int top, unsigned long long *bytes);
 const char *ALogProbs(float *log_probs, float *entropy, float *stats, int *top_tokens, float *top_log_probs, const void *logits,
@@ -296,7 +296,8 @@ const char *ALogProbs(float *log_probs, float *entropy, float *stats, int *top_t
  *   grad_logits[i][j] = scale * (grad_log_probs[i] * ([j == token i] - p_j)
  *                                - grad_entropy[i] * p_j * (log p_j + entropy[i]))
  * grad_entropy and entropy are both given or both NULL.  A row without a token has no part of the first kind, whatever
- * its grad_log_probs; logits of minus infinity, and rows of nothing else, have the gradient 0.  grad_logits has the logits' type,
+ * its grad_log_probs, and if its grad_entropy is 0, or not given, the gradient 0 whatever its logits.  Logits of minus infinity have the p 0, and so
+ * the gradient 0 but for the token itself; rows of nothing else have the gradient 0.  grad_logits has the logits' type,
  * and may be the logits themselves (same strides); otherwise the two must not overlap. */
 const char *ALogProbsGrad(void *grad_logits, const float *grad_log_probs, const float *grad_entropy, const void *logits,
                           const void *tokens, const float *stats, const float *entropy, long long n, long long vocab,
