@@ -17,7 +17,7 @@ __device__ __forceinline__ float ScaleOf(float most) { return most < __builtin_i
 
 // rint(v / scale).  With y = 1 / scale correctly rounded, q = v y is off by no more than a rounding or two and v - q scale is exact,
 // so that q + (v - q scale) y, rounded, is the quotient correctly rounded (Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000"): three operations, where a division takes about ten and bound the kernel (297 us for 65,536 x 4096, now 190).  Quotients are within
+// System/6000"): three operations, where a division takes about ten and bound the kernel (65,536 x 4096: 297 us, and 190 with nothing else changed).  Quotients are within
 // 127 and a rounding: the sum with 1.5 2^23, whose last bit is worth 1, rounds them to nearest, ties to even, with the code in its low eight bits.
 // (What a NaN becomes does not matter: the scale tells of it.)
 template <int N>

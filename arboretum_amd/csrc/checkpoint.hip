@@ -2,7 +2,8 @@
 //   scale = max |x| / 127,   code = x / scale, rounded to nearest (ties to even),   x ~ code * scale.
 // Codes of equal steps, not of 8-bit floating point: the values of a group differ little in size (their maximum is about 2.4
 // of their standard deviations where they are normal), where steps of max / 127 are off by 0.6 % of it and steps that grow with
-// the value, three bits each, by 2.6 % of the value.  One pass over memory bounds both: 65,536 x 4096 bf16, 0.83 GB each way, 157 and 162 us, 5.2 TB/s.
+// the value, three bits each, by 2.6 % of the value.  One pass over memory bounds both: 65,536 x 4096 bf16, 0.82 GB each way: 309 us there and back, 5.3 TB/s (one by
+// one under a profiler 173 and 200 at the median, 144 and 161 at best).
 #include "checkpoint.h"
 #include "operators_device.h"
 

@@ -42,12 +42,13 @@ __device__ __forceinline__ F4 Product(const Chunk<float> &a, const Chunk<float> 
 // ------------------------------------------------------------------ activations
 
 // (the instructions for powers of two and reciprocals, of a rounding each: a division and expf take three times the time, and an
-// epilogue of nothing but them is what bounds narrow layers)
+// epilogue of nothing but them is what bounds narrow layers.  Below -87.3, where 1 + e^-g passes 2^126, the reciprocal is 0: silu is 0 there instead of what is less than
+// 2^-119)
 __device__ __forceinline__ float PowerOfE(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ __forceinline__ float Sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + PowerOfE(-g)); }
 
 // Phi(g), and e^(-g^2/2) in two factors (which reach below 2^-126 together).  From -|g| on it is e^(-g^2/2) times Mills' ratio, here t P(t) with
-// t = 1 / (1 + 0.35 |g|): P has the least greatest relative error that a polynomial of its degree has for 0 <= |g| <= 16 (3e-8; summed in 32 bits 4e-7),
+// t = 1 / (1 + 0.35 |g|): P has the least greatest relative error that a polynomial of its degree has for 0 <= |g| <= 16 (3e-8, 9e-8 with its coefficients in 32 bits; summed in 32 bits 4e-7),
 // beyond which the other factor is 0.  (erfcf has a branch for either end, of which a wave runs both: 1003 x 771 x 2055 took 20.2 us.)
 __device__ __forceinline__ float Phi(float g, float *root) {
   const float a = fminf(fabsf(g), 16.0f), t = __builtin_amdgcn_rcpf(1.0f + 0.35f * a);
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_join(const Forward a, long l
 // Few rows (up to 16): 16 hidden columns a workgroup, whose eight waves share out the k's.  The weights are read once, from memory into the
 // registers that the products take them from: a lane's chunk is 16 bytes of a weight row, four steps of 64 bytes a row at once.
 // kApart: rows that begin anywhere.  Every eighth of them begins alike within 16 bytes, and the workgroup takes sixteen of those; behind as many k's as
-// the row's first 16 bytes hold its chunks are aligned.  Reading the weights bounds it: 1 x 4096 x 16384 bf16 48 us, 5.6 TB/s.
+// the row's first 16 bytes hold its chunks are aligned.  (In which order a sum is formed, and so its last bits, then depend on where the weights lie.)  Reading the weights bounds it: 1 x 4096 x 16384 bf16 48 us, 5.6 TB/s.
 constexpr int kFewWaves = 8;
 template <typename T, int kAct, bool kApart>
 __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
@@ -735,8 +736,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) k_gated_few(const Forward a) {
   }
 }
 
-// Up to three matrices of rows that begin anywhere, to rows that begin at multiples of 64 elements, 0 behind each row's end.  (12 MB in rows of 771 fp16: 8 us; 290 MB
-// in rows of 3033 57, 5.1 TB/s.)
+// Up to three matrices of rows that begin anywhere, to rows that begin at multiples of 64 elements, 0 behind each row's end.  (x and both weights of 1003 x 771 x 2055 fp16,
+// 16 MB read and written: 8 us; 290 MB in rows of 3033 57, 5.1 TB/s.)
 struct Padded {
   const void *from[3];
   void *to[3];

@@ -4,7 +4,7 @@
 //   grad_j   = scale (g ([j = token] - p_j) - h p_j (log p_j + entropy)),   p_j = exp(a_j - log S).
 // A row is read once: maximum, S and sum a exp a run along it, and a new maximum scales what was summed before
 // (sum (a + d) exp (a + d) = exp d (sum a exp a + d sum exp a)).  The gradient reads the row once more: what must be known of all of it, the maximum and
-// log S, is kept in 8 bytes a row.  Reading and writing the logits bounds both (4096 x 131,072 bf16: 1 GiB read in 190 us, read and written in 360, 5.7 and 6.0
+// log S, is kept in 8 bytes a row.  Reading and writing the logits bounds both (4096 x 131,072 bf16: 1 GiB read in 212 us, read and written in 362, 5.1 and 5.9
 // TB/s); with the likeliest tokens the search for them, where rows are short.
 #include <algorithm>
 #include <cmath>
